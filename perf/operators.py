@@ -73,16 +73,21 @@ def listed():
 
 
 def _log_int(rng, lo, hi):
-    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+    v = max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+    return v - 1 if v % 1024 == 0 and v > lo else v  # the listed cases have the round sizes
+
+
+def _log_multiple(rng, lo, hi, step):
+    """Mostly an odd multiple of `step`, as sizes of models are multiples; otherwise any size."""
+    v = _log_int(rng, lo, hi)
+    return max(lo, (v // step | 1) * step) if rng.random() < 0.7 and v >= 2 * step else v
 
 
 def draw(rng):
     op = rng.choice(["norm", "norm", "norm_bwd", "route", "route_bwd", "linear", "linear", "experts", "experts"])
     if op in ("norm", "norm_bwd"):
         dtype = rng.choice(["f16", "bf16", "bf16", "f32"])
-        H = _log_int(rng, 64, 16384)
-        if rng.random() < 0.7:  # most hidden sizes are multiples of 64, some are odd
-            H = max(64, H // 64 * 64)
+        H = _log_multiple(rng, 64, 16000, 64)
         c = {"op": op, "T": _log_int(rng, 1, 8192), "H": H, "dtype": dtype,
              "weight": rng.choice([dtype, "f32"]), "residual": rng.random() < 0.7}
         if op == "norm":
@@ -92,26 +97,22 @@ def draw(rng):
         groups = rng.choice([1, 1, 4, 8])
         E = groups * max(2, _log_int(rng, 8, 512) // groups)
         top_groups = 1 if groups == 1 else rng.randint(groups // 2, groups)
-        return {"op": op, "T": _log_int(rng, 1, 32768), "E": E,
-                "k": rng.randint(1, min(8, top_groups * (E // groups))),
+        k = rng.randint(1, min(8, top_groups * (E // groups)))
+        return {"op": op, "T": _log_int(rng, 1, 32768), "E": E, "k": k,
                 "dtype": rng.choice(["f32", "f32", "f16", "bf16"]), "scoring": rng.choice(["softmax", "sigmoid"]),
                 "bias": rng.random() < 0.5, "groups": groups, "top_groups": top_groups,
-                "renorm": rng.random() < 0.6, "scale": rng.choice([1.0, 2.5]),
+                # a single renormalised weight is a constant
+                "renorm": k > 1 and rng.random() < 0.6, "scale": rng.choice([1.0, 2.5]),
                 "masked": rng.choice([0.0, 0.0, 0.3])}
     group = rng.choice([32, 64, 128, 128])
     zeros = rng.random() < 0.5
     dtype = rng.choice(["f16", "bf16"])
     if op == "linear":
-        K = _log_int(rng, 64, 16384)
-        N = _log_int(rng, 64, 16384)
-        if rng.random() < 0.7:
-            K, N = max(64, K // 128 * 128), max(64, N // 16 * 16)
+        K, N = _log_multiple(rng, 64, 16000, 128), _log_multiple(rng, 64, 16000, 16)
         return {"op": op, "M": _log_int(rng, 1, 48), "N": N, "K": K, "group": group, "zeros": zeros, "dtype": dtype}
     E = rng.choice([8, 16, 32, 60, 64])
-    H = max(128, _log_int(rng, 256, 7168) // 64 * 64)
-    I = _log_int(rng, 128, min(4096, 7168 * 2048 // H))
-    if rng.random() < 0.7:
-        I = max(128, I // 64 * 64)
+    H = (_log_int(rng, 256, 7000) // 64 | 1) * 64
+    I = _log_multiple(rng, 128, min(4000, 7168 * 2048 // H - 64), 64)
     return {"op": op, "T": _log_int(rng, 1, 128), "H": H, "I": I, "E": E, "k": rng.choice([1, 2, 4, 8]),
             "group": group, "zeros": zeros, "dtype": dtype, "skew": rng.choice([0.0, 0.0, 1.1])}
 
