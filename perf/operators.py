@@ -271,8 +271,11 @@ def _run_own(s):
 
 
 def _quantised(case, q, scale, h):
-    """int8 codes as the values they stand for; e4m3 values are numbers already."""
-    return {"q": q if case["quant"] == "fp8" else torch.mul(q, scale[:, None]), "scale": scale, "h": h}
+    """int8 codes as the values they stand for, in the type of the activations; e4m3 values are
+    numbers already."""
+    if case["quant"] == "int8":
+        q = torch.mul(q, scale[:, None], out=torch.empty(q.shape, dtype=DTYPES[case["dtype"]], device=q.device))
+    return {"q": q, "scale": scale, "h": h}
 
 
 def _run_plain(s):
