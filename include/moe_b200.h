@@ -443,6 +443,35 @@ MOE_API int moe_ep_p2p_compute_push(const uint64_t* regions, void* own_region, i
 MOE_API int moe_ep_p2p_push_finish(const void* own_region, int64_t num_tokens, int64_t max_tokens, int64_t hidden,
                                    int64_t topk, int world, int64_t num_experts, int dtype, void* out, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Root-mean-square norm with the residual's addition (the step in front of the router and the
+ * experts; no reference counterpart, the reference starts at the stacked token rows).
+ *   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * weight
+ * The sum and the statistics are fp32; y and h are each rounded once.
+ *
+ * moe_add_rms_norm: x, residual (NULL: h = x) [T, H] dtype (MOE_F16 / MOE_BF16 / MOE_F32), row
+ *   pitches ld_x, ld_residual in elements; weight [H] weight_dtype (dtype or MOE_F32).
+ *   h_out [T, H] dtype, pitch ld_h, or NULL. out [T, H], pitch ld_out: dtype when out_dtype == dtype;
+ *   with out_dtype MOE_I8 / MOE_F8E4M3 8-bit rows with scale [T] fp32 = max|y| / 127 or / 448, as
+ *   moe_quantize_rows_int8 / _fp8 (y is not rounded to dtype in between). x, residual, h_out and (in
+ *   dtype) out may be the same rows.
+ * moe_add_rms_norm_backward: dy, h [T, H] dtype, dh (gradient of h from its other uses, or NULL);
+ *   dx [T, H] dtype = gradient of x, which is also that of the residual; dweight [H] weight_dtype.
+ *   The dweight sum has a fixed order. workspace: moe_add_rms_norm_backward_workspace_bytes(T, H).
+ * Inputs may have any pitch >= 0 (0: one row for all tokens), outputs any pitch >= H; rows that start on 16-byte
+ * boundaries are moved in 16-byte words. Requirements: 1 <= H <= 16384, 0 <= T, eps >= 0.
+ * ---------------------------------------------------------------------------------------- */
+MOE_API int moe_add_rms_norm(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* weight,
+                             int weight_dtype, void* out, int64_t ld_out, int out_dtype, float* scale, void* h_out,
+                             int64_t ld_h, int64_t num_tokens, int64_t hidden, float eps, int dtype, void* stream);
+
+MOE_API size_t moe_add_rms_norm_backward_workspace_bytes(int64_t num_tokens, int64_t hidden);
+
+MOE_API int moe_add_rms_norm_backward(const void* dy, int64_t ld_dy, const void* h, int64_t ld_h, const void* dh,
+                                      int64_t ld_dh, const void* weight, int weight_dtype, void* dx, int64_t ld_dx,
+                                      void* dweight, int64_t num_tokens, int64_t hidden, float eps, int dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

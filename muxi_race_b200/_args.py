@@ -1,0 +1,51 @@
+"""Argument helpers of the operators that are called many times per step (small calls, where the
+host time of a call counts)."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+FLOATS = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16, torch.float32: _lib.MOE_F32}
+HALVES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
+IDS = {torch.int32: _lib.MOE_I32, torch.int64: _lib.MOE_I64}
+
+#: handle of the current stream of a device ordinal, without building a Stream object
+raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def require(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def rows(t: torch.Tensor, name: str, device: torch.device | None = None) -> torch.Tensor:
+    """`t` [..., H] as a 2-D view whose rows are contiguous; raises if there is none."""
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name} must be a CUDA tensor" + (f" on {device}" if device is not None else ""))
+    if t.dim() != 2:
+        require(t.dim() >= 1, f"{name} must have at least one dimension")
+        try:
+            t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+        except RuntimeError:
+            raise ValueError(f"{name} must have one row pitch: its leading dimensions cannot be viewed as one") from None
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{name} must be contiguous along its last dimension")
+    return t
+
+
+def pitch(t: torch.Tensor) -> int:
+    """Row pitch of a 2-D tensor in elements (a single row has whatever pitch suits)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def launch(device: torch.device, name: str, *args) -> None:
+    """Call entry point `name` with the current stream of `device` appended, that device current."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        code = getattr(_lib.lib(), name)(*args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = getattr(_lib.lib(), name)(*args, raw_stream(index))
+    if code:
+        _lib.check(name, code)

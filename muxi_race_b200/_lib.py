@@ -36,6 +36,17 @@ SIGNATURES = {
     "moe_set_tile": (_int, [_int, ctypes.c_char_p]),
     "moe_set_a_path": (_int, [ctypes.c_char_p]),
     "moe_set_single_kernel": (_int, [_int]),
+    "moe_add_rms_norm": (
+        _int,
+        [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _i64, _int, _c_void_p, _c_void_p, _i64, _i64, _i64,
+         ctypes.c_float, _int, _c_void_p],
+    ),
+    "moe_add_rms_norm_backward_workspace_bytes": (_size, [_i64, _i64]),
+    "moe_add_rms_norm_backward": (
+        _int,
+        [_c_void_p, _i64] * 3 + [_c_void_p, _int, _c_void_p, _i64, _c_void_p, _i64, _i64, ctypes.c_float, _int, _c_void_p,
+                                 _size, _c_void_p],
+    ),
     "moe_ep_region_bytes": (_size, [_i64, _i64, _i64, _i64]),
     "moe_ep_region_alloc": (_int, [_size, ctypes.POINTER(_c_void_p)]),
     "moe_ep_region_free": (_int, [_c_void_p]),

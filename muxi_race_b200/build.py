@@ -10,13 +10,21 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libmoe_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
-SOURCES = ["moe_capi.cu"]
-HEADERS = ["moe_gemm.cuh", "moe_gemm_pair.cuh", "moe_gemm_tn.cuh", "ep_p2p.cuh", "route_align.cuh", "router_topk.cuh", "ordered_combine.cuh", "gather_quant.cuh", "ep_kernels.cuh", "sm100_ptx.cuh"]
+OBJ_DIR = os.path.join(PKG_DIR, "_build")
+API_HEADERS = ["capi_host.h", os.path.join("..", "..", "include", "moe_b200.h")]
+# translation unit -> the headers it includes besides API_HEADERS (one object each, so that a change
+# to one operator does not recompile the others)
+SOURCES = {
+    "moe_capi.cu": ["moe_gemm.cuh", "moe_gemm_pair.cuh", "moe_gemm_tn.cuh", "ep_p2p.cuh", "route_align.cuh",
+                    "router_topk.cuh", "ordered_combine.cuh", "gather_quant.cuh", "ep_kernels.cuh", "sm100_ptx.cuh"],
+    "norm_capi.cu": ["rms_norm.cuh"],
+}
 GENCODE = "arch=compute_100a,code=sm_100a"
 
 
@@ -34,21 +42,30 @@ def _stale(target: str, deps: list[str]) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _compile(source: str, force: bool, verbose: bool) -> str:
+    obj = os.path.join(OBJ_DIR, os.path.splitext(source)[0] + ".o")
+    deps = [os.path.join(CSRC, f) for f in [source] + SOURCES[source] + API_HEADERS]
+    if force or _stale(obj, deps):
+        cmd = [nvcc_path(), "-gencode", GENCODE, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+               "-Xcompiler", "-fvisibility=hidden", "-c", "-o", obj + ".tmp", os.path.join(CSRC, source)]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(obj + ".tmp", obj)
+    return obj
+
+
 def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile ``csrc/*.cu`` into ``libmoe_b200.so`` (skipped when up to date)."""
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(os.path.dirname(PKG_DIR), "include", "moe_b200.h"))
+    """Compile ``csrc/*.cu`` and link ``libmoe_b200.so`` (skipped when up to date)."""
+    deps = [os.path.join(CSRC, f) for src, headers in SOURCES.items() for f in [src] + headers + API_HEADERS]
     if not force and not _stale(LIB_PATH, deps):
         return LIB_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
+        objs = list(pool.map(lambda src: _compile(src, force, verbose), SOURCES))
     tmp = LIB_PATH + ".tmp"
-    cmd = [
-        nvcc_path(), "-gencode", GENCODE, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-        "-Xcompiler", "-fvisibility=hidden", "-shared", "-o", tmp,
-    ] + [os.path.join(CSRC, f) for f in SOURCES]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    subprocess.run([nvcc_path(), "-gencode", GENCODE, "-shared", "-o", tmp] + objs, check=True)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

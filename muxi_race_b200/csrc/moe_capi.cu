@@ -13,7 +13,7 @@
 #include <string>
 #include <type_traits>
 
-#include "../../include/moe_b200.h"
+#include "capi_host.h"
 #include "ep_kernels.cuh"
 #include "ep_p2p.cuh"
 #include "gather_quant.cuh"
@@ -38,7 +38,15 @@ void prof_record(int i, cudaStream_t s) {
   if (t_prof_events && i < t_prof_n && t_prof_events[i]) cudaEventRecord(static_cast<cudaEvent_t>(t_prof_events[i]), s);
 }
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+struct DeviceInfo {
+  std::atomic<int> sms{0};
+  std::atomic<uint32_t*> status{nullptr};
+  std::atomic<uint64_t> attr_done[48] = {};  // bit per kernel whose smem attribute has been raised
+};
+DeviceInfo g_dev[kMaxDevices];
+
+}  // namespace
+
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -49,27 +57,7 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-#define MOE_CUDA(call)                                                                        \
-  do {                                                                                        \
-    cudaError_t err_ = (call);                                                                \
-    if (err_ != cudaSuccess)                                                                  \
-      return fail(MOE_ERR_CUDA, "%s failed: %s (%s:%d)", #call, cudaGetErrorString(err_), __FILE__, __LINE__); \
-  } while (0)
-
-#define MOE_TRY(expr)          \
-  do {                         \
-    int rc_ = (expr);          \
-    if (rc_ != MOE_OK) return rc_; \
-  } while (0)
-
-constexpr int kMaxDevices = 64;
-
-struct DeviceInfo {
-  std::atomic<int> sms{0};
-  std::atomic<uint32_t*> status{nullptr};
-  std::atomic<uint64_t> attr_done[48] = {};  // bit per kernel whose smem attribute has been raised
-};
-DeviceInfo g_dev[kMaxDevices];
+void clear_error() { t_last_error.clear(); }
 
 int current_device(int* dev) {
   MOE_CUDA(cudaGetDevice(dev));
@@ -86,6 +74,8 @@ int device_sms(int dev, int* sms) {
   *sms = v;
   return MOE_OK;
 }
+
+namespace {
 
 int device_status_ptr(int dev, uint32_t** p) {
   uint32_t* v = g_dev[dev].status.load(std::memory_order_acquire);
