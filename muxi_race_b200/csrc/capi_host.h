@@ -18,6 +18,7 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 void clear_error();
 int current_device(int* dev);        // MOE_OK and the current device's ordinal (< kMaxDevices)
 int device_sms(int dev, int* sms);   // MOE_OK and the device's SM count (cached)
+int device_status_ptr(int dev, uint32_t** p);  // MOE_OK and the device's status word
 
 #define MOE_CUDA(call)                                                                        \
   do {                                                                                        \

@@ -75,8 +75,6 @@ int device_sms(int dev, int* sms) {
   return MOE_OK;
 }
 
-namespace {
-
 int device_status_ptr(int dev, uint32_t** p) {
   uint32_t* v = g_dev[dev].status.load(std::memory_order_acquire);
   if (v == nullptr) {
@@ -86,6 +84,8 @@ int device_status_ptr(int dev, uint32_t** p) {
   *p = v;
   return MOE_OK;
 }
+
+namespace {
 
 template <typename K>
 int raise_smem(int dev, int bit, K kernel, int bytes) {
