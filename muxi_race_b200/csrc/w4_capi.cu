@@ -1,5 +1,6 @@
 // w4_capi.cu — host side of the 4-bit products (include/moe_b200.h).
 #include <algorithm>
+#include <cmath>
 
 #include "capi_host.h"
 #include "w4_gemv.cuh"
@@ -14,33 +15,48 @@ size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
 // How one product is laid over the GPU.
 struct W4Plan {
-  int strips, kt, record;
-  int tile_rows, wps, strip_groups;
-  int slices, slice_kt, x_pitch, x_bytes, red_bytes, stages;
-  size_t smem() const { return static_cast<size_t>(x_bytes) + red_bytes + static_cast<size_t>(stages) * kW4Warps * record; }
+  int strips, kt, nt, warps, wps;
+  int tile_rows, slices, slice_kt, x_pitch, x_bytes, xsum_bytes, sum_bytes;
+  size_t smem() const { return static_cast<size_t>(x_bytes) + xsum_bytes + sum_bytes; }
 };
 
+#ifndef SUMCOST
+#define SUMCOST 1.0
+#endif
+constexpr double kW4SumCost = SUMCOST;
 constexpr int kW4Smem = kMaxDynamicSmem - 1024;  // static shared memory of the kernel, rounded up
-constexpr int kW4GoodStages = 8;                 // about 64 KB in flight: bandwidth times latency of an SM
 
-W4Plan w4_plan(int strips, int64_t K, int group, bool zeros, int tile_rows) {
+// `tiles`: token tiles expected, `sms`: CTAs.
+W4Plan w4_plan(int strips, int64_t K, int group, int tile_rows, double tiles, int sms) {
   W4Plan p{};
   p.strips = strips;
   p.kt = static_cast<int>(ceil_div(K, kW4TileK));
-  p.record = w4_record_bytes(group, zeros);
   p.tile_rows = tile_rows;
-  p.wps = p.kt >= 8 ? 8 : p.kt >= 4 ? 4 : p.kt >= 2 ? 2 : 1;
-  p.strip_groups = static_cast<int>(ceil_div(strips, kW4Warps / p.wps));
-  p.red_bytes = 2 * kW4Warps * 512 * (tile_rows <= 8 ? 1 : tile_rows <= 16 ? 2 : 4);
-  const int stage = kW4Warps * p.record;
-  const int64_t room = kW4Smem - p.red_bytes - kW4GoodStages * stage;
-  // K is cut so that the rows' slice of x fits beside the ring, in whole steps of the warps
-  const int64_t most = std::max<int64_t>((room / tile_rows - 64) / (2 * kW4TileK) / p.wps, 1) * p.wps;
-  p.slice_kt = static_cast<int>(ceil_div(ceil_div(p.kt, ceil_div(p.kt, most)), p.wps)) * p.wps;
+  p.nt = tile_rows <= 8 ? 1 : tile_rows <= 16 ? 2 : 4;
+  p.warps = w4_warps(p.nt);
+  p.sum_bytes = 2 * p.warps * p.nt * 512;
+  // K is cut so that the rows' slice of x (and its sums) fits in shared memory
+  const int xsum_kt = kW4TileK / group * kW4MaxRows * 4;
+  const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows + xsum_kt);
+  p.slice_kt = static_cast<int>(ceil_div(p.kt, ceil_div(p.kt, most)));
   p.slices = static_cast<int>(ceil_div(p.kt, p.slice_kt));
-  p.x_pitch = std::min(p.slice_kt, p.kt) * 2 * kW4TileK + 64;  // 64: rows r and r + 1 in different banks
+  p.x_pitch = p.slice_kt * 2 * kW4TileK + 64;  // 64: rows r and r + 1 in different banks
   p.x_bytes = static_cast<int>(ceil_div(static_cast<int64_t>(tile_rows) * p.x_pitch, 128) * 128);
-  p.stages = std::min(kW4MaxStages, (kW4Smem - p.red_bytes - p.x_bytes) / stage);
+  p.xsum_bytes = p.slice_kt * xsum_kt;
+  // Warps per strip: few make the sums rare, many give each CTA's groups of warps nearly the same
+  // number of strips. The cost of a choice in tile times: rounds of strips per CTA, each a warp's
+  // tiles and what handing on a sum takes.
+  const double per_cta = tiles * p.slices * strips / sms;
+  const int last_kt = p.kt - (p.slices - 1) * p.slice_kt;  // every warp has a tile in every slice
+  double best = 0;
+  for (int wps = 1; wps <= p.warps && wps <= last_kt; ++wps) {
+    const double rounds = std::ceil(per_cta / (p.warps / wps) - 1e-9);
+    const double cost = rounds * (static_cast<double>(ceil_div(p.slice_kt, wps)) + kW4SumCost);
+    if (p.wps == 0 || cost < best) {
+      best = cost;
+      p.wps = wps;
+    }
+  }
   return p;
 }
 
@@ -76,17 +92,26 @@ int launch(Kernel kernel, int grid, int threads, size_t smem, cudaStream_t s, bo
   return MOE_OK;
 }
 
-template <typename T, int GROUP>
+template <typename T, int GROUP, int NT>
 int launch_gemv_t(const W4Args& a, size_t smem, int grid, int dev, bool dependent, cudaStream_t s) {
-  MOE_TRY((allow_smem<w4_gemv_kernel<T, GROUP>>(dev)));
-  return launch(w4_gemv_kernel<T, GROUP>, grid, kW4Threads, smem, s, dependent, a);
+  MOE_TRY((allow_smem<w4_gemv_kernel<T, GROUP, NT>>(dev)));
+  return launch(w4_gemv_kernel<T, GROUP, NT>, grid, w4_threads(NT), smem, s, dependent, a);
+}
+
+template <typename T, int GROUP>
+int launch_gemv_g(const W4Args& a, const W4Plan& p, int grid, int dev, bool dependent, cudaStream_t s) {
+  if (p.nt == 1) return launch_gemv_t<T, GROUP, 1>(a, p.smem(), grid, dev, dependent, s);
+  if (p.nt == 2) return launch_gemv_t<T, GROUP, 2>(a, p.smem(), grid, dev, dependent, s);
+  return launch_gemv_t<T, GROUP, 4>(a, p.smem(), grid, dev, dependent, s);
 }
 
 template <typename T>
 int launch_gemv(const W4Args& a, const W4Plan& p, int group, int grid, int dev, bool dependent, cudaStream_t s) {
-  if (group == 32) return launch_gemv_t<T, 32>(a, p.smem(), grid, dev, dependent, s);
-  if (group == 64) return launch_gemv_t<T, 64>(a, p.smem(), grid, dev, dependent, s);
-  return launch_gemv_t<T, 128>(a, p.smem(), grid, dev, dependent, s);
+  if (p.wps < 1 || p.slice_kt < 1 || p.smem() > kW4Smem)
+    return fail(MOE_ERR_UNSUPPORTED, "no room for the rows of x: %zu bytes of shared memory", p.smem());
+  if (group == 32) return launch_gemv_g<T, 32>(a, p, grid, dev, dependent, s);
+  if (group == 64) return launch_gemv_g<T, 64>(a, p, grid, dev, dependent, s);
+  return launch_gemv_g<T, 128>(a, p, grid, dev, dependent, s);
 }
 
 W4Args w4_args(const W4Plan& p, const void* w, int zeros, int64_t expert_bytes, uint32_t* status) {
@@ -96,7 +121,6 @@ W4Args w4_args(const W4Plan& p, const void* w, int zeros, int64_t expert_bytes, 
   a.strips = p.strips;
   a.kt = p.kt;
   a.wps = p.wps;
-  a.strip_groups = p.strip_groups;
   a.slices = p.slices;
   a.slice_kt = p.slice_kt;
   a.zeros = zeros != 0;
@@ -104,8 +128,7 @@ W4Args w4_args(const W4Plan& p, const void* w, int zeros, int64_t expert_bytes, 
   a.gather_div = 1;
   a.x_pitch = p.x_pitch;
   a.x_bytes = p.x_bytes;
-  a.red_bytes = p.red_bytes;
-  a.stages = p.stages;
+  a.xsum_bytes = p.xsum_bytes;
   a.status = status;
   return a;
 }
@@ -149,7 +172,7 @@ int w4_linear_t(const void* x, int64_t ld_x, const void* packed, void* out, int6
   a.epilogue = p.slices == 1 ? kW4Out : kW4Partial;
   a.part = part;
   a.part_rows = M;
-  const int64_t units = ceil_div(M, p.tile_rows) * p.slices * p.strip_groups;
+  const int64_t units = ceil_div(M, p.tile_rows) * p.slices * p.strips;
   MOE_TRY(launch_gemv<T>(a, p, group, static_cast<int>(std::min<int64_t>(units, sms)), dev, false, s));
   if (p.slices == 1) return MOE_OK;
   return launch_combine_w<T, int32_t>(part, p.slices, M, p.strips * 16, nullptr, nullptr, MOE_F32, 0, 1, M, N,
@@ -172,12 +195,15 @@ int moe_tile_rows(int64_t R, int64_t E) {
   return static_cast<int>(std::min<int64_t>(rows, R));
 }
 
-W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int g13, int z13, int g2, int z2) {
+W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int g13, int g2, int sms) {
   W4MoeLayout L{};
   const int64_t R = T * topk;
   const int tile_rows = moe_tile_rows(R, E);
-  L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, z13 != 0, tile_rows);
-  L.p2 = w4_plan(w4_strips(H, 0), I, g2, z2 != 0, tile_rows);
+  // experts chosen by someone, if all are equally likely
+  const double active = static_cast<double>(E) * (1 - std::pow(1 - 1.0 / static_cast<double>(E), static_cast<double>(R)));
+  const double tiles = std::max(active, static_cast<double>(R) / tile_rows);
+  L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, tile_rows, tiles, sms);
+  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * 8, g2, tile_rows, tiles, sms);
   L.max_tiles = R / tile_rows + std::min(E, R);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -348,7 +374,7 @@ int moe_w4_unpack(const void* packed, int dtype, int64_t matrices, int64_t N, in
 size_t moe_w4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int has_zeros) {
   clear_error();
   if (M < 1 || check_format(1, N, K, group, 0) != MOE_OK) return 0;
-  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, has_zeros != 0, linear_tile_rows(M));
+  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, linear_tile_rows(M), 1, 1);
   return p.slices == 1 ? 0 : sizeof(float) * static_cast<size_t>(p.slices) * static_cast<size_t>(M) * p.strips * 16;
 }
 
@@ -362,7 +388,6 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
   if (!x || !packed || !out) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
   if (ld_x < 0 || ld_out < N) return fail(MOE_ERR_INVALID_ARG, "ld_x must be >= 0 and ld_out >= n");
   if (reinterpret_cast<uintptr_t>(packed) % 16 != 0) return fail(MOE_ERR_ALIGNMENT, "packed must be 16-byte aligned");
-  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, has_zeros != 0, linear_tile_rows(M));
   const size_t need = moe_w4_linear_workspace_bytes(M, N, K, group, has_zeros);
   if (need > 0) {
     if (!workspace || workspace_bytes < need) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", need);
@@ -373,6 +398,8 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &status));
+  const int tile_rows = linear_tile_rows(M);
+  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, tile_rows, ceil_div(M, tile_rows), sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   float* part = static_cast<float*>(workspace);
   return dtype == MOE_F16
@@ -385,7 +412,7 @@ size_t moe_fused_w4_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t 
                                     int group2, int has_zeros2) {
   clear_error();
   if (T < 1 || check_moe(T, topk, E, H, I, group13, group2) != MOE_OK) return 0;
-  return w4_moe_layout(T, topk, E, H, I, group13, has_zeros13, group2, has_zeros2).total;
+  return w4_moe_layout(T, topk, E, H, I, group13, group2, 1).total;
 }
 
 int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int has_zeros13, const void* w2, int group2,
@@ -403,14 +430,14 @@ int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int 
   if (ld_x < 0) return fail(MOE_ERR_INVALID_ARG, "ld_hidden must be >= 0");
   if (reinterpret_cast<uintptr_t>(w13) % 16 != 0 || reinterpret_cast<uintptr_t>(w2) % 16 != 0)
     return fail(MOE_ERR_ALIGNMENT, "packed weights must be 16-byte aligned");
-  const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, has_zeros13, group2, has_zeros2);
-  if (!workspace || workspace_bytes < L.total) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", L.total);
-  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(MOE_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   int dev, sms;
   uint32_t* status;
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &status));
+  const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, group2, sms);
+  if (!workspace || workspace_bytes < L.total) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", L.total);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(MOE_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MOE_F16)

@@ -7,16 +7,15 @@
 // fp32 on the tensor cores, and that sum is scaled and added in fp32.
 //
 // Few rows leave the weights' bytes as the bound: N K / 2 bytes for 2 M N K operations. So the
-// weights are laid out once (moe_w4_pack) as the stream that the kernel reads, and everything else is
-// arranged around that stream:
+// weights are laid out once (moe_w4_pack) as the stream that the kernel reads:
 //   tile    16 rows x 128 columns: 1024 bytes of values, the groups' scales, the zero points. In a
 //           tile, lane l's 16 bytes hold its mma.m16n8k16 A fragments of four steps, so a tile is two
-//           conflict-free 16-byte shared loads a lane and no shuffles.
+//           16-byte loads a lane straight into registers, with no shuffles and no shared memory.
 //   strip   the tiles of 16 rows, one after another along K; an expert's strips follow each other.
-// One CTA per SM: a producer thread streams tiles with bulk copies through a ring of mbarrier stages
-// (one tile per consumer warp and stage) across all the work of the CTA, so that the copies of the next
-// strip, expert or token tile run while this one is computed. x (at most 32 rows, one slice of K)
-// stays in shared memory. Warps that share a strip split K and add their sums in shared memory.
+// One CTA per SM. Its warps walk through strips with the loads of the next tiles in flight in
+// registers (kW4Ahead tiles a warp: about 64 KB an SM); x (at most 32 rows, one slice of K) stays in
+// shared memory. Warps that share a strip split K; their sums go through shared memory to the store
+// warps, which add them up, so that no consumer waits for another or for a store.
 // mma.sync and not tcgen05.mma: the weights must pass the registers to be unpacked, a 16-row strip
 // per warp keeps them there as the A operand, and with at most 32 columns the tensor rate is not
 // the bound.
@@ -29,12 +28,14 @@
 
 namespace moe {
 
-constexpr int kW4Warps = 8;            // consumer warps; one more warp produces
-constexpr int kW4Threads = kW4Warps * 32 + 32;
+constexpr int kW4StoreWarps = 2;       // warps that add up the consumers' sums and store them
+constexpr int kW4Ahead = 4;            // tiles that a warp has in flight
 constexpr int kW4TileK = 128;
 constexpr int kW4TileBytes = 1024;     // values of one tile
 constexpr int kW4MaxRows = 32;         // rows of x at a time
-constexpr int kW4MaxStages = 16;
+// consumer warps: with the store warps 16 of 128 registers, or 12 of 168 for four blocks of 8 rows
+__host__ __device__ constexpr int w4_warps(int nt) { return nt <= 2 ? 14 : 10; }
+__host__ __device__ constexpr int w4_threads(int nt) { return (w4_warps(nt) + kW4StoreWarps) * 32; }
 
 // bytes of a tile with its scales (half2 of rows r, r + 8 per group) and zero points (byte pairs)
 __host__ __device__ constexpr int w4_record_bytes(int group, bool zeros) {
@@ -47,8 +48,7 @@ struct W4Args {
   const uint8_t* w;         // [experts][strips][kt] records
   long long expert_bytes;
   int strips, kt;           // strips, and tiles along K
-  int wps;                  // warps that share a strip (kW4Warps / wps strips at a time)
-  int strip_groups;         // ceil(strips / (kW4Warps / wps))
+  int wps;                  // warps that share a strip
   int slices, slice_kt;     // K slices whose x fits in shared memory, and their tiles
   int zeros;                // records hold zero points
   const void* x;
@@ -68,17 +68,11 @@ struct W4Args {
   float* part;              // kW4Partial: [slice][row][strips * 16]
   long long part_rows;
   int x_pitch;              // bytes of a row of x in shared memory
-  int x_bytes, red_bytes;   // bytes of the x region and of the warps' sums
-  int stages;
+  int x_bytes, xsum_bytes;  // bytes of the rows of x, and of their sums per group (fp16)
   int early;                // the tile list is older than the kernel before this one
   uint32_t* status;
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void named_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -87,47 +81,48 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 
 // ------------------------------------------------------------------ unpacking
 // Eight values of a word as A fragments: nibble i of the low (high) half is the first (second) value
-// of register i; registers 0 and 2 are row r, 1 and 3 row r + 8. The nibbles become the low mantissa
-// bits of 1024 (fp16) or 128 (bf16), and one subtraction gives q - z, exactly.
+// of register i; registers 0 and 2 are row r, 1 and 3 row r + 8.
+//   fp16: the nibbles themselves, as the low bits of a subnormal number, are q 2^-24 (row r) and
+//     q 2^-20 (row r + 8, one nibble further up): no instruction but the masks. The powers of two go
+//     into the scales, and the zero points into one term per group: sum (q - z) x = sum q x - z sum x.
+//   bf16 (whose subnormal products fp32 cannot hold): the nibbles become the low bits of 128 + q, and
+//     one subtraction gives q - z, exactly.
 template <typename T> struct W4Type;
+__device__ __forceinline__ uint32_t w4_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));  // (w & mask) | bits
+  return v;
+}
 template <> struct W4Type<__half> {
-  // c[0]: 1024 + z of row r, c[1]: 64 + z of row r + 8 (its nibbles are read 16 times too large)
-  static __device__ __forceinline__ void offsets(int z0, int z1, uint32_t (&c)[2]) {
-    c[0] = (0x6400u + z0) * 0x10001u;
-    c[1] = (0x5400u + (z1 << 4)) * 0x10001u;  // fp16 64: 16 steps to a unit
-  }
-  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t c) {
-    uint32_t v = (w & 0x000f000fu) | 0x64006400u;
-    asm("sub.f16x2 %0, %0, %1;" : "+r"(v) : "r"(c));
-    return v;
-  }
-  static __device__ __forceinline__ uint32_t high(uint32_t w, uint32_t c) {
-    uint32_t v = (w & 0x00f000f0u) | 0x64006400u;
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(v) : "r"(0x2c002c00u), "r"(c ^ 0x80008000u));  // v / 16 - c
-    return v;
-  }
-  static __device__ __forceinline__ void unpack(uint32_t w, const uint32_t (&c)[2], uint32_t (&a)[4]) {
-    a[0] = low(w, c[0]);
-    a[1] = high(w, c[1]);
+  static constexpr bool kSums = true;
+  static constexpr float kScale0 = 16777216.0f, kScale1 = 1048576.0f;
+  static __device__ __forceinline__ void unpack(uint32_t w, const uint32_t (&)[2], uint32_t (&a)[4]) {
+    a[0] = w & 0x000f000fu;
+    a[1] = w & 0x00f000f0u;
     w >>= 8;
-    a[2] = low(w, c[0]);
-    a[3] = high(w, c[1]);
+    a[2] = w & 0x000f000fu;
+    a[3] = w & 0x00f000f0u;
   }
   static __device__ __forceinline__ float to_f(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+  template <bool FIRST>
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 template <> struct W4Type<__nv_bfloat16> {
-  static __device__ __forceinline__ void offsets(int z0, int z1, uint32_t (&c)[2]) {
-    c[0] = (0x4300u + z0) * 0x10001u;  // bf16 128: one step is a unit
-    c[1] = (0x4300u + z1) * 0x10001u;
-  }
+  static constexpr bool kSums = false;
+  static constexpr float kScale0 = 1.0f, kScale1 = 1.0f;
+  // c: 128 + z of rows r and r + 8 (bf16 128: one step is a unit)
   static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t c) {
-    uint32_t v = (w & 0x000f000fu) | 0x43004300u;
+    uint32_t v = w4_and_or(w, 0x000f000fu, 0x43004300u);
     asm("sub.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(c));
     return v;
   }
@@ -139,82 +134,144 @@ template <> struct W4Type<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float to_f(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+  template <bool FIRST>
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 
-// acc += tile * x for NT blocks of 8 rows of x. `tile`: a record; `x`: this lane's place in the
-// shared rows (row lane / 4, columns of lane % 4); rows at or past `rows` count as zero.
+// Loads from shared memory by 32-bit address.
+__device__ __forceinline__ uint4 lds128(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t p) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t p) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t p) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p));
+  return v;
+}
+
+// A lane's part of a record, loaded ahead.
+template <int GROUP>
+struct W4Frag {
+  static constexpr int kGroups = kW4TileK / GROUP;
+  uint4 w[2];
+  uint32_t s[kGroups];  // scales of rows r and r + 8
+  uint32_t z[kGroups];  // their zero points, one byte each
+  __device__ __forceinline__ void load(const uint8_t* record, bool zeros) {
+    const int lane = threadIdx.x & 31, r = lane >> 2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                   : "l"(record + i * 512 + lane * 16));
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(s[g]) : "l"(record + kW4TileBytes + g * 32 + r * 4));
+      z[g] = 0x0808;
+      if (zeros) {
+        uint16_t v;
+        asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];"
+                     : "=h"(v)
+                     : "l"(record + kW4TileBytes + kGroups * 32 + g * 16 + r * 2));
+        z[g] = v;
+      }
+    }
+  }
+};
+
+// acc += tile * x for NT blocks of 8 rows of x (shared addresses). `x`: this lane's columns of row 0;
+// xrow[t]: the offset of its row of block t (a lane whose row does not exist reads another's: the
+// column that it makes of it is not stored). `xsum`: this lane's two rows of the sums of x over the
+// tile's first group, [group][kW4MaxRows] fp32.
 template <typename T, int GROUP, int NT>
-__device__ __forceinline__ void w4_tile(const uint8_t* tile, bool zeros, const uint8_t* x, int x_pitch, int rows,
+__device__ __forceinline__ void w4_tile(const W4Frag<GROUP>& f, uint32_t x, const int (&xrow)[NT], uint32_t xsum,
                                         float (&acc)[NT][4]) {
   constexpr int kGroups = kW4TileK / GROUP;
-  constexpr int kBlocks = GROUP / 32;  // blocks of 32 columns in a group
-  const int lane = threadIdx.x & 31, r = lane >> 2;
-  const uint8_t* scales = tile + kW4TileBytes + r * 4;
-  const uint8_t* zp = tile + kW4TileBytes + kGroups * 32 + r * 2;
-  uint4 w[2];
-  w[0] = *reinterpret_cast<const uint4*>(tile + lane * 16);
-  w[1] = *reinterpret_cast<const uint4*>(tile + 512 + lane * 16);
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(w);
-  uint32_t off[2];
-  W4Type<T>::offsets(8, 8, off);
+  constexpr int kBlocks = GROUP / 32;        // blocks of 32 columns in a group
+  constexpr int kChains = NT == 1 ? 2 : 1;   // sums per block of rows: at least two independent chains
+  const uint32_t words[8] = {f.w[0].x, f.w[0].y, f.w[0].z, f.w[0].w, f.w[1].x, f.w[1].y, f.w[1].z, f.w[1].w};
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    if (zeros) {
-      const uint32_t z = *reinterpret_cast<const uint16_t*>(zp + g * 16);
-      W4Type<T>::offsets(z & 0xff, z >> 8, off);
-    }
-    const uint32_t s = *reinterpret_cast<const uint32_t*>(scales + g * 32);
-    float c[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[t][i] = 0.0f;
+    const uint32_t z0 = f.z[g] & 0xff, z1 = f.z[g] >> 8;
+    const uint32_t off[2] = {0x43004300u + z0 * 0x10001u, 0x43004300u + z1 * 0x10001u};
+    float c[NT][kChains][4];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const int block = g * kBlocks + b;
       uint4 xv[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        xv[t] = make_uint4(0, 0, 0, 0);
-        if (t * 8 + r < rows) xv[t] = *reinterpret_cast<const uint4*>(x + t * 8 * x_pitch + block * 64);
-      }
+      for (int t = 0; t < NT; ++t) xv[t] = lds128(x + xrow[t] + block * 64);
       uint32_t a[4];
       W4Type<T>::unpack(words[block * 2], off, a);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) W4Type<T>::mma(c[t], a, xv[t].x, xv[t].y);
+      for (int t = 0; t < NT; ++t)
+        if (b == 0) W4Type<T>::template mma<true>(c[t][0], a, xv[t].x, xv[t].y);
+        else W4Type<T>::template mma<false>(c[t][0], a, xv[t].x, xv[t].y);
       W4Type<T>::unpack(words[block * 2 + 1], off, a);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) W4Type<T>::mma(c[t], a, xv[t].z, xv[t].w);
+      for (int t = 0; t < NT; ++t)
+        if (b == 0 && kChains == 2) W4Type<T>::template mma<true>(c[t][kChains - 1], a, xv[t].z, xv[t].w);
+        else W4Type<T>::template mma<false>(c[t][kChains - 1], a, xv[t].z, xv[t].w);
     }
-    const float s0 = W4Type<T>::to_f(s & 0xffffu), s1 = W4Type<T>::to_f(s >> 16);
+    const float s0 = W4Type<T>::to_f(f.s[g] & 0xffffu), s1 = W4Type<T>::to_f(f.s[g] >> 16);
+    const float m0 = s0 * W4Type<T>::kScale0, m1 = s1 * W4Type<T>::kScale1;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      acc[t][0] = fmaf(s0, c[t][0], acc[t][0]);
-      acc[t][1] = fmaf(s0, c[t][1], acc[t][1]);
-      acc[t][2] = fmaf(s1, c[t][2], acc[t][2]);
-      acc[t][3] = fmaf(s1, c[t][3], acc[t][3]);
+      if constexpr (kChains == 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[t][0][i] += c[t][1][i];
+      acc[t][0] = fmaf(m0, c[t][0][0], acc[t][0]);
+      acc[t][1] = fmaf(m0, c[t][0][1], acc[t][1]);
+      acc[t][2] = fmaf(m1, c[t][0][2], acc[t][2]);
+      acc[t][3] = fmaf(m1, c[t][0][3], acc[t][3]);
+    }
+    if constexpr (W4Type<T>::kSums) {
+      const float n0 = -s0 * static_cast<float>(z0), n1 = -s1 * static_cast<float>(z1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 sum = lds_f2(xsum + (g * kW4MaxRows + t * 8) * 4);
+        acc[t][0] = fmaf(n0, sum.x, acc[t][0]);
+        acc[t][1] = fmaf(n0, sum.y, acc[t][1]);
+        acc[t][2] = fmaf(n1, sum.x, acc[t][2]);
+        acc[t][3] = fmaf(n1, sum.y, acc[t][3]);
+      }
     }
   }
 }
 
 __device__ __forceinline__ float w4_silu(float v) { return v / (1.0f + __expf(-v)); }
 
-// The sums of one strip leave: acc[t] = {row r: rows 2q, 2q + 1 of x; row r + 8: the same}.
+// The sums of block t of a strip leave: v = {row r: rows 2q, 2q + 1 of x; row r + 8: the same}.
+// `out_row`: the output row of x's row `lane`.
 template <typename T>
-__device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int first, int rows, int t,
+__device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int out_row, int rows, int t,
                                          const float4& v) {
   const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
   const float lo[2] = {v.x, v.y}, hi[2] = {v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int m = t * 8 + q * 2 + i;
+    const long long row = __shfl_sync(0xffffffffu, out_row, m);
     if (m >= rows) continue;
-    const long long row = a.scatter ? a.scatter[first + m] : first + m;
     if (a.epilogue == kW4Out) {
       T* o = static_cast<T*>(a.out) + row * a.ld_out + strip * 16;
       if (strip * 16 + r < a.n_out) o[r] = W4Type<T>::from_f(lo[i]);
@@ -230,90 +287,131 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, 
   }
 }
 
-struct W4Ring {
-  uint64_t *full, *empty;
-  uint8_t* slots;
-  int stages, stage_bytes;
-  int stage = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++stage == stages) {
-      stage = 0;
-      phase ^= 1;
+// The strips of a CTA: an equal run of all (token tile, slice of K, strip), taken in segments of one
+// tile and slice.
+struct W4Segments {
+  int tile, slice, strip, left;  // where the next segment starts, and the strips left in all
+  int s0, s1;                    // strips of this segment
+  __device__ __forceinline__ W4Segments(const W4Args& a, int tiles) {
+    const long long per_tile = static_cast<long long>(a.slices) * a.strips;
+    const long long all = tiles * per_tile;
+    const long long u0 = all * blockIdx.x / gridDim.x;
+    left = static_cast<int>(all * (blockIdx.x + 1) / gridDim.x - u0);
+    tile = static_cast<int>(u0 / per_tile);
+    const int in = static_cast<int>(u0 - tile * per_tile);
+    slice = in / a.strips;
+    strip = in - slice * a.strips;
+    s0 = s1 = 0;
+  }
+  // Opens the next segment: its tile and slice are returned.
+  __device__ __forceinline__ bool next(const W4Args& a, int& t, int& s) {
+    if (left == 0) return false;
+    t = tile;
+    s = slice;
+    s0 = strip;
+    s1 = min(a.strips, strip + left);
+    left -= s1 - s0;
+    strip = 0;
+    if (++slice == a.slices) {
+      slice = 0;
+      ++tile;
+    }
+    return true;
+  }
+};
+
+// Where a warp's sums go: one of two buffers per group of warps that share strips, in turn.
+struct W4Sums {
+  uint64_t *full, *empty;  // of this group: [2]
+  uint32_t at;             // shared address of its first buffer
+  uint32_t bytes;          // from one buffer to the next
+  int turn;                // buffers used so far
+  __device__ __forceinline__ int slot() const { return turn & 1; }
+  __device__ __forceinline__ uint32_t phase() const { return (turn >> 1) & 1; }
+};
+
+// The tiles of a warp in one segment, with the loads running kW4Ahead tiles before the products.
+template <int GROUP>
+struct W4Stream {
+  W4Frag<GROUP> frag[kW4Ahead];
+  const uint8_t* p;       // the next record to load
+  int k, nk, todo;        // tiles of its strip left, tiles of a strip, tiles left to load in the segment
+  long long step, jump;   // to the next tile of the strip, and further from its end to the next strip
+  __device__ __forceinline__ void load(int j, bool zeros) {
+    if (todo == 0) return;
+    frag[j].load(p, zeros);
+    --todo;
+    p += step;
+    if (--k == 0) {
+      k = nk;
+      p += jump;
     }
   }
 };
 
-// One unit of work (a token tile, a slice of K, a group of strips) of a consumer warp.
+// One segment of a consumer warp: its strips s0 + group, s0 + group + groups, ...
 template <typename T, int GROUP, int NT>
-__device__ __forceinline__ void w4_unit(const W4Args& a, W4Ring& ring, const uint8_t* x, float4* red, int unit, int slice,
-                                        int group, int first, int rows, volatile int* abort_flag) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wps = a.wps, part = warp % wps, sub = warp / wps;
-  const int strip = group * (kW4Warps / wps) + sub;
-  const int kt0 = slice * a.slice_kt, kt1 = min(kt0 + a.slice_kt, a.kt);
-  const int record = w4_record_bytes(GROUP, a.zeros);
-  const uint8_t* xl = x + (lane >> 2) * a.x_pitch + (lane & 3) * 16;
+__device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP>& in, W4Sums& sums, uint32_t x, uint32_t xsum,
+                                           int part, int rows, int strips, int rounds, volatile int* abort_flag) {
+  const int lane = threadIdx.x & 31;
+  int xrow[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) xrow[t] = min(t * 8 + (lane >> 2), rows - 1) * a.x_pitch;
+  constexpr int kXsumTile = kW4TileK / GROUP * kW4MaxRows * 4;
+  const uint32_t x0 = x + (lane & 3) * 16 + part * (kW4TileK * 2), sum0 = xsum + (lane & 3) * 8 + part * kXsumTile;
+  uint32_t xl = x0, sl = sum0;
   float acc[NT][4] = {};
-  for (int kt = kt0; kt < kt1; kt += wps) {
-    mbar_wait(&ring.full[ring.stage], ring.phase, abort_flag, a.status);
-    if (kt + part < kt1 && strip < a.strips)
-      w4_tile<T, GROUP, NT>(ring.slots + ring.stage * ring.stage_bytes + warp * record, a.zeros,
-                            xl + (kt + part - kt0) * (kW4TileK * 2), a.x_pitch, rows, acc);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ring.empty[ring.stage]);
-    ring.next();
-  }
-  if (wps == 1) {
-    if (strip < a.strips)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        w4_store<T>(a, strip, slice, first, rows, t, make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]));
-    return;
-  }
-  // The warps of a strip add up through one of two buffers; one warp, another each time, reads them
-  // after the barrier. A buffer is written again two units on, past the barrier that its reader joins
-  // only when it is done.
-  float4* buf = red + (unit & 1) * (kW4Warps * NT * 32) + sub * wps * (NT * 32);
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-    buf[(part * NT + t) * 32 + lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
-  named_sync(1 + sub, wps * 32);
-  if (part == unit % wps && strip < a.strips) {
+  auto flush = [&]() {
+    mbar_wait(&sums.empty[sums.slot()], sums.phase() ^ 1, abort_flag, a.status);
+    const uint32_t buf = sums.at + sums.slot() * sums.bytes + (part * NT * 32 + lane) * 16;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float4 s = buf[t * 32 + lane];
-      for (int p = 1; p < wps; ++p) {
-        const float4 v = buf[(p * NT + t) * 32 + lane];
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+      asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(buf + t * 512), "f"(acc[t][0]), "f"(acc[t][1]),
+                   "f"(acc[t][2]), "f"(acc[t][3])
+                   : "memory");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = 0.0f;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sums.full[sums.slot()]);
+    ++sums.turn;
+  };
+  int k = in.nk;
+  for (int n = strips * in.nk; n > 0; n -= kW4Ahead) {
+#pragma unroll
+    for (int j = 0; j < kW4Ahead; ++j) {
+      if (j < n) {
+        w4_tile<T, GROUP, NT>(in.frag[j], xl, xrow, sl, acc);
+        in.load(j, a.zeros);
+        xl += a.wps * (kW4TileK * 2);
+        sl += a.wps * kXsumTile;
+        if (--k == 0) {
+          k = in.nk;
+          xl = x0;
+          sl = sum0;
+          flush();
+        }
       }
-      w4_store<T>(a, strip, slice, first, rows, t, s);
     }
   }
+  if (strips < rounds) flush();  // the last round has no strip for this group
 }
 
-template <typename T, int GROUP>
-__global__ void __launch_bounds__(kW4Threads, 1) w4_gemv_kernel(const W4Args a) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kW4MaxStages], empty[kW4MaxStages];
+template <typename T, int GROUP, int NTMAX>
+__global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4Args a) {
+  constexpr int kWarps = w4_warps(NTMAX);
+  extern __shared__ __align__(128) uint8_t smem[];  // [x][sums of x][sums of the warps]
+  __shared__ uint64_t full[kWarps * 2], empty[kWarps * 2];
   __shared__ int abort_flag;
-  // [x][sums of the warps][ring]
-  uint8_t* xs = smem;
-  float4* red = reinterpret_cast<float4*>(smem + a.x_bytes);
   const int record = w4_record_bytes(GROUP, a.zeros);
-  W4Ring ring;
-  ring.full = full;
-  ring.empty = empty;
-  ring.slots = smem + a.x_bytes + a.red_bytes;
-  ring.stages = a.stages;
-  ring.stage_bytes = kW4Warps * record;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = kWarps / a.wps;
+  const uint32_t base = smem_u32(smem), xsum = base + a.x_bytes, sums_at = xsum + a.xsum_bytes;
+  constexpr int kSumBytes = kWarps * NTMAX * 512;  // of all groups, one turn
   if (threadIdx.x == 0) {
-    for (int i = 0; i < a.stages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kW4Warps);
+    for (int i = 0; i < groups * 2; ++i) {
+      mbar_init(&full[i], a.wps);
+      mbar_init(&empty[i], 1);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -322,92 +420,125 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_gemv_kernel(const W4Args a) 
   if (!a.early) grid_dep_wait();
   grid_dep_launch();  // after the wait: an early dependent may count on what is complete here
 
-  const int tiles = a.tiles ? *a.num_tiles : (a.rows + a.tile_rows - 1) / a.tile_rows;
-  const long long per_tile = static_cast<long long>(a.slices) * a.strip_groups;
-  const long long units = tiles * per_tile;
-  const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-  const int warp = threadIdx.x >> 5;
+  W4Segments seg(a, a.tiles ? *a.num_tiles : (a.rows + a.tile_rows - 1) / a.tile_rows);
+  int tile, slice, expert = 0, first = 0, rows = 0;
+  auto open_tile = [&]() {
+    if (a.tiles) {
+      const int4 t = a.tiles[tile];
+      expert = t.x;
+      first = t.y;
+      rows = t.z;
+    } else {
+      first = tile * a.tile_rows;
+      rows = min(a.tile_rows, a.rows - first);
+    }
+  };
 
-  if (warp == kW4Warps) {
-    if ((threadIdx.x & 31) == 0) {
-      const int sps = kW4Warps / a.wps;
-      ring.phase = 1;  // every stage starts empty
-      bool ok = true;
-      for (long long u = u0; u < u1 && ok; ++u) {
-        const int tile = static_cast<int>(u / per_tile);
-        const int in = static_cast<int>(u - tile * per_tile);
-        const int slice = in / a.strip_groups, group = in - slice * a.strip_groups;
-        const int expert = a.tiles ? a.tiles[tile].x : 0;
-        const int kt0 = slice * a.slice_kt, kt1 = min(kt0 + a.slice_kt, a.kt);
-        const int strips = min(sps, a.strips - group * sps);
-        const uint8_t* w = a.w + expert * a.expert_bytes + static_cast<long long>(group) * sps * a.kt * record;
-        for (int kt = kt0; kt < kt1; kt += a.wps) {
-          const uint32_t bytes = min(a.wps, kt1 - kt) * record;
-          ok = mbar_wait(&empty[ring.stage], ring.phase, &abort_flag, a.status);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&full[ring.stage], bytes * strips);
-          for (int s = 0; s < strips; ++s)
-            bulk_load(ring.slots + ring.stage * ring.stage_bytes + s * a.wps * record,
-                      w + (static_cast<long long>(s) * a.kt + kt) * record, bytes, &full[ring.stage]);
-          ring.next();
+  if (warp >= kWarps) {
+    // Store warps: each takes every kW4StoreWarps-th group of warps.
+    if (a.early) grid_dep_wait();
+    int turn = 0;
+    while (seg.next(a, tile, slice)) {
+      open_tile();
+      const int out_row = lane < rows ? (a.scatter ? a.scatter[first + lane] : first + lane) : 0;
+      const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+      for (int strip0 = seg.s0; strip0 < seg.s1; strip0 += groups, ++turn) {
+        for (int g = warp - kWarps; g < groups; g += kW4StoreWarps) {
+          const int at = g * 2 + (turn & 1);
+          mbar_wait(&full[at], (turn >> 1) & 1, &abort_flag, a.status);
+          if (strip0 + g < seg.s1) {
+            const float4* buf = reinterpret_cast<const float4*>(smem + (sums_at - base) + (turn & 1) * kSumBytes) +
+                                g * a.wps * NTMAX * 32 + lane;
+            for (int t = 0; t < nt; ++t) {
+              float4 v = buf[t * 32];
+              for (int p = 1; p < a.wps; ++p) {
+                const float4 o = buf[(p * nt + t) * 32];
+                v.x += o.x;
+                v.y += o.y;
+                v.z += o.z;
+                v.w += o.w;
+              }
+              w4_store<T>(a, strip0 + g, slice, out_row, rows, t, v);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[at]);
         }
       }
-      // Nothing may be in flight when the CTA ends. The consumers wait for every stage; where a wait
-      // gave up, the copies still under way are waited for here.
-      if (!ok || *static_cast<volatile int*>(&abort_flag))
-        for (int i = 0; i < a.stages; ++i) mbar_wait_drain(&full[i], i < ring.stage ? ring.phase ^ 1 : ring.phase);
     }
     return;
   }
 
-  if (a.early) grid_dep_wait();  // x is the kernel before's
-  int old_tile = -1, old_slice = -1, first = 0, rows = 0;
-  for (long long u = u0; u < u1; ++u) {
-    const int tile = static_cast<int>(u / per_tile);
-    const int in = static_cast<int>(u - tile * per_tile);
-    const int slice = in / a.strip_groups, group = in - slice * a.strip_groups;
-    if (tile != old_tile || slice != old_slice) {
-      if (a.tiles) {
-        const int4 t = a.tiles[tile];
-        first = t.y;
-        rows = t.z;
-      } else {
-        first = tile * a.tile_rows;
-        rows = min(a.tile_rows, a.rows - first);
-      }
-      old_tile = tile;
-      old_slice = slice;
-      named_sync(kW4Warps + 1, kW4Warps * 32);  // all have done with the rows before
-      const int k0 = slice * a.slice_kt * kW4TileK;
-      const int words = min(a.slice_kt, a.kt - slice * a.slice_kt) * (kW4TileK / 8);
-      for (int m = 0; m < rows; ++m) {
-        const long long row = a.gather ? a.gather[first + m] / a.gather_div : first + m;
-        const T* src = static_cast<const T*>(a.x) + row * a.ld_x + k0;
-        uint8_t* dst = xs + m * a.x_pitch;
-        for (int c = threadIdx.x; c < words; c += kW4Warps * 32) {
-          const int left = a.K - k0 - c * 8;  // columns of x from this word on
-          if (left >= 8 && a.x_words) {
-            cp_async_16(smem_u32(dst + c * 16), src + c * 8, 16);
-          } else {
-            uint16_t e[8];
+  const int part = warp % a.wps, group = warp / a.wps;
+  W4Sums sums{full + group * 2, empty + group * 2, sums_at + group * a.wps * NTMAX * 512, kSumBytes, 0};
+  W4Stream<GROUP> in;
+  in.step = static_cast<long long>(a.wps) * record;
+  bool fresh = a.early;
+  while (seg.next(a, tile, slice)) {
+    open_tile();
+    const int kt0 = slice * a.slice_kt, kts = min(a.slice_kt, a.kt - kt0);
+    // (warps past the last whole group have no strips)
+    const int rounds = group < groups ? (seg.s1 - seg.s0 + groups - 1) / groups : 0;
+    const int strips = group < groups ? (seg.s1 - seg.s0 - group + groups - 1) / groups : 0;
+    in.nk = in.k = (kts - part + a.wps - 1) / a.wps;
+    in.todo = strips * in.nk;
+    in.jump = (static_cast<long long>(groups) * a.kt - static_cast<long long>(in.nk) * a.wps) * record;
+    in.p = a.w + expert * a.expert_bytes + (static_cast<long long>(seg.s0 + group) * a.kt + kt0 + part) * record;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              e[i] = i < left ? reinterpret_cast<const uint16_t*>(src)[c * 8 + i] : static_cast<uint16_t>(0);
-            *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(e);
-          }
+    for (int j = 0; j < kW4Ahead; ++j) in.load(j, a.zeros);
+    if (fresh) grid_dep_wait();  // x is the kernel before's
+    fresh = false;
+
+    named_sync(1, kWarps * 32);  // all have done with the rows before
+    const int k0 = kt0 * kW4TileK, words = kts * (kW4TileK / 8);
+    for (int m = 0; m < rows; ++m) {
+      const long long row = a.gather ? a.gather[first + m] / a.gather_div : first + m;
+      const T* src = static_cast<const T*>(a.x) + row * a.ld_x + k0;
+      uint8_t* dst = smem + m * a.x_pitch;
+      for (int c = threadIdx.x; c < words; c += kWarps * 32) {
+        const int left = a.K - k0 - c * 8;  // columns of x from this word on
+        if (left >= 8 && a.x_words) {
+          cp_async_16(smem_u32(dst + c * 16), src + c * 8, 16);
+        } else {
+          uint16_t e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            e[i] = i < left ? reinterpret_cast<const uint16_t*>(src)[c * 8 + i] : static_cast<uint16_t>(0);
+          *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(e);
         }
       }
-      cp_async_wait_all();
-      named_sync(kW4Warps + 1, kW4Warps * 32);
     }
-    const int unit = static_cast<int>(u - u0);
-    if (rows <= 8)
-      w4_unit<T, GROUP, 1>(a, ring, xs, red, unit, slice, group, first, rows, &abort_flag);
-    else if (rows <= 16)
-      w4_unit<T, GROUP, 2>(a, ring, xs, red, unit, slice, group, first, rows, &abort_flag);
+    cp_async_wait_all();
+    named_sync(1, kWarps * 32);
+    if constexpr (W4Type<T>::kSums) {  // sums of each row over the groups, GROUP / 8 lanes each
+      const int chunks = (words + 31) / 32;
+      for (int i = warp; i < rows * chunks; i += kWarps) {
+        const int m = i / chunks, word = (i - m * chunks) * 32 + lane;
+        float sum = 0.0f;
+        if (word < words) {
+          const uint4 v = lds128(base + m * a.x_pitch + word * 16);
+          const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = __half22float2(h[e]);
+            sum += f.x + f.y;
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < GROUP / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane % (GROUP / 8) == 0 && word < words)
+          reinterpret_cast<float*>(smem + a.x_bytes)[word / (GROUP / 8) * kW4MaxRows + m] = sum;
+      }
+      named_sync(1, kWarps * 32);
+    }
+    if (NTMAX == 1 || rows <= 8)
+      w4_segment<T, GROUP, 1>(a, in, sums, base, xsum, part, rows, strips, rounds, &abort_flag);
+    else if (NTMAX == 2 || rows <= 16)
+      w4_segment<T, GROUP, NTMAX < 2 ? 1 : 2>(a, in, sums, base, xsum, part, rows, strips, rounds, &abort_flag);
     else
-      w4_unit<T, GROUP, 4>(a, ring, xs, red, unit, slice, group, first, rows, &abort_flag);
+      w4_segment<T, GROUP, NTMAX < 4 ? 1 : 4>(a, in, sums, base, xsum, part, rows, strips, rounds, &abort_flag);
   }
+  if (fresh) grid_dep_wait();  // a CTA without work: its end must still follow the kernel before
 }
 
 // ------------------------------------------------------------------ routing, activation, combine
