@@ -16,8 +16,8 @@ size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 // How one product is laid over the GPU.
 struct W4Plan {
   int strips, kt, nt, warps, wps;
-  int tile_rows, slices, slice_kt, x_pitch, x_bytes, xsum_bytes, sum_bytes;
-  size_t smem() const { return static_cast<size_t>(x_bytes) + xsum_bytes + sum_bytes; }
+  int tile_rows, slices, slice_kt, x_pitch, x_bytes, start_bytes, sum_bytes;
+  size_t smem() const { return static_cast<size_t>(x_bytes) + start_bytes + sum_bytes; }
 };
 
 #ifndef SUMCOST
@@ -35,14 +35,14 @@ W4Plan w4_plan(int strips, int64_t K, int group, int tile_rows, double tiles, in
   p.nt = tile_rows <= 8 ? 1 : tile_rows <= 16 ? 2 : 4;
   p.warps = w4_warps(p.nt);
   p.sum_bytes = 2 * p.warps * p.nt * 512;
-  // K is cut so that the rows' slice of x (and its sums) fits in shared memory
-  const int xsum_kt = kW4TileK / group * kW4MaxRows * 4;
-  const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows + xsum_kt);
+  // K is cut so that the rows' slice of x (and the starts of its sums) fits in shared memory
+  const int start_kt = kW4TileK / group * p.nt * 64;
+  const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows + start_kt);
   p.slice_kt = static_cast<int>(ceil_div(p.kt, ceil_div(p.kt, most)));
   p.slices = static_cast<int>(ceil_div(p.kt, p.slice_kt));
   p.x_pitch = p.slice_kt * 2 * kW4TileK + 64;  // 64: rows r and r + 1 in different banks
   p.x_bytes = static_cast<int>(ceil_div(static_cast<int64_t>(tile_rows) * p.x_pitch, 128) * 128);
-  p.xsum_bytes = p.slice_kt * xsum_kt;
+  p.start_bytes = p.slice_kt * start_kt;
   // Warps per strip: few make the sums rare, many give each CTA's groups of warps nearly the same
   // number of strips. The cost of a choice in tile times: rounds of strips per CTA, each a warp's
   // tiles and what handing on a sum takes.
@@ -92,29 +92,35 @@ int launch(Kernel kernel, int grid, int threads, size_t smem, cudaStream_t s, bo
   return MOE_OK;
 }
 
-template <typename T, int GROUP, int NT>
+template <typename T, int GROUP, bool ZEROS, int NT>
 int launch_gemv_t(const W4Args& a, size_t smem, int grid, int dev, bool dependent, cudaStream_t s) {
-  MOE_TRY((allow_smem<w4_gemv_kernel<T, GROUP, NT>>(dev)));
-  return launch(w4_gemv_kernel<T, GROUP, NT>, grid, w4_threads(NT), smem, s, dependent, a);
+  constexpr auto kernel = w4_gemv_kernel<T, GROUP, ZEROS, NT>;
+  MOE_TRY(allow_smem<kernel>(dev));
+  return launch(kernel, grid, w4_threads(NT), smem, s, dependent, a);
 }
 
-template <typename T, int GROUP>
-int launch_gemv_g(const W4Args& a, const W4Plan& p, int grid, int dev, bool dependent, cudaStream_t s) {
-  if (p.nt == 1) return launch_gemv_t<T, GROUP, 1>(a, p.smem(), grid, dev, dependent, s);
-  if (p.nt == 2) return launch_gemv_t<T, GROUP, 2>(a, p.smem(), grid, dev, dependent, s);
-  return launch_gemv_t<T, GROUP, 4>(a, p.smem(), grid, dev, dependent, s);
+template <typename T, int GROUP, bool ZEROS>
+int launch_gemv_z(const W4Args& a, const W4Plan& p, int grid, int dev, bool dependent, cudaStream_t s) {
+  if (p.nt == 1) return launch_gemv_t<T, GROUP, ZEROS, 1>(a, p.smem(), grid, dev, dependent, s);
+  if (p.nt == 2) return launch_gemv_t<T, GROUP, ZEROS, 2>(a, p.smem(), grid, dev, dependent, s);
+  return launch_gemv_t<T, GROUP, ZEROS, 4>(a, p.smem(), grid, dev, dependent, s);
 }
 
 template <typename T>
-int launch_gemv(const W4Args& a, const W4Plan& p, int group, int grid, int dev, bool dependent, cudaStream_t s) {
+int launch_gemv(const W4Args& a, const W4Plan& p, int group, int zeros, int grid, int dev, bool dependent, cudaStream_t s) {
   if (p.wps < 1 || p.slice_kt < 1 || p.smem() > kW4Smem)
     return fail(MOE_ERR_UNSUPPORTED, "no room for the rows of x: %zu bytes of shared memory", p.smem());
-  if (group == 32) return launch_gemv_g<T, 32>(a, p, grid, dev, dependent, s);
-  if (group == 64) return launch_gemv_g<T, 64>(a, p, grid, dev, dependent, s);
-  return launch_gemv_g<T, 128>(a, p, grid, dev, dependent, s);
+  if (group == 32)
+    return zeros ? launch_gemv_z<T, 32, true>(a, p, grid, dev, dependent, s)
+                 : launch_gemv_z<T, 32, false>(a, p, grid, dev, dependent, s);
+  if (group == 64)
+    return zeros ? launch_gemv_z<T, 64, true>(a, p, grid, dev, dependent, s)
+                 : launch_gemv_z<T, 64, false>(a, p, grid, dev, dependent, s);
+  return zeros ? launch_gemv_z<T, 128, true>(a, p, grid, dev, dependent, s)
+               : launch_gemv_z<T, 128, false>(a, p, grid, dev, dependent, s);
 }
 
-W4Args w4_args(const W4Plan& p, const void* w, int zeros, int64_t expert_bytes, uint32_t* status) {
+W4Args w4_args(const W4Plan& p, const void* w, int64_t expert_bytes, uint32_t* status) {
   W4Args a{};
   a.w = static_cast<const uint8_t*>(w);
   a.expert_bytes = expert_bytes;
@@ -123,12 +129,11 @@ W4Args w4_args(const W4Plan& p, const void* w, int zeros, int64_t expert_bytes, 
   a.wps = p.wps;
   a.slices = p.slices;
   a.slice_kt = p.slice_kt;
-  a.zeros = zeros != 0;
   a.tile_rows = p.tile_rows;
   a.gather_div = 1;
   a.x_pitch = p.x_pitch;
   a.x_bytes = p.x_bytes;
-  a.xsum_bytes = p.xsum_bytes;
+  a.start_bytes = p.start_bytes;
   a.status = status;
   return a;
 }
@@ -160,7 +165,7 @@ int launch_combine_w(const float* part, int slices, int64_t rows, int part_ld, c
 template <typename T>
 int w4_linear_t(const void* x, int64_t ld_x, const void* packed, void* out, int64_t ld_out, int64_t M, int64_t N, int64_t K,
                 int group, int zeros, const W4Plan& p, float* part, int dev, int sms, uint32_t* status, cudaStream_t s) {
-  W4Args a = w4_args(p, packed, zeros, 0, status);
+  W4Args a = w4_args(p, packed, 0, status);
   a.x = x;
   a.ld_x = ld_x;
   a.K = static_cast<int>(K);
@@ -173,7 +178,7 @@ int w4_linear_t(const void* x, int64_t ld_x, const void* packed, void* out, int6
   a.part = part;
   a.part_rows = M;
   const int64_t units = ceil_div(M, p.tile_rows) * p.slices * p.strips;
-  MOE_TRY(launch_gemv<T>(a, p, group, static_cast<int>(std::min<int64_t>(units, sms)), dev, false, s));
+  MOE_TRY(launch_gemv<T>(a, p, group, zeros, static_cast<int>(std::min<int64_t>(units, sms)), dev, false, s));
   if (p.slices == 1) return MOE_OK;
   return launch_combine_w<T, int32_t>(part, p.slices, M, p.strips * 16, nullptr, nullptr, MOE_F32, 0, 1, M, N,
                                       static_cast<T*>(out), ld_out, blocks_for(M * ceil_div(N, 4), 128, sms), s);
@@ -241,7 +246,7 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
     MOE_TRY(launch(w4_route_kernel<int64_t>, 1, 1024, 0, s, false, static_cast<const int64_t*>(ids), (int)R, (int)E,
                    tile_rows, sorted, tiles, num_tiles));
   // first product: x rows of the tokens, gate and up of a column in one thread
-  W4Args a = w4_args(L.p1, w13, z13, matrix_bytes(2 * I, H, g13, z13, 1), status);
+  W4Args a = w4_args(L.p1, w13, matrix_bytes(2 * I, H, g13, z13, 1), status);
   a.x = x;
   a.ld_x = ld_x;
   a.K = static_cast<int>(H);
@@ -256,12 +261,12 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
   a.n_out = L.p1.strips * 8;  // the padding's columns too: they are zero
   a.part = part1;
   a.part_rows = R;
-  MOE_TRY(launch_gemv<T>(a, L.p1, g13, sms, dev, true, s));
+  MOE_TRY(launch_gemv<T>(a, L.p1, g13, z13, sms, dev, true, s));
   if (L.p1.slices > 1)
     MOE_TRY(launch(w4_act_kernel<T>, blocks_for(R * L.p1.strips * 2, 128, sms), 128, 0, s, true, (const float*)part1,
                    L.p1.slices, (long long)R, L.p1.strips, h));
   // second product: the routes' rows in place, its sums per route
-  W4Args b = w4_args(L.p2, w2, z2, matrix_bytes(H, I, g2, z2, 0), status);
+  W4Args b = w4_args(L.p2, w2, matrix_bytes(H, I, g2, z2, 0), status);
   b.x = h;
   b.ld_x = L.p1.strips * 8;
   b.K = L.p1.strips * 8;
@@ -273,7 +278,7 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
   b.part = part2;
   b.part_rows = R;
   b.early = 1;
-  MOE_TRY(launch_gemv<T>(b, L.p2, g2, sms, dev, true, s));
+  MOE_TRY(launch_gemv<T>(b, L.p2, g2, z2, sms, dev, true, s));
   const int grid = blocks_for(T_ * ceil_div(H, 4), 128, sms);
   if (ids_dtype == MOE_I32)
     return launch_combine_w<T, int32_t>(part2, L.p2.slices, R, L.p2.strips * 16, ids, tw, w_dtype, E, topk, T_, H,

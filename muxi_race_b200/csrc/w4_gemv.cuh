@@ -13,7 +13,7 @@
 //           16-byte loads a lane straight into registers, with no shuffles and no shared memory.
 //   strip   the tiles of 16 rows, one after another along K; an expert's strips follow each other.
 // One CTA per SM. Its warps walk through strips with the loads of the next tiles in flight in
-// registers (kW4Ahead tiles a warp: about 64 KB an SM); x (at most 32 rows, one slice of K) stays in
+// registers (w4_ahead tiles a warp: 60 to 90 KB an SM); x (at most 32 rows, one slice of K) stays in
 // shared memory. Warps that share a strip split K; their sums go through shared memory to the store
 // warps, which add them up, so that no consumer waits for another or for a store.
 // mma.sync and not tcgen05.mma: the weights must pass the registers to be unpacked, a 16-row strip
@@ -29,13 +29,20 @@
 namespace moe {
 
 constexpr int kW4StoreWarps = 2;       // warps that add up the consumers' sums and store them
-constexpr int kW4Ahead = 4;            // tiles that a warp has in flight
 constexpr int kW4TileK = 128;
 constexpr int kW4TileBytes = 1024;     // values of one tile
 constexpr int kW4MaxRows = 32;         // rows of x at a time
 // consumer warps: with the store warps 16 of 128 registers, or 12 of 168 for four blocks of 8 rows
 __host__ __device__ constexpr int w4_warps(int nt) { return nt <= 2 ? 14 : 10; }
 __host__ __device__ constexpr int w4_threads(int nt) { return (w4_warps(nt) + kW4StoreWarps) * 32; }
+
+// tiles that a warp has in flight: as many as its registers hold
+#ifndef AH1
+#define AH1 6
+#endif
+__host__ __device__ constexpr int w4_ahead(int group, bool zeros, int nt) {
+  return nt > 1 ? 4 : group == 128 && !zeros ? AH1 : group >= 64 ? 5 : 4;
+}
 
 // bytes of a tile with its scales (half2 of rows r, r + 8 per group) and zero points (byte pairs)
 __host__ __device__ constexpr int w4_record_bytes(int group, bool zeros) {
@@ -50,7 +57,6 @@ struct W4Args {
   int strips, kt;           // strips, and tiles along K
   int wps;                  // warps that share a strip
   int slices, slice_kt;     // K slices whose x fits in shared memory, and their tiles
-  int zeros;                // records hold zero points
   const void* x;
   long long ld_x;
   int K;                    // columns of x
@@ -68,7 +74,7 @@ struct W4Args {
   float* part;              // kW4Partial: [slice][row][strips * 16]
   long long part_rows;
   int x_pitch;              // bytes of a row of x in shared memory
-  int x_bytes, xsum_bytes;  // bytes of the rows of x, and of their sums per group (fp16)
+  int x_bytes, start_bytes; // bytes of the rows of x, and of where the groups' sums start (fp16)
   int early;                // the tile list is older than the kernel before this one
   uint32_t* status;
 };
@@ -83,8 +89,9 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 // Eight values of a word as A fragments: nibble i of the low (high) half is the first (second) value
 // of register i; registers 0 and 2 are row r, 1 and 3 row r + 8.
 //   fp16: the nibbles themselves, as the low bits of a subnormal number, are q 2^-24 (row r) and
-//     q 2^-20 (row r + 8, one nibble further up): no instruction but the masks. The powers of two go
-//     into the scales, and the zero points into one term per group: sum (q - z) x = sum q x - z sum x.
+//     q 2^-20 (row r + 8, one nibble further up): no instruction but the masks. The sums carry those
+//     powers of two to their end, and the zero points enter as the start of each group's sum:
+//     sum (q - z) x = -z sum x + sum q x.
 //   bf16 (whose subnormal products fp32 cannot hold): the nibbles become the low bits of 128 + q, and
 //     one subtraction gives q - z, exactly.
 template <typename T> struct W4Type;
@@ -105,16 +112,11 @@ template <> struct W4Type<__half> {
   }
   static __device__ __forceinline__ float to_f(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-  template <bool FIRST>
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (FIRST)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 template <> struct W4Type<__nv_bfloat16> {
@@ -134,16 +136,11 @@ template <> struct W4Type<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float to_f(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-  template <bool FIRST>
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (FIRST)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   }
 };
 
@@ -163,20 +160,14 @@ __device__ __forceinline__ uint32_t lds16(uint32_t p) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p));
   return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t p) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p));
-  return v;
-}
-
 // A lane's part of a record, loaded ahead.
-template <int GROUP>
+template <int GROUP, bool ZEROS>
 struct W4Frag {
   static constexpr int kGroups = kW4TileK / GROUP;
   uint4 w[2];
-  uint32_t s[kGroups];  // scales of rows r and r + 8
-  uint32_t z[kGroups];  // their zero points, one byte each
-  __device__ __forceinline__ void load(const uint8_t* record, bool zeros) {
+  uint32_t s[kGroups];              // scales of rows r and r + 8
+  uint32_t z[ZEROS ? kGroups : 1];  // their zero points, one byte each
+  __device__ __forceinline__ void load(const uint8_t* record) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -186,8 +177,7 @@ struct W4Frag {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(s[g]) : "l"(record + kW4TileBytes + g * 32 + r * 4));
-      z[g] = 0x0808;
-      if (zeros) {
+      if constexpr (ZEROS) {
         uint16_t v;
         asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];"
                      : "=h"(v)
@@ -198,22 +188,39 @@ struct W4Frag {
   }
 };
 
-// acc += tile * x for NT blocks of 8 rows of x (shared addresses). `x`: this lane's columns of row 0;
-// xrow[t]: the offset of its row of block t (a lane whose row does not exist reads another's: the
-// column that it makes of it is not stored). `xsum`: this lane's two rows of the sums of x over the
-// tile's first group, [group][kW4MaxRows] fp32.
-template <typename T, int GROUP, int NT>
-__device__ __forceinline__ void w4_tile(const W4Frag<GROUP>& f, uint32_t x, const int (&xrow)[NT], uint32_t xsum,
-                                        float (&acc)[NT][4]) {
+// acc += tile * x for NT blocks of 8 rows of x (shared addresses), in units of 1 / kScale. `x`: this
+// lane's columns of row 0; xrow[t]: the offset of its row of block t (a lane whose row does not exist
+// reads another's: the column that it makes of it is not stored). `start` (fp16): this lane's starts
+// of the tile's first group, `start_group` bytes from one group to the next (see w4_load_x).
+template <typename T, int GROUP, bool ZEROS, int NT>
+__device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& f, uint32_t x, const int (&xrow)[NT], uint32_t start,
+                                        int start_group, float (&acc)[NT][4]) {
   constexpr int kGroups = kW4TileK / GROUP;
   constexpr int kBlocks = GROUP / 32;        // blocks of 32 columns in a group
   constexpr int kChains = NT == 1 ? 2 : 1;   // sums per block of rows: at least two independent chains
   const uint32_t words[8] = {f.w[0].x, f.w[0].y, f.w[0].z, f.w[0].w, f.w[1].x, f.w[1].y, f.w[1].z, f.w[1].w};
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    const uint32_t z0 = f.z[g] & 0xff, z1 = f.z[g] >> 8;
+    uint32_t z0 = 8, z1 = 8;
+    if constexpr (ZEROS) {
+      z0 = f.z[g] & 0xff;
+      z1 = f.z[g] >> 8;
+    }
     const uint32_t off[2] = {0x43004300u + z0 * 0x10001u, 0x43004300u + z1 * 0x10001u};
     float c[NT][kChains][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < kChains * 4; ++i) c[t][i / 4][i % 4] = 0.0f;
+      if constexpr (W4Type<T>::kSums) {
+        const uint4 v = lds128(start + g * start_group + t * 64);
+        const float f0 = ZEROS ? static_cast<float>(z0) : 1.0f, f1 = ZEROS ? static_cast<float>(z1) : 1.0f;
+        c[t][0][0] = f0 * __uint_as_float(v.x);
+        c[t][0][1] = f0 * __uint_as_float(v.y);
+        c[t][0][2] = f1 * __uint_as_float(v.z);
+        c[t][0][3] = f1 * __uint_as_float(v.w);
+      }
+    }
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const int block = g * kBlocks + b;
@@ -223,37 +230,21 @@ __device__ __forceinline__ void w4_tile(const W4Frag<GROUP>& f, uint32_t x, cons
       uint32_t a[4];
       W4Type<T>::unpack(words[block * 2], off, a);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (b == 0) W4Type<T>::template mma<true>(c[t][0], a, xv[t].x, xv[t].y);
-        else W4Type<T>::template mma<false>(c[t][0], a, xv[t].x, xv[t].y);
+      for (int t = 0; t < NT; ++t) W4Type<T>::mma(c[t][0], a, xv[t].x, xv[t].y, c[t][0]);
       W4Type<T>::unpack(words[block * 2 + 1], off, a);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (b == 0 && kChains == 2) W4Type<T>::template mma<true>(c[t][kChains - 1], a, xv[t].z, xv[t].w);
-        else W4Type<T>::template mma<false>(c[t][kChains - 1], a, xv[t].z, xv[t].w);
+      for (int t = 0; t < NT; ++t) W4Type<T>::mma(c[t][kChains - 1], a, xv[t].z, xv[t].w, c[t][kChains - 1]);
     }
     const float s0 = W4Type<T>::to_f(f.s[g] & 0xffffu), s1 = W4Type<T>::to_f(f.s[g] >> 16);
-    const float m0 = s0 * W4Type<T>::kScale0, m1 = s1 * W4Type<T>::kScale1;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if constexpr (kChains == 2)
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[t][0][i] += c[t][1][i];
-      acc[t][0] = fmaf(m0, c[t][0][0], acc[t][0]);
-      acc[t][1] = fmaf(m0, c[t][0][1], acc[t][1]);
-      acc[t][2] = fmaf(m1, c[t][0][2], acc[t][2]);
-      acc[t][3] = fmaf(m1, c[t][0][3], acc[t][3]);
-    }
-    if constexpr (W4Type<T>::kSums) {
-      const float n0 = -s0 * static_cast<float>(z0), n1 = -s1 * static_cast<float>(z1);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float2 sum = lds_f2(xsum + (g * kW4MaxRows + t * 8) * 4);
-        acc[t][0] = fmaf(n0, sum.x, acc[t][0]);
-        acc[t][1] = fmaf(n0, sum.y, acc[t][1]);
-        acc[t][2] = fmaf(n1, sum.x, acc[t][2]);
-        acc[t][3] = fmaf(n1, sum.y, acc[t][3]);
-      }
+      acc[t][0] = fmaf(s0, c[t][0][0], acc[t][0]);
+      acc[t][1] = fmaf(s0, c[t][0][1], acc[t][1]);
+      acc[t][2] = fmaf(s1, c[t][0][2], acc[t][2]);
+      acc[t][3] = fmaf(s1, c[t][0][3], acc[t][3]);
     }
   }
 }
@@ -266,7 +257,8 @@ template <typename T>
 __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int out_row, int rows, int t,
                                          const float4& v) {
   const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
-  const float lo[2] = {v.x, v.y}, hi[2] = {v.z, v.w};
+  const float lo[2] = {v.x * W4Type<T>::kScale0, v.y * W4Type<T>::kScale0};
+  const float hi[2] = {v.z * W4Type<T>::kScale1, v.w * W4Type<T>::kScale1};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int m = t * 8 + q * 2 + i;
@@ -330,36 +322,36 @@ struct W4Sums {
   __device__ __forceinline__ uint32_t phase() const { return (turn >> 1) & 1; }
 };
 
-// The tiles of a warp in one segment, with the loads running kW4Ahead tiles before the products.
-template <int GROUP>
+// The tiles of a warp in one segment, loaded AHEAD tiles before their products. Past the last strip
+// the loads go round in it (nothing reads them).
+template <int GROUP, bool ZEROS, int AHEAD>
 struct W4Stream {
-  W4Frag<GROUP> frag[kW4Ahead];
+  W4Frag<GROUP, ZEROS> frag[AHEAD];
   const uint8_t* p;       // the next record to load
-  int k, nk, todo;        // tiles of its strip left, tiles of a strip, tiles left to load in the segment
-  long long step, jump;   // to the next tile of the strip, and further from its end to the next strip
-  __device__ __forceinline__ void load(int j, bool zeros) {
-    if (todo == 0) return;
-    frag[j].load(p, zeros);
-    --todo;
+  int k, nk, strips;      // tiles of its strip left, tiles of a strip, strips left with this one
+  long long step, jump, back;  // to the next tile of the strip; from its end to the next strip, or to its start
+  __device__ __forceinline__ void load(int j) {
+    frag[j].load(p);
     p += step;
     if (--k == 0) {
       k = nk;
-      p += jump;
+      p += --strips > 0 ? jump : back;
     }
   }
 };
 
 // One segment of a consumer warp: its strips s0 + group, s0 + group + groups, ...
-template <typename T, int GROUP, int NT>
-__device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP>& in, W4Sums& sums, uint32_t x, uint32_t xsum,
-                                           int part, int rows, int strips, int rounds, volatile int* abort_flag) {
+template <typename T, int GROUP, bool ZEROS, int NTMAX, int NT, int AHEAD>
+__device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP, ZEROS, AHEAD>& in, W4Sums& sums, uint32_t x,
+                                           uint32_t start, int part, int rows, int strips, int rounds,
+                                           volatile int* abort_flag) {
   const int lane = threadIdx.x & 31;
   int xrow[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) xrow[t] = min(t * 8 + (lane >> 2), rows - 1) * a.x_pitch;
-  constexpr int kXsumTile = kW4TileK / GROUP * kW4MaxRows * 4;
-  const uint32_t x0 = x + (lane & 3) * 16 + part * (kW4TileK * 2), sum0 = xsum + (lane & 3) * 8 + part * kXsumTile;
-  uint32_t xl = x0, sl = sum0;
+  constexpr int kStartGroup = NTMAX * 64, kStartTile = kW4TileK / GROUP * kStartGroup;
+  const uint32_t x0 = x + (lane & 3) * 16 + part * (kW4TileK * 2), start0 = start + (lane & 3) * 16 + part * kStartTile;
+  uint32_t xl = x0, sl = start0;
   float acc[NT][4] = {};
   auto flush = [&]() {
     mbar_wait(&sums.empty[sums.slot()], sums.phase() ^ 1, abort_flag, a.status);
@@ -377,18 +369,18 @@ __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP>& in,
     ++sums.turn;
   };
   int k = in.nk;
-  for (int n = strips * in.nk; n > 0; n -= kW4Ahead) {
+  for (int n = strips * in.nk; n > 0; n -= AHEAD) {
 #pragma unroll
-    for (int j = 0; j < kW4Ahead; ++j) {
+    for (int j = 0; j < AHEAD; ++j) {
       if (j < n) {
-        w4_tile<T, GROUP, NT>(in.frag[j], xl, xrow, sl, acc);
-        in.load(j, a.zeros);
+        w4_tile<T, GROUP, ZEROS, NT>(in.frag[j], xl, xrow, sl, kStartGroup, acc);
+        in.load(j);
         xl += a.wps * (kW4TileK * 2);
-        sl += a.wps * kXsumTile;
+        sl += a.wps * kStartTile;
         if (--k == 0) {
           k = in.nk;
           xl = x0;
-          sl = sum0;
+          sl = start0;
           flush();
         }
       }
@@ -397,16 +389,72 @@ __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP>& in,
   if (strips < rounds) flush();  // the last round has no strip for this group
 }
 
-template <typename T, int GROUP, int NTMAX>
+// Rows first .. first + rows of x, columns of `kts` tiles from kt0, into shared memory; and for fp16
+// where each group's sums start: per group and pair of rows of x four numbers, -z 2^-24 sum x of the
+// two rows (z = 8, or 1 where the records hold zero points) and 16 times that.
+template <typename T, int GROUP, bool ZEROS, int NTMAX>
+__device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int first, int rows, int kt0, int kts) {
+  constexpr int kThreads = w4_warps(NTMAX) * 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k0 = kt0 * kW4TileK, words = kts * (kW4TileK / 8);
+  for (int m = 0; m < rows; ++m) {
+    const long long row = a.gather ? a.gather[first + m] / a.gather_div : first + m;
+    const T* src = static_cast<const T*>(a.x) + row * a.ld_x + k0;
+    uint8_t* dst = smem + m * a.x_pitch;
+    for (int c = threadIdx.x; c < words; c += kThreads) {
+      const int left = a.K - k0 - c * 8;  // columns of x from this word on
+      if (left >= 8 && a.x_words) {
+        cp_async_16(smem_u32(dst + c * 16), src + c * 8, 16);
+      } else {
+        uint16_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          e[i] = i < left ? reinterpret_cast<const uint16_t*>(src)[c * 8 + i] : static_cast<uint16_t>(0);
+        *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+  }
+  cp_async_wait_all();
+  named_sync(1, kThreads);
+  if constexpr (W4Type<T>::kSums) {
+    constexpr int kLanes = GROUP / 8;  // of a group
+    const int chunks = (words + 31) / 32;
+    for (int i = warp; i < rows * chunks; i += kThreads / 32) {
+      const int m = i / chunks, word = (i - m * chunks) * 32 + lane;
+      float sum = 0.0f;
+      if (word < words) {
+        const uint4 v = lds128(smem_u32(smem) + m * a.x_pitch + word * 16);
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __half22float2(h[e]);
+          sum += f.x + f.y;
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane % kLanes == 0 && word < words) {
+        const float start = sum * (ZEROS ? -1.0f : -8.0f) / W4Type<T>::kScale0;
+        float* to = reinterpret_cast<float*>(smem + a.x_bytes) + word / kLanes * (NTMAX * 16) + (m >> 1) * 4 + (m & 1);
+        to[0] = start;
+        to[2] = start * (W4Type<T>::kScale0 / W4Type<T>::kScale1);
+      }
+    }
+    named_sync(1, kThreads);
+  }
+}
+
+template <typename T, int GROUP, bool ZEROS, int NTMAX>
 __global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4Args a) {
   constexpr int kWarps = w4_warps(NTMAX);
-  extern __shared__ __align__(128) uint8_t smem[];  // [x][sums of x][sums of the warps]
+  extern __shared__ __align__(128) uint8_t smem[];  // [x][starts of the sums][sums of the warps]
   __shared__ uint64_t full[kWarps * 2], empty[kWarps * 2];
   __shared__ int abort_flag;
-  const int record = w4_record_bytes(GROUP, a.zeros);
+  constexpr int record = w4_record_bytes(GROUP, ZEROS);
+  constexpr int kAhead = w4_ahead(GROUP, ZEROS, NTMAX);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = kWarps / a.wps;
-  const uint32_t base = smem_u32(smem), xsum = base + a.x_bytes, sums_at = xsum + a.xsum_bytes;
+  const uint32_t base = smem_u32(smem), starts = base + a.x_bytes, sums_at = starts + a.start_bytes;
   constexpr int kSumBytes = kWarps * NTMAX * 512;  // of all groups, one turn
   if (threadIdx.x == 0) {
     for (int i = 0; i < groups * 2; ++i) {
@@ -471,7 +519,7 @@ __global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4A
 
   const int part = warp % a.wps, group = warp / a.wps;
   W4Sums sums{full + group * 2, empty + group * 2, sums_at + group * a.wps * NTMAX * 512, kSumBytes, 0};
-  W4Stream<GROUP> in;
+  W4Stream<GROUP, ZEROS, kAhead> in;
   in.step = static_cast<long long>(a.wps) * record;
   bool fresh = a.early;
   while (seg.next(a, tile, slice)) {
@@ -481,62 +529,24 @@ __global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4A
     const int rounds = group < groups ? (seg.s1 - seg.s0 + groups - 1) / groups : 0;
     const int strips = group < groups ? (seg.s1 - seg.s0 - group + groups - 1) / groups : 0;
     in.nk = in.k = (kts - part + a.wps - 1) / a.wps;
-    in.todo = strips * in.nk;
-    in.jump = (static_cast<long long>(groups) * a.kt - static_cast<long long>(in.nk) * a.wps) * record;
+    in.strips = strips;
+    in.back = -in.nk * in.step;
+    in.jump = static_cast<long long>(groups) * a.kt * record + in.back;
     in.p = a.w + expert * a.expert_bytes + (static_cast<long long>(seg.s0 + group) * a.kt + kt0 + part) * record;
+    if (strips > 0)
 #pragma unroll
-    for (int j = 0; j < kW4Ahead; ++j) in.load(j, a.zeros);
+      for (int j = 0; j < kAhead; ++j) in.load(j);
     if (fresh) grid_dep_wait();  // x is the kernel before's
     fresh = false;
 
     named_sync(1, kWarps * 32);  // all have done with the rows before
-    const int k0 = kt0 * kW4TileK, words = kts * (kW4TileK / 8);
-    for (int m = 0; m < rows; ++m) {
-      const long long row = a.gather ? a.gather[first + m] / a.gather_div : first + m;
-      const T* src = static_cast<const T*>(a.x) + row * a.ld_x + k0;
-      uint8_t* dst = smem + m * a.x_pitch;
-      for (int c = threadIdx.x; c < words; c += kWarps * 32) {
-        const int left = a.K - k0 - c * 8;  // columns of x from this word on
-        if (left >= 8 && a.x_words) {
-          cp_async_16(smem_u32(dst + c * 16), src + c * 8, 16);
-        } else {
-          uint16_t e[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            e[i] = i < left ? reinterpret_cast<const uint16_t*>(src)[c * 8 + i] : static_cast<uint16_t>(0);
-          *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(e);
-        }
-      }
-    }
-    cp_async_wait_all();
-    named_sync(1, kWarps * 32);
-    if constexpr (W4Type<T>::kSums) {  // sums of each row over the groups, GROUP / 8 lanes each
-      const int chunks = (words + 31) / 32;
-      for (int i = warp; i < rows * chunks; i += kWarps) {
-        const int m = i / chunks, word = (i - m * chunks) * 32 + lane;
-        float sum = 0.0f;
-        if (word < words) {
-          const uint4 v = lds128(base + m * a.x_pitch + word * 16);
-          const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = __half22float2(h[e]);
-            sum += f.x + f.y;
-          }
-        }
-#pragma unroll
-        for (int o = 1; o < GROUP / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane % (GROUP / 8) == 0 && word < words)
-          reinterpret_cast<float*>(smem + a.x_bytes)[word / (GROUP / 8) * kW4MaxRows + m] = sum;
-      }
-      named_sync(1, kWarps * 32);
-    }
+    w4_load_x<T, GROUP, ZEROS, NTMAX>(a, smem, first, rows, kt0, kts);
     if (NTMAX == 1 || rows <= 8)
-      w4_segment<T, GROUP, 1>(a, in, sums, base, xsum, part, rows, strips, rounds, &abort_flag);
+      w4_segment<T, GROUP, ZEROS, NTMAX, 1>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
     else if (NTMAX == 2 || rows <= 16)
-      w4_segment<T, GROUP, NTMAX < 2 ? 1 : 2>(a, in, sums, base, xsum, part, rows, strips, rounds, &abort_flag);
+      w4_segment<T, GROUP, ZEROS, NTMAX, NTMAX < 2 ? 1 : 2>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
     else
-      w4_segment<T, GROUP, NTMAX < 4 ? 1 : 4>(a, in, sums, base, xsum, part, rows, strips, rounds, &abort_flag);
+      w4_segment<T, GROUP, ZEROS, NTMAX, NTMAX < 4 ? 1 : 4>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
   }
   if (fresh) grid_dep_wait();  // a CTA without work: its end must still follow the kernel before
 }
