@@ -20,10 +20,7 @@ struct W4Plan {
   size_t smem() const { return static_cast<size_t>(x_bytes) + start_bytes + sum_bytes; }
 };
 
-#ifndef SUMCOST
-#define SUMCOST 1.0
-#endif
-constexpr double kW4SumCost = SUMCOST;
+constexpr double kW4SumCost = 1.0;
 constexpr int kW4Smem = kMaxDynamicSmem - 1024;  // static shared memory of the kernel, rounded up
 
 // `tiles`: token tiles expected, `sms`: CTAs.
@@ -33,8 +30,8 @@ W4Plan w4_plan(int strips, int64_t K, int group, int tile_rows, double tiles, in
   p.kt = static_cast<int>(ceil_div(K, kW4TileK));
   p.tile_rows = tile_rows;
   p.nt = tile_rows <= 8 ? 1 : tile_rows <= 16 ? 2 : 4;
-  p.warps = w4_warps(p.nt);
-  p.sum_bytes = 2 * p.warps * p.nt * 512;
+  p.warps = w4_warps(group, p.nt);
+  p.sum_bytes = 2 * p.warps * p.nt * 1024;
   // K is cut so that the rows' slice of x (and the starts of its sums) fits in shared memory
   const int start_kt = kW4TileK / group * p.nt * 64;
   const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows + start_kt);
@@ -68,7 +65,7 @@ int check_format(int64_t matrices, int64_t N, int64_t K, int group, int gate_up)
   return MOE_OK;
 }
 
-int w4_strips(int64_t N, int gate_up) { return static_cast<int>(gate_up ? ceil_div(N / 2, 8) : ceil_div(N, 16)); }
+int w4_strips(int64_t N, int gate_up) { return static_cast<int>(ceil_div(gate_up ? N / 2 : N, gate_up ? kW4TileRows / 2 : kW4TileRows)); }
 
 int64_t matrix_bytes(int64_t N, int64_t K, int group, int zeros, int gate_up) {
   return static_cast<int64_t>(w4_strips(N, gate_up)) * ceil_div(K, kW4TileK) * w4_record_bytes(group, zeros != 0);
@@ -96,7 +93,7 @@ template <typename T, int GROUP, bool ZEROS, int NT>
 int launch_gemv_t(const W4Args& a, size_t smem, int grid, int dev, bool dependent, cudaStream_t s) {
   constexpr auto kernel = w4_gemv_kernel<T, GROUP, ZEROS, NT>;
   MOE_TRY(allow_smem<kernel>(dev));
-  return launch(kernel, grid, w4_threads(NT), smem, s, dependent, a);
+  return launch(kernel, grid, w4_threads(GROUP, NT), smem, s, dependent, a);
 }
 
 template <typename T, int GROUP, bool ZEROS>
@@ -180,7 +177,7 @@ int w4_linear_t(const void* x, int64_t ld_x, const void* packed, void* out, int6
   const int64_t units = ceil_div(M, p.tile_rows) * p.slices * p.strips;
   MOE_TRY(launch_gemv<T>(a, p, group, zeros, static_cast<int>(std::min<int64_t>(units, sms)), dev, false, s));
   if (p.slices == 1) return MOE_OK;
-  return launch_combine_w<T, int32_t>(part, p.slices, M, p.strips * 16, nullptr, nullptr, MOE_F32, 0, 1, M, N,
+  return launch_combine_w<T, int32_t>(part, p.slices, M, p.strips * kW4TileRows, nullptr, nullptr, MOE_F32, 0, 1, M, N,
                                       static_cast<T*>(out), ld_out, blocks_for(M * ceil_div(N, 4), 128, sms), s);
 }
 
@@ -208,7 +205,7 @@ W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t
   const double active = static_cast<double>(E) * (1 - std::pow(1 - 1.0 / static_cast<double>(E), static_cast<double>(R)));
   const double tiles = std::max(active, static_cast<double>(R) / tile_rows);
   L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, tile_rows, tiles, sms);
-  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * 8, g2, tile_rows, tiles, sms);
+  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * (kW4TileRows / 2), g2, tile_rows, tiles, sms);
   L.max_tiles = R / tile_rows + std::min(E, R);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -219,9 +216,9 @@ W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t
   L.num_tiles = take(sizeof(int));
   L.tiles = take(sizeof(int4) * static_cast<size_t>(L.max_tiles));
   L.sorted = take(sizeof(int) * static_cast<size_t>(R));
-  L.h = take(2 * static_cast<size_t>(R) * L.p1.strips * 8);
-  L.part1 = take(L.p1.slices > 1 ? sizeof(float) * static_cast<size_t>(L.p1.slices) * R * L.p1.strips * 16 : 0);
-  L.part2 = take(sizeof(float) * static_cast<size_t>(L.p2.slices) * R * L.p2.strips * 16);
+  L.h = take(2 * static_cast<size_t>(R) * L.p1.strips * (kW4TileRows / 2));
+  L.part1 = take(L.p1.slices > 1 ? sizeof(float) * static_cast<size_t>(L.p1.slices) * R * L.p1.strips * kW4TileRows : 0);
+  L.part2 = take(sizeof(float) * static_cast<size_t>(L.p2.slices) * R * L.p2.strips * kW4TileRows);
   L.total = off;
   return L;
 }
@@ -257,19 +254,19 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
   a.gather_div = static_cast<int>(topk);
   a.epilogue = L.p1.slices == 1 ? kW4GateUp : kW4Partial;
   a.out = h;
-  a.ld_out = L.p1.strips * 8;
-  a.n_out = L.p1.strips * 8;  // the padding's columns too: they are zero
+  a.ld_out = L.p1.strips * (kW4TileRows / 2);
+  a.n_out = L.p1.strips * (kW4TileRows / 2);  // the padding's columns too: they are zero
   a.part = part1;
   a.part_rows = R;
   MOE_TRY(launch_gemv<T>(a, L.p1, g13, z13, sms, dev, true, s));
   if (L.p1.slices > 1)
-    MOE_TRY(launch(w4_act_kernel<T>, blocks_for(R * L.p1.strips * 2, 128, sms), 128, 0, s, true, (const float*)part1,
-                   L.p1.slices, (long long)R, L.p1.strips, h));
+    MOE_TRY(launch(w4_act_kernel<T>, blocks_for(R * L.p1.strips * 4, 128, sms), 128, 0, s, true, (const float*)part1,
+                   L.p1.slices, (long long)R, L.p1.strips * 2, h));
   // second product: the routes' rows in place, its sums per route
   W4Args b = w4_args(L.p2, w2, matrix_bytes(H, I, g2, z2, 0), status);
   b.x = h;
-  b.ld_x = L.p1.strips * 8;
-  b.K = L.p1.strips * 8;
+  b.ld_x = L.p1.strips * (kW4TileRows / 2);
+  b.K = L.p1.strips * (kW4TileRows / 2);
   b.x_words = 1;
   b.tiles = tiles;
   b.num_tiles = num_tiles;
@@ -281,9 +278,9 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
   MOE_TRY(launch_gemv<T>(b, L.p2, g2, z2, sms, dev, true, s));
   const int grid = blocks_for(T_ * ceil_div(H, 4), 128, sms);
   if (ids_dtype == MOE_I32)
-    return launch_combine_w<T, int32_t>(part2, L.p2.slices, R, L.p2.strips * 16, ids, tw, w_dtype, E, topk, T_, H,
+    return launch_combine_w<T, int32_t>(part2, L.p2.slices, R, L.p2.strips * kW4TileRows, ids, tw, w_dtype, E, topk, T_, H,
                                         static_cast<T*>(out), H, grid, s);
-  return launch_combine_w<T, int64_t>(part2, L.p2.slices, R, L.p2.strips * 16, ids, tw, w_dtype, E, topk, T_, H,
+  return launch_combine_w<T, int64_t>(part2, L.p2.slices, R, L.p2.strips * kW4TileRows, ids, tw, w_dtype, E, topk, T_, H,
                                       static_cast<T*>(out), H, grid, s);
 }
 
@@ -380,7 +377,7 @@ size_t moe_w4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int group,
   clear_error();
   if (M < 1 || check_format(1, N, K, group, 0) != MOE_OK) return 0;
   const W4Plan p = w4_plan(w4_strips(N, 0), K, group, linear_tile_rows(M), 1, 1);
-  return p.slices == 1 ? 0 : sizeof(float) * static_cast<size_t>(p.slices) * static_cast<size_t>(M) * p.strips * 16;
+  return p.slices == 1 ? 0 : sizeof(float) * static_cast<size_t>(p.slices) * static_cast<size_t>(M) * p.strips * kW4TileRows;
 }
 
 int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, int64_t ld_out, int64_t M, int64_t N, int64_t K,

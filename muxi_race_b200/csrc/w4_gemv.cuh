@@ -8,15 +8,15 @@
 //
 // Few rows leave the weights' bytes as the bound: N K / 2 bytes for 2 M N K operations. So the
 // weights are laid out once (moe_w4_pack) as the stream that the kernel reads:
-//   tile    16 rows x 128 columns: 1024 bytes of values, the groups' scales, the zero points. In a
-//           tile, lane l's 16 bytes hold its mma.m16n8k16 A fragments of four steps, so a tile is two
-//           16-byte loads a lane straight into registers, with no shuffles and no shared memory.
-//   strip   the tiles of 16 rows, one after another along K; an expert's strips follow each other.
+//   tile    32 rows x 128 columns: 2048 bytes of values, the groups' scales, the zero points. In a
+//           tile, lane l's 16-byte words hold its mma.m16n8k16 A fragments of four steps, so a tile is
+//           four 16-byte loads a lane straight into registers, with no shuffles and no shared memory.
+//   strip   the tiles of 32 rows, one after another along K; an expert's strips follow each other.
 // One CTA per SM. Its warps walk through strips with the loads of the next tiles in flight in
-// registers (w4_ahead tiles a warp: 60 to 90 KB an SM); x (at most 32 rows, one slice of K) stays in
+// registers (w4_ahead tiles a warp: 59 to 89 KB an SM); x (at most 32 rows, one slice of K) stays in
 // shared memory. Warps that share a strip split K; their sums go through shared memory to the store
 // warps, which add them up, so that no consumer waits for another or for a store.
-// mma.sync and not tcgen05.mma: the weights must pass the registers to be unpacked, a 16-row strip
+// mma.sync and not tcgen05.mma: the weights must pass the registers to be unpacked, a 32-row strip
 // per warp keeps them there as the A operand, and with at most 32 columns the tensor rate is not
 // the bound.
 #pragma once
@@ -30,23 +30,24 @@ namespace moe {
 
 constexpr int kW4StoreWarps = 2;       // warps that add up the consumers' sums and store them
 constexpr int kW4TileK = 128;
-constexpr int kW4TileBytes = 1024;     // values of one tile
+constexpr int kW4TileRows = 32;
+constexpr int kW4TileBytes = 2048;     // values of one tile
 constexpr int kW4MaxRows = 32;         // rows of x at a time
-// consumer warps: with the store warps 16 of 128 registers, or 12 of 168 for four blocks of 8 rows
-__host__ __device__ constexpr int w4_warps(int nt) { return nt <= 2 ? 14 : 10; }
-__host__ __device__ constexpr int w4_threads(int nt) { return (w4_warps(nt) + kW4StoreWarps) * 32; }
+// Consumer warps. With the store warps 16 of 128 registers, 12 of 168 or 8 of 255: with small groups a
+// lane holds more scales and zero points, and with more blocks of rows more sums, and what spills
+// costs more than the warps (17 rows of K = 14336, group 32: 51 us with 6 warps, 75 us with 10; 16 rows
+// of K = 7168, N = 131072, group 128: 125 us with 14, 128 us with 10).
+__host__ __device__ constexpr int w4_warps(int group, int nt) {
+  return nt == 1 || (nt == 2 && group == 128) ? 14 : nt == 2 || group == 128 ? 10 : 6;
+}
+__host__ __device__ constexpr int w4_threads(int group, int nt) { return (w4_warps(group, nt) + kW4StoreWarps) * 32; }
 
 // tiles that a warp has in flight: as many as its registers hold
-#ifndef AH1
-#define AH1 6
-#endif
-__host__ __device__ constexpr int w4_ahead(int group, bool zeros, int nt) {
-  return nt > 1 ? 4 : group == 128 && !zeros ? AH1 : group >= 64 ? 5 : 4;
-}
+__host__ __device__ constexpr int w4_ahead(int group, int nt) { return group == 128 && nt == 1 ? 3 : 2; }
 
-// bytes of a tile with its scales (half2 of rows r, r + 8 per group) and zero points (byte pairs)
+// bytes of a tile with its scales (of rows r, r + 8, r + 16, r + 24 together, per group) and zero points
 __host__ __device__ constexpr int w4_record_bytes(int group, bool zeros) {
-  return kW4TileBytes + kW4TileK / group * (32 + (zeros ? 16 : 0));
+  return kW4TileBytes + kW4TileK / group * (64 + (zeros ? 32 : 0));
 }
 
 enum { kW4Out = 0, kW4GateUp = 1, kW4Partial = 2 };
@@ -71,7 +72,7 @@ struct W4Args {
   void* out;                // kW4Out: [row][n]; kW4GateUp: [row][i]
   long long ld_out;
   int n_out;                // columns to write
-  float* part;              // kW4Partial: [slice][row][strips * 16]
+  float* part;              // kW4Partial: [slice][row][strips * 32]
   long long part_rows;
   int x_pitch;              // bytes of a row of x in shared memory
   int x_bytes, start_bytes; // bytes of the rows of x, and of where the groups' sums start (fp16)
@@ -160,65 +161,61 @@ __device__ __forceinline__ uint32_t lds16(uint32_t p) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p));
   return v;
 }
-// A lane's part of a record, loaded ahead.
+// A lane's part of a record, loaded ahead: its fragments of rows r, r + 8 ([0]) and r + 16, r + 24 ([1]).
 template <int GROUP, bool ZEROS>
 struct W4Frag {
   static constexpr int kGroups = kW4TileK / GROUP;
-  uint4 w[2];
-  uint32_t s[kGroups];              // scales of rows r and r + 8
-  uint32_t z[ZEROS ? kGroups : 1];  // their zero points, one byte each
+  uint4 w[2][2];                    // [half of the columns][rows]
+  uint2 s[kGroups];                 // scales: .x of the first rows' two, .y of the second's
+  uint32_t z[ZEROS ? kGroups : 1];  // zero points of the four rows, one byte each
   __device__ __forceinline__ void load(const uint8_t* record) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
       asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                   : "=r"(w[i / 2][i % 2].x), "=r"(w[i / 2][i % 2].y), "=r"(w[i / 2][i % 2].z), "=r"(w[i / 2][i % 2].w)
                    : "l"(record + i * 512 + lane * 16));
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(s[g]) : "l"(record + kW4TileBytes + g * 32 + r * 4));
-      if constexpr (ZEROS) {
-        uint16_t v;
-        asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];"
-                     : "=h"(v)
-                     : "l"(record + kW4TileBytes + kGroups * 32 + g * 16 + r * 2));
-        z[g] = v;
-      }
+      asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+                   : "=r"(s[g].x), "=r"(s[g].y)
+                   : "l"(record + kW4TileBytes + g * 64 + r * 8));
+      if constexpr (ZEROS)
+        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];"
+                     : "=r"(z[g])
+                     : "l"(record + kW4TileBytes + kGroups * 64 + g * 32 + r * 4));
     }
   }
 };
 
-// acc += tile * x for NT blocks of 8 rows of x (shared addresses), in units of 1 / kScale. `x`: this
-// lane's columns of row 0; xrow[t]: the offset of its row of block t (a lane whose row does not exist
-// reads another's: the column that it makes of it is not stored). `start` (fp16): this lane's starts
-// of the tile's first group, `start_group` bytes from one group to the next (see w4_load_x).
+// acc[f] += fragment rows f of the tile * x for NT blocks of 8 rows of x (shared addresses), in units
+// of 1 / kScale. `x`: this lane's columns of row 0; xrow[t]: the offset of its row of block t (a lane
+// whose row does not exist reads another's: the column that it makes of it is not stored). `start`
+// (fp16): this lane's starts of the tile's first group, `start_group` bytes from one group to the next
+// (see w4_load_x).
 template <typename T, int GROUP, bool ZEROS, int NT>
-__device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& f, uint32_t x, const int (&xrow)[NT], uint32_t start,
-                                        int start_group, float (&acc)[NT][4]) {
+__device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& in, uint32_t x, const int (&xrow)[NT], uint32_t start,
+                                        int start_group, float (&acc)[2][NT][4]) {
   constexpr int kGroups = kW4TileK / GROUP;
-  constexpr int kBlocks = GROUP / 32;        // blocks of 32 columns in a group
-  constexpr int kChains = NT == 1 ? 2 : 1;   // sums per block of rows: at least two independent chains
-  const uint32_t words[8] = {f.w[0].x, f.w[0].y, f.w[0].z, f.w[0].w, f.w[1].x, f.w[1].y, f.w[1].z, f.w[1].w};
+  constexpr int kBlocks = GROUP / 32;  // blocks of 32 columns in a group
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    uint32_t z0 = 8, z1 = 8;
-    if constexpr (ZEROS) {
-      z0 = f.z[g] & 0xff;
-      z1 = f.z[g] >> 8;
-    }
-    const uint32_t off[2] = {0x43004300u + z0 * 0x10001u, 0x43004300u + z1 * 0x10001u};
-    float c[NT][kChains][4];
+    uint32_t z[4] = {8, 8, 8, 8};
+    if constexpr (ZEROS)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = (in.z[g] >> (8 * i)) & 0xff;
+    float c[2][NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if constexpr (W4Type<T>::kSums) v = lds128(start + g * start_group + t * 64);
 #pragma unroll
-      for (int i = 0; i < kChains * 4; ++i) c[t][i / 4][i % 4] = 0.0f;
-      if constexpr (W4Type<T>::kSums) {
-        const uint4 v = lds128(start + g * start_group + t * 64);
-        const float f0 = ZEROS ? static_cast<float>(z0) : 1.0f, f1 = ZEROS ? static_cast<float>(z1) : 1.0f;
-        c[t][0][0] = f0 * __uint_as_float(v.x);
-        c[t][0][1] = f0 * __uint_as_float(v.y);
-        c[t][0][2] = f1 * __uint_as_float(v.z);
-        c[t][0][3] = f1 * __uint_as_float(v.w);
+      for (int f = 0; f < 2; ++f) {
+        const float f0 = ZEROS ? static_cast<float>(z[2 * f]) : 1.0f, f1 = ZEROS ? static_cast<float>(z[2 * f + 1]) : 1.0f;
+        c[f][t][0] = f0 * __uint_as_float(v.x);
+        c[f][t][1] = f0 * __uint_as_float(v.y);
+        c[f][t][2] = f1 * __uint_as_float(v.z);
+        c[f][t][3] = f1 * __uint_as_float(v.w);
       }
     }
 #pragma unroll
@@ -227,34 +224,40 @@ __device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& f, uint32_t 
       uint4 xv[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) xv[t] = lds128(x + xrow[t] + block * 64);
-      uint32_t a[4];
-      W4Type<T>::unpack(words[block * 2], off, a);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) W4Type<T>::mma(c[t][0], a, xv[t].x, xv[t].y, c[t][0]);
-      W4Type<T>::unpack(words[block * 2 + 1], off, a);
+      for (int step = 0; step < 2; ++step)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) W4Type<T>::mma(c[t][kChains - 1], a, xv[t].z, xv[t].w, c[t][kChains - 1]);
+        for (int f = 0; f < 2; ++f) {
+          const uint4& w = in.w[block / 2][f];
+          const uint32_t off[2] = {0x43004300u + z[2 * f] * 0x10001u, 0x43004300u + z[2 * f + 1] * 0x10001u};
+          uint32_t a[4];
+          W4Type<T>::unpack(block % 2 == 0 ? (step == 0 ? w.x : w.y) : (step == 0 ? w.z : w.w), off, a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            W4Type<T>::mma(c[f][t], a, step == 0 ? xv[t].x : xv[t].z, step == 0 ? xv[t].y : xv[t].w, c[f][t]);
+        }
     }
-    const float s0 = W4Type<T>::to_f(f.s[g] & 0xffffu), s1 = W4Type<T>::to_f(f.s[g] >> 16);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if constexpr (kChains == 2)
+    for (int f = 0; f < 2; ++f) {
+      const uint32_t s = f == 0 ? in.s[g].x : in.s[g].y;
+      const float s0 = W4Type<T>::to_f(s & 0xffffu), s1 = W4Type<T>::to_f(s >> 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[t][0][i] += c[t][1][i];
-      acc[t][0] = fmaf(s0, c[t][0][0], acc[t][0]);
-      acc[t][1] = fmaf(s0, c[t][0][1], acc[t][1]);
-      acc[t][2] = fmaf(s1, c[t][0][2], acc[t][2]);
-      acc[t][3] = fmaf(s1, c[t][0][3], acc[t][3]);
+      for (int t = 0; t < NT; ++t) {
+        acc[f][t][0] = fmaf(s0, c[f][t][0], acc[f][t][0]);
+        acc[f][t][1] = fmaf(s0, c[f][t][1], acc[f][t][1]);
+        acc[f][t][2] = fmaf(s1, c[f][t][2], acc[f][t][2]);
+        acc[f][t][3] = fmaf(s1, c[f][t][3], acc[f][t][3]);
+      }
     }
   }
 }
 
 __device__ __forceinline__ float w4_silu(float v) { return v / (1.0f + __expf(-v)); }
 
-// The sums of block t of a strip leave: v = {row r: rows 2q, 2q + 1 of x; row r + 8: the same}.
-// `out_row`: the output row of x's row `lane`.
+// The sums of block t and fragment rows f of a strip leave: v = {row r: rows 2q, 2q + 1 of x; row
+// r + 8: the same}. `out_row`: the output row of x's row `lane`.
 template <typename T>
-__device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int out_row, int rows, int t,
+__device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int out_row, int rows, int t, int f,
                                          const float4& v) {
   const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
   const float lo[2] = {v.x * W4Type<T>::kScale0, v.y * W4Type<T>::kScale0};
@@ -264,17 +267,18 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, 
     const int m = t * 8 + q * 2 + i;
     const long long row = __shfl_sync(0xffffffffu, out_row, m);
     if (m >= rows) continue;
+    const int n = strip * kW4TileRows + f * 16 + r;
     if (a.epilogue == kW4Out) {
-      T* o = static_cast<T*>(a.out) + row * a.ld_out + strip * 16;
-      if (strip * 16 + r < a.n_out) o[r] = W4Type<T>::from_f(lo[i]);
-      if (strip * 16 + r + 8 < a.n_out) o[r + 8] = W4Type<T>::from_f(hi[i]);
+      T* o = static_cast<T*>(a.out) + row * a.ld_out;
+      if (n < a.n_out) o[n] = W4Type<T>::from_f(lo[i]);
+      if (n + 8 < a.n_out) o[n + 8] = W4Type<T>::from_f(hi[i]);
     } else if (a.epilogue == kW4GateUp) {
-      if (strip * 8 + r < a.n_out)
-        static_cast<T*>(a.out)[row * a.ld_out + strip * 8 + r] = W4Type<T>::from_f(w4_silu(lo[i]) * hi[i]);
+      const int c = strip * 16 + f * 8 + r;
+      if (c < a.n_out) static_cast<T*>(a.out)[row * a.ld_out + c] = W4Type<T>::from_f(w4_silu(lo[i]) * hi[i]);
     } else {
-      float* o = a.part + (slice * a.part_rows + row) * (a.strips * 16ll) + strip * 16;
-      o[r] = lo[i];
-      o[r + 8] = hi[i];
+      float* o = a.part + (slice * a.part_rows + row) * (a.strips * static_cast<long long>(kW4TileRows)) + n;
+      o[0] = lo[i];
+      o[8] = hi[i];
     }
   }
 }
@@ -352,17 +356,16 @@ __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP, ZERO
   constexpr int kStartGroup = NTMAX * 64, kStartTile = kW4TileK / GROUP * kStartGroup;
   const uint32_t x0 = x + (lane & 3) * 16 + part * (kW4TileK * 2), start0 = start + (lane & 3) * 16 + part * kStartTile;
   uint32_t xl = x0, sl = start0;
-  float acc[NT][4] = {};
+  float acc[2][NT][4] = {};
   auto flush = [&]() {
     mbar_wait(&sums.empty[sums.slot()], sums.phase() ^ 1, abort_flag, a.status);
-    const uint32_t buf = sums.at + sums.slot() * sums.bytes + (part * NT * 32 + lane) * 16;
+    const uint32_t buf = sums.at + sums.slot() * sums.bytes + (part * NT * 64 + lane) * 16;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(buf + t * 512), "f"(acc[t][0]), "f"(acc[t][1]),
-                   "f"(acc[t][2]), "f"(acc[t][3])
+    for (int i = 0; i < 2 * NT; ++i) {
+      float(&v)[4] = acc[i & 1][i / 2];
+      asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(buf + i * 512), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3])
                    : "memory");
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = 0.0f;
+      v[0] = v[1] = v[2] = v[3] = 0.0f;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sums.full[sums.slot()]);
@@ -394,7 +397,7 @@ __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP, ZERO
 // two rows (z = 8, or 1 where the records hold zero points) and 16 times that.
 template <typename T, int GROUP, bool ZEROS, int NTMAX>
 __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int first, int rows, int kt0, int kts) {
-  constexpr int kThreads = w4_warps(NTMAX) * 32;
+  constexpr int kThreads = w4_warps(GROUP, NTMAX) * 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k0 = kt0 * kW4TileK, words = kts * (kW4TileK / 8);
   for (int m = 0; m < rows; ++m) {
@@ -445,17 +448,17 @@ __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int fi
 }
 
 template <typename T, int GROUP, bool ZEROS, int NTMAX>
-__global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4Args a) {
-  constexpr int kWarps = w4_warps(NTMAX);
+__global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(const W4Args a) {
+  constexpr int kWarps = w4_warps(GROUP, NTMAX);
   extern __shared__ __align__(128) uint8_t smem[];  // [x][starts of the sums][sums of the warps]
   __shared__ uint64_t full[kWarps * 2], empty[kWarps * 2];
   __shared__ int abort_flag;
   constexpr int record = w4_record_bytes(GROUP, ZEROS);
-  constexpr int kAhead = w4_ahead(GROUP, ZEROS, NTMAX);
+  constexpr int kAhead = w4_ahead(GROUP, NTMAX);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = kWarps / a.wps;
   const uint32_t base = smem_u32(smem), starts = base + a.x_bytes, sums_at = starts + a.start_bytes;
-  constexpr int kSumBytes = kWarps * NTMAX * 512;  // of all groups, one turn
+  constexpr int kSumBytes = kWarps * NTMAX * 1024;  // of all groups, one turn
   if (threadIdx.x == 0) {
     for (int i = 0; i < groups * 2; ++i) {
       mbar_init(&full[i], a.wps);
@@ -496,17 +499,17 @@ __global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4A
           mbar_wait(&full[at], (turn >> 1) & 1, &abort_flag, a.status);
           if (strip0 + g < seg.s1) {
             const float4* buf = reinterpret_cast<const float4*>(smem + (sums_at - base) + (turn & 1) * kSumBytes) +
-                                g * a.wps * NTMAX * 32 + lane;
-            for (int t = 0; t < nt; ++t) {
-              float4 v = buf[t * 32];
+                                g * a.wps * NTMAX * 64 + lane;
+            for (int i = 0; i < 2 * nt; ++i) {
+              float4 v = buf[i * 32];
               for (int p = 1; p < a.wps; ++p) {
-                const float4 o = buf[(p * nt + t) * 32];
+                const float4 o = buf[(p * 2 * nt + i) * 32];
                 v.x += o.x;
                 v.y += o.y;
                 v.z += o.z;
                 v.w += o.w;
               }
-              w4_store<T>(a, strip0 + g, slice, out_row, rows, t, v);
+              w4_store<T>(a, strip0 + g, slice, out_row, rows, i / 2, i & 1, v);
             }
           }
           __syncwarp();
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(w4_threads(NTMAX), 1) w4_gemv_kernel(const W4A
   }
 
   const int part = warp % a.wps, group = warp / a.wps;
-  W4Sums sums{full + group * 2, empty + group * 2, sums_at + group * a.wps * NTMAX * 512, kSumBytes, 0};
+  W4Sums sums{full + group * 2, empty + group * 2, sums_at + group * a.wps * NTMAX * 1024, kSumBytes, 0};
   W4Stream<GROUP, ZEROS, kAhead> in;
   in.step = static_cast<long long>(a.wps) * record;
   bool fresh = a.early;
@@ -614,27 +617,27 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// h[p][i] = silu(sum over the slices of gate) * (the same of up); part [slices][rows][strips * 16],
-// each strip 8 gate rows then 8 up rows. A thread takes 4 columns; h has strips * 8 columns.
+// h[p][i] = silu(sum over the slices of gate) * (the same of up); part [slices][rows][blocks * 16],
+// each block 8 gate rows then 8 up rows. A thread takes 4 columns; h has blocks * 8 columns.
 template <typename T>
-__global__ void w4_act_kernel(const float* __restrict__ part, int slices, long long rows, int strips, T* __restrict__ h) {
+__global__ void w4_act_kernel(const float* __restrict__ part, int slices, long long rows, int blocks, T* __restrict__ h) {
   grid_dep_launch();
   grid_dep_wait();
-  const long long n = rows * strips * 2;
+  const long long n = rows * blocks * 2;
   for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
        i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long row = i / (strips * 2);
-    const int c = static_cast<int>(i - row * (strips * 2));  // strip c / 2, its columns 4 (c % 2) ..
+    const long long row = i / (blocks * 2);
+    const int c = static_cast<int>(i - row * (blocks * 2));  // block c / 2, its columns 4 (c % 2) ..
     float4 g = make_float4(0, 0, 0, 0), u = g;
     for (int s = 0; s < slices; ++s) {
-      const float* p = part + (s * rows + row) * (strips * 16ll) + (c >> 1) * 16 + (c & 1) * 4;
+      const float* p = part + (s * rows + row) * (blocks * 16ll) + (c >> 1) * 16 + (c & 1) * 4;
       const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 8);
       g.x += x.x; g.y += x.y; g.z += x.z; g.w += x.w;
       u.x += y.x; u.y += y.y; u.z += y.z; u.w += y.w;
     }
     T o[4] = {W4Type<T>::from_f(w4_silu(g.x) * u.x), W4Type<T>::from_f(w4_silu(g.y) * u.y),
               W4Type<T>::from_f(w4_silu(g.z) * u.z), W4Type<T>::from_f(w4_silu(g.w) * u.w)};
-    *reinterpret_cast<uint2*>(h + row * (strips * 8ll) + c * 4) = *reinterpret_cast<const uint2*>(o);
+    *reinterpret_cast<uint2*>(h + row * (blocks * 8ll) + c * 4) = *reinterpret_cast<const uint2*>(o);
   }
 }
 
@@ -680,12 +683,17 @@ __global__ void w4_combine_kernel(const float* __restrict__ part, int slices, lo
 }
 
 // ------------------------------------------------------------------ layout
-// The row of W that row `r` of strip `s` holds (gate_up: 8 gate rows, then the same 8 of up), or -1.
+// The row of W that row `r` of strip `s` holds, or -1. gate_up: rows 0..7 and 16..23 of a strip are
+// gate rows, the 8 after each the same rows of up.
 __device__ __forceinline__ int w4_row(int s, int r, int N, bool gate_up) {
-  if (!gate_up) return s * 16 + r < N ? s * 16 + r : -1;
-  const int i = s * 8 + (r & 7);
-  return i < N / 2 ? (r < 8 ? i : N / 2 + i) : -1;
+  if (!gate_up) return s * kW4TileRows + r < N ? s * kW4TileRows + r : -1;
+  const int i = s * 16 + (r >> 4) * 8 + (r & 7);
+  return i < N / 2 ? ((r & 8) == 0 ? i : N / 2 + i) : -1;
 }
+// Where a value of a tile lies: lane 4 (row & 7) + q holds columns 32 b + 8 q .. + 7 of block b. Word
+// 2 (b & 1) + step of its 16 bytes [b / 2][row / 16]; nibble h + 2 (i / 2) of the low (even i) or high
+// half, h = row / 8 & 1, i = the column's place among the step's four.
+__device__ __forceinline__ int w4_shift(int h, int i) { return 4 * (h + 2 * (i >> 1)) + 16 * (i & 1); }
 
 // One warp per tile: q [N][ceil(K / 2)] (low half first), scales and zeros [N][ceil(K / group)] of
 // one matrix after another -> records. Rows and columns past the matrix get scale and value 0.
@@ -702,27 +710,27 @@ __global__ void w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __
     const int s = static_cast<int>(t / kt % strips);
     const long long m = t / kt / strips;
     uint8_t* o = out + t * record;
-    for (int half = 0; half < 2; ++half) {
-      uint32_t words[4] = {};
-      for (int block = 0; block < 2; ++block)
-        for (int h = 0; h < 2; ++h) {
-          const int row = w4_row(s, r + 8 * h, N, gate_up);
-          for (int i = 0; i < 8; ++i) {
-            const int c = k * kW4TileK + half * 64 + block * 32 + col + i;
-            if (row < 0 || c >= K) continue;
-            const uint32_t v = (q[(m * N + row) * row_bytes + c / 2] >> (c & 1 ? 4 : 0)) & 15u;
-            // step i / 4; register h + 2 (i % 4 / 2), first or second half
-            words[block * 2 + i / 4] |= v << (4 * (h + 2 * (i % 4 / 2)) + 16 * (i & 1));
+    for (int half = 0; half < 2; ++half)
+      for (int f = 0; f < 2; ++f) {
+        uint32_t words[4] = {};
+        for (int block = 0; block < 2; ++block)
+          for (int h = 0; h < 2; ++h) {
+            const int row = w4_row(s, f * 16 + h * 8 + r, N, gate_up);
+            for (int i = 0; i < 8; ++i) {
+              const int c = k * kW4TileK + half * 64 + block * 32 + col + i;
+              if (row < 0 || c >= K) continue;
+              const uint32_t v = (q[(m * N + row) * row_bytes + c / 2] >> (c & 1 ? 4 : 0)) & 15u;
+              words[block * 2 + i / 4] |= v << w4_shift(h, i % 4);
+            }
           }
-        }
-      *reinterpret_cast<uint4*>(o + half * 512 + lane * 16) = make_uint4(words[0], words[1], words[2], words[3]);
-    }
-    for (int i = lane; i < groups * 16; i += 32) {
-      const int g = k * groups + i / 16, row = w4_row(s, i % 16, N, gate_up);
+        *reinterpret_cast<uint4*>(o + (half * 2 + f) * 512 + lane * 16) = make_uint4(words[0], words[1], words[2], words[3]);
+      }
+    for (int i = lane; i < groups * kW4TileRows; i += 32) {
+      const int g = k * groups + i / kW4TileRows, rr = i % kW4TileRows, row = w4_row(s, rr, N, gate_up);
       const bool in = row >= 0 && g < G;
-      const int at = (i % 16 & 7) * 2 + (i % 16 >> 3);
-      reinterpret_cast<uint16_t*>(o + kW4TileBytes + i / 16 * 32)[at] = in ? scales[(m * N + row) * G + g] : 0;
-      if (zeros) o[kW4TileBytes + groups * 32 + i / 16 * 16 + at] = in ? zeros[(m * N + row) * G + g] & 15 : 0;
+      const int at = (rr & 7) * 4 + (rr >> 3);
+      reinterpret_cast<uint16_t*>(o + kW4TileBytes + i / kW4TileRows * 64)[at] = in ? scales[(m * N + row) * G + g] : 0;
+      if (zeros) o[kW4TileBytes + groups * 64 + i / kW4TileRows * 32 + at] = in ? zeros[(m * N + row) * G + g] & 15 : 0;
     }
   }
 }
@@ -741,25 +749,27 @@ __global__ void w4_unpack_kernel(const uint8_t* __restrict__ w, long long matric
     const int s = static_cast<int>(t / kt % strips);
     const long long m = t / kt / strips;
     const uint8_t* p = w + t * record;
-    for (int half = 0; half < 2; ++half) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + half * 512 + lane * 16);
-      const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-      for (int block = 0; block < 2; ++block) {
-        const int g = (half * 64 + block * 32) / group;
-        for (int h = 0; h < 2; ++h) {
-          const int row = w4_row(s, r + 8 * h, N, gate_up);
-          if (row < 0) continue;
-          const float scale = W4Type<T>::to_f(reinterpret_cast<const uint16_t*>(p + kW4TileBytes + g * 32)[r * 2 + h]);
-          const int z = zeros ? p[kW4TileBytes + groups * 32 + g * 16 + r * 2 + h] : 8;
-          for (int i = 0; i < 8; ++i) {
-            const int c = k * kW4TileK + half * 64 + block * 32 + col + i;
-            if (c >= K) continue;
-            const int n = (words[block * 2 + i / 4] >> (4 * (h + 2 * (i % 4 / 2)) + 16 * (i & 1))) & 15;
-            out[(m * N + row) * K + c] = W4Type<T>::from_f(scale * static_cast<float>(n - z));
+    for (int half = 0; half < 2; ++half)
+      for (int f = 0; f < 2; ++f) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p + (half * 2 + f) * 512 + lane * 16);
+        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+        for (int block = 0; block < 2; ++block) {
+          const int g = (half * 64 + block * 32) / group;
+          for (int h = 0; h < 2; ++h) {
+            const int row = w4_row(s, f * 16 + h * 8 + r, N, gate_up);
+            if (row < 0) continue;
+            const int at = r * 4 + f * 2 + h;
+            const float scale = W4Type<T>::to_f(reinterpret_cast<const uint16_t*>(p + kW4TileBytes + g * 64)[at]);
+            const int z = zeros ? p[kW4TileBytes + groups * 64 + g * 32 + at] : 8;
+            for (int i = 0; i < 8; ++i) {
+              const int c = k * kW4TileK + half * 64 + block * 32 + col + i;
+              if (c >= K) continue;
+              const int n = (words[block * 2 + i / 4] >> w4_shift(h, i % 4)) & 15;
+              out[(m * N + row) * K + c] = W4Type<T>::from_f(scale * static_cast<float>(n - z));
+            }
           }
         }
       }
-    }
   }
 }
 
