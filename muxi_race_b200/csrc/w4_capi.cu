@@ -9,6 +9,7 @@ namespace moe {
 namespace {
 
 constexpr int64_t kMaxSize = int64_t(1) << 24;  // rows, columns and experts stay far inside 32 bits
+constexpr int64_t kMaxStrips = int64_t(1) << 31;  // strips of all token tiles and slices of a call
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
@@ -40,14 +41,17 @@ W4Plan w4_plan(int strips, int64_t K, int group, int tile_rows, double tiles, in
   p.x_pitch = p.slice_kt * 2 * kW4TileK + 64;  // 64: rows r and r + 1 in different banks
   p.x_bytes = static_cast<int>(ceil_div(static_cast<int64_t>(tile_rows) * p.x_pitch, 128) * 128);
   p.start_bytes = p.slice_kt * start_kt;
-  // Warps per strip: few make the sums rare, many give each CTA's groups of warps nearly the same
-  // number of strips. The cost of a choice in tile times: rounds of strips per CTA, each a warp's
-  // tiles and what handing on a sum takes.
-  const double per_cta = tiles * p.slices * strips / sms;
+  // Warps per strip: few make the sums rare, many let a CTA's groups of warps finish together. The
+  // cost of a choice in tile times: the rounds of the worst CTA, each a warp's tiles and what handing
+  // on a sum takes. A CTA whose strips are of two token tiles (or slices) starts a round for each.
+  // (One token, 8 experts, H = 7168: 14 warps a strip instead of 2, in whose second round one or two
+  // groups of 7 work, take the first product from 43 to 30 us.)
+  const int64_t strips_cta = static_cast<int64_t>(std::ceil(tiles * p.slices * strips / sms));
   const int last_kt = p.kt - (p.slices - 1) * p.slice_kt;  // every warp has a tile in every slice
   double best = 0;
   for (int wps = 1; wps <= p.warps && wps <= last_kt; ++wps) {
-    const double rounds = std::ceil(per_cta / (p.warps / wps) - 1e-9);
+    const int64_t groups = p.warps / wps;
+    const int64_t rounds = tiles * p.slices <= 1 || strips_cta < 2 ? ceil_div(strips_cta, groups) : (strips_cta - 2) / groups + 2;
     const double cost = rounds * (static_cast<double>(ceil_div(p.slice_kt, wps)) + kW4SumCost);
     if (p.wps == 0 || cost < best) {
       best = cost;
@@ -124,10 +128,12 @@ W4Args w4_args(const W4Plan& p, const void* w, int64_t expert_bytes, uint32_t* s
   a.strips = p.strips;
   a.kt = p.kt;
   a.wps = p.wps;
+  a.groups = p.warps / p.wps;
+  a.by_wps = w4_div_by(a.wps);
+  a.by_groups = w4_div_by(a.groups);
   a.slices = p.slices;
   a.slice_kt = p.slice_kt;
   a.tile_rows = p.tile_rows;
-  a.gather_div = 1;
   a.x_pitch = p.x_pitch;
   a.x_bytes = p.x_bytes;
   a.start_bytes = p.start_bytes;
@@ -185,7 +191,7 @@ int w4_linear_t(const void* x, int64_t ld_x, const void* packed, void* out, int6
 struct W4MoeLayout {
   W4Plan p1, p2;
   int64_t max_tiles;
-  size_t num_tiles, tiles, sorted, h, part1, part2, total;
+  size_t tiles, sorted, tokens, h, part1, part2, total;
 };
 
 // Rows per tile: an expert of more rows reads its weights once for each tile. 8 rows cost least where
@@ -213,9 +219,9 @@ W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t
     off += pad256(bytes);
     return o;
   };
-  L.num_tiles = take(sizeof(int));
-  L.tiles = take(sizeof(int4) * static_cast<size_t>(L.max_tiles));
+  L.tiles = take(sizeof(int4) * static_cast<size_t>(L.max_tiles + 1));  // the first holds their number
   L.sorted = take(sizeof(int) * static_cast<size_t>(R));
+  L.tokens = take(sizeof(int) * static_cast<size_t>(R));
   L.h = take(2 * static_cast<size_t>(R) * L.p1.strips * (kW4TileRows / 2));
   L.part1 = take(L.p1.slices > 1 ? sizeof(float) * static_cast<size_t>(L.p1.slices) * R * L.p1.strips * kW4TileRows : 0);
   L.part2 = take(sizeof(float) * static_cast<size_t>(L.p2.slices) * R * L.p2.strips * kW4TileRows);
@@ -229,19 +235,19 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
                int64_t E, int64_t topk, const W4MoeLayout& L, uint8_t* ws, int dev, int sms, uint32_t* status,
                cudaStream_t s) {
   const int64_t R = T_ * topk;
-  int* num_tiles = reinterpret_cast<int*>(ws + L.num_tiles);
-  int4* tiles = reinterpret_cast<int4*>(ws + L.tiles);
+  int4* tiles = reinterpret_cast<int4*>(ws + L.tiles) + 1;
   int* sorted = reinterpret_cast<int*>(ws + L.sorted);
+  int* tokens = reinterpret_cast<int*>(ws + L.tokens);
   T* h = reinterpret_cast<T*>(ws + L.h);
   float* part1 = reinterpret_cast<float*>(ws + L.part1);
   float* part2 = reinterpret_cast<float*>(ws + L.part2);
   const int tile_rows = L.p1.tile_rows;
   if (ids_dtype == MOE_I32)
     MOE_TRY(launch(w4_route_kernel<int32_t>, 1, 1024, 0, s, false, static_cast<const int32_t*>(ids), (int)R, (int)E,
-                   tile_rows, sorted, tiles, num_tiles));
+                   (int)topk, tile_rows, sorted, tokens, tiles));
   else
     MOE_TRY(launch(w4_route_kernel<int64_t>, 1, 1024, 0, s, false, static_cast<const int64_t*>(ids), (int)R, (int)E,
-                   tile_rows, sorted, tiles, num_tiles));
+                   (int)topk, tile_rows, sorted, tokens, tiles));
   // first product: x rows of the tokens, gate and up of a column in one thread
   W4Args a = w4_args(L.p1, w13, matrix_bytes(2 * I, H, g13, z13, 1), status);
   a.x = x;
@@ -249,9 +255,7 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
   a.K = static_cast<int>(H);
   a.x_words = in_words(x, ld_x);
   a.tiles = tiles;
-  a.num_tiles = num_tiles;
-  a.gather = sorted;
-  a.gather_div = static_cast<int>(topk);
+  a.gather = tokens;
   a.epilogue = L.p1.slices == 1 ? kW4GateUp : kW4Partial;
   a.out = h;
   a.ld_out = L.p1.strips * (kW4TileRows / 2);
@@ -269,7 +273,6 @@ int fused_w4_t(const void* x, int64_t ld_x, const void* w13, int g13, int z13, c
   b.K = L.p1.strips * (kW4TileRows / 2);
   b.x_words = 1;
   b.tiles = tiles;
-  b.num_tiles = num_tiles;
   b.scatter = sorted;
   b.epilogue = kW4Partial;
   b.part = part2;
@@ -401,6 +404,8 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &status));
   const int tile_rows = linear_tile_rows(M);
+  if (M / tile_rows > kMaxStrips / w4_strips(N, 0) / ceil_div(K, kW4TileK))
+    return fail(MOE_ERR_INVALID_ARG, "too many rows for one call");
   const W4Plan p = w4_plan(w4_strips(N, 0), K, group, tile_rows, ceil_div(M, tile_rows), sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   float* part = static_cast<float*>(workspace);
@@ -438,6 +443,8 @@ int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int 
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &status));
   const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, group2, sms);
+  if (L.max_tiles > kMaxStrips / std::max<int64_t>(L.p1.strips * L.p1.slices, L.p2.strips * L.p2.slices))
+    return fail(MOE_ERR_INVALID_ARG, "too many tokens for one call");
   if (!workspace || workspace_bytes < L.total) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", L.total);
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(MOE_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);

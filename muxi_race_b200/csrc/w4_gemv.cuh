@@ -56,17 +56,16 @@ struct W4Args {
   const uint8_t* w;         // [experts][strips][kt] records
   long long expert_bytes;
   int strips, kt;           // strips, and tiles along K
-  int wps;                  // warps that share a strip
+  int wps, groups;          // warps that share a strip, and strips at a time
+  uint32_t by_wps, by_groups;  // w4_div by these
   int slices, slice_kt;     // K slices whose x fits in shared memory, and their tiles
   const void* x;
   long long ld_x;
   int K;                    // columns of x
   int x_words;              // x can be read in 16-byte words
-  const int4* tiles;        // {expert, first position, rows, -} or null: dense
-  const int* num_tiles;
+  const int4* tiles;        // {expert, first position, rows, -}, tiles[-1].x their number; null: dense
   int rows, tile_rows;      // dense: rows of x, rows per tile
-  const int* gather;        // x row of position p is gather[p] / gather_div, or p
-  int gather_div;
+  const int* gather;        // x row of position p is gather[p], or p
   const int* scatter;       // output row of position p is scatter[p], or p
   int epilogue;
   void* out;                // kW4Out: [row][n]; kW4GateUp: [row][i]
@@ -283,32 +282,36 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, 
   }
 }
 
+// n / d for 0 <= n < 2^24 and 1 <= d <= 16, m = w4_div_by(d).
+__host__ __device__ constexpr uint32_t w4_div_by(int d) { return d == 1 ? 0 : static_cast<uint32_t>(0xffffffffu / d) + 1; }
+__device__ __forceinline__ int w4_div(int n, uint32_t m) { return m == 0 ? n : static_cast<int>(__umulhi(n, m)); }
+
 // The strips of a CTA: an equal run of all (token tile, slice of K, strip), taken in segments of one
 // tile and slice.
 struct W4Segments {
+  int strips, slices;
   int tile, slice, strip, left;  // where the next segment starts, and the strips left in all
   int s0, s1;                    // strips of this segment
-  __device__ __forceinline__ W4Segments(const W4Args& a, int tiles) {
-    const long long per_tile = static_cast<long long>(a.slices) * a.strips;
-    const long long all = tiles * per_tile;
-    const long long u0 = all * blockIdx.x / gridDim.x;
-    left = static_cast<int>(all * (blockIdx.x + 1) / gridDim.x - u0);
-    tile = static_cast<int>(u0 / per_tile);
-    const int in = static_cast<int>(u0 - tile * per_tile);
-    slice = in / a.strips;
-    strip = in - slice * a.strips;
+  __device__ __forceinline__ W4Segments(uint32_t tiles, uint32_t slices_, uint32_t strips_) : strips(strips_), slices(slices_) {
+    const uint32_t all = tiles * slices_ * strips_, each = all / gridDim.x, more = all - each * gridDim.x;
+    const uint32_t u0 = each * blockIdx.x + min(blockIdx.x, more);
+    left = each + (blockIdx.x < more ? 1 : 0);
+    const uint32_t run = u0 / strips_;
+    strip = u0 - run * strips_;
+    tile = slices_ == 1 ? run : run / slices_;
+    slice = run - tile * slices_;
     s0 = s1 = 0;
   }
   // Opens the next segment: its tile and slice are returned.
-  __device__ __forceinline__ bool next(const W4Args& a, int& t, int& s) {
+  __device__ __forceinline__ bool next(int& t, int& s) {
     if (left == 0) return false;
     t = tile;
     s = slice;
     s0 = strip;
-    s1 = min(a.strips, strip + left);
+    s1 = min(strips, strip + left);
     left -= s1 - s0;
     strip = 0;
-    if (++slice == a.slices) {
+    if (++slice == slices) {
       slice = 0;
       ++tile;
     }
@@ -392,38 +395,38 @@ __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP, ZERO
   if (strips < rounds) flush();  // the last round has no strip for this group
 }
 
-// Rows first .. first + rows of x, columns of `kts` tiles from kt0, into shared memory; and for fp16
-// where each group's sums start: per group and pair of rows of x four numbers, -z 2^-24 sum x of the
-// two rows (z = 8, or 1 where the records hold zero points) and 16 times that.
-template <typename T, int GROUP, bool ZEROS, int NTMAX>
+// Rows first .. first + rows of x, columns of `kts` tiles from kt0, on their way into shared memory.
+template <typename T, int NTMAX, int THREADS>
 __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int first, int rows, int kt0, int kts) {
-  constexpr int kThreads = w4_warps(GROUP, NTMAX) * 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k0 = kt0 * kW4TileK, words = kts * (kW4TileK / 8);
+  const int whole = a.x_words ? min(words, (a.K - k0) / 8) : 0;  // 16-byte words that lie in x
   for (int m = 0; m < rows; ++m) {
-    const long long row = a.gather ? a.gather[first + m] / a.gather_div : first + m;
+    const long long row = a.gather ? a.gather[first + m] : first + m;
     const T* src = static_cast<const T*>(a.x) + row * a.ld_x + k0;
     uint8_t* dst = smem + m * a.x_pitch;
-    for (int c = threadIdx.x; c < words; c += kThreads) {
+    int c = threadIdx.x;
+    for (; c < whole; c += THREADS) cp_async_16(smem_u32(dst + c * 16), src + c * 8, 16);
+    for (; c < words; c += THREADS) {
       const int left = a.K - k0 - c * 8;  // columns of x from this word on
-      if (left >= 8 && a.x_words) {
-        cp_async_16(smem_u32(dst + c * 16), src + c * 8, 16);
-      } else {
-        uint16_t e[8];
+      uint16_t e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          e[i] = i < left ? reinterpret_cast<const uint16_t*>(src)[c * 8 + i] : static_cast<uint16_t>(0);
-        *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(e);
-      }
+      for (int i = 0; i < 8; ++i)
+        e[i] = i < left ? reinterpret_cast<const uint16_t*>(src)[c * 8 + i] : static_cast<uint16_t>(0);
+      *reinterpret_cast<uint4*>(dst + c * 16) = *reinterpret_cast<const uint4*>(e);
     }
   }
-  cp_async_wait_all();
-  named_sync(1, kThreads);
-  if constexpr (W4Type<T>::kSums) {
-    constexpr int kLanes = GROUP / 8;  // of a group
-    const int chunks = (words + 31) / 32;
-    for (int i = warp; i < rows * chunks; i += kThreads / 32) {
-      const int m = i / chunks, word = (i - m * chunks) * 32 + lane;
+}
+
+// fp16: where each group's sums start: per group and pair of rows of x four numbers, -z 2^-24 sum x of
+// the two rows (z = 8, or 1 where the records hold zero points) and 16 times that.
+template <typename T, int GROUP, bool ZEROS, int NTMAX, int WARPS>
+__device__ __forceinline__ void w4_starts(const W4Args& a, uint8_t* smem, int rows, int kts) {
+  constexpr int kLanes = GROUP / 8;  // of a group
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int words = kts * (kW4TileK / 8);
+  for (int m = 0; m < rows; ++m)
+    for (int w0 = warp * 32; w0 < words; w0 += WARPS * 32) {
+      const int word = w0 + lane;
       float sum = 0.0f;
       if (word < words) {
         const uint4 v = lds128(smem_u32(smem) + m * a.x_pitch + word * 16);
@@ -443,8 +446,6 @@ __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int fi
         to[2] = start * (W4Type<T>::kScale0 / W4Type<T>::kScale1);
       }
     }
-    named_sync(1, kThreads);
-  }
 }
 
 template <typename T, int GROUP, bool ZEROS, int NTMAX>
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
   constexpr int record = w4_record_bytes(GROUP, ZEROS);
   constexpr int kAhead = w4_ahead(GROUP, NTMAX);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = kWarps / a.wps;
+  const int groups = a.groups;
   const uint32_t base = smem_u32(smem), starts = base + a.x_bytes, sums_at = starts + a.start_bytes;
   constexpr int kSumBytes = kWarps * NTMAX * 1024;  // of all groups, one turn
   if (threadIdx.x == 0) {
@@ -471,7 +472,8 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
   if (!a.early) grid_dep_wait();
   grid_dep_launch();  // after the wait: an early dependent may count on what is complete here
 
-  W4Segments seg(a, a.tiles ? *a.num_tiles : (a.rows + a.tile_rows - 1) / a.tile_rows);
+  const int tiles = a.tiles ? a.tiles[-1].x : (a.rows + a.tile_rows - 1) / a.tile_rows;
+  W4Segments seg(tiles, a.slices, a.strips);
   int tile, slice, expert = 0, first = 0, rows = 0;
   auto open_tile = [&]() {
     if (a.tiles) {
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
     // Store warps: each takes every kW4StoreWarps-th group of warps.
     if (a.early) grid_dep_wait();
     int turn = 0;
-    while (seg.next(a, tile, slice)) {
+    while (seg.next(tile, slice)) {
       open_tile();
       const int out_row = lane < rows ? (a.scatter ? a.scatter[first + lane] : first + lane) : 0;
       const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
@@ -520,30 +522,41 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
     return;
   }
 
-  const int part = warp % a.wps, group = warp / a.wps;
+  const int group = w4_div(warp, a.by_wps), part = warp - group * a.wps;
   W4Sums sums{full + group * 2, empty + group * 2, sums_at + group * a.wps * NTMAX * 1024, kSumBytes, 0};
   W4Stream<GROUP, ZEROS, kAhead> in;
   in.step = static_cast<long long>(a.wps) * record;
   bool fresh = a.early;
-  while (seg.next(a, tile, slice)) {
+  while (seg.next(tile, slice)) {
     open_tile();
     const int kt0 = slice * a.slice_kt, kts = min(a.slice_kt, a.kt - kt0);
     // (warps past the last whole group have no strips)
-    const int rounds = group < groups ? (seg.s1 - seg.s0 + groups - 1) / groups : 0;
-    const int strips = group < groups ? (seg.s1 - seg.s0 - group + groups - 1) / groups : 0;
-    in.nk = in.k = (kts - part + a.wps - 1) / a.wps;
+    const int rounds = group < groups ? w4_div(seg.s1 - seg.s0 + groups - 1, a.by_groups) : 0;
+    const int strips = group < groups ? w4_div(seg.s1 - seg.s0 - group + groups - 1, a.by_groups) : 0;
+    in.nk = in.k = w4_div(kts - part + a.wps - 1, a.by_wps);
     in.strips = strips;
     in.back = -in.nk * in.step;
     in.jump = static_cast<long long>(groups) * a.kt * record + in.back;
     in.p = a.w + expert * a.expert_bytes + (static_cast<long long>(seg.s0 + group) * a.kt + kt0 + part) * record;
-    if (strips > 0)
+    auto load_w = [&]() {
+      if (strips > 0)
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) in.load(j);
-    if (fresh) grid_dep_wait();  // x is the kernel before's
-    fresh = false;
-
+        for (int j = 0; j < kAhead; ++j) in.load(j);
+    };
+    if (fresh) {  // x is the kernel before's: the weights' loads go first
+      load_w();
+      grid_dep_wait();
+    }
     named_sync(1, kWarps * 32);  // all have done with the rows before
-    w4_load_x<T, GROUP, ZEROS, NTMAX>(a, smem, first, rows, kt0, kts);
+    w4_load_x<T, NTMAX, kWarps * 32>(a, smem, first, rows, kt0, kts);
+    if (!fresh) load_w();
+    fresh = false;
+    cp_async_wait_all();
+    named_sync(1, kWarps * 32);
+    if constexpr (W4Type<T>::kSums) {
+      w4_starts<T, GROUP, ZEROS, NTMAX, kWarps>(a, smem, rows, kts);
+      named_sync(1, kWarps * 32);
+    }
     if (NTMAX == 1 || rows <= 8)
       w4_segment<T, GROUP, ZEROS, NTMAX, 1>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
     else if (NTMAX == 2 || rows <= 16)
@@ -555,13 +568,14 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
 }
 
 // ------------------------------------------------------------------ routing, activation, combine
-// Routes by expert, in tiles of at most tile_rows: one CTA. An expert's routes are split evenly over
+// Routes by expert (sorted[p], of token tokens[p]), in tiles of at most tile_rows, their number in
+// tiles[-1].x: one CTA. An expert's routes are split evenly over
 // its tiles; which of its rows a route gets does not matter for the result (a column of the product
 // does not depend on its place). Ids outside [0, E) get no row.
 template <typename IdT>
 __global__ void __launch_bounds__(1024)
-    w4_route_kernel(const IdT* __restrict__ ids, int R, int E, int tile_rows, int* __restrict__ sorted,
-                    int4* __restrict__ tiles, int* __restrict__ num_tiles) {
+    w4_route_kernel(const IdT* __restrict__ ids, int R, int E, int topk, int tile_rows, int* __restrict__ sorted,
+                    int* __restrict__ tokens, int4* __restrict__ tiles) {
   __shared__ int count[1024], next[1024], wsum[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dep_launch();
@@ -609,11 +623,15 @@ __global__ void __launch_bounds__(1024)
     tiles[tile + i] = make_int4(tid, at, size, 0);
     at += size;
   }
-  if (tid == 1023) *num_tiles = tile + nt;
+  if (tid == 1023) tiles[-1].x = tile + nt;
   __syncthreads();
   for (int i = tid; i < R; i += 1024) {
     const long long id = static_cast<long long>(ids[i]);
-    if (id >= 0 && id < E) sorted[atomicAdd(&next[id], 1)] = i;
+    if (id >= 0 && id < E) {
+      const int p = atomicAdd(&next[id], 1);
+      sorted[p] = i;
+      tokens[p] = i / topk;
+    }
   }
 }
 
@@ -655,24 +673,41 @@ __global__ void w4_combine_kernel(const float* __restrict__ part, int slices, lo
     const long long t = i / quads;
     const int c = static_cast<int>(i - t * quads) * 4;
     float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int j = 0; j < topk; ++j) {
-      const long long row = t * topk + j;
-      float w = 1.0f;
-      if (ids) {
-        const long long id = static_cast<long long>(ids[row]);
-        if (id < 0 || id >= E) continue;
-        w = static_cast<float>(weights[row]);
+    // eight routes at a time: their weights first, then their sums, all loads of a kind in flight
+    for (int j0 = 0; j0 < topk; j0 += 8) {
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = j0 + j < topk ? 1.0f : 0.0f;
+        if (ids && j0 + j < topk) w[j] = static_cast<float>(weights[t * topk + j0 + j]);
       }
-      float4 v = make_float4(0, 0, 0, 0);
-      for (int s = 0; s < slices; ++s) {
-        const float4 p = *reinterpret_cast<const float4*>(part + (s * rows + row) * part_ld + c);
-        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+      bool in[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        in[j] = j0 + j < topk;
+        if (ids && in[j]) {
+          const long long id = static_cast<long long>(ids[t * topk + j0 + j]);
+          in[j] = id >= 0 && id < E;
+        }
       }
-      sum.x = fmaf(w, v.x, sum.x);
-      sum.y = fmaf(w, v.y, sum.y);
-      sum.z = fmaf(w, v.z, sum.z);
-      sum.w = fmaf(w, v.w, sum.w);
+      float4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = make_float4(0, 0, 0, 0);
+      for (int s = 0; s < slices; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (in[j]) {
+            const float4 p = *reinterpret_cast<const float4*>(part + (s * rows + t * topk + j0 + j) * part_ld + c);
+            v[j].x += p.x; v[j].y += p.y; v[j].z += p.z; v[j].w += p.w;
+          }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (in[j]) {
+          sum.x = fmaf(w[j], v[j].x, sum.x);
+          sum.y = fmaf(w[j], v[j].y, sum.y);
+          sum.z = fmaf(w[j], v[j].z, sum.z);
+          sum.w = fmaf(w[j], v[j].w, sum.w);
+        }
     }
     T* o = out + t * ld_out + c;
     const float f[4] = {sum.x, sum.y, sum.z, sum.w};

@@ -7,7 +7,7 @@ of tiles that the kernels read.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional
 
 import torch
@@ -27,6 +27,7 @@ class W4Weights:
     group_size: int
     has_zeros: bool
     gate_up: bool         # gate rows and up rows interleaved, for fused_moe_w4
+    sizes: dict = field(default_factory=dict, repr=False, compare=False)  # workspace bytes by rows, asked once each
 
     def nbytes(self) -> int:
         return self.packed.numel()
@@ -119,15 +120,19 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
         raise ValueError(f"x must be {w.dtype} [..., {K}]")
     M = x2.shape[0]
     if out is None:
-        out = torch.empty(x.shape[:-1] + (N,), dtype=w.dtype, device=dev)
+        out = x2.new_empty((*x.shape[:-1], N))
         ld_out = N
     else:
         require(tuple(out.shape) == (*x.shape[:-1], N) and out.dtype == w.dtype, f"out must be {w.dtype} [..., {N}]")
         ld_out = pitch(rows(out, "out", dev))
-    nbytes = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, w.has_zeros)
-    ws = _workspace(("w4_linear", dev, raw_stream(dev.index)), nbytes, dev)
+    nbytes = w.sizes.get(M)
+    if nbytes is None:
+        nbytes = w.sizes[M] = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, w.has_zeros)
+    ws_ptr = None
+    if nbytes:
+        ws_ptr = _workspace(("w4_linear", dev, raw_stream(dev.index)), nbytes, dev).data_ptr()
     launch(dev, "moe_w4_linear", x2.data_ptr(), pitch(x2), w.packed.data_ptr(), out.data_ptr(), ld_out, M, N, K,
-           w.group_size, w.has_zeros, FLOATS[w.dtype], ws.data_ptr(), ws.numel())
+           w.group_size, w.has_zeros, FLOATS[w.dtype], ws_ptr, nbytes)
     return out
 
 
@@ -165,12 +170,15 @@ def fused_moe_w4(
         raise ValueError(f"topk_ids and topk_weights must be contiguous tensors on {dev}")
     k = topk_ids.shape[1]
     if out is None:
-        out = torch.empty((T, H), dtype=w13.dtype, device=dev)
+        out = x.new_empty((T, H))
     else:
         require(tuple(out.shape) == (T, H) and out.dtype == w13.dtype and out.is_contiguous() and out.device == dev, "bad out")
     if T == 0:
         return out
-    nbytes = _lib.lib().moe_fused_w4_workspace_bytes(T, k, E, H, I, w13.group_size, w13.has_zeros, w2.group_size, w2.has_zeros)
+    nbytes = w13.sizes.get((T, k))
+    if nbytes is None:
+        nbytes = w13.sizes[T, k] = _lib.lib().moe_fused_w4_workspace_bytes(
+            T, k, E, H, I, w13.group_size, w13.has_zeros, w2.group_size, w2.has_zeros)
     ws = _workspace(("fused_w4", dev, raw_stream(dev.index)), nbytes, dev)
     launch(dev, "moe_fused_w4", x.data_ptr(), pitch(x), w13.packed.data_ptr(), w13.group_size, w13.has_zeros,
            w2.packed.data_ptr(), w2.group_size, w2.has_zeros, topk_ids.data_ptr(), IDS[topk_ids.dtype],
