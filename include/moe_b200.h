@@ -485,7 +485,7 @@ MOE_API int moe_add_rms_norm_backward(const void* dy, int64_t ld_dy, const void*
  *   gate_up != 0: N = 2I rows, gate then up, for moe_fused_w4's first product.
  *   packed_bytes >= moe_w4_packed_bytes(...), 16-byte aligned. moe_w4_unpack: back to 16 bits.
  * moe_w4_linear: out [M, N] = x [M, K] W^T, row pitches ld_x, ld_out. Sums in fp32. Meant for few rows
- *   (the weights are read once per 32); any M, N, K >= 1.
+ *   (the weights are read once per 16); any M, N, K >= 1.
  * moe_fused_w4: moe_fused with 4-bit w13 (packed with gate_up) and w2; the same sums, h = silu(gate) *
  *   up rounded to dtype in between, the top-k combine in fp32 in route order: the same bits on every
  *   run. Ids outside [0, E) are skipped. Meant for decode batches; any T.
@@ -502,15 +502,14 @@ MOE_API int moe_w4_pack(const void* q, const void* scales, const void* zeros, in
 MOE_API int moe_w4_unpack(const void* packed, int dtype, int64_t matrices, int64_t n, int64_t k, int group, int has_zeros,
                           int gate_up, void* out, void* stream);
 
-MOE_API size_t moe_w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int group, int has_zeros);
+MOE_API size_t moe_w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int group, int dtype);
 
 MOE_API int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, int64_t ld_out, int64_t m, int64_t n,
                           int64_t k, int group, int has_zeros, int dtype, void* workspace, size_t workspace_bytes,
                           void* stream);
 
 MOE_API size_t moe_fused_w4_workspace_bytes(int64_t num_tokens, int64_t topk, int64_t num_experts, int64_t hidden,
-                                            int64_t intermediate, int group13, int has_zeros13, int group2,
-                                            int has_zeros2);
+                                            int64_t intermediate, int group13, int group2, int dtype);
 
 MOE_API int moe_fused_w4(const void* hidden_states, int64_t ld_hidden, const void* w13, int group13, int has_zeros13,
                          const void* w2, int group2, int has_zeros2, const void* topk_ids, int ids_dtype,

@@ -45,7 +45,7 @@ SIGNATURES = {
         _int,
         [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _int, _int, _int, _c_void_p, _size, _c_void_p],
     ),
-    "moe_fused_w4_workspace_bytes": (_size, [_i64] * 5 + [_int] * 4),
+    "moe_fused_w4_workspace_bytes": (_size, [_i64] * 5 + [_int] * 3),
     "moe_fused_w4": (
         _int,
         [_c_void_p, _i64, _c_void_p, _int, _int, _c_void_p, _int, _int, _c_void_p, _int, _c_void_p, _int, _c_void_p]

@@ -25,16 +25,16 @@ constexpr double kW4SumCost = 1.0;
 constexpr int kW4Smem = kMaxDynamicSmem - 1024;  // static shared memory of the kernel, rounded up
 
 // `tiles`: token tiles expected, `sms`: CTAs.
-W4Plan w4_plan(int strips, int64_t K, int group, int tile_rows, double tiles, int sms) {
+W4Plan w4_plan(int strips, int64_t K, int group, int dtype, int tile_rows, double tiles, int sms) {
   W4Plan p{};
   p.strips = strips;
   p.kt = static_cast<int>(ceil_div(K, kW4TileK));
   p.tile_rows = tile_rows;
-  p.nt = tile_rows <= 8 ? 1 : tile_rows <= 16 ? 2 : 4;
+  p.nt = tile_rows <= 8 ? 1 : 2;
   p.warps = w4_warps(group, p.nt);
   p.sum_bytes = 2 * p.warps * p.nt * 1024;
   // K is cut so that the rows' slice of x (and the starts of its sums) fits in shared memory
-  const int start_kt = kW4TileK / group * p.nt * 64;
+  const int start_kt = dtype == MOE_F16 ? kW4TileK / group * p.nt * 64 : 0;
   const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows + start_kt);
   p.slice_kt = static_cast<int>(ceil_div(p.kt, ceil_div(p.kt, most)));
   p.slices = static_cast<int>(ceil_div(p.kt, p.slice_kt));
@@ -103,8 +103,7 @@ int launch_gemv_t(const W4Args& a, size_t smem, int grid, int dev, bool dependen
 template <typename T, int GROUP, bool ZEROS>
 int launch_gemv_z(const W4Args& a, const W4Plan& p, int grid, int dev, bool dependent, cudaStream_t s) {
   if (p.nt == 1) return launch_gemv_t<T, GROUP, ZEROS, 1>(a, p.smem(), grid, dev, dependent, s);
-  if (p.nt == 2) return launch_gemv_t<T, GROUP, ZEROS, 2>(a, p.smem(), grid, dev, dependent, s);
-  return launch_gemv_t<T, GROUP, ZEROS, 4>(a, p.smem(), grid, dev, dependent, s);
+  return launch_gemv_t<T, GROUP, ZEROS, 2>(a, p.smem(), grid, dev, dependent, s);
 }
 
 template <typename T>
@@ -143,7 +142,7 @@ W4Args w4_args(const W4Plan& p, const void* w, int64_t expert_bytes, uint32_t* s
 
 bool in_words(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 
-// Rows of x at a time of a dense product: 32, evenly.
+// Rows of x at a time of a dense product: up to 16, evenly.
 int linear_tile_rows(int64_t M) { return static_cast<int>(ceil_div(M, ceil_div(M, kW4MaxRows))); }
 
 int blocks_for(int64_t items, int threads, int sms) {
@@ -195,23 +194,22 @@ struct W4MoeLayout {
 };
 
 // Rows per tile: an expert of more rows reads its weights once for each tile. 8 rows cost least where
-// the experts have few (one block of the tensor instruction, x of all of K in shared memory); with
-// more rows per expert on average 16, then 32.
+// the experts have few (one block of the tensor instruction); with more on average, 16.
 int moe_tile_rows(int64_t R, int64_t E) {
   const double per_expert = static_cast<double>(R) / static_cast<double>(std::min(E, R));
-  const int rows = per_expert <= 4 ? 8 : per_expert <= 10 ? 16 : kW4MaxRows;
-  return static_cast<int>(std::min<int64_t>(rows, R));
+  return static_cast<int>(std::min<int64_t>(per_expert <= 4 ? 8 : kW4MaxRows, R));
 }
 
-W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int g13, int g2, int sms) {
+W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int g13, int g2, int dtype,
+                          int sms) {
   W4MoeLayout L{};
   const int64_t R = T * topk;
   const int tile_rows = moe_tile_rows(R, E);
   // experts chosen by someone, if all are equally likely
   const double active = static_cast<double>(E) * (1 - std::pow(1 - 1.0 / static_cast<double>(E), static_cast<double>(R)));
   const double tiles = std::max(active, static_cast<double>(R) / tile_rows);
-  L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, tile_rows, tiles, sms);
-  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * (kW4TileRows / 2), g2, tile_rows, tiles, sms);
+  L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, dtype, tile_rows, tiles, sms);
+  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * (kW4TileRows / 2), g2, dtype, tile_rows, tiles, sms);
   L.max_tiles = R / tile_rows + std::min(E, R);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -376,10 +374,10 @@ int moe_w4_unpack(const void* packed, int dtype, int64_t matrices, int64_t N, in
   return MOE_OK;
 }
 
-size_t moe_w4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int has_zeros) {
+size_t moe_w4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int dtype) {
   clear_error();
-  if (M < 1 || check_format(1, N, K, group, 0) != MOE_OK) return 0;
-  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, linear_tile_rows(M), 1, 1);
+  if (M < 1 || M > kMaxSize || check_format(1, N, K, group, 0) != MOE_OK) return 0;
+  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, dtype, linear_tile_rows(M), 1, 1);
   return p.slices == 1 ? 0 : sizeof(float) * static_cast<size_t>(p.slices) * static_cast<size_t>(M) * p.strips * kW4TileRows;
 }
 
@@ -393,7 +391,7 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
   if (!x || !packed || !out) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
   if (ld_x < 0 || ld_out < N) return fail(MOE_ERR_INVALID_ARG, "ld_x must be >= 0 and ld_out >= n");
   if (reinterpret_cast<uintptr_t>(packed) % 16 != 0) return fail(MOE_ERR_ALIGNMENT, "packed must be 16-byte aligned");
-  const size_t need = moe_w4_linear_workspace_bytes(M, N, K, group, has_zeros);
+  const size_t need = moe_w4_linear_workspace_bytes(M, N, K, group, dtype);
   if (need > 0) {
     if (!workspace || workspace_bytes < need) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", need);
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(MOE_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
@@ -406,7 +404,7 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
   const int tile_rows = linear_tile_rows(M);
   if (M / tile_rows > kMaxStrips / w4_strips(N, 0) / ceil_div(K, kW4TileK))
     return fail(MOE_ERR_INVALID_ARG, "too many rows for one call");
-  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, tile_rows, ceil_div(M, tile_rows), sms);
+  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, dtype, tile_rows, ceil_div(M, tile_rows), sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   float* part = static_cast<float*>(workspace);
   return dtype == MOE_F16
@@ -415,11 +413,11 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
                                           s);
 }
 
-size_t moe_fused_w4_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int group13, int has_zeros13,
-                                    int group2, int has_zeros2) {
+size_t moe_fused_w4_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int group13, int group2,
+                                    int dtype) {
   clear_error();
   if (T < 1 || check_moe(T, topk, E, H, I, group13, group2) != MOE_OK) return 0;
-  return w4_moe_layout(T, topk, E, H, I, group13, group2, 1).total;
+  return w4_moe_layout(T, topk, E, H, I, group13, group2, dtype, 1).total;
 }
 
 int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int has_zeros13, const void* w2, int group2,
@@ -442,7 +440,7 @@ int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int 
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &status));
-  const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, group2, sms);
+  const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, group2, dtype, sms);
   if (L.max_tiles > kMaxStrips / std::max<int64_t>(L.p1.strips * L.p1.slices, L.p2.strips * L.p2.slices))
     return fail(MOE_ERR_INVALID_ARG, "too many tokens for one call");
   if (!workspace || workspace_bytes < L.total) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", L.total);

@@ -13,11 +13,11 @@
 //           four 16-byte loads a lane straight into registers, with no shuffles and no shared memory.
 //   strip   the tiles of 32 rows, one after another along K; an expert's strips follow each other.
 // One CTA per SM. Its warps walk through strips with the loads of the next tiles in flight in
-// registers (w4_ahead tiles a warp: 59 to 89 KB an SM); x (at most 32 rows, one slice of K) stays in
+// registers (w4_ahead tiles a warp: 59 to 89 KB an SM); x (at most 16 rows, one slice of K) stays in
 // shared memory. Warps that share a strip split K; their sums go through shared memory to the store
 // warps, which add them up, so that no consumer waits for another or for a store.
 // mma.sync and not tcgen05.mma: the weights must pass the registers to be unpacked, a 32-row strip
-// per warp keeps them there as the A operand, and with at most 32 columns the tensor rate is not
+// per warp keeps them there as the A operand, and with at most 16 columns the tensor rate is not
 // the bound.
 #pragma once
 #include <cuda_bf16.h>
@@ -32,14 +32,13 @@ constexpr int kW4StoreWarps = 2;       // warps that add up the consumers' sums 
 constexpr int kW4TileK = 128;
 constexpr int kW4TileRows = 32;
 constexpr int kW4TileBytes = 2048;     // values of one tile
-constexpr int kW4MaxRows = 32;         // rows of x at a time
-// Consumer warps. With the store warps 16 of 128 registers, 12 of 168 or 8 of 255: with small groups a
-// lane holds more scales and zero points, and with more blocks of rows more sums, and what spills
-// costs more than the warps (17 rows of K = 14336, group 32: 51 us with 6 warps, 75 us with 10; 16 rows
-// of K = 7168, N = 131072, group 128: 125 us with 14, 128 us with 10).
-__host__ __device__ constexpr int w4_warps(int group, int nt) {
-  return nt == 1 || (nt == 2 && group == 128) ? 14 : nt == 2 || group == 128 ? 10 : 6;
-}
+// Rows of x at a time: two blocks of 8. (Four blocks read the weights half as often, but their sums
+// take the registers of the loads ahead and of the other warps: 32 rows of K = 4096, N = 14336 took
+// 51 us in one pass of 32 and take 41 us in two of 16, the second from L2.)
+constexpr int kW4MaxRows = 16;
+// Consumer warps: with the store warps 16 of 128 registers, or 12 of 168 where two blocks of rows meet
+// small groups, whose scales and zero points fill more registers.
+__host__ __device__ constexpr int w4_warps(int group, int nt) { return nt == 2 && group < 128 ? 10 : 14; }
 __host__ __device__ constexpr int w4_threads(int group, int nt) { return (w4_warps(group, nt) + kW4StoreWarps) * 32; }
 
 // tiles that a warp has in flight: as many as its registers hold
@@ -494,7 +493,7 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
     while (seg.next(tile, slice)) {
       open_tile();
       const int out_row = lane < rows ? (a.scatter ? a.scatter[first + lane] : first + lane) : 0;
-      const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+      const int nt = rows <= 8 ? 1 : NTMAX;
       for (int strip0 = seg.s0; strip0 < seg.s1; strip0 += groups, ++turn) {
         for (int g = warp - kWarps; g < groups; g += kW4StoreWarps) {
           const int at = g * 2 + (turn & 1);
@@ -559,10 +558,8 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
     }
     if (NTMAX == 1 || rows <= 8)
       w4_segment<T, GROUP, ZEROS, NTMAX, 1>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
-    else if (NTMAX == 2 || rows <= 16)
-      w4_segment<T, GROUP, ZEROS, NTMAX, NTMAX < 2 ? 1 : 2>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
     else
-      w4_segment<T, GROUP, ZEROS, NTMAX, NTMAX < 4 ? 1 : 4>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
+      w4_segment<T, GROUP, ZEROS, NTMAX, NTMAX>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
   }
   if (fresh) grid_dep_wait();  // a CTA without work: its end must still follow the kernel before
 }

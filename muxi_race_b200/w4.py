@@ -108,7 +108,7 @@ def dequantize_w4(w: W4Weights) -> torch.Tensor:
 def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ W.T`` for a few rows x [..., K] (fp16 / bf16, the dtype of the weight's scales).
 
-    Sums in fp32, rounded once. The weights are read once for up to 32 rows, and again for every 32
+    Sums in fp32, rounded once. The weights are read once for up to 16 rows, and again for every 16
     more: for a prompt, ``torch.matmul`` with :func:`dequantize_w4` is the better call.
     """
     if len(w.shape) != 2 or w.gate_up:
@@ -127,7 +127,7 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
         ld_out = pitch(rows(out, "out", dev))
     nbytes = w.sizes.get(M)
     if nbytes is None:
-        nbytes = w.sizes[M] = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, w.has_zeros)
+        nbytes = w.sizes[M] = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, HALVES[w.dtype])
     ws_ptr = None
     if nbytes:
         ws_ptr = _workspace(("w4_linear", dev, raw_stream(dev.index)), nbytes, dev).data_ptr()
@@ -148,8 +148,8 @@ def fused_moe_w4(
 
     hidden_states [T, H] in the dtype of the scales (rows of any pitch); topk_ids [T, k] int32 / int64,
     ids outside [0, E) are skipped; topk_weights [T, k] fp32 / fp16 / bf16. Meant for decode batches:
-    each chosen expert's weights are read once for up to 8, 16 or 32 of its tokens (more with more
-    tokens per expert). The same bits on every run.
+    each chosen expert's weights are read once for up to 8 of its tokens (16 where the experts have
+    more than 4 on average). The same bits on every run.
     """
     if len(w13.shape) != 3 or not w13.gate_up or len(w2.shape) != 3 or w2.gate_up:
         raise ValueError("w13 must be [E, 2I, H] packed with gate_up, w2 [E, H, I] without")
@@ -178,7 +178,7 @@ def fused_moe_w4(
     nbytes = w13.sizes.get((T, k))
     if nbytes is None:
         nbytes = w13.sizes[T, k] = _lib.lib().moe_fused_w4_workspace_bytes(
-            T, k, E, H, I, w13.group_size, w13.has_zeros, w2.group_size, w2.has_zeros)
+            T, k, E, H, I, w13.group_size, w2.group_size, HALVES[w13.dtype])
     ws = _workspace(("fused_w4", dev, raw_stream(dev.index)), nbytes, dev)
     launch(dev, "moe_fused_w4", x.data_ptr(), pitch(x), w13.packed.data_ptr(), w13.group_size, w13.has_zeros,
            w2.packed.data_ptr(), w2.group_size, w2.has_zeros, topk_ids.data_ptr(), IDS[topk_ids.dtype],
