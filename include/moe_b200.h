@@ -473,6 +473,31 @@ MOE_API int moe_add_rms_norm_backward(const void* dy, int64_t ld_dy, const void*
                                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Routing in its general form, with its gradient (moe_router_topk and moe_router_grouped_topk are its
+ * two fixed forms for contiguous, finite logits).
+ *   scores s = softmax(logits) (scoring 0) or sigmoid(logits) (1) of [T, E] logits, row pitch
+ *   ld_logits >= 0; choice by s + bias (bias [E] fp32 or NULL) among the experts of the topk_group best
+ *   of n_group equal groups, a group's score being the sum of its group_top (1 or 2) best (-inf where
+ *   fewer are eligible); the topk
+ *   largest in descending order, equal ones by the lower id (without bias and groups the order is the
+ *   logits'); topk_weights [T, topk] fp32 = s of the chosen, divided by their sum when renormalize,
+ *   times scale. A logit of -inf is never chosen; a slot without an expert holds id -1, weight 0.
+ *   counts [E] int32 or NULL: tokens per expert.
+ * moe_route_topk_backward: dlogits [T, E] (contiguous, logits' dtype) from dweights [T, topk] fp32 and the
+ *   ids that were chosen (each at most once per token; -1 allowed).
+ * Requirements: 1 <= E <= 1024, 1 <= topk <= min(32, topk_group * E / n_group), 1 <= n_group <= 32,
+ *   E % n_group == 0.
+ * ---------------------------------------------------------------------------------------- */
+MOE_API int moe_route_topk(const void* logits, int64_t ld_logits, int logits_dtype, const float* bias,
+                           int64_t num_tokens, int64_t num_experts, int64_t topk, int scoring, int64_t n_group,
+                           int64_t topk_group, int group_top, int renormalize, float scale, int32_t* topk_ids,
+                           float* topk_weights, int32_t* counts, void* stream);
+
+MOE_API int moe_route_topk_backward(const float* dweights, const void* logits, int64_t ld_logits, int logits_dtype,
+                                    const int32_t* topk_ids, int64_t num_tokens, int64_t num_experts, int64_t topk,
+                                    int scoring, int renormalize, float scale, void* dlogits, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * 4-bit weights with group scales (weights of 16-bit activations; no reference counterpart, the
  * reference's quantised experiments are 8-bit).
  *   W[n, k] = scales[n, g] * (q[n, k] - zeros[n, g]),  g = k / group,  q in 0..15;

@@ -8,6 +8,8 @@ Entry points:
   moe_align(...)       device-side routing metadata
   fused_topk(...)      softmax top-k routing of router logits; fused_moe_router(...) routes + runs
   grouped_topk(...)    group-limited sigmoid routing (DeepSeek-V3 router)
+  route_topk(...)      routing in its general form (softmax / sigmoid, bias, groups, masked experts, counts),
+                       differentiable; route_topk_backward(...) its gradient
   add_rms_norm(...)    norm with the residual's addition; add_rms_norm_quant(...) with int8 / e4m3 rows;
                        add_rms_norm_backward(...) its gradient (add_rms_norm is differentiable)
   quantize_w4(...), pack_w4(...)  4-bit weights with group scales -> W4Weights; dequantize_w4(...) back
@@ -27,12 +29,14 @@ from .fused import (Alignment, clear_workspace_cache, device_status, fused_moe, 
                     quantize_rows_int8)
 from .norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_quant
 from .packed import PackedWeights, fused_moe_packed, pack_weights
+from .route import route_topk, route_topk_backward
 from .submission import run_kernel
 from .w4 import W4Weights, dequantize_w4, fused_moe_w4, pack_w4, quantize_w4, w4_linear
 
 __all__ = [
     "Alignment", "clear_workspace_cache", "device_status", "fused_moe", "fused_moe_fp8", "fused_moe_int8",
     "fused_moe_router", "fused_topk", "grouped_topk", "max_padded_rows", "moe_align", "quantize_rows_fp8", "quantize_rows_int8",
-    "add_rms_norm", "add_rms_norm_backward", "add_rms_norm_quant", "run_kernel", "PackedWeights", "fused_moe_packed", "pack_weights",
+    "add_rms_norm", "add_rms_norm_backward", "add_rms_norm_quant",
+    "route_topk", "route_topk_backward", "run_kernel", "PackedWeights", "fused_moe_packed", "pack_weights",
     "W4Weights", "dequantize_w4", "fused_moe_w4", "pack_w4", "quantize_w4", "w4_linear",
 ]

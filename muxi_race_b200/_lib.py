@@ -36,6 +36,15 @@ SIGNATURES = {
     "moe_set_tile": (_int, [_int, ctypes.c_char_p]),
     "moe_set_a_path": (_int, [ctypes.c_char_p]),
     "moe_set_single_kernel": (_int, [_int]),
+    "moe_route_topk": (
+        _int,
+        [_c_void_p, _i64, _int, _c_void_p, _i64, _i64, _i64, _int, _i64, _i64, _int, _int, ctypes.c_float, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p],
+    ),
+    "moe_route_topk_backward": (
+        _int,
+        [_c_void_p, _c_void_p, _i64, _int, _c_void_p, _i64, _i64, _i64, _int, _int, ctypes.c_float, _c_void_p, _c_void_p],
+    ),
     "moe_w4_quantize": (_int, [_c_void_p, _int, _i64, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "moe_w4_packed_bytes": (_size, [_i64, _i64, _i64, _int, _int, _int]),
     "moe_w4_pack": (_int, [_c_void_p] * 3 + [_i64] * 3 + [_int, _int, _c_void_p, _size, _c_void_p]),

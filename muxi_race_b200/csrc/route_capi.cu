@@ -1,0 +1,140 @@
+// route_capi.cu — host side of moe_route_topk and its gradient (include/moe_b200.h).
+#include "capi_host.h"
+#include "route_topk.cuh"
+
+namespace moe {
+namespace {
+
+int check_route(const RouteArgs& a, int64_t T, int64_t E, int64_t topk, int dtype) {
+  if (dtype != MOE_F32 && dtype != MOE_F16 && dtype != MOE_BF16)
+    return fail(MOE_ERR_INVALID_ARG, "logits must be fp32, fp16 or bf16");
+  if (E < 1 || E > kRouteMaxExperts) return fail(MOE_ERR_INVALID_ARG, "num_experts must be in [1, %d]", kRouteMaxExperts);
+  if (topk < 1 || topk > kRouteMaxTopk || topk > E)
+    return fail(MOE_ERR_INVALID_ARG, "topk must be in [1, min(num_experts, %d)]", kRouteMaxTopk);
+  if (T < 0 || T > (int64_t(1) << 31) - 1) return fail(MOE_ERR_INVALID_ARG, "bad token count");
+  if (a.scoring != kRouteSoftmax && a.scoring != kRouteSigmoid)
+    return fail(MOE_ERR_INVALID_ARG, "scoring must be 0 (softmax) or 1 (sigmoid)");
+  if (a.ld < 0) return fail(MOE_ERR_INVALID_ARG, "ld_logits must be >= 0");
+  return MOE_OK;
+}
+
+constexpr int kRouteBlocksPerSm = 8;  // all warps of an SM
+
+// E up to 32 * VPL experts; four neighbours per load where rows and sizes allow it.
+template <typename LogitT, bool GRAD, int VPL>
+int launch_vpl(const RouteArgs& a, size_t smem, int grid, cudaStream_t s) {
+  constexpr int V = VPL >= 4 ? 4 : 1;
+  constexpr int bytes = V * static_cast<int>(sizeof(LogitT));
+  const bool words = a.E % V == 0 && a.ld % V == 0 && reinterpret_cast<uintptr_t>(a.logits) % bytes == 0 &&
+                     (!GRAD || reinterpret_cast<uintptr_t>(a.dlogits) % bytes == 0);
+  if constexpr (GRAD) {
+    if (words) route_topk_grad_kernel<LogitT, VPL, V><<<grid, kRouteWarps * 32, 0, s>>>(a);
+    else route_topk_grad_kernel<LogitT, VPL, 1><<<grid, kRouteWarps * 32, 0, s>>>(a);
+  } else {
+    if (words) route_topk_kernel<LogitT, VPL, V><<<grid, kRouteWarps * 32, smem, s>>>(a);
+    else route_topk_kernel<LogitT, VPL, 1><<<grid, kRouteWarps * 32, smem, s>>>(a);
+  }
+  MOE_CUDA(cudaGetLastError());
+  return MOE_OK;
+}
+
+template <typename LogitT, bool GRAD>
+int launch_route(const RouteArgs& a, size_t smem, int grid, cudaStream_t s) {
+  if (a.E <= 32) return launch_vpl<LogitT, GRAD, 1>(a, smem, grid, s);
+  if (a.E <= 64) return launch_vpl<LogitT, GRAD, 2>(a, smem, grid, s);
+  if (a.E <= 128) return launch_vpl<LogitT, GRAD, 4>(a, smem, grid, s);
+  if (a.E <= 256) return launch_vpl<LogitT, GRAD, 8>(a, smem, grid, s);
+  if (a.E <= 512) return launch_vpl<LogitT, GRAD, 16>(a, smem, grid, s);
+  return launch_vpl<LogitT, GRAD, 32>(a, smem, grid, s);
+}
+
+template <bool GRAD>
+int launch_route_dtype(const RouteArgs& a, int dtype, size_t smem, int grid, cudaStream_t s) {
+  if (dtype == MOE_F32) return launch_route<float, GRAD>(a, smem, grid, s);
+  if (dtype == MOE_F16) return launch_route<__half, GRAD>(a, smem, grid, s);
+  return launch_route<__nv_bfloat16, GRAD>(a, smem, grid, s);
+}
+
+int route_grid(int64_t T, int* grid) {
+  int dev, sms;
+  MOE_TRY(current_device(&dev));
+  MOE_TRY(device_sms(dev, &sms));
+  const int64_t want = (T + kRouteWarps - 1) / kRouteWarps, most = static_cast<int64_t>(sms) * kRouteBlocksPerSm;
+  *grid = static_cast<int>(want < most ? want : most);
+  return MOE_OK;
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int moe_route_topk(const void* logits, int64_t ld_logits, int logits_dtype, const float* bias, int64_t T, int64_t E,
+                   int64_t topk, int scoring, int64_t n_group, int64_t topk_group, int group_top, int renormalize,
+                   float scale, int32_t* topk_ids, float* topk_weights, int32_t* counts, void* stream) {
+  clear_error();
+  RouteArgs a{};
+  a.logits = logits;
+  a.ld = ld_logits;
+  a.scoring = scoring;
+  MOE_TRY(check_route(a, T, E, topk, logits_dtype));
+  if (n_group < 1 || n_group > kRouteMaxGroups || E % n_group != 0)
+    return fail(MOE_ERR_INVALID_ARG, "num_groups must be in [1, %d] and divide the experts", kRouteMaxGroups);
+  if (topk_group < 1 || topk_group > n_group) return fail(MOE_ERR_INVALID_ARG, "topk_groups must be in [1, num_groups]");
+  if (group_top != 1 && group_top != 2) return fail(MOE_ERR_INVALID_ARG, "group_top must be 1 or 2");
+  if (topk > topk_group * (E / n_group))
+    return fail(MOE_ERR_INVALID_ARG, "topk must be within the experts of topk_groups groups");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    if (counts) MOE_CUDA(cudaMemsetAsync(counts, 0, sizeof(int32_t) * static_cast<size_t>(E), s));
+    return MOE_OK;
+  }
+  if (!logits || !topk_ids || !topk_weights) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  a.bias = bias;
+  a.T = static_cast<int>(T);
+  a.E = static_cast<int>(E);
+  a.topk = static_cast<int>(topk);
+  a.n_group = static_cast<int>(n_group);
+  a.topk_group = static_cast<int>(topk_group);
+  a.group_top = group_top;
+  a.renorm = renormalize != 0;
+  a.scale = scale;
+  a.ids = topk_ids;
+  a.weights = topk_weights;
+  a.counts = counts;
+  int grid;
+  MOE_TRY(route_grid(T, &grid));
+  if (counts && grid > 1) MOE_CUDA(cudaMemsetAsync(counts, 0, sizeof(int32_t) * static_cast<size_t>(E), s));
+  // counts, and each warp's candidates with up to a lane's distance between the groups
+  const size_t smem = (counts ? sizeof(int) * static_cast<size_t>(E) : 0) +
+                      (n_group > 1 ? sizeof(float) * kRouteWarps * (static_cast<size_t>(E) + 32) : 0);
+  return launch_route_dtype<false>(a, logits_dtype, smem, grid, s);
+}
+
+int moe_route_topk_backward(const float* dweights, const void* logits, int64_t ld_logits, int logits_dtype,
+                            const int32_t* topk_ids, int64_t T, int64_t E, int64_t topk, int scoring, int renormalize,
+                            float scale, void* dlogits, void* stream) {
+  clear_error();
+  RouteArgs a{};
+  a.logits = logits;
+  a.ld = ld_logits;
+  a.scoring = scoring;
+  MOE_TRY(check_route(a, T, E, topk, logits_dtype));
+  if (T == 0) return MOE_OK;
+  if (!dweights || !logits || !topk_ids || !dlogits) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  a.T = static_cast<int>(T);
+  a.E = static_cast<int>(E);
+  a.topk = static_cast<int>(topk);
+  a.renorm = renormalize != 0;
+  a.scale = scale;
+  a.dweights = dweights;
+  a.chosen = topk_ids;
+  a.dlogits = dlogits;
+  int grid;
+  MOE_TRY(route_grid(T, &grid));
+  return launch_route_dtype<true>(a, logits_dtype, 0, grid, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

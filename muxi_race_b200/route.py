@@ -1,0 +1,113 @@
+"""Routing of tokens to experts in its general form, differentiable: softmax or sigmoid scores, a
+selection bias, groups, experts that are switched off, strided logits, tokens per expert.
+
+``fused_topk`` and ``grouped_topk`` are the two fixed forms of serving (contiguous finite logits, no
+gradient); :func:`route_topk` covers training and masked experts.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._args import FLOATS, launch, pitch, require, rows
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def _forward(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale, counts):
+    l2 = rows(logits, "logits")
+    require(logits.dim() == 2, "logits must be [T, E]")
+    require(l2.dtype in FLOATS, "logits must be fp32, fp16 or bf16")
+    require(scoring in _SCORING, "scoring must be 'softmax' or 'sigmoid'")
+    T, E = l2.shape
+    dev = l2.device
+    bias_ptr = None
+    if bias is not None:
+        require(bias.device == dev and bias.dtype == torch.float32 and bias.is_contiguous() and tuple(bias.shape) == (E,),
+                f"bias must be a contiguous fp32 tensor [{E}] on {dev}")
+        bias_ptr = bias.data_ptr()
+    ids = l2.new_empty((T, topk), dtype=torch.int32)
+    weights = l2.new_empty((T, topk), dtype=torch.float32)
+    number = l2.new_empty((E,), dtype=torch.int32) if counts else None
+    launch(dev, "moe_route_topk", l2.data_ptr(), pitch(l2), FLOATS[l2.dtype], bias_ptr, T, E, topk, _SCORING[scoring],
+           num_groups, topk_groups, group_top, renormalize, scale, ids.data_ptr(), weights.data_ptr(),
+           None if number is None else number.data_ptr())
+    return weights, ids, number
+
+
+class _RouteTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale, counts):
+        weights, ids, number = _forward(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale,
+                                        counts)
+        ctx.save_for_backward(logits, ids)
+        ctx.how = scoring, renormalize, scale
+        ctx.mark_non_differentiable(ids)
+        if number is not None:
+            ctx.mark_non_differentiable(number)
+        return weights, ids, number
+
+    @staticmethod
+    def backward(ctx, dweights, *_):
+        logits, ids = ctx.saved_tensors
+        scoring, renormalize, scale = ctx.how
+        return (route_topk_backward(dweights, logits, ids, scoring=scoring, renormalize=renormalize, scale=scale),
+                *[None] * 9)
+
+
+def route_topk(
+    logits: torch.Tensor,
+    topk: int,
+    scoring: str = "softmax",
+    bias: Optional[torch.Tensor] = None,
+    num_groups: int = 1,
+    topk_groups: int = 1,
+    group_top: int = 2,
+    renormalize: bool = True,
+    scale: float = 1.0,
+    return_counts: bool = False,
+):
+    """``(topk_weights [T, k] fp32, topk_ids [T, k] int32)``, and with ``return_counts`` the number of
+    tokens of each expert ([E] int32).
+
+    logits [T, E] fp32 / fp16 / bf16, rows of any pitch. Scores are ``softmax(logits)`` or
+    ``sigmoid(logits)``; the ``topk`` largest ``score + bias`` are chosen (bias [E] fp32, for balance:
+    it moves the choice only) among the experts of the ``topk_groups`` best of ``num_groups`` groups,
+    a group counting the sum of its ``group_top`` (1 or 2) best (-inf where fewer are eligible). Ids come in descending order, equal
+    ones by the lower id; weights are the chosen scores, divided by their sum when ``renormalize``,
+    times ``scale``. An expert whose logit is -inf is never chosen; slots left without one hold id -1
+    (which the expert operators skip) and weight 0. The weights are differentiable in the logits.
+    """
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out = _RouteTopk.apply(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale,
+                               return_counts)
+    else:
+        out = _forward(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale, return_counts)
+    return out if return_counts else out[:2]
+
+
+def route_topk_backward(
+    dweights: torch.Tensor,
+    logits: torch.Tensor,
+    topk_ids: torch.Tensor,
+    scoring: str = "softmax",
+    renormalize: bool = True,
+    scale: float = 1.0,
+) -> torch.Tensor:
+    """Gradient of :func:`route_topk`'s weights for the logits ([T, E], the logits' dtype), given the
+    ids that it chose (each expert at most once per token)."""
+    l2 = rows(logits, "logits")
+    require(logits.dim() == 2 and l2.dtype in FLOATS, "logits must be fp32, fp16 or bf16 [T, E]")
+    require(scoring in _SCORING, "scoring must be 'softmax' or 'sigmoid'")
+    T, E = l2.shape
+    dev = l2.device
+    require(topk_ids.device == dev and topk_ids.dtype == torch.int32 and topk_ids.is_contiguous() and topk_ids.dim() == 2
+            and topk_ids.shape[0] == T, "topk_ids must be a contiguous int32 tensor [T, k] on the logits' device")
+    require(dweights.shape == topk_ids.shape and dweights.dtype == torch.float32 and dweights.device == dev,
+            "dweights must be an fp32 tensor of topk_ids' shape")
+    dweights = dweights.contiguous()
+    out = l2.new_empty((T, E))
+    launch(dev, "moe_route_topk_backward", dweights.data_ptr(), l2.data_ptr(), pitch(l2), FLOATS[l2.dtype],
+           topk_ids.data_ptr(), T, E, topk_ids.shape[1], _SCORING[scoring], renormalize, scale, out.data_ptr())
+    return out

@@ -103,3 +103,58 @@ def router_grouped_ref(logits: torch.Tensor, topk: int, n_group: int, topk_group
         ggap = torch.where((ggap == 0) & same, inf, ggap)
     margins = torch.minimum(ggap / gsorted[:, 0].abs().clamp_min(1e-30), cgap / csorted[:, 0].abs().clamp_min(1e-30))
     return w.contiguous(), torch.from_numpy(np.ascontiguousarray(ids)), margins
+
+
+def route_scores64(logits: torch.Tensor, scoring: str) -> torch.Tensor:
+    """fp64 scores of the general router; an expert whose logit is -inf scores 0."""
+    l = logits.double()
+    if scoring == "sigmoid":
+        return torch.sigmoid(l)
+    m = l.amax(-1, keepdim=True)
+    e = torch.exp(l - torch.where(torch.isinf(m), torch.zeros_like(m), m))
+    return e / e.sum(-1, keepdim=True).clamp_min(1e-300)
+
+
+def route_topk_ref(logits, topk, scoring, bias=None, num_groups=1, topk_groups=1, group_top=2, renormalize=True,
+                   scale=1.0):
+    """(topk_weights fp64, topk_ids int64 with -1 for empty slots, sure): the general router from its
+    definition in fp64. ``sure`` [T]: no two candidates that the choice or its order hangs on are nearer
+    than 1e-5 of their value (equal ones are taken by the lower id and are sure)."""
+    T, E = logits.shape
+    l = logits.double()
+    s = route_scores64(logits, scoring)
+    plain = bias is None and num_groups == 1
+    c = l.clone() if plain else s + (0.0 if bias is None else bias.double())
+    c[l == -float("inf")] = -float("inf")
+    sure = torch.ones(T, dtype=torch.bool, device=logits.device)
+
+    def near(v):
+        gap = v[:, :-1] - v[:, 1:]
+        return ((gap > 0) & (gap < 1e-5 * v[:, :-1].abs().clamp_min(1e-3))).any(-1)
+
+    if num_groups > 1:
+        g = c.view(T, num_groups, -1).sort(dim=-1, descending=True).values[..., :group_top].sum(-1)
+        v, order = g.sort(dim=-1, descending=True, stable=True)
+        sure &= ~near(v[:, :topk_groups + 1])
+        keep = torch.zeros_like(g, dtype=torch.bool).scatter_(1, order[:, :topk_groups], True)
+        c[~keep.repeat_interleave(E // num_groups, 1)] = -float("inf")
+    v, ids = c.sort(dim=-1, descending=True, stable=True)
+    if not plain:
+        sure &= ~near(v[:, :topk + 1])
+    ids = torch.where(v == -float("inf"), -1, ids)[:, :topk]
+    return route_weights64(logits, ids, scoring, renormalize, scale), ids, sure
+
+
+def route_weights64(logits, ids, scoring, renormalize, scale):
+    """fp64 weights of the chosen ids; differentiable in the logits. (The renormalised softmax is
+    taken over the chosen logits themselves: the gradient of the others is 0, not a cancellation.)"""
+    there = ids >= 0
+    zero = torch.zeros((), dtype=torch.float64, device=logits.device)
+    at = ids.clamp_min(0).long()
+    if scoring == "softmax" and renormalize:
+        chosen = logits.double().gather(1, at)
+        return route_scores64(torch.where(there, chosen, torch.full_like(chosen, -float("inf"))), "softmax") * scale
+    w = torch.where(there, route_scores64(logits, scoring).gather(1, at), zero)
+    if renormalize:
+        w = w / w.sum(-1, keepdim=True).clamp_min(1e-290)
+    return w * scale
