@@ -18,50 +18,52 @@ int check_route(const RouteArgs& a, int64_t T, int64_t E, int64_t topk, int dtyp
   return MOE_OK;
 }
 
-constexpr int kRouteBlocksPerSm = 8;  // all warps of an SM
+constexpr int kRouteWarpsPerSm = 64;
 
 // E up to 32 * VPL experts; four neighbours per load where rows and sizes allow it.
 template <typename LogitT, bool GRAD, int VPL>
-int launch_vpl(const RouteArgs& a, size_t smem, int grid, cudaStream_t s) {
+int launch_vpl(const RouteArgs& a, int sms, cudaStream_t s) {
   constexpr int V = VPL >= 4 ? 4 : 1;
   constexpr int bytes = V * static_cast<int>(sizeof(LogitT));
+  constexpr int warps = GRAD ? kRouteGradWarps : route_warps(VPL);
   const bool words = a.E % V == 0 && a.ld % V == 0 && reinterpret_cast<uintptr_t>(a.logits) % bytes == 0 &&
                      (!GRAD || reinterpret_cast<uintptr_t>(a.dlogits) % bytes == 0);
+  const int want = (a.T - 1) / warps + 1, most = sms * (kRouteWarpsPerSm / warps);
+  const int grid = want < most ? want : most;
   if constexpr (GRAD) {
-    if (words) route_topk_grad_kernel<LogitT, VPL, V><<<grid, kRouteWarps * 32, 0, s>>>(a);
-    else route_topk_grad_kernel<LogitT, VPL, 1><<<grid, kRouteWarps * 32, 0, s>>>(a);
+    if (words) route_topk_grad_kernel<LogitT, VPL, V><<<grid, warps * 32, 0, s>>>(a);
+    else route_topk_grad_kernel<LogitT, VPL, 1><<<grid, warps * 32, 0, s>>>(a);
   } else {
-    if (words) route_topk_kernel<LogitT, VPL, V><<<grid, kRouteWarps * 32, smem, s>>>(a);
-    else route_topk_kernel<LogitT, VPL, 1><<<grid, kRouteWarps * 32, smem, s>>>(a);
+    if (a.counts && grid > 1) MOE_CUDA(cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * static_cast<size_t>(a.E), s));
+    const size_t smem = sizeof(uint2) * warps * (static_cast<size_t>(a.E) + 32) + (a.counts ? sizeof(int) * a.E : 0);
+    const bool scored = a.bias || a.n_group > 1;
+    if (words && scored) route_topk_kernel<LogitT, VPL, V, true><<<grid, warps * 32, smem, s>>>(a);
+    else if (words) route_topk_kernel<LogitT, VPL, V, false><<<grid, warps * 32, smem, s>>>(a);
+    else if (scored) route_topk_kernel<LogitT, VPL, 1, true><<<grid, warps * 32, smem, s>>>(a);
+    else route_topk_kernel<LogitT, VPL, 1, false><<<grid, warps * 32, smem, s>>>(a);
   }
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
 
 template <typename LogitT, bool GRAD>
-int launch_route(const RouteArgs& a, size_t smem, int grid, cudaStream_t s) {
-  if (a.E <= 32) return launch_vpl<LogitT, GRAD, 1>(a, smem, grid, s);
-  if (a.E <= 64) return launch_vpl<LogitT, GRAD, 2>(a, smem, grid, s);
-  if (a.E <= 128) return launch_vpl<LogitT, GRAD, 4>(a, smem, grid, s);
-  if (a.E <= 256) return launch_vpl<LogitT, GRAD, 8>(a, smem, grid, s);
-  if (a.E <= 512) return launch_vpl<LogitT, GRAD, 16>(a, smem, grid, s);
-  return launch_vpl<LogitT, GRAD, 32>(a, smem, grid, s);
+int launch_route(const RouteArgs& a, int sms, cudaStream_t s) {
+  if (a.E <= 32) return launch_vpl<LogitT, GRAD, 1>(a, sms, s);
+  if (a.E <= 64) return launch_vpl<LogitT, GRAD, 2>(a, sms, s);
+  if (a.E <= 128) return launch_vpl<LogitT, GRAD, 4>(a, sms, s);
+  if (a.E <= 256) return launch_vpl<LogitT, GRAD, 8>(a, sms, s);
+  if (a.E <= 512) return launch_vpl<LogitT, GRAD, 16>(a, sms, s);
+  return launch_vpl<LogitT, GRAD, 32>(a, sms, s);
 }
 
 template <bool GRAD>
-int launch_route_dtype(const RouteArgs& a, int dtype, size_t smem, int grid, cudaStream_t s) {
-  if (dtype == MOE_F32) return launch_route<float, GRAD>(a, smem, grid, s);
-  if (dtype == MOE_F16) return launch_route<__half, GRAD>(a, smem, grid, s);
-  return launch_route<__nv_bfloat16, GRAD>(a, smem, grid, s);
-}
-
-int route_grid(int64_t T, int* grid) {
+int launch_route_dtype(const RouteArgs& a, int dtype, cudaStream_t s) {
   int dev, sms;
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
-  const int64_t want = (T + kRouteWarps - 1) / kRouteWarps, most = static_cast<int64_t>(sms) * kRouteBlocksPerSm;
-  *grid = static_cast<int>(want < most ? want : most);
-  return MOE_OK;
+  if (dtype == MOE_F32) return launch_route<float, GRAD>(a, sms, s);
+  if (dtype == MOE_F16) return launch_route<__half, GRAD>(a, sms, s);
+  return launch_route<__nv_bfloat16, GRAD>(a, sms, s);
 }
 
 }  // namespace
@@ -104,13 +106,7 @@ int moe_route_topk(const void* logits, int64_t ld_logits, int logits_dtype, cons
   a.ids = topk_ids;
   a.weights = topk_weights;
   a.counts = counts;
-  int grid;
-  MOE_TRY(route_grid(T, &grid));
-  if (counts && grid > 1) MOE_CUDA(cudaMemsetAsync(counts, 0, sizeof(int32_t) * static_cast<size_t>(E), s));
-  // counts, and each warp's candidates with up to a lane's distance between the groups
-  const size_t smem = (counts ? sizeof(int) * static_cast<size_t>(E) : 0) +
-                      (n_group > 1 ? sizeof(float) * kRouteWarps * (static_cast<size_t>(E) + 32) : 0);
-  return launch_route_dtype<false>(a, logits_dtype, smem, grid, s);
+  return launch_route_dtype<false>(a, logits_dtype, s);
 }
 
 int moe_route_topk_backward(const float* dweights, const void* logits, int64_t ld_logits, int logits_dtype,
@@ -132,9 +128,7 @@ int moe_route_topk_backward(const float* dweights, const void* logits, int64_t l
   a.dweights = dweights;
   a.chosen = topk_ids;
   a.dlogits = dlogits;
-  int grid;
-  MOE_TRY(route_grid(T, &grid));
-  return launch_route_dtype<true>(a, logits_dtype, 0, grid, static_cast<cudaStream_t>(stream));
+  return launch_route_dtype<true>(a, logits_dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -15,11 +15,12 @@
 //   softmax                 dl_e = (g_e p_e at the chosen) - p_e sum g p
 //   sigmoid                 dl_j = d_j s_j (1 - s_j), d = g, renormalised (g - sum g s / D) / D, D = sum s
 //
-// One warp per token, its logits in registers. A lane keeps its best and second-best candidate; each
-// of the topk rounds is two warp reductions (the largest key, then the lowest id that has it) and one
-// step of the winner, which scans its logits again only when it has won twice since. The work is a
-// read of T * E logits; what bounds it is that scan and the exponentials (about 300 instructions a
-// token at E = 256, topk = 8).
+// One warp per token, its logits in registers. The topk-th largest of the 32 lanes' own maxima is a
+// lower bound of the topk-th largest of all, and few candidates reach it (about 10 for topk = 8 of 256):
+// those go to shared memory, and each counts how many are before it. The
+// next token's logits are loaded meanwhile. T = 32768, E = 256, topk = 8: 22 us, against 34 us with topk
+// rounds of a warp-wide maximum; the 33.5 MB of logits take 5 us, the instructions and the latencies of
+// the steps bound it. The gradient writes (and, softmax, reads) those bytes: 13 us for 67 MB.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,7 +28,9 @@
 
 namespace moe {
 
-constexpr int kRouteWarps = 8;
+// warps of a block; their candidates (8 bytes for each expert) stay within 32 KB
+__host__ __device__ constexpr int route_warps(int vpl) { return vpl > 16 ? 4 : 8; }
+constexpr int kRouteGradWarps = 8;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
 constexpr int kRouteMaxGroups = 32;
@@ -56,17 +59,15 @@ __device__ __forceinline__ void route_set(float& o, float v) { o = v; }
 __device__ __forceinline__ void route_set(__half& o, float v) { o = __float2half_rn(v); }
 __device__ __forceinline__ void route_set(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
 
-// Order-preserving image of a candidate's value: 0 for -inf (never chosen), the largest for NaN;
-// -0 and +0 are equal.
+// Order-preserving image of a value: -0 and +0 alike, any NaN above everything. Keys up to kRouteNone
+// (that of -inf) are never chosen.
+constexpr uint32_t kRouteNone = 0x007fffffu;
 __device__ __forceinline__ uint32_t route_key(float v) {
-  const uint32_t u = __float_as_uint(v + 0.0f);
-  if (v != v) return 0xffffffffu;
-  if (u == 0xff800000u) return 0u;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint(v + 0.0f);  // the sum of a NaN is the positive one
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float route_unkey(uint32_t k) {
-  if (k == 0u) return -INFINITY;
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);  // the key of NaN is a NaN again
+  return __uint_as_float(k ^ (static_cast<uint32_t>(static_cast<int32_t>(~k) >> 31) | 0x80000000u));
 }
 __device__ __forceinline__ float route_sum(float v) {
 #pragma unroll
@@ -96,70 +97,120 @@ __device__ __forceinline__ void route_load(const LogitT* row, int E, int lane, f
   }
 }
 
-// The largest logit (0 where all are -inf, so that the exponentials are 0) and the sum of exp(l - m).
+// m: the largest logit (0 where all are -inf, so that the exponentials are 0); e = exp(l - m) and their
+// sum. (A NaN is passed over for m and shows in the sum.)
 template <int VPL>
-__device__ __forceinline__ void route_softmax(const float (&l)[VPL], float& m, float& sum) {
-  uint32_t k = 0u;
+__device__ __forceinline__ void route_softmax(const float (&l)[VPL], float& m, float (&e)[VPL], float& sum) {
+  m = l[0];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) k = max(k, route_key(l[i]));
-  k = __reduce_max_sync(kAllLanes, k);
-  m = k == 0u ? 0.0f : route_unkey(k);
+  for (int i = 1; i < VPL; ++i) m = fmaxf(m, l[i]);
+  m = route_unkey(__reduce_max_sync(kAllLanes, route_key(m == m ? m : -INFINITY)));
+  if (m == -INFINITY) m = 0.0f;
   sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) sum += expf(l[i] - m);
-  sum = fmaxf(route_sum(sum), 1e-30f);
+  for (int i = 0; i < VPL; ++i) {
+    e[i] = expf(l[i] - m);
+    sum += e[i];
+  }
+  sum = route_sum(sum);
+  if (sum < 1e-30f) sum = 1e-30f;
 }
 
-template <typename LogitT, int VPL, int VEC>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_topk_kernel(const RouteArgs a) {
-  extern __shared__ int route_smem[];  // [E] counts, then per warp its candidates by group
+// The 32 lanes' values in descending order, lane 0 first (a bitonic network).
+__device__ __forceinline__ uint32_t route_sort(uint32_t v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+    for (int j = k / 2; j > 0; j /= 2) {
+      const uint32_t o = __shfl_xor_sync(kAllLanes, v, j);
+      v = ((lane & j) == 0) == ((lane & k) == 0) ? max(v, o) : min(v, o);
+    }
+  return v;
+}
+
+// SCORED: the choice needs the scores (a bias or groups), not the logits' order alone.
+template <typename LogitT, int VPL, int VEC, bool SCORED>
+__global__ void __launch_bounds__(route_warps(VPL) * 32, VPL <= 8 ? 4 : 1) route_topk_kernel(const RouteArgs a) {
+  constexpr int kWarps = route_warps(VPL);
+  extern __shared__ uint2 route_smem[];  // per warp its candidates, or their scores by group; [E] counts
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gsz = a.E / a.n_group;
-  // lanes per group, and the distance of the groups' candidates in shared memory (other banks)
+  // lanes per group, and the distance of the groups' scores in shared memory (other banks)
   int per_group = 1;
   while (per_group * 2 * a.n_group <= 32) per_group *= 2;
   const int pitch = gsz + per_group;
-  int* hist = route_smem;
-  float* cand = reinterpret_cast<float*>(route_smem + (a.counts ? a.E : 0)) + warp * a.n_group * pitch;
+  uint2* cand = route_smem + warp * (a.E + 32);
+  uint32_t* by_group = reinterpret_cast<uint32_t*>(cand);
+  int* hist = reinterpret_cast<int*>(route_smem + kWarps * (a.E + 32));
   if (a.counts) {
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
     __syncthreads();
   }
-  const bool scored = a.bias || a.n_group > 1;  // the choice needs the scores, not the logits' order alone
-  for (long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp; t < a.T;
-       t += static_cast<long long>(gridDim.x) * kRouteWarps) {
-    const LogitT* row = static_cast<const LogitT*>(a.logits) + t * a.ld;
+  const LogitT* logits = static_cast<const LogitT*>(a.logits);
+  const long long step = static_cast<long long>(gridDim.x) * kWarps;
+  constexpr bool kAhead = VPL <= 8;  // the next token's logits are on their way during this one
+  float next[VPL];
+  long long t = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  if (kAhead && t < a.T) route_load<LogitT, VPL, VEC>(logits + t * a.ld, a.E, lane, next);
+  for (; t < a.T; t += step) {
+    const LogitT* row = logits + t * a.ld;
     float l[VPL];
-    route_load<LogitT, VPL, VEC>(row, a.E, lane, l);
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) l[i] = next[i];
+      if (t + step < a.T) route_load<LogitT, VPL, VEC>(row + step * a.ld, a.E, lane, next);
+    } else {
+      route_load<LogitT, VPL, VEC>(row, a.E, lane, l);
+    }
     float m = 0.0f, sum = 1.0f;
-    if (a.scoring == kRouteSoftmax && (scored || !a.renorm)) route_softmax<VPL>(l, m, sum);
     uint32_t key[VPL];
-    if (scored) {
-      const float inv = 1.0f / sum;
+    if constexpr (!SCORED) {
+      if (a.scoring == kRouteSoftmax && !a.renorm) {
+        float ex[VPL];
+        route_softmax<VPL>(l, m, ex, sum);
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) key[i] = route_key(l[i]);
+    } else {
+      float c[VPL];
+      if (a.scoring == kRouteSoftmax) {
+        route_softmax<VPL>(l, m, c, sum);
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) c[i] *= inv;
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) c[i] = route_sigmoid(l[i]);
+      }
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const int e = route_expert<VEC>(i, lane);
-        float c = a.scoring == kRouteSoftmax ? expf(l[i] - m) * inv : route_sigmoid(l[i]);
-        if (a.bias && e < a.E) c += __ldg(a.bias + e);
-        key[i] = l[i] == -INFINITY ? 0u : route_key(c);
+        if (a.bias && e < a.E) c[i] += __ldg(a.bias + e);
+        key[i] = l[i] == -INFINITY ? kRouteNone : route_key(c[i]);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = route_key(l[i]);
     }
-    if (a.n_group > 1) {
-      __syncwarp();  // the last token's candidates have been read
+    __syncwarp();  // the last token's candidates have been read
+    if (SCORED && a.n_group > 1) {
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
+      for (int i = 0; i < VPL; i += VEC) {
         const int e = route_expert<VEC>(i, lane), g = e / gsz;
-        if (e < a.E) cand[e + g * per_group] = route_unkey(key[i]);
+        int ge = g, left = (g + 1) * gsz - e;  // this entry's group, and its experts from here on
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if (left == 0) {
+            ++ge;
+            left = gsz;
+          }
+          if (e + j < a.E) by_group[e + j + ge * per_group] = key[i + j];
+          --left;
+        }
       }
       __syncwarp();
       const int g = lane / per_group;
-      uint32_t k1 = 0u, k2 = 0u;  // the two best of this lane's part of its group
+      uint32_t k1 = kRouteNone, k2 = kRouteNone;  // the two best of this lane's part of its group
       if (g < a.n_group)
         for (int j = lane % per_group; j < gsz; j += per_group) {
-          const uint32_t k = route_key(cand[g * pitch + j]);
+          const uint32_t k = by_group[g * pitch + j];
           k2 = max(k2, min(k1, k));
           k1 = max(k1, k);
         }
@@ -178,59 +229,63 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_topk_kernel(const Rout
       }
       const uint32_t in = __ballot_sync(kAllLanes, g < a.n_group && rank < a.topk_group);
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int e = route_expert<VEC>(i, lane);
-        if (e < a.E && !((in >> (e / gsz * per_group)) & 1u)) key[i] = 0u;
+      for (int i = 0; i < VPL; i += VEC) {
+        const int e = route_expert<VEC>(i, lane), ge = e / gsz;
+        int at = ge * per_group, left = (ge + 1) * gsz - e;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if (left == 0) {
+            at += per_group;
+            left = gsz;
+          }
+          if (e + j < a.E && !((in >> at) & 1u)) key[i + j] = kRouteNone;
+          --left;
+        }
       }
+      __syncwarp();  // the groups' scores have been read
     }
-    // this lane's best and second best; equal keys in ascending order of their ids
-    uint32_t taken = 0u, best = 0u, second = 0u;
-    int at = 0, at2 = 0;
-    bool known = true;  // `second` is what its name says
-    auto scan = [&]() {
-      best = second = 0u;
-      at = at2 = 0;
-      known = true;
+    // the candidates that reach the topk-th largest of the lanes' maxima
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) best = max(best, key[i]);
+    const uint32_t least = max(__shfl_sync(kAllLanes, route_sort(best, lane), a.topk - 1), kRouteNone + 1);
+    int n = 0;
+    if (__any_sync(kAllLanes, best >= least)) {
+      const uint32_t below = (1u << lane) - 1u;
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
-        const uint32_t k = (taken >> i) & 1u ? 0u : key[i];
-        if (k > best) {
-          second = best;
-          at2 = at;
-          best = k;
-          at = i;
-        } else if (k > second) {
-          second = k;
-          at2 = i;
-        }
-      }
-    };
-    scan();
-    int my_e = -1;
-    for (int j = 0; j < a.topk; ++j) {
-      const uint32_t top = __reduce_max_sync(kAllLanes, best);
-      if (top == 0u) break;
-      const uint32_t own = best == top ? static_cast<uint32_t>(route_expert<VEC>(at, lane)) : 0xffffffffu;
-      const uint32_t e = __reduce_min_sync(kAllLanes, own);
-      if (lane == j) my_e = static_cast<int>(e);
-      if (own == e) {
-        taken |= 1u << at;
-        if (known) {
-          best = second;
-          at = at2;
-          known = false;
-          second = 0u;
-        } else {
-          scan();
-        }
+        const bool in = key[i] >= least;
+        const uint32_t mask = __ballot_sync(kAllLanes, in);
+        // the second half orders equal keys: a lower expert is larger
+        if (in) cand[n + __popc(mask & below)] = make_uint2(~static_cast<uint32_t>(route_expert<VEC>(i, lane)), key[i]);
+        n += __popc(mask);
       }
     }
+    __syncwarp();
+    // where each stands among them; the place of the topk first in the order of their rank
+    uint2* chosen = cand + a.E;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      const uint2 mine = i < n ? cand[i] : make_uint2(0u, 0u);
+      int rank = 0;
+#pragma unroll 4
+      for (int o = 0; o < n; ++o) {
+        const uint2 other = cand[o];
+        rank += other.y > mine.y || (other.y == mine.y && other.x > mine.x);
+      }
+      if (i < n && rank < a.topk) chosen[rank] = mine;
+    }
+    __syncwarp();
+    const bool have = lane < a.topk && lane < n;
+    const uint2 mine = have ? chosen[lane] : make_uint2(0u, kRouteNone);
+    const int my_e = have ? static_cast<int>(~mine.x) : -1;
+    float v = route_unkey(mine.y);  // its logit, where the choice went by the logits
+    if (SCORED && have) v = route_f(row[my_e]);
     float w = 0.0f;
     if (a.scoring == kRouteSoftmax) {
-      const float v = my_e >= 0 ? route_f(row[my_e]) : -INFINITY;
       if (a.renorm) {
-        const uint32_t k = __reduce_max_sync(kAllLanes, route_key(v));
-        m = k == 0u ? 0.0f : route_unkey(k);
+        m = route_unkey(__reduce_max_sync(kAllLanes, route_key(v)));
+        if (m == -INFINITY) m = 0.0f;
         w = my_e >= 0 ? expf(v - m) : 0.0f;
         sum = fmaxf(route_sum(w), 1e-30f);
         w /= sum;
@@ -238,7 +293,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_topk_kernel(const Rout
         w = expf(v - m) / sum;
       }
     } else {
-      w = my_e >= 0 ? route_sigmoid(route_f(row[my_e])) : 0.0f;
+      w = my_e >= 0 ? route_sigmoid(v) : 0.0f;
       if (a.renorm) {
         const float d = route_sum(w);
         w /= d < kRouteLeast ? kRouteLeast : d;  // NaN stays
@@ -260,12 +315,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_topk_kernel(const Rout
 }
 
 template <typename LogitT, int VPL, int VEC>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_topk_grad_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(kRouteGradWarps * 32) route_topk_grad_kernel(const RouteArgs a) {
   struct alignas(sizeof(LogitT) * VEC) Pack { LogitT v[VEC]; };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool dense = a.scoring == kRouteSoftmax && !a.renorm;
-  for (long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + warp; t < a.T;
-       t += static_cast<long long>(gridDim.x) * kRouteWarps) {
+  for (long long t = static_cast<long long>(blockIdx.x) * kRouteGradWarps + warp; t < a.T;
+       t += static_cast<long long>(gridDim.x) * kRouteGradWarps) {
     const LogitT* row = static_cast<const LogitT*>(a.logits) + t * a.ld;
     LogitT* out = static_cast<LogitT*>(a.dlogits) + t * a.E;
     int e = -1;
@@ -278,17 +333,18 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_topk_grad_kernel(const
         v = route_f(row[e]);
       }
     }
-    float l[VPL], m = 0.0f, sum = 1.0f, d, all = 0.0f;
+    float ex[VPL], m = 0.0f, sum = 1.0f, d, all = 0.0f;
     if (dense) {
+      float l[VPL];
       route_load<LogitT, VPL, VEC>(row, a.E, lane, l);
-      route_softmax<VPL>(l, m, sum);
+      route_softmax<VPL>(l, m, ex, sum);
       const float p = e >= 0 ? expf(v - m) / sum : 0.0f;
       d = g * p;
       all = route_sum(d);
       d -= p * all;
     } else if (a.scoring == kRouteSoftmax) {
-      const uint32_t k = __reduce_max_sync(kAllLanes, route_key(v));
-      m = k == 0u ? 0.0f : route_unkey(k);
+      m = route_unkey(__reduce_max_sync(kAllLanes, route_key(v)));
+      if (m == -INFINITY) m = 0.0f;
       float p = e >= 0 ? expf(v - m) : 0.0f;
       p /= fmaxf(route_sum(p), 1e-30f);
       d = p * (g - route_sum(g * p));
@@ -301,14 +357,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_topk_grad_kernel(const
       }
       d = g * s * (1.0f - s);
     }
-    const float inv = 1.0f / sum;
+    const float factor = -all / sum;
 #pragma unroll
     for (int i = 0; i < VPL; i += VEC) {
       const int first = route_expert<VEC>(i, lane);
       if (first < a.E) {
         Pack p;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) route_set(p.v[j], dense ? -all * (expf(l[i + j] - m) * inv) : 0.0f);
+        for (int j = 0; j < VEC; ++j) route_set(p.v[j], dense ? factor * ex[i + j] : 0.0f);
         *reinterpret_cast<Pack*>(out + first) = p;
       }
     }
