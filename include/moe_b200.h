@@ -305,6 +305,15 @@ MOE_API int moe_fused_fp8(const void* hidden_states, const void* w13_q, const fl
                           int64_t num_experts, int64_t topk, int dtype, void* workspace, size_t workspace_bytes,
                           void* stream);
 
+/* moe_fused_q8_rows: moe_fused_int8 (kind MOE_I8) / moe_fused_fp8 (MOE_F8E4M3) on token rows that are 8-bit
+ *   already: x_q [T, H] with x_scale [T] fp32, as moe_add_rms_norm writes them. dtype is that of out.
+ *   Workspace: moe_fused_int8_workspace_bytes / moe_fused_fp8_workspace_bytes. No reference counterpart. */
+MOE_API int moe_fused_q8_rows(const void* x_q, const float* x_scale, int kind, const void* w13_q, const float* w13_scale,
+                              const void* w2_q, const float* w2_scale, const void* topk_ids, int ids_dtype,
+                              const void* topk_weights, int weights_dtype, void* out, int64_t num_tokens, int64_t hidden,
+                              int64_t intermediate, int64_t num_experts, int64_t topk, int dtype, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Packed weights: one buffer holding an expert set in the layout the fused kernels read (no
  * reference counterpart: the reference takes gate_w, up_w [E, I, H] and down_w [E, H, I] as

@@ -128,6 +128,11 @@ SIGNATURES = {
         _int,
         [_c_void_p] * 6 + [_int, _c_void_p, _int, _c_void_p] + [_i64] * 5 + [_int, _c_void_p, _size, _c_void_p],
     ),
+    "moe_fused_q8_rows": (
+        _int,
+        [_c_void_p, _c_void_p, _int] + [_c_void_p] * 5 + [_int, _c_void_p, _int, _c_void_p] + [_i64] * 5
+        + [_int, _c_void_p, _size, _c_void_p],
+    ),
     "moe_packed_weights_layout": (_int, [_i64, _i64, _i64, _int, ctypes.POINTER(_size), ctypes.POINTER(_size)]),
     "moe_pack_weights": (_int, [_c_void_p] * 3 + [_int, _i64, _i64, _i64, _int, _c_void_p, _size, _c_void_p]),
     "moe_fused_packed_workspace_bytes": (_size, [_i64] * 5 + [_int, _int]),

@@ -6,6 +6,8 @@
 //                     epilogue accumulates into. One warp per row, 16-byte vectors.
 //   gather_rows_q8    the same gather with per-token symmetric int8 quantisation fused in:
 //                     scale = amax(|x[t]|) / 127, q = clamp(round_half_away(x / scale), +-127).
+//   gather_rows_q8in  the gather of rows that are 8-bit already, with their scales (the rows of
+//                     moe_add_rms_norm): bytes and scale are copied as they are.
 //   quantize_rows_q8  per-row amax int8 (or fp8) quantisation of a [rows, K] 16-bit matrix
 //                     (weights offline: one scale per output row; the Stage1 intermediate online).
 // The rounding and clamp follow the reference's int8 experiment
@@ -123,6 +125,32 @@ __global__ void gather_rows_q8_kernel(const T* __restrict__ x, const int32_t* __
     } else {
       uint4* dst = reinterpret_cast<uint4*>(zero_out + (item - R) * static_cast<size_t>(H));
       for (int v = lane; v < vecs; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const long long tid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (long long i = tid; i < n_zero_f32; i += static_cast<long long>(gridDim.x) * blockDim.x) zero_f32[i] = 0.0f;
+}
+
+// x [tokens][H] bytes, x_scale [tokens]; H a multiple of 16. zero_out: rows of H 2-byte elements.
+__global__ void gather_rows_q8in_kernel(const uint8_t* __restrict__ x, const float* __restrict__ x_scale,
+                                        const int32_t* __restrict__ route_slot, int R, int topk, int H,
+                                        uint8_t* __restrict__ xq, float* __restrict__ xscale, uint16_t* __restrict__ zero_out,
+                                        int zero_rows, float* __restrict__ zero_f32, int n_zero_f32) {
+  const int lane = threadIdx.x & 31;
+  const long long warp_id = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const long long n_warps = (static_cast<long long>(gridDim.x) * blockDim.x) >> 5;
+  for (long long item = warp_id; item < static_cast<long long>(R) + zero_rows; item += n_warps) {
+    if (item < R) {
+      const int slot = route_slot[item];
+      if (slot < 0) continue;
+      const long long t = item / topk;
+      const uint4* src = reinterpret_cast<const uint4*>(x + t * H);
+      uint4* dst = reinterpret_cast<uint4*>(xq + static_cast<size_t>(slot) * H);
+      for (int v = lane; v < H / 16; v += 32) dst[v] = __ldg(src + v);
+      if (lane == 0) xscale[slot] = x_scale[t];
+    } else {
+      uint4* dst = reinterpret_cast<uint4*>(zero_out + (item - R) * static_cast<size_t>(H));
+      for (int v = lane; v < H / 8; v += 32) dst[v] = make_uint4(0, 0, 0, 0);
     }
   }
   const long long tid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;

@@ -1363,7 +1363,8 @@ static int fused_common(bool int8, const void* x, const void* w13, const float* 
                         const float* w2_scale, const void* ids, int ids_dtype, const void* tw, int w_dtype, void* out,
                         int64_t T, int64_t H, int64_t I, int64_t E, int64_t topk, int dtype, void* workspace,
                         size_t workspace_bytes, void* stream, const PeerSource* peer = nullptr,
-                        const RouterSource* router = nullptr, bool ordered = false, bool fp8 = false) {
+                        const RouterSource* router = nullptr, bool ordered = false, bool fp8 = false,
+                        const float* x_scale = nullptr) {  // x_scale: x holds 8-bit rows with these scales
   t_last_error.clear();
   MOE_TRY(check_common(H, I, E, dtype, int8 ? 16 : 8));
   if (T < 0 || topk < 1) return fail(MOE_ERR_INVALID_ARG, "num_tokens must be >= 0 and topk >= 1");
@@ -1461,7 +1462,16 @@ static int fused_common(bool int8, const void* x, const void* w13, const float* 
   const int gblocks = sms * 4;
   float* amax = int8 ? reinterpret_cast<float*>(ws + L.amax) : nullptr;
   float* xscale = int8 ? reinterpret_cast<float*>(ws + L.xscale) : nullptr;
-  if (lsu || gather) {
+  if (x_scale && (lsu || gather)) {  // 8-bit rows already
+    MOE_CUDA(cudaMemcpyAsync(xs, x, static_cast<size_t>(T) * H, cudaMemcpyDeviceToDevice, s));
+    MOE_CUDA(cudaMemcpyAsync(xscale, x_scale, sizeof(float) * static_cast<size_t>(T), cudaMemcpyDeviceToDevice, s));
+    MOE_CUDA(cudaMemsetAsync(amax, 0, sizeof(float) * (size_t)L.P_max, s));
+  } else if (x_scale) {
+    gather_rows_q8in_kernel<<<gblocks, 256, 0, s>>>(static_cast<const uint8_t*>(x), x_scale, slot, (int)R, (int)topk,
+                                                    (int)H, static_cast<uint8_t*>(xs), xscale, static_cast<uint16_t*>(out),
+                                                    (int)T, amax, (int)L.P_max);
+    MOE_CUDA(cudaGetLastError());
+  } else if (lsu || gather) {
     if (int8) {  // quantised per token, once (each token's k routes share its row and scale)
       if (dtype == MOE_F16 && fp8)
         quantize_rows_q8_kernel<__half, kQF8><<<gblocks, 256, 0, s>>>(
@@ -1899,6 +1909,17 @@ int moe_fused_fp8(const void* x, const void* w13_q, const float* w13_scale, cons
                   void* stream) {
   return fused_common(true, x, w13_q, w13_scale, w2_q, w2_scale, ids, ids_dtype, tw, w_dtype, out, T, H, I, E, topk,
                       dtype, workspace, workspace_bytes, stream, nullptr, nullptr, false, true);
+}
+
+int moe_fused_q8_rows(const void* x_q, const float* x_scale, int kind, const void* w13_q, const float* w13_scale,
+                      const void* w2_q, const float* w2_scale, const void* ids, int ids_dtype, const void* tw, int w_dtype,
+                      void* out, int64_t T, int64_t H, int64_t I, int64_t E, int64_t topk, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  t_last_error.clear();
+  if (kind != MOE_I8 && kind != MOE_F8E4M3) return fail(MOE_ERR_INVALID_ARG, "kind must be MOE_I8 or MOE_F8E4M3");
+  if (T > 0 && !x_scale) return fail(MOE_ERR_INVALID_ARG, "null row scales");
+  return fused_common(true, x_q, w13_q, w13_scale, w2_q, w2_scale, ids, ids_dtype, tw, w_dtype, out, T, H, I, E, topk,
+                      dtype, workspace, workspace_bytes, stream, nullptr, nullptr, false, kind == MOE_F8E4M3, x_scale);
 }
 
 // ---------------------------------------------------------------------------- packed weights

@@ -295,6 +295,38 @@ def quantize_rows_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
+def _fused_q8_rows(x_q, x_scale, q_dtype, w13_q, w13_scale, w2_q, w2_scale, topk_ids, topk_weights, out, out_dtype):
+    """fused_moe_int8 / fused_moe_fp8 on rows that are 8-bit already."""
+    _check(out_dtype in _DTYPES, "out_dtype must be fp16 or bf16")
+    _check(x_q.dim() == 2 and x_q.dtype == q_dtype, f"hidden_states must be {q_dtype} [T, H]")
+    T, H = x_q.shape
+    _check(x_scale.dtype == torch.float32 and x_scale.numel() == T and x_scale.is_contiguous() and x_scale.device == x_q.device,
+           "hidden_scale must be contiguous fp32 [T]")
+    _check(x_q.is_cuda and x_q.is_contiguous(), "hidden_states must be a contiguous CUDA tensor")
+    if out is None:
+        out = torch.empty((T, H), dtype=out_dtype, device=x_q.device)
+    _check(out.dtype in _DTYPES, "out must be fp16 or bf16")
+    _, _, I, E, k = _check_fused(out, w13_q, w2_q, topk_ids, topk_weights, True, q_dtype)
+    _check(tuple(out.shape) == (T, H) and out.device == x_q.device, "bad out")
+    _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
+           "w13_scale must be fp32 [E, 2I]")
+    _check(w2_scale.dtype == torch.float32 and w2_scale.numel() == E * H and w2_scale.is_contiguous(),
+           "w2_scale must be fp32 [E, H]")
+    if T == 0:
+        return out
+    dev, dt = x_q.device, _DTYPES[out.dtype]
+    int8 = q_dtype == torch.int8
+    nbytes = getattr(_lib.lib(), "moe_fused_int8_workspace_bytes" if int8 else "moe_fused_fp8_workspace_bytes")(T, k, E, H, I, dt)
+    ws = _workspace(("fused_i8" if int8 else "fused_f8", dev, _stream(dev)), nbytes, dev)
+    _lib.call(
+        "moe_fused_q8_rows", x_q.data_ptr(), x_scale.data_ptr(), _lib.MOE_I8 if int8 else _lib.MOE_F8E4M3, w13_q.data_ptr(),
+        w13_scale.data_ptr(), w2_q.data_ptr(), w2_scale.data_ptr(), topk_ids.data_ptr(), _ID_DTYPES[topk_ids.dtype],
+        topk_weights.data_ptr(), _W_DTYPES[topk_weights.dtype], out.data_ptr(), T, H, I, E, k, dt, ws.data_ptr(), ws.numel(),
+        _stream(dev),
+    )
+    return out
+
+
 def fused_moe_int8(
     hidden_states: torch.Tensor,
     w13_q: torch.Tensor,
@@ -304,9 +336,17 @@ def fused_moe_int8(
     topk_ids: torch.Tensor,
     topk_weights: torch.Tensor,
     out: Optional[torch.Tensor] = None,
+    hidden_scale: Optional[torch.Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
     """W8A8 ``fused_moe``: int8 weights with per-output-row scales (from :func:`quantize_rows_int8`),
-    activations quantised per token on the device, int32 accumulation, output in the activation dtype."""
+    activations quantised per token on the device, int32 accumulation, output in the activation dtype.
+
+    With ``hidden_scale`` [T] fp32 the rows are int8 already (:func:`add_rms_norm_quant`) and the output
+    is in ``out_dtype``."""
+    if hidden_scale is not None:
+        return _fused_q8_rows(hidden_states, hidden_scale, torch.int8, w13_q, w13_scale, w2_q, w2_scale, topk_ids,
+                              topk_weights, out, out_dtype)
     T, H, I, E, k = _check_fused(hidden_states, w13_q, w2_q, topk_ids, topk_weights, True)
     _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
            "w13_scale must be fp32 [E, 2I]")
@@ -354,10 +394,18 @@ def fused_moe_fp8(
     topk_ids: torch.Tensor,
     topk_weights: torch.Tensor,
     out: Optional[torch.Tensor] = None,
+    hidden_scale: Optional[torch.Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
 ) -> torch.Tensor:
     """fp8 ``fused_moe``: e4m3 weights with per-output-row scales (from :func:`quantize_rows_fp8`),
     activations quantised to e4m3 per token on the device, fp32 accumulation, output in the
-    activation dtype."""
+    activation dtype.
+
+    With ``hidden_scale`` [T] fp32 the rows are e4m3 already (:func:`add_rms_norm_quant`) and the output
+    is in ``out_dtype``."""
+    if hidden_scale is not None:
+        return _fused_q8_rows(hidden_states, hidden_scale, torch.float8_e4m3fn, w13_q, w13_scale, w2_q, w2_scale, topk_ids,
+                              topk_weights, out, out_dtype)
     T, H, I, E, k = _check_fused(hidden_states, w13_q, w2_q, topk_ids, topk_weights, True, torch.float8_e4m3fn)
     _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
            "w13_scale must be fp32 [E, 2I]")

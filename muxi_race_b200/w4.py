@@ -29,6 +29,17 @@ class W4Weights:
     gate_up: bool         # gate rows and up rows interleaved, for fused_moe_w4
     sizes: dict = field(default_factory=dict, repr=False, compare=False)  # workspace bytes by rows, asked once each
 
+    def __post_init__(self):
+        *lead, N, K = self.shape
+        matrices = 1
+        for n in lead:
+            matrices *= n
+        _check_group(self.group_size)
+        want = _lib.lib().moe_w4_packed_bytes(matrices, N, K, self.group_size, int(self.has_zeros), int(self.gate_up))
+        require(self.packed.dtype == torch.uint8 and self.packed.is_contiguous() and self.packed.numel() == want,
+                f"packed must be a contiguous uint8 tensor of {want} bytes for this shape")
+        require(self.dtype in HALVES, "dtype must be fp16 or bf16")
+
     def nbytes(self) -> int:
         return self.packed.numel()
 
