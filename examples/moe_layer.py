@@ -77,7 +77,7 @@ def train_step(layer: Layer, x: torch.Tensor, residual: torch.Tensor, target: to
         layer.norm.copy_(norm - lr * norm.grad)
         layer.gate.copy_(gate - lr * gate.grad)
         layer.bias += step * torch.sign(counts.float().mean() - counts.float())
-    return float(loss)
+    return float(loss.detach())
 
 
 def main() -> None:

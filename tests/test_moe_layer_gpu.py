@@ -64,10 +64,9 @@ def test_int8(cuda_device, example):
     """int8 rows and weights: steps of 1/127 of each row's largest value (about 3.5 sigma), a relative
     error of 3.5 / 127 / sqrt(12) = 0.8 % per factor; x, w13, h, w2 are four: under 4 %."""
     layer = example.make_layer(kind="int8")
-    plain = example.make_layer(kind="w4", seed=0)
     x, residual = inputs(48)
     out, _ = example.serve_int8(layer, x, residual)
-    q, scale, _ = m.add_rms_norm_quant(x, plain.norm, residual)
+    q, scale, _ = m.add_rms_norm_quant(x, layer.norm, residual)
     weights, ids = layer.route(q.float() * scale[:, None])
     y, _ = rms_norm_ref(x, layer.norm, residual)
     w13, w2 = (v.double() * s.double()[..., None] for v, s in (layer.w13, layer.w2))
