@@ -91,8 +91,9 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 //     q 2^-20 (row r + 8, one nibble further up): no instruction but the masks. The sums carry those
 //     powers of two to their end, and the zero points enter as the start of each group's sum:
 //     sum (q - z) x = -z sum x + sum q x.
-//   bf16 (whose subnormal products fp32 cannot hold): the nibbles become the low bits of 128 + q, and
-//     one subtraction gives q - z, exactly.
+//   bf16 (whose subnormal products fp32 cannot hold): the nibbles become the low bits of 1/2 + q / 256,
+//     and one subtraction gives (q - z) / 256, exactly. (At this size a group's sum overflows fp32 only
+//     where x is beyond 4e37; with whole numbers it would at 2e37 / 128.)
 template <typename T> struct W4Type;
 __device__ __forceinline__ uint32_t w4_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
   uint32_t v;
@@ -120,10 +121,10 @@ template <> struct W4Type<__half> {
 };
 template <> struct W4Type<__nv_bfloat16> {
   static constexpr bool kSums = false;
-  static constexpr float kScale0 = 1.0f, kScale1 = 1.0f;
-  // c: 128 + z of rows r and r + 8 (bf16 128: one step is a unit)
+  static constexpr float kScale0 = 256.0f, kScale1 = 256.0f;
+  // c: 1/2 + z / 256 of rows r and r + 8 (bf16 1/2: one step is 1 / 256)
   static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t c) {
-    uint32_t v = w4_and_or(w, 0x000f000fu, 0x43004300u);
+    uint32_t v = w4_and_or(w, 0x000f000fu, 0x3f003f00u);
     asm("sub.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(c));
     return v;
   }
@@ -227,7 +228,7 @@ __device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& in, uint32_t
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const uint4& w = in.w[block / 2][f];
-          const uint32_t off[2] = {0x43004300u + z[2 * f] * 0x10001u, 0x43004300u + z[2 * f + 1] * 0x10001u};
+          const uint32_t off[2] = {0x3f003f00u + z[2 * f] * 0x10001u, 0x3f003f00u + z[2 * f + 1] * 0x10001u};
           uint32_t a[4];
           W4Type<T>::unpack(block % 2 == 0 ? (step == 0 ? w.x : w.y) : (step == 0 ? w.z : w.w), off, a);
 #pragma unroll
@@ -399,8 +400,10 @@ template <typename T, int NTMAX, int THREADS>
 __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int first, int rows, int kt0, int kts) {
   const int k0 = kt0 * kW4TileK, words = kts * (kW4TileK / 8);
   const int whole = a.x_words ? min(words, (a.K - k0) / 8) : 0;  // 16-byte words that lie in x
+  const int lane = threadIdx.x & 31;
+  const int rows_of_x = lane < rows ? (a.gather ? a.gather[first + lane] : first + lane) : 0;
   for (int m = 0; m < rows; ++m) {
-    const long long row = a.gather ? a.gather[first + m] : first + m;
+    const long long row = __shfl_sync(0xffffffffu, rows_of_x, m);
     const T* src = static_cast<const T*>(a.x) + row * a.ld_x + k0;
     uint8_t* dst = smem + m * a.x_pitch;
     int c = threadIdx.x;
@@ -421,28 +424,43 @@ __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int fi
 template <typename T, int GROUP, bool ZEROS, int NTMAX, int WARPS>
 __device__ __forceinline__ void w4_starts(const W4Args& a, uint8_t* smem, int rows, int kts) {
   constexpr int kLanes = GROUP / 8;  // of a group
+  constexpr int kBatch = 4;          // rows at a time, so that their loads are in flight together
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int words = kts * (kW4TileK / 8);
-  for (int m = 0; m < rows; ++m)
+  for (int m0 = 0; m0 < rows; m0 += kBatch)
     for (int w0 = warp * 32; w0 < words; w0 += WARPS * 32) {
       const int word = w0 + lane;
-      float sum = 0.0f;
-      if (word < words) {
-        const uint4 v = lds128(smem_u32(smem) + m * a.x_pitch + word * 16);
-        const __half2* h = reinterpret_cast<const __half2*>(&v);
+      uint4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        v[j] = make_uint4(0, 0, 0, 0);
+        if (m0 + j < rows && word < words) v[j] = lds128(smem_u32(smem) + (m0 + j) * a.x_pitch + word * 16);
+      }
+      float sum[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v[j]);
+        sum[j] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = __half22float2(h[e]);
-          sum += f.x + f.y;
+          sum[j] += f.x + f.y;
         }
       }
 #pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
       if (lane % kLanes == 0 && word < words) {
-        const float start = sum * (ZEROS ? -1.0f : -8.0f) / W4Type<T>::kScale0;
-        float* to = reinterpret_cast<float*>(smem + a.x_bytes) + word / kLanes * (NTMAX * 16) + (m >> 1) * 4 + (m & 1);
-        to[0] = start;
-        to[2] = start * (W4Type<T>::kScale0 / W4Type<T>::kScale1);
+        float* group = reinterpret_cast<float*>(smem + a.x_bytes) + word / kLanes * (NTMAX * 16);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int m = m0 + j;
+          const float start = sum[j] * (ZEROS ? -1.0f : -8.0f) / W4Type<T>::kScale0;
+          float* to = group + (m >> 1) * 4 + (m & 1);  // m < 8 NTMAX: rows of a block are whole batches
+          to[0] = start;
+          to[2] = start * (W4Type<T>::kScale0 / W4Type<T>::kScale1);
+        }
       }
     }
 }

@@ -176,6 +176,29 @@ def test_spoilt_rows_stay_alone(cuda_device):
     assert torch.equal(y[keep], y2[keep])
 
 
+@pytest.mark.parametrize("group,zeros", [(128, False), (32, True)])
+def test_bf16_rows_of_any_range(cuda_device, group, zeros):
+    """Tiny and huge rows (1e37: the products of whole numbers would overflow fp32), rows of zeros and of
+    subnormal values, values of any size in one row; NaN and infinity stay in their row."""
+    M, N, K = 14, 50, 700
+    q, s, z = w4_inputs(42, (), N, K, group, zeros, BF16)
+    w, values = pack_w4(q, s, z, in_features=K, group_size=group), w4_values_ref(q, s, z, K, group)
+    x = torch.randn(M, K, generator=gen(43))
+    scale = torch.tensor([1e-30, 1e30, 0.0, 1e-39, 1, 1e-6, 3e4, 1e37, 1e-20, 1, 1, 1, 1, 1])
+    x = x * scale[:, None]
+    x[9] *= 2.0 ** torch.randint(-30, 1, (K,), generator=gen(44))
+    x[9, 5] = 4.0
+    x = x.to(BF16).cuda()
+    x[11, 3], x[12, 4] = float("nan"), float("-inf")
+    y = w4_linear(x, w)
+    fine = [i for i in range(M) if i not in (11, 12)]
+    ref, mag = linear_ref(x[fine], values)
+    tiny = 2.0 ** -133  # subnormal results and products are not part of the bound
+    within(y[fine], ref, U[BF16] * ref.abs() + F32 * mag + tiny, "y")
+    assert bool(y[11].isnan().all()) and not bool(y[12].isfinite().any())
+    assert device_status() == 0
+
+
 def test_empty_and_other_stream(cuda_device):
     q13, q2, x, ids, w = moe_case(50, 9, 256, 128, 8, 2, 128, False, F16)
     w13, w2 = pack_w4(*q13, group_size=128, gate_up=True), pack_w4(*q2, group_size=128)
