@@ -12,6 +12,8 @@ IDS = {torch.int32: _lib.MOE_I32, torch.int64: _lib.MOE_I64}
 
 #: handle of the current stream of a device ordinal, without building a Stream object
 raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_functions: dict = {}
 
 
 def require(cond: bool, msg: str) -> None:
@@ -29,23 +31,31 @@ def rows(t: torch.Tensor, name: str, device: torch.device | None = None) -> torc
             t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
         except RuntimeError:
             raise ValueError(f"{name} must have one row pitch: its leading dimensions cannot be viewed as one") from None
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    if not t.is_contiguous() and t.stride(1) != 1 and t.shape[1] > 1:
         raise ValueError(f"{name} must be contiguous along its last dimension")
     return t
 
 
 def pitch(t: torch.Tensor) -> int:
     """Row pitch of a 2-D tensor in elements (a single row has whatever pitch suits)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t.shape[1] if t.is_contiguous() or t.shape[0] == 1 else t.stride(0)
+
+
+def empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """An uninitialised contiguous [rows, cols] tensor (the cheapest way to one)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def launch(device: torch.device, name: str, *args) -> None:
     """Call entry point `name` with the current stream of `device` appended, that device current."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.lib(), name)
     index = device.index
-    if torch._C._cuda_getDevice() == index:
-        code = getattr(_lib.lib(), name)(*args, raw_stream(index))
+    if _current_device() == index:
+        code = fn(*args, raw_stream(index))
     else:
         with torch.cuda.device(index):
-            code = getattr(_lib.lib(), name)(*args, raw_stream(index))
+            code = fn(*args, raw_stream(index))
     if code:
         _lib.check(name, code)

@@ -30,7 +30,7 @@ def _check_weight(weight: torch.Tensor, H: int, dtype: torch.dtype, dev: torch.d
 def _output(t: Optional[torch.Tensor], x: torch.Tensor, name: str):
     """`t`, or a new tensor of x's shape and dtype, with its address and row pitch."""
     if t is None:
-        t = torch.empty_like(x, memory_format=torch.contiguous_format)
+        t = torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
         return t, t.data_ptr(), x.shape[-1]
     require(t.shape == x.shape and t.dtype == x.dtype, f"{name} must have the shape and dtype of x")
     t2 = rows(t, name, x.device)

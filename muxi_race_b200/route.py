@@ -10,27 +10,28 @@ from typing import Optional
 
 import torch
 
-from ._args import FLOATS, launch, pitch, require, rows
+from ._args import FLOATS, empty2, launch, pitch, require, rows
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
 
 
 def _forward(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale, counts):
     l2 = rows(logits, "logits")
-    require(logits.dim() == 2, "logits must be [T, E]")
-    require(l2.dtype in FLOATS, "logits must be fp32, fp16 or bf16")
-    require(scoring in _SCORING, "scoring must be 'softmax' or 'sigmoid'")
     T, E = l2.shape
-    dev = l2.device
+    dev, dtype = l2.device, l2.dtype
+    if logits.dim() != 2 or dtype not in FLOATS:
+        raise ValueError("logits must be fp32, fp16 or bf16 [T, E]")
+    if scoring not in _SCORING:
+        raise ValueError("scoring must be 'softmax' or 'sigmoid'")
     bias_ptr = None
     if bias is not None:
-        require(bias.device == dev and bias.dtype == torch.float32 and bias.is_contiguous() and tuple(bias.shape) == (E,),
-                f"bias must be a contiguous fp32 tensor [{E}] on {dev}")
+        if bias.device != dev or bias.dtype != torch.float32 or not bias.is_contiguous() or bias.dim() != 1 or bias.shape[0] != E:
+            raise ValueError(f"bias must be a contiguous fp32 tensor [{E}] on {dev}")
         bias_ptr = bias.data_ptr()
-    ids = l2.new_empty((T, topk), dtype=torch.int32)
-    weights = l2.new_empty((T, topk), dtype=torch.float32)
-    number = l2.new_empty((E,), dtype=torch.int32) if counts else None
-    launch(dev, "moe_route_topk", l2.data_ptr(), pitch(l2), FLOATS[l2.dtype], bias_ptr, T, E, topk, _SCORING[scoring],
+    ids = empty2(T, topk, torch.int32, dev)
+    weights = empty2(T, topk, torch.float32, dev)
+    number = torch.empty_strided((E,), (1,), dtype=torch.int32, device=dev) if counts else None
+    launch(dev, "moe_route_topk", l2.data_ptr(), pitch(l2), FLOATS[dtype], bias_ptr, T, E, topk, _SCORING[scoring],
            num_groups, topk_groups, group_top, renormalize, scale, ids.data_ptr(), weights.data_ptr(),
            None if number is None else number.data_ptr())
     return weights, ids, number
@@ -107,7 +108,7 @@ def route_topk_backward(
     require(dweights.shape == topk_ids.shape and dweights.dtype == torch.float32 and dweights.device == dev,
             "dweights must be an fp32 tensor of topk_ids' shape")
     dweights = dweights.contiguous()
-    out = l2.new_empty((T, E))
+    out = empty2(T, E, l2.dtype, dev)
     launch(dev, "moe_route_topk_backward", dweights.data_ptr(), l2.data_ptr(), pitch(l2), FLOATS[l2.dtype],
            topk_ids.data_ptr(), T, E, topk_ids.shape[1], _SCORING[scoring], renormalize, scale, out.data_ptr())
     return out

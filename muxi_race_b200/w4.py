@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, launch, pitch, raw_stream, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, launch, pitch, raw_stream, require, rows
 from .fused import _workspace
 
 
@@ -131,7 +131,9 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
         raise ValueError(f"x must be {w.dtype} [..., {K}]")
     M = x2.shape[0]
     if out is None:
-        out = x2.new_empty((*x.shape[:-1], N))
+        out = empty2(M, N, w.dtype, dev)
+        if x.dim() != 2:
+            out = out.view(*x.shape[:-1], N)
         ld_out = N
     else:
         require(tuple(out.shape) == (*x.shape[:-1], N) and out.dtype == w.dtype, f"out must be {w.dtype} [..., {N}]")
@@ -181,7 +183,7 @@ def fused_moe_w4(
         raise ValueError(f"topk_ids and topk_weights must be contiguous tensors on {dev}")
     k = topk_ids.shape[1]
     if out is None:
-        out = x.new_empty((T, H))
+        out = empty2(T, H, w13.dtype, dev)
     else:
         require(tuple(out.shape) == (T, H) and out.dtype == w13.dtype and out.is_contiguous() and out.device == dev, "bad out")
     if T == 0:
