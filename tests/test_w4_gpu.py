@@ -141,6 +141,13 @@ def test_experts_with_uneven_loads(cuda_device, T):
     run_moe(*moe_case(20, T, 384, 200, 40, 2, 128, False, BF16, skew=True), 128)
 
 
+@pytest.mark.parametrize("T,H,I,E,k", [(100, 96, 40, 600, 8), (60, 130, 70, 1000, 4), (250, 64, 16, 700, 8), (9, 1024, 300, 900, 8)])
+@pytest.mark.parametrize("group,zeros,dtype", [(128, False, F16), (64, True, BF16), (32, True, F16)])
+def test_many_experts_of_few_tokens(cuda_device, T, H, I, E, k, group, zeros, dtype):
+    """A CTA's strips belong to many experts of one to a few tokens each, whose rows it holds together."""
+    run_moe(*moe_case(25, T, H, I, E, k, group, zeros, dtype), group)
+
+
 def test_experts_ids(cuda_device):
     """Skipped ids, a token without any expert, an expert twice in a token, int64 ids, 16-bit weights,
     rows at odd starts."""
