@@ -319,24 +319,40 @@ __global__ void __launch_bounds__(kRouteGradWarps * 32) route_topk_grad_kernel(c
   struct alignas(sizeof(LogitT) * VEC) Pack { LogitT v[VEC]; };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool dense = a.scoring == kRouteSoftmax && !a.renorm;
-  for (long long t = static_cast<long long>(blockIdx.x) * kRouteGradWarps + warp; t < a.T;
-       t += static_cast<long long>(gridDim.x) * kRouteGradWarps) {
-    const LogitT* row = static_cast<const LogitT*>(a.logits) + t * a.ld;
-    LogitT* out = static_cast<LogitT*>(a.dlogits) + t * a.E;
-    int e = -1;
-    float g = 0.0f, v = -INFINITY;
+  const LogitT* logits = static_cast<const LogitT*>(a.logits);
+  const long long step = static_cast<long long>(gridDim.x) * kRouteGradWarps;
+  constexpr bool kAhead = VPL <= 8;  // the next token's logits, ids and gradients are on their way during this one
+  float next[VPL];
+  int next_e = -1;
+  float next_g = 0.0f;
+  auto load_chosen = [&](long long t) {
     if (lane < a.topk) {
-      e = a.chosen[t * a.topk + lane];
-      if (e >= a.E) e = -1;
-      if (e >= 0) {
-        g = a.dweights[t * a.topk + lane] * a.scale;
-        v = route_f(row[e]);
-      }
+      next_e = a.chosen[t * a.topk + lane];
+      next_g = a.dweights[t * a.topk + lane] * a.scale;
     }
+  };
+  long long t = static_cast<long long>(blockIdx.x) * kRouteGradWarps + warp;
+  if (t < a.T) {
+    load_chosen(t);
+    if (kAhead && dense) route_load<LogitT, VPL, VEC>(logits + t * a.ld, a.E, lane, next);
+  }
+  for (; t < a.T; t += step) {
+    const LogitT* row = logits + t * a.ld;
+    LogitT* out = static_cast<LogitT*>(a.dlogits) + t * a.E;
+    const int e = next_e < a.E ? next_e : -1;
+    float g = e >= 0 ? next_g : 0.0f;
+    const float v = e >= 0 ? route_f(row[e]) : -INFINITY;
+    if (t + step < a.T) load_chosen(t + step);
     float ex[VPL], m = 0.0f, sum = 1.0f, d, all = 0.0f;
     if (dense) {
       float l[VPL];
-      route_load<LogitT, VPL, VEC>(row, a.E, lane, l);
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) l[i] = next[i];
+        if (t + step < a.T) route_load<LogitT, VPL, VEC>(row + step * a.ld, a.E, lane, next);
+      } else {
+        route_load<LogitT, VPL, VEC>(row, a.E, lane, l);
+      }
       route_softmax<VPL>(l, m, ex, sum);
       const float p = e >= 0 ? expf(v - m) / sum : 0.0f;
       d = g * p;

@@ -21,7 +21,9 @@ struct W4Plan {
   size_t smem() const { return static_cast<size_t>(x_bytes) + start_bytes + sum_bytes; }
 };
 
-constexpr double kW4SumCost = 1.0;
+// What handing on a strip's sum takes in tile times, and what each further strip at a time adds (more
+// streams, each read by fewer warps). Of 0.2 to 3 and 0 to 0.03 the best over eleven sizes of 1 to 100 rows.
+constexpr double kW4SumCost = 0.4, kW4GroupCost = 0.03;
 constexpr int kW4Smem = kMaxDynamicSmem - 1024;  // static shared memory of the kernel, rounded up
 
 // `tiles`: token tiles expected, `sms`: CTAs.
@@ -47,12 +49,13 @@ W4Plan w4_plan(int strips, int64_t K, int group, int dtype, int tile_rows, doubl
   // (One token, 8 experts, H = 7168: 14 warps a strip instead of 2, in whose second round one or two
   // groups of 7 work, take the first product from 43 to 30 us.)
   const int64_t strips_cta = static_cast<int64_t>(std::ceil(tiles * p.slices * strips / sms));
+  const bool apart = w4_apart(std::max<int64_t>(1, std::llround(tiles * p.slices)), strips, sms);
   const int last_kt = p.kt - (p.slices - 1) * p.slice_kt;  // every warp has a tile in every slice
   double best = 0;
   for (int wps = 1; wps <= p.warps && wps <= last_kt; ++wps) {
     const int64_t groups = p.warps / wps;
-    const int64_t rounds = tiles * p.slices <= 1 || strips_cta < 2 ? ceil_div(strips_cta, groups) : (strips_cta - 2) / groups + 2;
-    const double cost = rounds * (static_cast<double>(ceil_div(p.slice_kt, wps)) + kW4SumCost);
+    const int64_t rounds = apart || strips_cta < 2 ? ceil_div(strips_cta, groups) : (strips_cta - 2) / groups + 2;
+    const double cost = rounds * (static_cast<double>(ceil_div(p.slice_kt, wps)) + kW4SumCost) * (1 + kW4GroupCost * groups);
     if (p.wps == 0 || cost < best) {
       best = cost;
       p.wps = wps;

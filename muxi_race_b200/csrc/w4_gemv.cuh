@@ -286,18 +286,36 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, 
 __host__ __device__ constexpr uint32_t w4_div_by(int d) { return d == 1 ? 0 : static_cast<uint32_t>(0xffffffffu / d) + 1; }
 __device__ __forceinline__ int w4_div(int n, uint32_t m) { return m == 0 ? n : static_cast<int>(__umulhi(n, m)); }
 
-// The strips of a CTA: an equal run of all (token tile, slice of K, strip), taken in segments of one
-// tile and slice.
+// Whether each (token tile, slice) gets CTAs of its own: where that gives no CTA more strips than equal
+// runs over all of them would. No CTA then has rows of x of two of them to load.
+__host__ __device__ inline bool w4_apart(long long units, long long strips, long long ctas) {
+  return units <= ctas && (strips + ctas / units - 1) / (ctas / units) <= (units * strips + ctas - 1) / ctas;
+}
+
+// The strips of a CTA: of one (token tile, slice of K) or an equal run over all, taken in segments of
+// one tile and slice.
 struct W4Segments {
   int strips, slices;
   int tile, slice, strip, left;  // where the next segment starts, and the strips left in all
   int s0, s1;                    // strips of this segment
   __device__ __forceinline__ W4Segments(uint32_t tiles, uint32_t slices_, uint32_t strips_) : strips(strips_), slices(slices_) {
-    const uint32_t all = tiles * slices_ * strips_, each = all / gridDim.x, more = all - each * gridDim.x;
-    const uint32_t u0 = each * blockIdx.x + min(blockIdx.x, more);
-    left = each + (blockIdx.x < more ? 1 : 0);
-    const uint32_t run = u0 / strips_;
-    strip = u0 - run * strips_;
+    const uint32_t units = tiles * slices_;
+    uint32_t run = 0;
+    if (units > 0 && w4_apart(units, strips_, gridDim.x)) {
+      // the first `more` units have a CTA more than the others
+      const uint32_t each = gridDim.x / units, more = gridDim.x - each * units, big = more * (each + 1);
+      const uint32_t c = blockIdx.x;
+      run = c < big ? c / (each + 1) : more + (c - big) / each;
+      const uint32_t n = run < more ? each + 1 : each, i = c < big ? c - run * (each + 1) : c - big - (run - more) * each;
+      strip = strips_ * i / n;
+      left = strips_ * (i + 1) / n - strip;
+    } else {
+      const uint32_t all = units * strips_, each = all / gridDim.x, more = all - each * gridDim.x;
+      const uint32_t u0 = each * blockIdx.x + min(blockIdx.x, more);
+      left = each + (blockIdx.x < more ? 1 : 0);
+      run = u0 / strips_;
+      strip = u0 - run * strips_;
+    }
     tile = slices_ == 1 ? run : run / slices_;
     slice = run - tile * slices_;
     s0 = s1 = 0;
