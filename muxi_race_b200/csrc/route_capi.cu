@@ -34,13 +34,26 @@ int launch_vpl(const RouteArgs& a, int sms, cudaStream_t s) {
     if (words) route_topk_grad_kernel<LogitT, VPL, V><<<grid, warps * 32, 0, s>>>(a);
     else route_topk_grad_kernel<LogitT, VPL, 1><<<grid, warps * 32, 0, s>>>(a);
   } else {
-    if (a.counts && grid > 1) MOE_CUDA(cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * static_cast<size_t>(a.E), s));
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    if (a.counts && grid > 1) {
+      route_clear_kernel<<<1, 256, 0, s>>>(a.counts, a.E);
+      MOE_CUDA(cudaGetLastError());
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+    }
     const size_t smem = sizeof(uint2) * warps * (static_cast<size_t>(a.E) + 32) + (a.counts ? sizeof(int) * a.E : 0);
     const bool scored = a.bias || a.n_group > 1;
-    if (words && scored) route_topk_kernel<LogitT, VPL, V, true><<<grid, warps * 32, smem, s>>>(a);
-    else if (words) route_topk_kernel<LogitT, VPL, V, false><<<grid, warps * 32, smem, s>>>(a);
-    else if (scored) route_topk_kernel<LogitT, VPL, 1, true><<<grid, warps * 32, smem, s>>>(a);
-    else route_topk_kernel<LogitT, VPL, 1, false><<<grid, warps * 32, smem, s>>>(a);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    if (words && scored) MOE_CUDA(cudaLaunchKernelEx(&cfg, route_topk_kernel<LogitT, VPL, V, true>, a));
+    else if (words) MOE_CUDA(cudaLaunchKernelEx(&cfg, route_topk_kernel<LogitT, VPL, V, false>, a));
+    else if (scored) MOE_CUDA(cudaLaunchKernelEx(&cfg, route_topk_kernel<LogitT, VPL, 1, true>, a));
+    else MOE_CUDA(cudaLaunchKernelEx(&cfg, route_topk_kernel<LogitT, VPL, 1, false>, a));
   }
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;

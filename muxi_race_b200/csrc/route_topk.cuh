@@ -18,9 +18,11 @@
 // One warp per token, its logits in registers. The topk-th largest of the 32 lanes' own maxima is a
 // lower bound of the topk-th largest of all, and few candidates reach it (about 10 for topk = 8 of 256):
 // those go to shared memory, and each counts how many are before it. The
-// next token's logits are loaded meanwhile. T = 32768, E = 256, topk = 8: 22 us, against 34 us with topk
-// rounds of a warp-wide maximum; the 33.5 MB of logits take 5 us, the instructions and the latencies of
-// the steps bound it. The gradient writes (and, softmax, reads) those bytes: 13 us for 67 MB.
+// next token's logits are loaded meanwhile. T = 32768, E = 256, topk = 8: 21 us (softmax of the chosen;
+// with the softmax of all and counts 23 us, sigmoid with bias and groups 46 us), against 34 us with topk
+// rounds of a warp-wide maximum over all; the 33.5 MB of logits take 5 us, the instructions and the
+// latencies of the steps bound it. The gradient writes (and, softmax of all, reads) those bytes: 18 us for
+// 67 MB, 13 us with the logits in L2.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -34,6 +36,9 @@ constexpr int kRouteGradWarps = 8;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
 constexpr int kRouteMaxGroups = 32;
+// A bound by rounds up to this topk, by sorting above (T = 32768, E = 256, softmax: topk 4 18.2 against
+// 19.4 us, 6 19.6 against 20.3, 8 20.4 against 20.8, 10 the same, 12 23.2 against 22.9).
+constexpr int kRouteRounds = 8;
 constexpr float kRouteLeast = 1e-37f;  // a sum of scores that rounds to nothing divides as this
 constexpr unsigned kAllLanes = 0xffffffffu;
 enum { kRouteSoftmax = 0, kRouteSigmoid = 1 };
@@ -126,6 +131,18 @@ __device__ __forceinline__ uint32_t route_sort(uint32_t v, int lane) {
       v = ((lane & j) == 0) == ((lane & k) == 0) ? max(v, o) : min(v, o);
     }
   return v;
+}
+
+// A bound that at least topk of the lanes' values reach, or all: in topk rounds, each of which drops the
+// largest, or from their order.
+__device__ __forceinline__ uint32_t route_bound(uint32_t v, int topk, int lane) {
+  if (topk > kRouteRounds) return __shfl_sync(kAllLanes, route_sort(v, lane), topk - 1);
+  uint32_t most = 0;
+  for (int i = 0; i < topk; ++i) {
+    most = __reduce_max_sync(kAllLanes, v);
+    if (v == most) v = 0;
+  }
+  return most;
 }
 
 // SCORED: the choice needs the scores (a bias or groups), not the logits' order alone.
@@ -248,7 +265,7 @@ __global__ void __launch_bounds__(route_warps(VPL) * 32, VPL <= 8 ? 4 : 1) route
     uint32_t best = key[0];
 #pragma unroll
     for (int i = 1; i < VPL; ++i) best = max(best, key[i]);
-    const uint32_t least = max(__shfl_sync(kAllLanes, route_sort(best, lane), a.topk - 1), kRouteNone + 1);
+    const uint32_t least = max(route_bound(best, a.topk, lane), kRouteNone + 1);
     int n = 0;
     if (__any_sync(kAllLanes, best >= least)) {
       const uint32_t below = (1u << lane) - 1u;
@@ -307,11 +324,18 @@ __global__ void __launch_bounds__(route_warps(VPL) * 32, VPL <= 8 ? 4 : 1) route
   }
   if (a.counts) {
     __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the counts are cleared
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
       if (gridDim.x == 1) a.counts[e] = hist[e];
       else if (hist[e]) atomicAdd(&a.counts[e], hist[e]);  // whole numbers: any order gives the same
     }
   }
+}
+
+// Clears the counts while route_topk_kernel already runs.
+__global__ void route_clear_kernel(int32_t* counts, int E) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = threadIdx.x; e < E; e += blockDim.x) counts[e] = 0;
 }
 
 template <typename LogitT, int VPL, int VEC>
