@@ -4,6 +4,8 @@ Tolerances: u = half a unit in the last place of the output type (2^-11 fp16, 2^
 rounding. The products q - z are exact; a sum is at most 8 tensor instructions per group of 128 (whose
 accumulation may truncate, 2^-23), then at most 16 groups of a warp and 8 warps: 32 steps, so an error
 below 32 * 2^-23 = 3.8e-6 of the sum of the terms' magnitudes: F32 = 5e-6 with the scaling products.
+(A plan may give one warp all of a long K, 128 steps of 2^-24 at K = 16384, whose rounding errors are of
+either sign and stay far below their bound.)
 """
 import pytest
 import torch
