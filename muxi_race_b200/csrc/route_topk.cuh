@@ -28,6 +28,8 @@
 #include <cuda_fp16.h>
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
+
 namespace moe {
 
 // warps of a block; their candidates (8 bytes for each expert) stay within 32 KB
@@ -51,7 +53,9 @@ struct RouteArgs {
   float scale;
   int32_t* ids;
   float* weights;
-  int32_t* counts;   // [E] or null; one block stores it, more blocks add to it (cleared before)
+  int32_t* counts;   // [E] or null
+  int cluster;       // the blocks are one cluster that adds up its counts itself; otherwise one block
+                     // stores them, more blocks add to them (cleared before)
   const float* dweights;  // gradient only
   const int32_t* chosen;
   void* dlogits;
@@ -322,7 +326,19 @@ __global__ void __launch_bounds__(route_warps(VPL) * 32, VPL <= 8 ? 4 : 1) route
       if (a.counts && my_e >= 0) atomicAdd(&hist[my_e], 1);
     }
   }
-  if (a.counts) {
+  if (a.counts && a.cluster) {
+    cluster_sync();
+    for (int e = blockIdx.x * blockDim.x + threadIdx.x; e < a.E; e += gridDim.x * blockDim.x) {
+      int n = 0;
+      for (uint32_t c = 0; c < gridDim.x; ++c) {
+        int of_c;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(of_c) : "r"(mapa_shared(smem_u32(hist + e), c)) : "memory");
+        n += of_c;
+      }
+      a.counts[e] = n;
+    }
+    cluster_sync();  // no block ends while its counts are read
+  } else if (a.counts) {
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the counts are cleared
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {

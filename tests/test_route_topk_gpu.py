@@ -57,6 +57,14 @@ def test_by_logits(cuda_device, T, E, k, scoring, renormalize, dtype, masked):
     check(logits_of(1, T, E, dtype, masked), k, scoring=scoring, renormalize=renormalize, scale=2.5)
 
 
+@pytest.mark.parametrize("E,k", [(8, 2), (60, 8), (100, 9), (256, 8), (512, 10), (1024, 8)])
+@pytest.mark.parametrize("T", [1, 8, 9, 16, 17, 63, 64, 65, 127, 128, 129, 257])
+def test_counts_of_every_launch_form(cuda_device, T, E, k):
+    """One block, one cluster of blocks, and many blocks add their counts up."""
+    for seed in (2, 3):
+        check(logits_of(seed, T, E, masked=0.1), k)
+
+
 @pytest.mark.parametrize("T,E,k,groups,top_groups", [(200, 256, 8, 8, 4), (33, 256, 8, 8, 1), (100, 60, 6, 5, 3),
                                                      (100, 96, 2, 32, 7), (64, 12, 3, 3, 2), (50, 40, 4, 1, 1),
                                                      (30, 1024, 8, 16, 2), (30, 8, 4, 8, 5)])
