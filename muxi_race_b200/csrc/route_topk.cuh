@@ -34,6 +34,11 @@ namespace moe {
 
 // warps of a block; their candidates (8 bytes for each expert) stay within 32 KB
 __host__ __device__ constexpr int route_warps(int vpl) { return vpl > 16 ? 4 : 8; }
+// Blocks of an SM at once, which sets the registers (64 or 80): a token is a chain of dependent steps, so
+// many warps matter more than what stays in registers. (Sigmoid with bias, T = 16384: E = 512 at one block of
+// 149 registers 54 us, at 4 blocks of 64 23 us; E = 1024 at 2 blocks of 240 registers 73 us, at 4 48 us, at 6
+// 44 us.)
+__host__ __device__ constexpr int route_blocks(int vpl) { return vpl > 16 ? 6 : 4; }
 constexpr int kRouteGradWarps = 8;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 32;
@@ -151,7 +156,7 @@ __device__ __forceinline__ uint32_t route_bound(uint32_t v, int topk, int lane) 
 
 // SCORED: the choice needs the scores (a bias or groups), not the logits' order alone.
 template <typename LogitT, int VPL, int VEC, bool SCORED>
-__global__ void __launch_bounds__(route_warps(VPL) * 32, VPL <= 8 ? 4 : 1) route_topk_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(route_warps(VPL) * 32, route_blocks(VPL)) route_topk_kernel(const RouteArgs a) {
   constexpr int kWarps = route_warps(VPL);
   extern __shared__ uint2 route_smem[];  // per warp its candidates, or their scores by group; [E] counts
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
