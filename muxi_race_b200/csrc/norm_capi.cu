@@ -90,10 +90,11 @@ int norm_grad_groups(int64_t T, int64_t rows_per_block, int64_t ctas) {
   return static_cast<int>(groups < kNormGradMaxGroups ? groups : kNormGradMaxGroups);
 }
 
-// Elements of a row per thread of the ring form. 32 against 16: with few elements the reductions and
-// addresses of a row outweigh its arithmetic (T = 8191, H = 4096, bf16: 56.6 us against 60.0 us; 2 or
-// 3 rows in the ring are the same, 4 leave one CTA less per SM, 62.0 us).
-constexpr int kGradElems = 32;
+// Elements of a row per thread of the ring form. With few, the reductions and addresses of a row outweigh
+// its arithmetic (T = 8191, H = 4096, bf16: 32 elements 52 us, 16 55 us); with many, short rows leave an SM
+// few warps, and fp32 rows too, whose ring leaves room for few CTAs (T = 8192, H = 1000, bf16: 8 elements
+// 21 us, 32 27 us; T = 4096, H = 7168, fp32: 16 elements 76 us, 32 85 us).
+constexpr int grad_elems(int hidden, int size) { return hidden <= 2048 ? 8 : size == 4 && hidden <= 8192 ? 16 : 32; }
 constexpr int kGradThreads = 512;  // per SM: 128 registers each
 
 template <typename WT>
@@ -117,10 +118,10 @@ int launch_grad_form(const NormGradArgs& a, int sms, void* dweight, cudaStream_t
   return launch_dweight<WT>(a, groups, dweight, s);
 }
 
-template <typename XT, typename WT, int VEC, int STAGES>
+template <typename XT, typename WT, int VEC, int ELEMS, int STAGES>
 int launch_grad_rows(const NormGradArgs& a, int threads, size_t stage_bytes, int dev, int sms, void* dweight,
                      cudaStream_t s) {
-  constexpr auto kernel = rms_norm_grad_rows_kernel<XT, WT, VEC, kGradElems / VEC, STAGES>;
+  constexpr auto kernel = rms_norm_grad_rows_kernel<XT, WT, VEC, ELEMS / VEC, STAGES>;
   MOE_TRY(allow_smem<kernel>(dev));
   int per_sm = static_cast<int>((kMaxDynamicSmem - 1024) / (STAGES * stage_bytes + 1024));
   if (per_sm > kGradThreads / threads) per_sm = kGradThreads / threads;
@@ -129,6 +130,21 @@ int launch_grad_rows(const NormGradArgs& a, int threads, size_t stage_bytes, int
   kernel<<<groups, threads, STAGES * stage_bytes, s>>>(a);
   MOE_CUDA(cudaGetLastError());
   return launch_dweight<WT>(a, groups, dweight, s);
+}
+
+// 3 rows in the ring; 2 where that puts two CTAs on an SM instead of one (T = 8191, H = 4096, fp32: 86 us
+// against 99 us; T = 4096, H = 7168, bf16: 48 against 55 us) or where 3 do not fit. `done`: 2 fit.
+template <typename XT, typename WT, int V, int ELEMS>
+int launch_grad_ring(const NormGradArgs& a, int dev, int sms, void* dweight, cudaStream_t s, bool* done) {
+  const int threads = round32((a.hidden + ELEMS - 1) / ELEMS);
+  const size_t stage_bytes = static_cast<size_t>(a.dh ? 3 : 2) * threads * ELEMS * sizeof(XT);
+  constexpr size_t most = kMaxDynamicSmem - 2048;
+  *done = true;
+  if (3 * stage_bytes <= most && (6 * stage_bytes <= most || 4 * stage_bytes > most))
+    return launch_grad_rows<XT, WT, V, ELEMS, 3>(a, threads, stage_bytes, dev, sms, dweight, s);
+  if (2 * stage_bytes <= most) return launch_grad_rows<XT, WT, V, ELEMS, 2>(a, threads, stage_bytes, dev, sms, dweight, s);
+  *done = false;
+  return MOE_OK;
 }
 
 // Rows that a warp holds: one row per warp. Longer ones: one per CTA, through the ring of 3 (or 2)
@@ -140,12 +156,12 @@ int launch_grad(const NormGradArgs& a, bool vec16, int dev, int sms, void* dweig
     if (a.hidden <= 32 * 8) return launch_grad_form<XT, WT, V, 8, false, true>(a, sms, dweight, s);
     if constexpr (V == 8)
       if (a.hidden <= 32 * 16) return launch_grad_form<XT, WT, V, 16, false, true>(a, sms, dweight, s);
-    const int threads = round32((a.hidden + kGradElems - 1) / kGradElems);
-    const size_t stage_bytes = static_cast<size_t>(a.dh ? 3 : 2) * threads * kGradElems * sizeof(XT);
-    if (3 * stage_bytes <= kMaxDynamicSmem - 2048)
-      return launch_grad_rows<XT, WT, V, 3>(a, threads, stage_bytes, dev, sms, dweight, s);
-    if (2 * stage_bytes <= kMaxDynamicSmem - 2048)
-      return launch_grad_rows<XT, WT, V, 2>(a, threads, stage_bytes, dev, sms, dweight, s);
+    bool done;
+    const int elems = grad_elems(a.hidden, sizeof(XT));
+    const int rc = elems == 8    ? launch_grad_ring<XT, WT, V, 8>(a, dev, sms, dweight, s, &done)
+                   : elems == 16 ? launch_grad_ring<XT, WT, V, 16>(a, dev, sms, dweight, s, &done)
+                                 : launch_grad_ring<XT, WT, V, 32>(a, dev, sms, dweight, s, &done);
+    if (done) return rc;
     if constexpr (V == 4) return launch_grad_form<XT, WT, V, 16, true, false>(a, sms, dweight, s);
   }
   if (a.hidden <= 32 * 8) return launch_grad_form<XT, WT, 1, 8, false, true>(a, sms, dweight, s);

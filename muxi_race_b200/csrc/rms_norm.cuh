@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(CTA ? (AHEAD ? 512 : 1024) : kNormWarpBlock)
 // its places twice, for the sums and for the gradients, so that registers hold only dweight and the
 // weight.
 template <typename XT, typename WT, int VEC, int NV, int STAGES>
-__global__ void __launch_bounds__(NV * VEC > 16 ? 512 : 1024)
+__global__ void __launch_bounds__(512)
     rms_norm_grad_rows_kernel(const NormGradArgs a) {
   __shared__ float2 red[2][32];
   extern __shared__ uint4 ring[];  // [STAGES][dy, h, dh][NV][threads]
