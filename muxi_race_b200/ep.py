@@ -124,7 +124,7 @@ class CudaOps:
                  torch.empty(4, **i32))
         offsets = torch.empty(W + 1, **i32)
         nbytes = _lib.lib().moe_ep_plan_workspace_bytes(T, W)
-        ws = _workspace(("ep_plan", self.device, _stream(self.device)), nbytes, self.device)
+        ws = _workspace(nbytes, self.device)
         _lib.call("moe_ep_plan", topk_ids.data_ptr(), _ID_DTYPES[topk_ids.dtype], T, k, self.expert_rank.data_ptr(),
                   self.E, W, p.send_counts.data_ptr(), offsets.data_ptr(), p.send_pairs.data_ptr(),
                   p.pair_slot.data_ptr(), p.meta.data_ptr(), ws.data_ptr(), ws.numel(), _stream(self.device))
@@ -397,8 +397,7 @@ class PeerMemoryEP:
         if self.push:
             _lib.call("moe_ep_p2p_push_prepare", self._region, T, self.T_max, self.H, self.k, self.world, dt, stream)
         self._barrier(stream)
-        ws = _workspace(("ep_p2p", self.device, self.T_max, self.k, self.world, self.E_local, stream), self._ws_bytes,
-                        self.device)
+        ws = _workspace(self._ws_bytes, self.device)
         _lib.call("moe_ep_p2p_compute_push" if self.push else "moe_ep_p2p_compute", self.regions.data_ptr(),
                   self._region, self.rank, self.world, self.T_max, self.H, self.I, self.k,
                   self.expert_rank.data_ptr(), self.expert_local.data_ptr(), self.E, self.w13.data_ptr(),

@@ -9,7 +9,6 @@ counts stay on the device, so a call never synchronises the host.
 """
 from __future__ import annotations
 
-import threading
 from dataclasses import dataclass
 from typing import Optional
 
@@ -22,30 +21,23 @@ _DTYPES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
 _W_DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
 _ID_DTYPES = {torch.int32: _lib.MOE_I32, torch.int64: _lib.MOE_I64}
 
-_WS: dict = {}
-_WS_LOCK = threading.Lock()
-
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _workspace(key, nbytes: int, device: torch.device) -> torch.Tensor:
-    """Scratch buffer of at least `nbytes`, one per (entry point, device, stream), grown when a call
-    needs more. Calls on one stream run in stream order, so they can share it whatever their
-    shapes, and the cache stays bounded by the largest call (not one buffer per shape). A buffer
-    replaced by a larger one goes back to the caching allocator of its own stream."""
-    with _WS_LOCK:
-        ws = _WS.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-            _WS[key] = ws
-    return ws
+def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Scratch buffer of one call, allocated on the device's current stream. Its block goes back to
+    PyTorch's caching allocator when the call has been launched, and the next call on that stream
+    gets it again behind this one. Not shared between calls: an entry point launches several kernels
+    without the interpreter's lock, so two threads on one stream may interleave theirs; and a buffer that is
+    allocated during a graph capture belongs to that graph's memory for as long as the graph lives."""
+    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
 
 
 def clear_workspace_cache() -> None:
-    with _WS_LOCK:
-        _WS.clear()
+    """Nothing to do: no call keeps its workspace. (``torch.cuda.empty_cache()`` returns the allocator's
+    unused memory to the device.)"""
 
 
 def _check(cond: bool, msg: str) -> None:
@@ -95,7 +87,7 @@ def moe_align(topk_ids: torch.Tensor, num_experts: int, block_m: int = BLOCK_M) 
         meta=torch.empty(4, **i32),
     )
     nbytes = _lib.lib().moe_align_workspace_bytes(R, num_experts)
-    ws = _workspace(("align", dev, _stream(dev)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     _lib.call(
         "moe_align", topk_ids.data_ptr(), _ID_DTYPES[topk_ids.dtype], R, num_experts, block_m,
         al.group_sizes.data_ptr(), al.group_offsets.data_ptr(), al.group_padded_offsets.data_ptr(),
@@ -156,7 +148,7 @@ def fused_moe(
     dt = _DTYPES[hidden_states.dtype]
     fn = "moe_fused_ordered" if deterministic else "moe_fused"
     nbytes = getattr(_lib.lib(), fn + "_workspace_bytes")(T, k, E, H, I, dt)
-    ws = _workspace(("fused", dev, _stream(dev)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     _lib.call(
         fn, hidden_states.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(), topk_ids.data_ptr(),
         _ID_DTYPES[topk_ids.dtype], topk_weights.data_ptr(), _W_DTYPES[topk_weights.dtype], out.data_ptr(),
@@ -269,7 +261,7 @@ def fused_moe_router(
     if T:
         dt = _DTYPES[hidden_states.dtype]
         nbytes = _lib.lib().moe_fused_workspace_bytes(T, k, E, H, I, dt)
-        ws = _workspace(("fused", dev, _stream(dev)), nbytes, dev)
+        ws = _workspace(nbytes, dev)
         _lib.call(
             "moe_fused_router", hidden_states.data_ptr(), w_gate_up.data_ptr(), w_down.data_ptr(),
             gating_output.data_ptr(), _LOGIT_DTYPES[gating_output.dtype], int(bool(renormalize)), ids.data_ptr(),
@@ -317,7 +309,7 @@ def _fused_q8_rows(x_q, x_scale, q_dtype, w13_q, w13_scale, w2_q, w2_scale, topk
     dev, dt = x_q.device, _DTYPES[out.dtype]
     int8 = q_dtype == torch.int8
     nbytes = getattr(_lib.lib(), "moe_fused_int8_workspace_bytes" if int8 else "moe_fused_fp8_workspace_bytes")(T, k, E, H, I, dt)
-    ws = _workspace(("fused_i8" if int8 else "fused_f8", dev, _stream(dev)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     _lib.call(
         "moe_fused_q8_rows", x_q.data_ptr(), x_scale.data_ptr(), _lib.MOE_I8 if int8 else _lib.MOE_F8E4M3, w13_q.data_ptr(),
         w13_scale.data_ptr(), w2_q.data_ptr(), w2_scale.data_ptr(), topk_ids.data_ptr(), _ID_DTYPES[topk_ids.dtype],
@@ -359,7 +351,7 @@ def fused_moe_int8(
     dev = hidden_states.device
     dt = _DTYPES[hidden_states.dtype]
     nbytes = _lib.lib().moe_fused_int8_workspace_bytes(T, k, E, H, I, dt)
-    ws = _workspace(("fused_i8", dev, _stream(dev)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     _lib.call(
         "moe_fused_int8", hidden_states.data_ptr(), w13_q.data_ptr(), w13_scale.data_ptr(), w2_q.data_ptr(),
         w2_scale.data_ptr(), topk_ids.data_ptr(), _ID_DTYPES[topk_ids.dtype], topk_weights.data_ptr(),
@@ -418,7 +410,7 @@ def fused_moe_fp8(
     dev = hidden_states.device
     dt = _DTYPES[hidden_states.dtype]
     nbytes = _lib.lib().moe_fused_fp8_workspace_bytes(T, k, E, H, I, dt)
-    ws = _workspace(("fused_f8", dev, _stream(dev)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     _lib.call(
         "moe_fused_fp8", hidden_states.data_ptr(), w13_q.data_ptr(), w13_scale.data_ptr(), w2_q.data_ptr(),
         w2_scale.data_ptr(), topk_ids.data_ptr(), _ID_DTYPES[topk_ids.dtype], topk_weights.data_ptr(),

@@ -1,7 +1,7 @@
 """CUDA-graph capture of a fused MoE call.
 
-Every library entry point is stream-ordered, keeps its block counts on the device and reuses a
-cached workspace, so one call (alignment, gather, both grouped GEMMs) can be captured into a
+Every library entry point is stream-ordered and keeps its block counts on the device, and its
+workspace is allocated per call (in the graph's own memory during a capture), so one call (alignment, gather, both grouped GEMMs) can be captured into a
 CUDA graph and replayed with one launch: the per-kernel host launch cost (seven launches per call)
 disappears, which is what dominates small, decode-sized calls.
 

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, launch, pitch, raw_stream, require, rows
+from ._args import FLOATS, launch, pitch, require, rows
 from .fused import _workspace
 
 _Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -158,7 +158,7 @@ def add_rms_norm_backward(
     dx = torch.empty_like(h, memory_format=torch.contiguous_format)
     dweight = torch.empty_like(weight)
     nbytes = _lib.lib().moe_add_rms_norm_backward_workspace_bytes(T, H)
-    ws = _workspace(("norm_bwd", dev, raw_stream(dev.index)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     launch(dev, "moe_add_rms_norm_backward", y2.data_ptr(), pitch(y2), h2.data_ptr(), pitch(h2), *dh_args,
            weight.data_ptr(), wdt, dx.data_ptr(), H, dweight.data_ptr(), T, H, eps, FLOATS[h2.dtype], ws.data_ptr(),
            ws.numel())

@@ -2,22 +2,17 @@
 
 ``run_kernel`` keeps the reference signature and semantics (初审材料/源代码/submission.py:2098-2184):
 ten positional tensors, ``out`` is the only tensor written, padding rows of ``out`` end up 0,
-empty inputs take the same shortcuts (:2117-2153), the ``up_logits`` scratch is cached (:2081-2095;
-here per device and stream, grown as needed) and both fp32 and fp16 routed weights are accepted
+empty inputs take the same shortcuts (:2117-2153), the ``up_logits`` scratch is reused (:2081-2095;
+here through PyTorch's caching allocator) and both fp32 and fp16 routed weights are accepted
 (:2125-2128). The work runs in
 two sm_100a kernels of ``libmoe_b200.so`` on the current CUDA stream, with no host
 synchronisation.
 """
 from __future__ import annotations
 
-import threading
-
 import torch
 
 from . import _lib
-
-_WORKSPACE_CACHE: dict = {}
-_WS_LOCK = threading.Lock()
 
 _DTYPES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
 _ROUTED_DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16}
@@ -29,17 +24,11 @@ def _stream_handle(device: torch.device) -> int:
 
 def _get_workspace(x: torch.Tensor, intermediate: int) -> torch.Tensor:
     """Scratch for the Stage1 output ``up_logits`` [P, I] (reference ``_get_workspace``, which caches
-    one buffer per shape). Here one buffer per device and stream, grown when a call needs more:
-    calls on one stream run in order, so they can share it whatever their shapes, calls on
-    different streams never share it, and the cache is bounded by the largest call."""
+    one buffer per shape). Here each call has its own from PyTorch's caching allocator, which hands the
+    same memory to the next call on the stream: two threads may call on one stream, and a captured
+    graph keeps its buffer."""
     nbytes = _lib.lib().moe_run_kernel_workspace_bytes(x.shape[0], intermediate, _DTYPES[x.dtype])
-    key = (x.device, _stream_handle(x.device))
-    with _WS_LOCK:
-        ws = _WORKSPACE_CACHE.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=x.device)
-            _WORKSPACE_CACHE[key] = ws
-    return ws
+    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=x.device)
 
 
 def _require(cond: bool, msg: str) -> None:

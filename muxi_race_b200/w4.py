@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, launch, pitch, raw_stream, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, launch, pitch, require, rows
 from .fused import _workspace
 
 
@@ -141,11 +141,9 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
     nbytes = w.sizes.get(M)
     if nbytes is None:
         nbytes = w.sizes[M] = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, HALVES[w.dtype])
-    ws_ptr = None
-    if nbytes:
-        ws_ptr = _workspace(("w4_linear", dev, raw_stream(dev.index)), nbytes, dev).data_ptr()
+    ws = _workspace(nbytes, dev) if nbytes else None  # held until the call has been launched
     launch(dev, "moe_w4_linear", x2.data_ptr(), pitch(x2), w.packed.data_ptr(), out.data_ptr(), ld_out, M, N, K,
-           w.group_size, w.has_zeros, FLOATS[w.dtype], ws_ptr, nbytes)
+           w.group_size, w.has_zeros, FLOATS[w.dtype], None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
@@ -194,7 +192,7 @@ def fused_moe_w4(
     if nbytes is None:
         nbytes = w13.sizes[T, k] = _lib.lib().moe_fused_w4_workspace_bytes(
             T, k, E, H, I, w13.group_size, w2.group_size, HALVES[w13.dtype])
-    ws = _workspace(("fused_w4", dev, raw_stream(dev.index)), nbytes, dev)
+    ws = _workspace(nbytes, dev)
     launch(dev, "moe_fused_w4", x.data_ptr(), pitch(x), w13.packed.data_ptr(), w13.group_size, w13.has_zeros,
            w2.packed.data_ptr(), w2.group_size, w2.has_zeros, topk_ids.data_ptr(), IDS[topk_ids.dtype],
            topk_weights.data_ptr(), FLOATS[topk_weights.dtype], out.data_ptr(), T, H, I, E, k, FLOATS[w13.dtype],
