@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, launch, pitch, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, launch, overlap, pitch, require, rows
 from .fused import _workspace
 
 
@@ -119,7 +119,7 @@ def dequantize_w4(w: W4Weights) -> torch.Tensor:
 def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ W.T`` for a few rows x [..., K] (fp16 / bf16, the dtype of the weight's scales).
 
-    Sums in fp32, rounded once. The weights are read once for up to 16 rows, and again for every 16
+    Sums in fp32, rounded once. ``out`` must not share memory with x. The weights are read once for up to 16 rows, and again for every 16
     more: for a prompt, ``torch.matmul`` with :func:`dequantize_w4` is the better call.
     """
     if len(w.shape) != 2 or w.gate_up:
@@ -137,7 +137,10 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
         ld_out = N
     else:
         require(tuple(out.shape) == (*x.shape[:-1], N) and out.dtype == w.dtype, f"out must be {w.dtype} [..., {N}]")
-        ld_out = pitch(rows(out, "out", dev))
+        out2 = rows(out, "out", dev)
+        # a block may still read rows of x when another stores its columns of them
+        require(not overlap(out2, x2), "out must not share memory with x")
+        ld_out = pitch(out2)
     nbytes = w.sizes.get(M)
     if nbytes is None:
         nbytes = w.sizes[M] = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, HALVES[w.dtype])
