@@ -462,8 +462,8 @@ MOE_API int moe_ep_p2p_push_finish(const void* own_region, int64_t num_tokens, i
  *   pitches ld_x, ld_residual in elements; weight [H] weight_dtype (dtype or MOE_F32).
  *   h_out [T, H] dtype, pitch ld_h, or NULL. out [T, H], pitch ld_out: dtype when out_dtype == dtype;
  *   with out_dtype MOE_I8 / MOE_F8E4M3 8-bit rows with scale [T] fp32 = max|y| / 127 or / 448, as
- *   moe_quantize_rows_int8 / _fp8 (y is not rounded to dtype in between). x, residual, h_out and (in
- *   dtype) out may be the same rows.
+ *   moe_quantize_rows_int8 / _fp8 (y is not rounded to dtype in between). h_out and (in dtype)
+ *   out may each be the rows of x or of residual themselves; other overlaps are not allowed.
  * moe_add_rms_norm_backward: dy, h [T, H] dtype, dh (gradient of h from its other uses, or NULL);
  *   dx [T, H] dtype = gradient of x, which is also that of the residual; dweight [H] weight_dtype.
  *   The dweight sum has a fixed order. workspace: moe_add_rms_norm_backward_workspace_bytes(T, H).

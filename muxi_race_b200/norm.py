@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, launch, pitch, require, rows
+from ._args import FLOATS, launch, overlap, pitch, require, rows
 from .fused import _workspace
 
 _Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -27,26 +27,32 @@ def _check_weight(weight: torch.Tensor, H: int, dtype: torch.dtype, dev: torch.d
     return FLOATS[weight.dtype]
 
 
-def _output(t: Optional[torch.Tensor], x: torch.Tensor, name: str):
-    """`t`, or a new tensor of x's shape and dtype, with its address and row pitch."""
+def _output(t: Optional[torch.Tensor], x: torch.Tensor, name: str, *others: Optional[torch.Tensor]):
+    """`t`, or a new tensor of x's shape and dtype, with its address and row pitch. `t` may be one of
+    `others` (2-D), row for row: a row is read before it is written. It may not share memory with them
+    in another way, where a row would be written while another is read from the same place."""
     if t is None:
         t = torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
         return t, t.data_ptr(), x.shape[-1]
     require(t.shape == x.shape and t.dtype == x.dtype, f"{name} must have the shape and dtype of x")
     t2 = rows(t, name, x.device)
-    return t, t2.data_ptr(), pitch(t2)
+    ptr, ld = t2.data_ptr(), pitch(t2)
+    for o in others:
+        if o is not None and not (o.data_ptr() == ptr and pitch(o) == ld) and overlap(t2, o):
+            raise ValueError(f"{name} must be x or residual itself, or share no memory with them")
+    return t, ptr, ld
 
 
-def _sum_args(x, residual, residual_out):
-    """(h, residual's address and pitch, h's address and pitch); no residual: h is None."""
+def _sum_args(x, x2, residual, residual_out):
+    """(residual's rows, h, residual's address and pitch, h's address and pitch); no residual: h is None."""
     if residual is None:
         require(residual_out is None, "residual_out needs a residual")
-        return None, None, 0, None, 0
+        return None, None, None, 0, None, 0
     if residual.shape != x.shape or residual.dtype != x.dtype:
         raise ValueError("residual must have the shape and dtype of x")
     r2 = rows(residual, "residual", x.device)
-    h, h_ptr, h_ld = _output(residual_out, x, "residual_out")
-    return h, r2.data_ptr(), pitch(r2), h_ptr, h_ld
+    h, h_ptr, h_ld = _output(residual_out, x, "residual_out", x2, r2)
+    return r2, h, r2.data_ptr(), pitch(r2), h_ptr, h_ld
 
 
 def _forward(x, weight, residual, eps, out, residual_out):
@@ -54,8 +60,10 @@ def _forward(x, weight, residual, eps, out, residual_out):
     T, H = x2.shape
     dtype, dev = x2.dtype, x2.device
     wdt = _check_weight(weight, H, dtype, dev)
-    y, y_ptr, y_ld = _output(out, x, "out")
-    h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, residual, residual_out)
+    r2, h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x2, residual, residual_out)
+    y, y_ptr, y_ld = _output(out, x, "out", x2, r2)
+    if out is not None and residual_out is not None:
+        require(not overlap(rows(out, "out"), rows(residual_out, "residual_out")), "out and residual_out share memory")
     dt = FLOATS[dtype]
     launch(dev, "moe_add_rms_norm", x2.data_ptr(), pitch(x2), r_ptr, r_ld, weight.data_ptr(), wdt, y_ptr, y_ld, dt, None,
            h_ptr, h_ld, T, H, eps, dt)
@@ -94,7 +102,8 @@ def add_rms_norm(
 
     x, residual [..., H] fp16 / bf16 / fp32 with contiguous rows of any one pitch; weight [H] in x's
     dtype or fp32. The sum and the statistics are fp32, y is normalised from the unrounded sum.
-    ``out`` and ``residual_out`` may be x or residual themselves (updated in place). Differentiable
+    ``out`` and ``residual_out`` may be x or residual themselves (updated in place), but share no other memory
+    with them or with each other. Differentiable
     in x, weight and residual when neither is given.
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
@@ -126,7 +135,7 @@ def add_rms_norm_quant(
     wdt = _check_weight(weight, H, dtype, dev)
     q = torch.empty_like(x, dtype=q_dtype, memory_format=torch.contiguous_format)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, residual, residual_out)
+    _, h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x2, residual, residual_out)
     launch(dev, "moe_add_rms_norm", x2.data_ptr(), pitch(x2), r_ptr, r_ld, weight.data_ptr(), wdt, q.data_ptr(), H,
            _Q_DTYPES[q_dtype], scale.data_ptr(), h_ptr, h_ld, T, H, eps, FLOATS[dtype])
     return q, scale, h
