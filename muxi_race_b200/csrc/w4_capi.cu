@@ -17,8 +17,8 @@ size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 // How one product is laid over the GPU.
 struct W4Plan {
   int strips, kt, nt, warps, wps;
-  int tile_rows, slices, slice_kt, x_pitch, x_bytes, start_bytes, sum_bytes;
-  size_t smem() const { return static_cast<size_t>(x_bytes) + start_bytes + sum_bytes; }
+  int tile_rows, slices, slice_kt, x_pitch, x_bytes, sum_bytes;
+  size_t smem() const { return static_cast<size_t>(x_bytes) + sum_bytes; }
 };
 
 // What handing on a strip's sum takes in tile times, and what each further strip at a time adds (more
@@ -27,7 +27,7 @@ constexpr double kW4SumCost = 0.4, kW4GroupCost = 0.03;
 constexpr int kW4Smem = kMaxDynamicSmem - 1024;  // static shared memory of the kernel, rounded up
 
 // `tiles`: token tiles expected, `sms`: CTAs.
-W4Plan w4_plan(int strips, int64_t K, int group, int dtype, int tile_rows, double tiles, int sms) {
+W4Plan w4_plan(int strips, int64_t K, int group, int tile_rows, double tiles, int sms) {
   W4Plan p{};
   p.strips = strips;
   p.kt = static_cast<int>(ceil_div(K, kW4TileK));
@@ -35,14 +35,12 @@ W4Plan w4_plan(int strips, int64_t K, int group, int dtype, int tile_rows, doubl
   p.nt = tile_rows <= 8 ? 1 : 2;
   p.warps = w4_warps(group, p.nt);
   p.sum_bytes = 2 * p.warps * p.nt * 1024;
-  // K is cut so that the rows' slice of x (and the starts of its sums) fits in shared memory
-  const int start_kt = dtype == MOE_F16 ? kW4TileK / group * p.nt * 64 : 0;
-  const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows + start_kt);
+  // K is cut so that the rows' slice of x fits in shared memory
+  const int64_t most = (kW4Smem - p.sum_bytes - 128 - tile_rows * 64) / (2 * kW4TileK * tile_rows);
   p.slice_kt = static_cast<int>(ceil_div(p.kt, ceil_div(p.kt, most)));
   p.slices = static_cast<int>(ceil_div(p.kt, p.slice_kt));
   p.x_pitch = p.slice_kt * 2 * kW4TileK + 64;  // 64: rows r and r + 1 in different banks
   p.x_bytes = static_cast<int>(ceil_div(static_cast<int64_t>(tile_rows) * p.x_pitch, 128) * 128);
-  p.start_bytes = p.slice_kt * start_kt;
   // Warps per strip: few make the sums rare, many let a CTA's groups of warps finish together. The
   // cost of a choice in tile times: the rounds of the worst CTA, each a warp's tiles and what handing
   // on a sum takes. A CTA whose strips are of two token tiles (or slices) starts a round for each.
@@ -138,7 +136,6 @@ W4Args w4_args(const W4Plan& p, const void* w, int64_t expert_bytes, uint32_t* s
   a.tile_rows = p.tile_rows;
   a.x_pitch = p.x_pitch;
   a.x_bytes = p.x_bytes;
-  a.start_bytes = p.start_bytes;
   a.status = status;
   return a;
 }
@@ -203,16 +200,15 @@ int moe_tile_rows(int64_t R, int64_t E) {
   return static_cast<int>(std::min<int64_t>(per_expert <= 4 ? 8 : kW4MaxRows, R));
 }
 
-W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int g13, int g2, int dtype,
-                          int sms) {
+W4MoeLayout w4_moe_layout(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int g13, int g2, int sms) {
   W4MoeLayout L{};
   const int64_t R = T * topk;
   const int tile_rows = moe_tile_rows(R, E);
   // experts chosen by someone, if all are equally likely
   const double active = static_cast<double>(E) * (1 - std::pow(1 - 1.0 / static_cast<double>(E), static_cast<double>(R)));
   const double tiles = std::max(active, static_cast<double>(R) / tile_rows);
-  L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, dtype, tile_rows, tiles, sms);
-  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * (kW4TileRows / 2), g2, dtype, tile_rows, tiles, sms);
+  L.p1 = w4_plan(w4_strips(2 * I, 1), H, g13, tile_rows, tiles, sms);
+  L.p2 = w4_plan(w4_strips(H, 0), L.p1.strips * (kW4TileRows / 2), g2, tile_rows, tiles, sms);
   L.max_tiles = R / tile_rows + std::min(E, R);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -378,9 +374,10 @@ int moe_w4_unpack(const void* packed, int dtype, int64_t matrices, int64_t N, in
 }
 
 size_t moe_w4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int dtype) {
+  (void)dtype;
   clear_error();
   if (M < 1 || M > kMaxSize || check_format(1, N, K, group, 0) != MOE_OK) return 0;
-  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, dtype, linear_tile_rows(M), 1, 1);
+  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, linear_tile_rows(M), 1, 1);
   return p.slices == 1 ? 0 : sizeof(float) * static_cast<size_t>(p.slices) * static_cast<size_t>(M) * p.strips * kW4TileRows;
 }
 
@@ -407,7 +404,7 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
   const int tile_rows = linear_tile_rows(M);
   if (M / tile_rows > kMaxStrips / w4_strips(N, 0) / ceil_div(K, kW4TileK))
     return fail(MOE_ERR_INVALID_ARG, "too many rows for one call");
-  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, dtype, tile_rows, ceil_div(M, tile_rows), sms);
+  const W4Plan p = w4_plan(w4_strips(N, 0), K, group, tile_rows, ceil_div(M, tile_rows), sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   float* part = static_cast<float*>(workspace);
   return dtype == MOE_F16
@@ -418,9 +415,10 @@ int moe_w4_linear(const void* x, int64_t ld_x, const void* packed, void* out, in
 
 size_t moe_fused_w4_workspace_bytes(int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I, int group13, int group2,
                                     int dtype) {
+  (void)dtype;
   clear_error();
   if (T < 1 || check_moe(T, topk, E, H, I, group13, group2) != MOE_OK) return 0;
-  return w4_moe_layout(T, topk, E, H, I, group13, group2, dtype, 1).total;
+  return w4_moe_layout(T, topk, E, H, I, group13, group2, 1).total;
 }
 
 int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int has_zeros13, const void* w2, int group2,
@@ -443,7 +441,7 @@ int moe_fused_w4(const void* x, int64_t ld_x, const void* w13, int group13, int 
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &status));
-  const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, group2, dtype, sms);
+  const W4MoeLayout L = w4_moe_layout(T, topk, E, H, I, group13, group2, sms);
   if (L.max_tiles > kMaxStrips / std::max<int64_t>(L.p1.strips * L.p1.slices, L.p2.strips * L.p2.slices))
     return fail(MOE_ERR_INVALID_ARG, "too many tokens for one call");
   if (!workspace || workspace_bytes < L.total) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", L.total);

@@ -73,7 +73,7 @@ struct W4Args {
   float* part;              // kW4Partial: [slice][row][strips * 32]
   long long part_rows;
   int x_pitch;              // bytes of a row of x in shared memory
-  int x_bytes, start_bytes; // bytes of the rows of x, and of where the groups' sums start (fp16)
+  int x_bytes;              // bytes of the rows of x
   int early;                // the tile list is older than the kernel before this one
   uint32_t* status;
 };
@@ -87,13 +87,16 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 // ------------------------------------------------------------------ unpacking
 // Eight values of a word as A fragments: nibble i of the low (high) half is the first (second) value
 // of register i; registers 0 and 2 are row r, 1 and 3 row r + 8.
-//   fp16: the nibbles themselves, as the low bits of a subnormal number, are q 2^-24 (row r) and
-//     q 2^-20 (row r + 8, one nibble further up): no instruction but the masks. The sums carry those
-//     powers of two to their end, and the zero points enter as the start of each group's sum:
-//     sum (q - z) x = -z sum x + sum q x.
-//   bf16 (whose subnormal products fp32 cannot hold): the nibbles become the low bits of 1/2 + q / 256,
-//     and one subtraction gives (q - z) / 256, exactly. (At this size a group's sum overflows fp32 only
-//     where x is beyond 4e37; with whole numbers it would at 2e37 / 128.)
+//   fp16: nibbles in bits 0..3 (row r) become the low bits of 1024 + q, nibbles in bits 4..7 (row
+//     r + 8) those of 64 + q, and one subtraction gives q - z.
+//   bf16 (of 8 bits): the nibbles become the low bits of 1/2 + q / 256, and one subtraction gives
+//     (q - z) / 256. (At this size a group's sum overflows fp32 only where x is beyond 4e37; with whole
+//     numbers it would at 2e37 / 128.)
+// The differences are formed before the products, exactly: a weight of 0 adds nothing, whatever its x. (As
+// -z sum x + sum q x, with the nibbles as they are, fp16 would take four instructions less per eight
+// values: 128 tokens over 256 experts of 7168 x 2048 1103 us instead of 1240, one token over 8 54 instead of
+// 57, a single row of 14336 x 4096 the same. But the terms of a large x at q = z would cancel only to
+// fp32's rounding of them: with x of 6e4 beside 1e-3 nothing of the small columns' sum is left.)
 template <typename T> struct W4Type;
 __device__ __forceinline__ uint32_t w4_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
   uint32_t v;
@@ -101,14 +104,22 @@ __device__ __forceinline__ uint32_t w4_and_or(uint32_t w, uint32_t mask, uint32_
   return v;
 }
 template <> struct W4Type<__half> {
-  static constexpr bool kSums = true;
-  static constexpr float kScale0 = 16777216.0f, kScale1 = 1048576.0f;
-  static __device__ __forceinline__ void unpack(uint32_t w, const uint32_t (&)[2], uint32_t (&a)[4]) {
-    a[0] = w & 0x000f000fu;
-    a[1] = w & 0x00f000f0u;
+  static constexpr float kScale = 1.0f;
+  // the subtrahends of rows r and r + 8: 1024 + z (one step is 1) and 64 + z (one step is 1/16)
+  static __device__ __forceinline__ void offsets(uint32_t z0, uint32_t z1, uint32_t (&c)[2]) {
+    c[0] = 0x64006400u + z0 * 0x10001u;
+    c[1] = 0x54005400u + z1 * 0x100010u;
+  }
+  static __device__ __forceinline__ uint32_t sub(uint32_t v, uint32_t c) {
+    asm("sub.f16x2 %0, %0, %1;" : "+r"(v) : "r"(c));
+    return v;
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, const uint32_t (&c)[2], uint32_t (&a)[4]) {
+    a[0] = sub(w4_and_or(w, 0x000f000fu, 0x64006400u), c[0]);
+    a[1] = sub(w4_and_or(w, 0x00f000f0u, 0x54005400u), c[1]);
     w >>= 8;
-    a[2] = w & 0x000f000fu;
-    a[3] = w & 0x00f000f0u;
+    a[2] = sub(w4_and_or(w, 0x000f000fu, 0x64006400u), c[0]);
+    a[3] = sub(w4_and_or(w, 0x00f000f0u, 0x54005400u), c[1]);
   }
   static __device__ __forceinline__ float to_f(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits))); }
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
@@ -120,9 +131,12 @@ template <> struct W4Type<__half> {
   }
 };
 template <> struct W4Type<__nv_bfloat16> {
-  static constexpr bool kSums = false;
-  static constexpr float kScale0 = 256.0f, kScale1 = 256.0f;
-  // c: 1/2 + z / 256 of rows r and r + 8 (bf16 1/2: one step is 1 / 256)
+  static constexpr float kScale = 256.0f;
+  // the subtrahends of rows r and r + 8: 1/2 + z / 256 (one step is 1 / 256)
+  static __device__ __forceinline__ void offsets(uint32_t z0, uint32_t z1, uint32_t (&c)[2]) {
+    c[0] = 0x3f003f00u + z0 * 0x10001u;
+    c[1] = 0x3f003f00u + z1 * 0x10001u;
+  }
   static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t c) {
     uint32_t v = w4_and_or(w, 0x000f000fu, 0x3f003f00u);
     asm("sub.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(c));
@@ -189,34 +203,21 @@ struct W4Frag {
 
 // acc[f] += fragment rows f of the tile * x for NT blocks of 8 rows of x (shared addresses), in units
 // of 1 / kScale. `x`: this lane's columns of row 0; xrow[t]: the offset of its row of block t (a lane
-// whose row does not exist reads another's: the column that it makes of it is not stored). `start`
-// (fp16): this lane's starts of the tile's first group, `start_group` bytes from one group to the next
-// (see w4_load_x).
+// whose row does not exist reads another's: the column that it makes of it is not stored).
 template <typename T, int GROUP, bool ZEROS, int NT>
-__device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& in, uint32_t x, const int (&xrow)[NT], uint32_t start,
-                                        int start_group, float (&acc)[2][NT][4]) {
+__device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& in, uint32_t x, const int (&xrow)[NT],
+                                        float (&acc)[2][NT][4]) {
   constexpr int kGroups = kW4TileK / GROUP;
   constexpr int kBlocks = GROUP / 32;  // blocks of 32 columns in a group
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    uint32_t z[4] = {8, 8, 8, 8};
-    if constexpr (ZEROS)
+    uint32_t off[2][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z[i] = (in.z[g] >> (8 * i)) & 0xff;
-    float c[2][NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if constexpr (W4Type<T>::kSums) v = lds128(start + g * start_group + t * 64);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float f0 = ZEROS ? static_cast<float>(z[2 * f]) : 1.0f, f1 = ZEROS ? static_cast<float>(z[2 * f + 1]) : 1.0f;
-        c[f][t][0] = f0 * __uint_as_float(v.x);
-        c[f][t][1] = f0 * __uint_as_float(v.y);
-        c[f][t][2] = f1 * __uint_as_float(v.z);
-        c[f][t][3] = f1 * __uint_as_float(v.w);
-      }
+    for (int f = 0; f < 2; ++f) {
+      const uint32_t z = ZEROS ? in.z[g] >> (16 * f) : 0x0808u;
+      W4Type<T>::offsets(z & 0xff, (z >> 8) & 0xff, off[f]);
     }
+    float c[2][NT][4] = {};
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const int block = g * kBlocks + b;
@@ -228,9 +229,8 @@ __device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& in, uint32_t
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const uint4& w = in.w[block / 2][f];
-          const uint32_t off[2] = {0x3f003f00u + z[2 * f] * 0x10001u, 0x3f003f00u + z[2 * f + 1] * 0x10001u};
           uint32_t a[4];
-          W4Type<T>::unpack(block % 2 == 0 ? (step == 0 ? w.x : w.y) : (step == 0 ? w.z : w.w), off, a);
+          W4Type<T>::unpack(block % 2 == 0 ? (step == 0 ? w.x : w.y) : (step == 0 ? w.z : w.w), off[f], a);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
             W4Type<T>::mma(c[f][t], a, step == 0 ? xv[t].x : xv[t].z, step == 0 ? xv[t].y : xv[t].w, c[f][t]);
@@ -259,8 +259,8 @@ template <typename T>
 __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int out_row, int rows, int t, int f,
                                          const float4& v) {
   const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
-  const float lo[2] = {v.x * W4Type<T>::kScale0, v.y * W4Type<T>::kScale0};
-  const float hi[2] = {v.z * W4Type<T>::kScale1, v.w * W4Type<T>::kScale1};
+  const float lo[2] = {v.x * W4Type<T>::kScale, v.y * W4Type<T>::kScale};
+  const float hi[2] = {v.z * W4Type<T>::kScale, v.w * W4Type<T>::kScale};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int m = t * 8 + q * 2 + i;
@@ -366,17 +366,16 @@ struct W4Stream {
 };
 
 // One segment of a consumer warp: its strips s0 + group, s0 + group + groups, ...
-template <typename T, int GROUP, bool ZEROS, int NTMAX, int NT, int AHEAD>
+template <typename T, int GROUP, bool ZEROS, int NT, int AHEAD>
 __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP, ZEROS, AHEAD>& in, W4Sums& sums, uint32_t x,
-                                           uint32_t start, int part, int rows, int strips, int rounds,
+                                           int part, int rows, int strips, int rounds,
                                            volatile int* abort_flag) {
   const int lane = threadIdx.x & 31;
   int xrow[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) xrow[t] = min(t * 8 + (lane >> 2), rows - 1) * a.x_pitch;
-  constexpr int kStartGroup = NTMAX * 64, kStartTile = kW4TileK / GROUP * kStartGroup;
-  const uint32_t x0 = x + (lane & 3) * 16 + part * (kW4TileK * 2), start0 = start + (lane & 3) * 16 + part * kStartTile;
-  uint32_t xl = x0, sl = start0;
+  const uint32_t x0 = x + (lane & 3) * 16 + part * (kW4TileK * 2);
+  uint32_t xl = x0;
   float acc[2][NT][4] = {};
   auto flush = [&]() {
     mbar_wait(&sums.empty[sums.slot()], sums.phase() ^ 1, abort_flag, a.status);
@@ -397,14 +396,12 @@ __device__ __forceinline__ void w4_segment(const W4Args& a, W4Stream<GROUP, ZERO
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (j < n) {
-        w4_tile<T, GROUP, ZEROS, NT>(in.frag[j], xl, xrow, sl, kStartGroup, acc);
+        w4_tile<T, GROUP, ZEROS, NT>(in.frag[j], xl, xrow, acc);
         in.load(j);
         xl += a.wps * (kW4TileK * 2);
-        sl += a.wps * kStartTile;
         if (--k == 0) {
           k = in.nk;
           xl = x0;
-          sl = start0;
           flush();
         }
       }
@@ -437,63 +434,17 @@ __device__ __forceinline__ void w4_load_x(const W4Args& a, uint8_t* smem, int fi
   }
 }
 
-// fp16: where each group's sums start: per group and pair of rows of x four numbers, -z 2^-24 sum x of
-// the two rows (z = 8, or 1 where the records hold zero points) and 16 times that.
-template <typename T, int GROUP, bool ZEROS, int NTMAX, int WARPS>
-__device__ __forceinline__ void w4_starts(const W4Args& a, uint8_t* smem, int rows, int kts) {
-  constexpr int kLanes = GROUP / 8;  // of a group
-  constexpr int kBatch = 4;          // rows at a time, so that their loads are in flight together
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int words = kts * (kW4TileK / 8);
-  for (int m0 = 0; m0 < rows; m0 += kBatch)
-    for (int w0 = warp * 32; w0 < words; w0 += WARPS * 32) {
-      const int word = w0 + lane;
-      uint4 v[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        v[j] = make_uint4(0, 0, 0, 0);
-        if (m0 + j < rows && word < words) v[j] = lds128(smem_u32(smem) + (m0 + j) * a.x_pitch + word * 16);
-      }
-      float sum[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const __half2* h = reinterpret_cast<const __half2*>(&v[j]);
-        sum[j] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __half22float2(h[e]);
-          sum[j] += f.x + f.y;
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1)
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
-      if (lane % kLanes == 0 && word < words) {
-        float* group = reinterpret_cast<float*>(smem + a.x_bytes) + word / kLanes * (NTMAX * 16);
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int m = m0 + j;
-          const float start = sum[j] * (ZEROS ? -1.0f : -8.0f) / W4Type<T>::kScale0;
-          float* to = group + (m >> 1) * 4 + (m & 1);  // m < 8 NTMAX: rows of a block are whole batches
-          to[0] = start;
-          to[2] = start * (W4Type<T>::kScale0 / W4Type<T>::kScale1);
-        }
-      }
-    }
-}
-
 template <typename T, int GROUP, bool ZEROS, int NTMAX>
 __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(const W4Args a) {
   constexpr int kWarps = w4_warps(GROUP, NTMAX);
-  extern __shared__ __align__(128) uint8_t smem[];  // [x][starts of the sums][sums of the warps]
+  extern __shared__ __align__(128) uint8_t smem[];  // [x][sums of the warps]
   __shared__ uint64_t full[kWarps * 2], empty[kWarps * 2];
   __shared__ int abort_flag;
   constexpr int record = w4_record_bytes(GROUP, ZEROS);
   constexpr int kAhead = w4_ahead(GROUP, NTMAX);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = a.groups;
-  const uint32_t base = smem_u32(smem), starts = base + a.x_bytes, sums_at = starts + a.start_bytes;
+  const uint32_t base = smem_u32(smem), sums_at = base + a.x_bytes;
   constexpr int kSumBytes = kWarps * NTMAX * 1024;  // of all groups, one turn
   if (threadIdx.x == 0) {
     for (int i = 0; i < groups * 2; ++i) {
@@ -535,7 +486,7 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
           const int at = g * 2 + (turn & 1);
           mbar_wait(&full[at], (turn >> 1) & 1, &abort_flag, a.status);
           if (strip0 + g < seg.s1) {
-            const float4* buf = reinterpret_cast<const float4*>(smem + (sums_at - base) + (turn & 1) * kSumBytes) +
+            const float4* buf = reinterpret_cast<const float4*>(smem + a.x_bytes + (turn & 1) * kSumBytes) +
                                 g * a.wps * NTMAX * 64 + lane;
             for (int i = 0; i < 2 * nt; ++i) {
               float4 v = buf[i * 32];
@@ -588,14 +539,10 @@ __global__ void __launch_bounds__(w4_threads(GROUP, NTMAX), 1) w4_gemv_kernel(co
     fresh = false;
     cp_async_wait_all();
     named_sync(1, kWarps * 32);
-    if constexpr (W4Type<T>::kSums) {
-      w4_starts<T, GROUP, ZEROS, NTMAX, kWarps>(a, smem, rows, kts);
-      named_sync(1, kWarps * 32);
-    }
     if (NTMAX == 1 || rows <= 8)
-      w4_segment<T, GROUP, ZEROS, NTMAX, 1>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
+      w4_segment<T, GROUP, ZEROS, 1>(a, in, sums, base, part, rows, strips, rounds, &abort_flag);
     else
-      w4_segment<T, GROUP, ZEROS, NTMAX, NTMAX>(a, in, sums, base, starts, part, rows, strips, rounds, &abort_flag);
+      w4_segment<T, GROUP, ZEROS, NTMAX>(a, in, sums, base, part, rows, strips, rounds, &abort_flag);
   }
   if (fresh) grid_dep_wait();  // a CTA without work: its end must still follow the kernel before
 }

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import muxi_race_b200 as m
+from oracle.w4_ref import linear_ref, w4_values_ref
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -56,3 +57,62 @@ def test_norm_refuses_outputs_over_other_rows(cuda_device):
     wide[:, :H], wide[:, H:2 * H] = x, res
     m.add_rms_norm(wide[:, :H], w, wide[:, H:2 * H], out=wide[:, 2 * H:], residual_out=wide[:, H:2 * H])
     assert torch.equal(wide[:, 2 * H:], y) and torch.equal(wide[:, H:2 * H], h) and torch.equal(wide[:, :H], x)
+
+
+U = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
+TINY = {F16: 2.0 ** -25, BF16: 0.0}
+F32 = 5e-6  # of the sum of |x| |W|, as derived in test_w4_gpu.py: the products are of exact q - z
+
+
+def w4_random(seed, N, K, group, zeros, dtype):
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    G = -(-K // group)
+    v = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8)
+    s = ((torch.rand((N, G), generator=g) + 0.5) * 0.2 * K ** -0.5).to(dtype)
+    z = torch.randint(0, 16, (N, G), generator=g, dtype=torch.uint8) if zeros else None
+    return v, s, z
+
+
+def w4_packed(v, s, z, group):
+    """(the package's weights, their values in fp64) of codes v [N, K]."""
+    N, K = v.shape
+    v = torch.nn.functional.pad(v, (0, K % 2))
+    q = (v[:, 0::2] | v[:, 1::2] << 4).contiguous().cuda()
+    s, z = s.cuda(), None if z is None else z.cuda()
+    return (m.pack_w4(q, s, z, in_features=K, group_size=group), w4_values_ref(q, s, z, K, group))
+
+
+@pytest.mark.parametrize("M", [1, 8, 11, 16, 40])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size,outlier", [(0.1, 1e4), (0.01, 2000.0), (1e-3, 6e4)])
+def test_w4_outliers_where_the_weight_is_zero(cuda_device, M, group, zeros, dtype, size, outlier):
+    """A few channels of x far above the others, whose codes are the zero point: they add exactly nothing."""
+    N, K = 70, 700
+    v, s, z = w4_random(7, N, K, group, zeros, dtype)
+    x = randn(8, M, K, scale=size)
+    for c in (3, 77, 130, 131, 400, 699):
+        v[:, c] = 8 if z is None else z[:, c // group]
+        x[:, c] = outlier * (1 if c % 2 else -0.7)
+    w, values = w4_packed(v, s, z, group)
+    x = x.to(dtype)
+    ref, mag = linear_ref(x, values)
+    assert float(mag.amax()) < 100 * size  # the outliers are in no term
+    within(m.w4_linear(x, w), ref, U[dtype] * ref.abs() + F32 * mag + TINY[dtype], "y")
+    assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_w4_infinities_keep_their_sign(cuda_device, dtype, zeros):
+    """An infinite value makes a sum infinite with the sign of its weight, and NaN where that is 0."""
+    v, s, z = w4_random(9, 96, 300, 32, zeros, dtype)
+    w, values = w4_packed(v, s, z, 32)
+    x = randn(10, 12, 300).to(dtype)
+    x[2, 5], x[7, 250], x[9, 0], x[9, 299] = float("inf"), float("-inf"), float("inf"), float("inf")
+    y, ref = m.w4_linear(x, w).double(), x.double() @ values.mT
+    spoilt = [2, 7, 9]
+    assert torch.equal(y[spoilt].nan_to_num(nan=1e9), ref[spoilt].nan_to_num(nan=1e9)) and bool(ref[2].isinf().any())
+    fine = [i for i in range(12) if i not in spoilt]
+    within(y[fine], ref[fine], U[dtype] * ref[fine].abs() + F32 * (x.double().abs() @ values.abs().mT)[fine] + TINY[dtype], "y")
