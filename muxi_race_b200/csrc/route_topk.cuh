@@ -13,7 +13,8 @@
 // Gradient for the logits, with g = scale * dweights and p the weights before the scale:
 //   softmax, renormalised   dl_j = p_j (g_j - sum g p)          at the chosen j, 0 elsewhere
 //   softmax                 dl_e = (g_e p_e at the chosen) - p_e sum g p
-//   sigmoid                 dl_j = d_j s_j (1 - s_j), d = g, renormalised (g - sum g s / D) / D, D = sum s
+//   sigmoid                 dl_j = g_j s_j (1 - s_j)            at the chosen j, 0 elsewhere
+//   sigmoid, renormalised   dl_j = p_j (g_j - sum g p) (1 - s_j)  at the chosen j, 0 elsewhere
 //
 // One warp per token, its logits in registers. The topk-th largest of the 32 lanes' own maxima is a
 // lower bound of the topk-th largest of all, and few candidates reach it (about 10 for topk = 8 of 256):
@@ -411,12 +412,13 @@ __global__ void __launch_bounds__(kRouteGradWarps * 32) route_topk_grad_kernel(c
       d = p * (g - route_sum(g * p));
     } else {
       const float s = e >= 0 ? route_sigmoid(v) : 0.0f;
-      if (a.renorm) {
-        float den = route_sum(s);
-        den = den < kRouteLeast ? kRouteLeast : den;
-        g = (g - route_sum(g * s) / den) / den;
+      float p = s;
+      if (a.renorm) {  // the weights first (at most 1), so that nothing is larger than the g
+        const float den = route_sum(s);
+        p = den == 0.0f ? 0.0f : s / den;
+        g -= route_sum(g * p);
       }
-      d = g * s * (1.0f - s);
+      d = g * p * (1.0f - s);
     }
     const float factor = -all / sum;
 #pragma unroll

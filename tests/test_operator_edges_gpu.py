@@ -116,3 +116,40 @@ def test_w4_infinities_keep_their_sign(cuda_device, dtype, zeros):
     assert torch.equal(y[spoilt].nan_to_num(nan=1e9), ref[spoilt].nan_to_num(nan=1e9)) and bool(ref[2].isinf().any())
     fine = [i for i in range(12) if i not in spoilt]
     within(y[fine], ref[fine], U[dtype] * ref[fine].abs() + F32 * (x.double().abs() @ values.abs().mT)[fine] + TINY[dtype], "y")
+
+
+def sigmoid_grad64(l, ids, dw, scale):
+    x = l.double().requires_grad_()
+    s = torch.sigmoid(x).gather(1, ids.long())
+    p = s / s.sum(-1, keepdim=True)
+    (p * dw.double() * scale).sum().backward()
+    p, g = p.detach(), dw.double().abs() * scale
+    return x.grad, torch.zeros_like(x.grad).scatter_add_(1, ids.long(), p * (g + (g * p).sum(-1, keepdim=True)))
+
+
+@pytest.mark.parametrize("size", [1.0, 100.0, 65536.0])
+def test_route_gradient_of_far_sigmoids(cuda_device, size):
+    """Renormalised sigmoid, every chosen logit far below 0 (a masked row, or a training that ran off) and
+    large gradients. While the scores are numbers of fp32 (above -88) the gradient is the formula's; below,
+    where every score and weight is 0, it is 0. W = 5e-6 as derived in test_route_topk_gpu.py; a subnormal
+    score adds half its spacing, 2e-7 of it at -88.5."""
+    T, E, k = 60, 16, 4
+    l = randn(20, T, E, scale=0.3) - torch.linspace(60, 88, T).cuda()[:, None]
+    l = l.clamp_min(-88.5)
+    dw = randn(21, T, k, scale=size)
+    _, ids = m.route_topk(l, k, scoring="sigmoid")
+    got = m.route_topk_backward(dw, l, ids, scoring="sigmoid", scale=2.5)
+    ref, mag = sigmoid_grad64(l, ids, dw, 2.5)
+    within(got, ref, 4 * 5e-6 * mag + 1e-37, "dlogits")
+    for far in (-100.0, -1e4):
+        l = torch.full((8, E), far, device="cuda")
+        l[4:] += randn(22, 4, E)
+        _, ids = m.route_topk(l, k, scoring="sigmoid")
+        got = m.route_topk_backward(dw[:8], l, ids, scoring="sigmoid", scale=2.5)
+        assert bool((got == 0).all())
+    l = torch.tensor([[-87.0, -88.0]], device="cuda")
+    got = m.route_topk_backward(torch.tensor([[100.0, 1.0]], device="cuda"), l, torch.tensor([[0, 1]], device="cuda", dtype=torch.int32),
+                                scoring="sigmoid")
+    p = 1 / (1 + 2.718281828459045 ** -1)
+    want = p * (100 - 100 * p - (1 - p))
+    within(got, torch.tensor([[want, -want]], dtype=torch.float64, device="cuda"), 4 * 5e-6 * 200, "dlogits")
