@@ -47,7 +47,6 @@ constexpr int kRouteMaxGroups = 32;
 // A bound by rounds up to this topk, by sorting above (T = 32768, E = 256, softmax: topk 4 18.2 against
 // 19.4 us, 6 19.6 against 20.3, 8 20.4 against 20.8, 10 the same, 12 23.2 against 22.9).
 constexpr int kRouteRounds = 8;
-constexpr float kRouteLeast = 1e-37f;  // a sum of scores that rounds to nothing divides as this
 constexpr unsigned kAllLanes = 0xffffffffu;
 enum { kRouteSoftmax = 0, kRouteSigmoid = 1 };
 
@@ -323,7 +322,7 @@ __global__ void __launch_bounds__(route_warps(VPL) * 32, route_blocks(VPL)) rout
       w = my_e >= 0 ? route_sigmoid(v) : 0.0f;
       if (a.renorm) {
         const float d = route_sum(w);
-        w /= d < kRouteLeast ? kRouteLeast : d;  // NaN stays
+        w = d == 0.0f ? 0.0f : w / d;  // every score rounded to 0 (logits below -88): no weights; NaN stays
       }
     }
     if (lane < a.topk) {

@@ -78,7 +78,8 @@ def route_topk(
     a group counting the sum of its ``group_top`` (1 or 2) best (-inf where fewer are eligible). Ids come in descending order, equal
     ones by the lower id; weights are the chosen scores, divided by their sum when ``renormalize``,
     times ``scale``. An expert whose logit is -inf is never chosen; slots left without one hold id -1
-    (which the expert operators skip) and weight 0. The weights are differentiable in the logits.
+    (which the expert operators skip) and weight 0. (A sigmoid below -88 is 0 in fp32: a token whose chosen scores are
+    all 0 has weights 0, renormalised or not.) The weights are differentiable in the logits.
     """
     if torch.is_grad_enabled() and logits.requires_grad:
         out = _RouteTopk.apply(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale,

@@ -153,3 +153,15 @@ def test_route_gradient_of_far_sigmoids(cuda_device, size):
     p = 1 / (1 + 2.718281828459045 ** -1)
     want = p * (100 - 100 * p - (1 - p))
     within(got, torch.tensor([[want, -want]], dtype=torch.float64, device="cuda"), 4 * 5e-6 * 200, "dlogits")
+
+
+def test_route_weights_of_far_sigmoids_add_up_to_one(cuda_device):
+    """Scores down to fp32's subnormal numbers (logits to -88.5, whose sum is below 1e-37) are divided by their
+    own sum."""
+    T, E, k = 100, 24, 5
+    l = (randn(30, T, E, scale=0.2) - torch.linspace(20, 88, T).cuda()[:, None]).clamp_min(-88.5)
+    w, ids = m.route_topk(l, k, scoring="sigmoid")
+    s = torch.sigmoid(l.double()).gather(1, ids.long())
+    ref = s / s.sum(-1, keepdim=True)
+    within(w, ref, 5e-6 * ref, "weights")
+    within(w.double().sum(-1), torch.ones(T, dtype=torch.float64, device="cuda"), 5e-6, "sum")
