@@ -63,6 +63,27 @@ def empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> to
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
+class _OnceDifferentiable(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, grads, *sources):
+        ctx.name = name
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} can be differentiated once: its gradient comes from a kernel without a graph")
+
+
+def once_differentiable(name: str, grads: tuple, *sources):
+    """The gradients that a kernel made of `sources`, as a backward function returns them. Where a graph of
+    them is being built (``create_graph=True``), differentiating them for whatever the sources come from
+    raises instead of passing them for constants. (``torch.autograd.function.once_differentiable`` sees the
+    incoming gradient only, and is passed over by ``torch.autograd.grad``, whose inputs it does not lead to.)"""
+    if not torch.is_grad_enabled():
+        return grads
+    return _OnceDifferentiable.apply(name, grads, *sources)
+
+
 def launch(device: torch.device, name: str, *args) -> None:
     """Call entry point `name` with the current stream of `device` appended, that device current."""
     fn = _functions.get(name)

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, launch, overlap, pitch, require, rows
+from ._args import FLOATS, launch, once_differentiable, overlap, pitch, require, rows
 from .fused import _workspace
 
 _Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -85,8 +85,8 @@ class _AddRmsNorm(torch.autograd.Function):
         if dy is None:  # only the sum was used
             dx, dweight = dh, None
         else:
-            dx, dweight = add_rms_norm_backward(dy.contiguous(), h, weight,
-                                                None if dh is None else dh.contiguous(), eps=ctx.eps)
+            dx, dweight = once_differentiable("add_rms_norm", add_rms_norm_backward(
+                dy.contiguous(), h, weight, None if dh is None else dh.contiguous(), eps=ctx.eps), dy, dh, h, weight)
         return dx, dweight, (dx if ctx.has_residual else None), None
 
 
@@ -104,7 +104,7 @@ def add_rms_norm(
     dtype or fp32. The sum and the statistics are fp32, y is normalised from the unrounded sum.
     ``out`` and ``residual_out`` may be x or residual themselves (updated in place), but share no other memory
     with them or with each other. Differentiable
-    in x, weight and residual when neither is given.
+    once in x, weight and residual when neither is given.
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (residual is not None and residual.requires_grad)):

@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from ._args import FLOATS, empty2, launch, pitch, require, rows
+from ._args import FLOATS, empty2, launch, once_differentiable, pitch, require, rows
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
 
@@ -53,8 +53,9 @@ class _RouteTopk(torch.autograd.Function):
     def backward(ctx, dweights, *_):
         logits, ids = ctx.saved_tensors
         scoring, renormalize, scale = ctx.how
-        return (route_topk_backward(dweights, logits, ids, scoring=scoring, renormalize=renormalize, scale=scale),
-                *[None] * 9)
+        dlogits, = once_differentiable("route_topk", (route_topk_backward(
+            dweights, logits, ids, scoring=scoring, renormalize=renormalize, scale=scale),), dweights, logits)
+        return (dlogits, *[None] * 9)
 
 
 def route_topk(
@@ -79,7 +80,8 @@ def route_topk(
     ones by the lower id; weights are the chosen scores, divided by their sum when ``renormalize``,
     times ``scale``. An expert whose logit is -inf is never chosen; slots left without one hold id -1
     (which the expert operators skip) and weight 0. (A sigmoid below -88 is 0 in fp32: a token whose chosen scores are
-    all 0 has weights 0, renormalised or not.) The weights are differentiable in the logits.
+    all 0 has weights 0, renormalised or not.) The weights are differentiable once in
+    the logits.
     """
     if torch.is_grad_enabled() and logits.requires_grad:
         out = _RouteTopk.apply(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale,

@@ -165,3 +165,14 @@ def test_route_weights_of_far_sigmoids_add_up_to_one(cuda_device):
     ref = s / s.sum(-1, keepdim=True)
     within(w, ref, 5e-6 * ref, "weights")
     within(w.double().sum(-1), torch.ones(T, dtype=torch.float64, device="cuda"), 5e-6, "sum")
+
+
+def test_second_derivatives_raise(cuda_device):
+    x, w, l = randn(40, 4, 64).requires_grad_(), randn(41, 64).requires_grad_(), randn(42, 4, 16).requires_grad_()
+    for leaf, loss in ((x, lambda: m.add_rms_norm(x, w).sum()), (w, lambda: m.add_rms_norm(x, w, x)[0].square().sum()),
+                       (l, lambda: m.route_topk(l, 3)[0][:, 0].sum()), (l, lambda: m.route_topk(l, 3, "sigmoid")[0].square().sum())):
+        plain, = torch.autograd.grad(loss(), leaf)
+        g, = torch.autograd.grad(loss(), leaf, create_graph=True)
+        assert torch.equal(g.detach(), plain)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            torch.autograd.grad(g.square().sum(), leaf)
