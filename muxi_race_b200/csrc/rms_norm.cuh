@@ -160,7 +160,15 @@ __device__ __forceinline__ void norm_finish(const NormArgs& a, long long row, in
       }
     amax = norm_row_max<CTA>(amax, red);
     constexpr float kMax = OUT == kNormOutI8 ? 127.0f : 448.0f;
-    const float inv = amax > 0.0f ? kMax / amax : 0.0f;
+    float inv = amax > 0.0f ? kMax / amax : 0.0f;
+    if (inv == INFINITY) {  // amax below 1.4e-36: the row is moved up by a power of two first
+      constexpr float kUp = 18446744073709551616.0f;  // 2^64
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) h[j][i] *= kUp;
+      inv = kMax / (amax * kUp);
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int e = (j * lanes + tid) * VEC;

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import muxi_race_b200 as m
+from oracle.norm_ref import rms_norm_ref
 from oracle.w4_ref import linear_ref, w4_values_ref
 
 pytestmark = pytest.mark.gpu
@@ -176,3 +177,26 @@ def test_second_derivatives_raise(cuda_device):
         assert torch.equal(g.detach(), plain)
         with pytest.raises(RuntimeError, match="differentiated once"):
             torch.autograd.grad(g.square().sum(), leaf)
+
+
+@pytest.mark.parametrize("q_dtype,kmax", [(torch.int8, 127.0), (torch.float8_e4m3fn, 448.0)])
+@pytest.mark.parametrize("T,H", [(3, 64), (3, 100), (5, 4096), (400, 7168), (400, 999)])
+@pytest.mark.parametrize("size", [1e-36, 1e-37, 1e-38, 1e-41, 1e-44])
+def test_quant_of_tiny_rows(cuda_device, q_dtype, kmax, T, H, size):
+    """Rows whose largest |y| is near or below fp32's least normal number, with zeros in them. Bounds as in
+    test_norm_gpu.py, with half a spacing of the subnormal numbers (2^-150) for y and, times a code of up to
+    kmax, for the scale."""
+    x, w = randn(50, T, H, dtype=F16), randn(51, H, scale=size)
+    x[:, ::7] = 0
+    x[0] = 0
+    q, scale, _ = m.add_rms_norm_quant(x, w, q_dtype=q_dtype)
+    codes = q.float().double()
+    assert bool(codes.isfinite().all()) and bool((codes[:, ::7] == 0).all()) and bool((codes[0] == 0).all())
+    y, _ = rms_norm_ref(x, w)
+    rscale, tiny = y.abs().amax(-1) / kmax, 2.0 ** -150
+    within(scale, rscale, 8e-6 * rscale + 2 * tiny, "scale")
+    s = rscale[:, None]
+    step = 0.5 * s if q_dtype == torch.int8 else torch.maximum(y.abs() * 2.0 ** -4, s * 2.0 ** -10)
+    within(codes * scale.double()[:, None], y, step + 1.6e-5 * (y.abs() + s * kmax) + (kmax + 2) * tiny, "q * scale")
+    if size >= 1e-37:  # the largest value of a row still has the largest code
+        assert bool((codes[1:].abs().amax(-1) == kmax).all())
