@@ -55,6 +55,35 @@ template <> struct QuantKind<kQF8> {
   }
 };
 
+// The factor of a row's values, kMax / amax, as a power of two (1 but for the tiniest rows) and the rest:
+// below an amax of 1.4e-36 the quotient itself is beyond fp32.
+struct RowFactor {
+  float up, inv;
+};
+template <int Q8>
+__device__ __forceinline__ RowFactor row_factor(float amax) {
+  RowFactor r{1.0f, amax > 0.0f ? QuantKind<Q8>::kMax / amax : 0.0f};
+  if (r.inv == INFINITY) {
+    r.up = 18446744073709551616.0f;  // 2^64
+    r.inv = QuantKind<Q8>::kMax / (amax * r.up);
+  }
+  return r;
+}
+// Eight scaled values as bytes.
+template <int Q8>
+__device__ __forceinline__ uint2 enc8(float (&f)[8], const RowFactor& r) {
+  if (r.up != 1.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= r.up;
+  }
+  uint2 w = make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w.x |= QuantKind<Q8>::enc(f[i], r.inv) << (8 * i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w.y |= QuantKind<Q8>::enc(f[4 + i], r.inv) << (8 * i);
+  return w;
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -109,17 +138,12 @@ __global__ void gather_rows_q8_kernel(const T* __restrict__ x, const int32_t* __
         for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
       }
       amax = warp_max(amax);
-      const float inv = amax > 0.0f ? QuantKind<Q8>::kMax / amax : 0.0f;
+      const RowFactor factor = row_factor<Q8>(amax);
       uint2* dst = reinterpret_cast<uint2*>(xq + static_cast<size_t>(slot) * H);
       for (int v = lane; v < vecs; v += 32) {
         float f[8];
         unpack8<T>(__ldg(src + v), f);
-        uint32_t w0 = 0, w1 = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w0 |= QuantKind<Q8>::enc(f[i], inv) << (8 * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w1 |= QuantKind<Q8>::enc(f[4 + i], inv) << (8 * i);
-        dst[v] = make_uint2(w0, w1);
+        dst[v] = enc8<Q8>(f, factor);
       }
       if (lane == 0) xscale[slot] = amax / QuantKind<Q8>::kMax;
     } else {
@@ -184,17 +208,12 @@ __global__ void quantize_rows_q8_kernel(const T* __restrict__ w, long long rows,
       }
       amax = warp_max(amax);
     }
-    const float inv = amax > 0.0f ? QuantKind<Q8>::kMax / amax : 0.0f;
+    const RowFactor factor = row_factor<Q8>(amax);
     uint2* dst = reinterpret_cast<uint2*>(q + r * K);
     for (int v = lane; v < vecs; v += 32) {
       float f[8];
       unpack8<T>(__ldg(src + v), f);
-      uint32_t w0 = 0, w1 = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w0 |= QuantKind<Q8>::enc(f[i], inv) << (8 * i);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w1 |= QuantKind<Q8>::enc(f[4 + i], inv) << (8 * i);
-      dst[v] = make_uint2(w0, w1);
+      dst[v] = enc8<Q8>(f, factor);
     }
     if (lane == 0) scale[r] = amax / QuantKind<Q8>::kMax;
   }

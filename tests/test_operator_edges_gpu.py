@@ -200,3 +200,24 @@ def test_quant_of_tiny_rows(cuda_device, q_dtype, kmax, T, H, size):
     within(codes * scale.double()[:, None], y, step + 1.6e-5 * (y.abs() + s * kmax) + (kmax + 2) * tiny, "q * scale")
     if size >= 1e-37:  # the largest value of a row still has the largest code
         assert bool((codes[1:].abs().amax(-1) == kmax).all())
+
+
+@pytest.mark.parametrize("kind,kmax", [("int8", 127.0), ("fp8", 448.0)])
+@pytest.mark.parametrize("size", [1e-36, 1e-37, 1e-38, 3e-40])
+def test_quantised_tiny_rows(cuda_device, kind, kmax, size):
+    """The same at the quantisation of 16-bit rows, by itself and inside the experts' calls (bf16: fp16 has no
+    values this small). Bounds: half a step, and half a spacing of fp32's subnormal numbers for the scale."""
+    quantize, fused = {"int8": (m.quantize_rows_int8, m.fused_moe_int8), "fp8": (m.quantize_rows_fp8, m.fused_moe_fp8)}[kind]
+    x = randn(52, 20, 256, dtype=BF16, scale=size)
+    x[:, ::5] = 0
+    q, scale = quantize(x)
+    codes, y = q.float().double(), x.double()
+    assert bool(codes.isfinite().all()) and bool((codes[:, ::5] == 0).all())
+    s = y.abs().amax(-1, keepdim=True) / kmax
+    step = 0.5 * s if kind == "int8" else torch.maximum(y.abs() * 2.0 ** -4, s * 2.0 ** -10)
+    within(codes * scale.double()[:, None], y, step + 1e-6 * s * kmax + kmax * 2.0 ** -150, "q * scale")
+    w13, w2 = quantize(randn(53, 4, 256, 256, dtype=BF16)), quantize(randn(54, 4, 256, 128, dtype=BF16))
+    ids = torch.arange(20, device="cuda", dtype=torch.int32)[:, None] % 4
+    out = fused(x, *w13, *w2, ids, torch.ones(20, 1, device="cuda"))
+    assert bool((out == 0).all())  # silu(gate) * up is below the least bf16 number
+    assert m.device_status() == 0
