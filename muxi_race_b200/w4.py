@@ -7,7 +7,8 @@ of tiles that the kernels read.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -15,6 +16,12 @@ import torch
 from . import _lib
 from ._args import FLOATS, HALVES, IDS, empty2, launch, overlap, pitch, require, rows
 from .fused import _workspace
+
+
+@lru_cache(maxsize=1024)
+def _workspace_bytes(name: str, *sizes: int) -> int:
+    """What entry point `name` says of these sizes, asked once for each (a call counts its microseconds)."""
+    return getattr(_lib.lib(), name)(*sizes)
 
 
 @dataclass
@@ -27,7 +34,6 @@ class W4Weights:
     group_size: int
     has_zeros: bool
     gate_up: bool         # gate rows and up rows interleaved, for fused_moe_w4
-    sizes: dict = field(default_factory=dict, repr=False, compare=False)  # workspace bytes by rows, asked once each
 
     def __post_init__(self):
         *lead, N, K = self.shape
@@ -141,9 +147,7 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
         # a block may still read rows of x when another stores its columns of them
         require(not overlap(out2, x2), "out must not share memory with x")
         ld_out = pitch(out2)
-    nbytes = w.sizes.get(M)
-    if nbytes is None:
-        nbytes = w.sizes[M] = _lib.lib().moe_w4_linear_workspace_bytes(M, N, K, w.group_size, HALVES[w.dtype])
+    nbytes = _workspace_bytes("moe_w4_linear_workspace_bytes", M, N, K, w.group_size, HALVES[w.dtype])
     ws = _workspace(nbytes, dev) if nbytes else None  # held until the call has been launched
     launch(dev, "moe_w4_linear", x2.data_ptr(), pitch(x2), w.packed.data_ptr(), out.data_ptr(), ld_out, M, N, K,
            w.group_size, w.has_zeros, FLOATS[w.dtype], None if ws is None else ws.data_ptr(), nbytes)
@@ -191,10 +195,8 @@ def fused_moe_w4(
         require(tuple(out.shape) == (T, H) and out.dtype == w13.dtype and out.is_contiguous() and out.device == dev, "bad out")
     if T == 0:
         return out
-    nbytes = w13.sizes.get((T, k))
-    if nbytes is None:
-        nbytes = w13.sizes[T, k] = _lib.lib().moe_fused_w4_workspace_bytes(
-            T, k, E, H, I, w13.group_size, w2.group_size, HALVES[w13.dtype])
+    nbytes = _workspace_bytes("moe_fused_w4_workspace_bytes", T, k, E, H, I, w13.group_size, w2.group_size,
+                              HALVES[w13.dtype])
     ws = _workspace(nbytes, dev)
     launch(dev, "moe_fused_w4", x.data_ptr(), pitch(x), w13.packed.data_ptr(), w13.group_size, w13.has_zeros,
            w2.packed.data_ptr(), w2.group_size, w2.has_zeros, topk_ids.data_ptr(), IDS[topk_ids.dtype],

@@ -4,7 +4,7 @@ import torch
 
 import muxi_race_b200 as m
 from oracle.norm_ref import rms_norm_ref
-from oracle.w4_ref import linear_ref, w4_values_ref
+from oracle.w4_ref import experts_ref, linear_ref, w4_values_ref
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = torch.float16, torch.bfloat16
@@ -220,4 +220,29 @@ def test_quantised_tiny_rows(cuda_device, kind, kmax, size):
     ids = torch.arange(20, device="cuda", dtype=torch.int32)[:, None] % 4
     out = fused(x, *w13, *w2, ids, torch.ones(20, 1, device="cuda"))
     assert bool((out == 0).all())  # silu(gate) * up is below the least bf16 number
+    assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("groups", [(32, 128), (128, 32)])
+def test_one_w13_with_w2_of_other_groups(cuda_device, groups):
+    """At I = 5632 and 16 rows a tile, w2 in groups of 128 takes two slices of K and in groups of 32 one: each
+    call asks for its own workspace."""
+    T, H, I, E, k = 16, 64, 5632, 4, 2
+    size = m._lib.lib().moe_fused_w4_workspace_bytes
+    assert size(T, k, E, H, I, 64, 32, m._lib.MOE_F16) != size(T, k, E, H, I, 64, 128, m._lib.MOE_F16)
+
+    def experts(seed, N, K, group, gate_up):  # (packed, values in fp64) of E matrices
+        g = torch.Generator(device="cpu").manual_seed(seed)
+        q = torch.randint(0, 256, (E, N, K // 2), generator=g, dtype=torch.uint8).cuda()
+        s = ((torch.rand((E, N, -(-K // group)), generator=g) + 0.5) * 0.2 * K ** -0.5).half().cuda()
+        return m.pack_w4(q, s, group_size=group, gate_up=gate_up), w4_values_ref(q, s, None, K, group)
+
+    q13, w13 = experts(60, 2 * I, H, 64, True)
+    x = randn(62, T, H, dtype=F16)
+    ids = torch.stack([torch.arange(T) % E, (torch.arange(T) + 1) % E], 1).int().cuda()
+    weights = torch.full((T, k), 0.5, device="cuda")
+    for group in groups:
+        q2, w2 = experts(61, H, I, group, False)
+        ref, tol = experts_ref(x, w13, w2, ids, weights, U[F16], F32)
+        within(m.fused_moe_w4(x, q13, q2, ids, weights), ref, tol + TINY[F16], "out")
     assert m.device_status() == 0
