@@ -289,7 +289,10 @@ def quantize_rows_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _fused_q8_rows(x_q, x_scale, q_dtype, w13_q, w13_scale, w2_q, w2_scale, topk_ids, topk_weights, out, out_dtype):
     """fused_moe_int8 / fused_moe_fp8 on rows that are 8-bit already."""
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if out is None else out.dtype
     _check(out_dtype in _DTYPES, "out_dtype must be fp16 or bf16")
+    _check(out is None or out.dtype == out_dtype, "out must have out_dtype")
     _check(x_q.dim() == 2 and x_q.dtype == q_dtype, f"hidden_states must be {q_dtype} [T, H]")
     T, H = x_q.shape
     _check(x_scale.dtype == torch.float32 and x_scale.numel() == T and x_scale.is_contiguous() and x_scale.device == x_q.device,
@@ -297,7 +300,6 @@ def _fused_q8_rows(x_q, x_scale, q_dtype, w13_q, w13_scale, w2_q, w2_scale, topk
     _check(x_q.is_cuda and x_q.is_contiguous(), "hidden_states must be a contiguous CUDA tensor")
     if out is None:
         out = torch.empty((T, H), dtype=out_dtype, device=x_q.device)
-    _check(out.dtype in _DTYPES, "out must be fp16 or bf16")
     _, _, I, E, k = _check_fused(out, w13_q, w2_q, topk_ids, topk_weights, True, q_dtype)
     _check(tuple(out.shape) == (T, H) and out.device == x_q.device, "bad out")
     _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
@@ -329,16 +331,17 @@ def fused_moe_int8(
     topk_weights: torch.Tensor,
     out: Optional[torch.Tensor] = None,
     hidden_scale: Optional[torch.Tensor] = None,
-    out_dtype: torch.dtype = torch.bfloat16,
+    out_dtype: Optional[torch.dtype] = None,
 ) -> torch.Tensor:
     """W8A8 ``fused_moe``: int8 weights with per-output-row scales (from :func:`quantize_rows_int8`),
     activations quantised per token on the device, int32 accumulation, output in the activation dtype.
 
     With ``hidden_scale`` [T] fp32 the rows are int8 already (:func:`add_rms_norm_quant`) and the output
-    is in ``out_dtype``."""
+    is in ``out_dtype`` (default: that of ``out``, or bf16), which is for this form only."""
     if hidden_scale is not None:
         return _fused_q8_rows(hidden_states, hidden_scale, torch.int8, w13_q, w13_scale, w2_q, w2_scale, topk_ids,
                               topk_weights, out, out_dtype)
+    _check(out_dtype is None, "out_dtype needs hidden_scale: otherwise the output has the dtype of hidden_states")
     T, H, I, E, k = _check_fused(hidden_states, w13_q, w2_q, topk_ids, topk_weights, True)
     _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
            "w13_scale must be fp32 [E, 2I]")
@@ -387,17 +390,18 @@ def fused_moe_fp8(
     topk_weights: torch.Tensor,
     out: Optional[torch.Tensor] = None,
     hidden_scale: Optional[torch.Tensor] = None,
-    out_dtype: torch.dtype = torch.bfloat16,
+    out_dtype: Optional[torch.dtype] = None,
 ) -> torch.Tensor:
     """fp8 ``fused_moe``: e4m3 weights with per-output-row scales (from :func:`quantize_rows_fp8`),
     activations quantised to e4m3 per token on the device, fp32 accumulation, output in the
     activation dtype.
 
     With ``hidden_scale`` [T] fp32 the rows are e4m3 already (:func:`add_rms_norm_quant`) and the output
-    is in ``out_dtype``."""
+    is in ``out_dtype`` (default: that of ``out``, or bf16), which is for this form only."""
     if hidden_scale is not None:
         return _fused_q8_rows(hidden_states, hidden_scale, torch.float8_e4m3fn, w13_q, w13_scale, w2_q, w2_scale, topk_ids,
                               topk_weights, out, out_dtype)
+    _check(out_dtype is None, "out_dtype needs hidden_scale: otherwise the output has the dtype of hidden_states")
     T, H, I, E, k = _check_fused(hidden_states, w13_q, w2_q, topk_ids, topk_weights, True, torch.float8_e4m3fn)
     _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
            "w13_scale must be fp32 [E, 2I]")

@@ -246,3 +246,23 @@ def test_one_w13_with_w2_of_other_groups(cuda_device, groups):
         ref, tol = experts_ref(x, w13, w2, ids, weights, U[F16], F32)
         within(m.fused_moe_w4(x, q13, q2, ids, weights), ref, tol + TINY[F16], "out")
     assert m.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_out_dtype_is_refused_where_it_has_no_effect(cuda_device, kind):
+    quantize, fused = {"int8": (m.quantize_rows_int8, m.fused_moe_int8), "fp8": (m.quantize_rows_fp8, m.fused_moe_fp8)}[kind]
+    x = randn(70, 6, 256, dtype=F16)
+    w = (*quantize(randn(71, 4, 256, 256, dtype=F16, scale=0.06)), *quantize(randn(72, 4, 256, 128, dtype=F16, scale=0.09)))
+    ids, tw = torch.arange(6, device="cuda", dtype=torch.int32)[:, None] % 4, torch.ones(6, 1, device="cuda")
+    for dtype in (F16, BF16):
+        with pytest.raises(ValueError, match="needs hidden_scale"):
+            fused(x, *w, ids, tw, out_dtype=dtype)
+    q, scale = quantize(x)
+    want = fused(x, *w, ids, tw)
+    assert want.dtype == F16
+    with pytest.raises(ValueError, match="out_dtype"):
+        fused(q, *w, ids, tw, out=torch.empty_like(x), hidden_scale=scale, out_dtype=BF16)
+    assert fused(q, *w, ids, tw, hidden_scale=scale).dtype == BF16
+    out = torch.empty_like(x)
+    assert fused(q, *w, ids, tw, out=out, hidden_scale=scale) is out and torch.equal(out, want)  # one route a token
+    assert torch.equal(fused(q, *w, ids, tw, hidden_scale=scale, out_dtype=F16), want)
