@@ -10,9 +10,10 @@ FLOATS = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16, torch.floa
 HALVES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
 IDS = {torch.int32: _lib.MOE_I32, torch.int64: _lib.MOE_I64}
 
-#: handle of the current stream of a device ordinal, without building a Stream object
-raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+#: handle of the current stream of a device ordinal, without building a Stream object; None in a torch
+#: without CUDA, where the package can be imported and its argument checks work, but no call gets as far
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 _functions: dict = {}
 
 
@@ -91,9 +92,9 @@ def launch(device: torch.device, name: str, *args) -> None:
         fn = _functions[name] = getattr(_lib.lib(), name)
     index = device.index
     if _current_device() == index:
-        code = fn(*args, raw_stream(index))
+        code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            code = fn(*args, raw_stream(index))
+            code = fn(*args, _raw_stream(index))
     if code:
         _lib.check(name, code)
