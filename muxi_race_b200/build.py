@@ -24,7 +24,7 @@ SOURCES = {
     "moe_capi.cu": ["moe_gemm.cuh", "moe_gemm_pair.cuh", "moe_gemm_tn.cuh", "ep_p2p.cuh", "route_align.cuh",
                     "router_topk.cuh", "ordered_combine.cuh", "gather_quant.cuh", "ep_kernels.cuh", "sm100_ptx.cuh"],
     "norm_capi.cu": ["rms_norm.cuh"],
-    "route_capi.cu": ["route_topk.cuh"],
+    "route_capi.cu": ["route_topk.cuh", "sm100_ptx.cuh"],
     "w4_capi.cu": ["w4_gemv.cuh", "sm100_ptx.cuh"],
 }
 GENCODE = "arch=compute_100a,code=sm_100a"
