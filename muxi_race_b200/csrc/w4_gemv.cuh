@@ -788,9 +788,16 @@ __global__ void w4_unpack_kernel(const uint8_t* __restrict__ w, long long matric
   }
 }
 
+__device__ __forceinline__ float w4_max_nan(float a, float b) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 // 16-bit weights to 4 bits, one warp per group of a row. Symmetric: s = amax / 7, q = round(w / s) + 8;
 // otherwise s = (max - min) / 15 over the range widened to hold 0, z = round(-min / s). s is rounded to
-// its stored type first; values are rounded to nearest, ties to even, and clamped to 0..15.
+// its stored type first; values are rounded to nearest, ties to even, and clamped to 0..15. A group with NaN
+// or an infinity gets that as its scale.
 template <typename T>
 __global__ void w4_quantize_kernel(const T* __restrict__ w, long long rows, int K, int group, uint8_t* __restrict__ q,
                                    T* __restrict__ scales, uint8_t* __restrict__ zeros) {
@@ -802,21 +809,21 @@ __global__ void w4_quantize_kernel(const T* __restrict__ w, long long rows, int 
     const long long row = t / G;
     const int c0 = static_cast<int>(t - row * G) * group, c1 = min(c0 + group, K);
     const T* p = w + row * K;
-    float lo = 0.0f, hi = 0.0f;
+    float down = 0.0f, hi = 0.0f;  // -min and max
     for (int c = c0 + lane; c < c1; c += 32) {
       const float v = static_cast<float>(p[c]);
-      lo = fminf(lo, v);
-      hi = fmaxf(hi, v);
+      down = w4_max_nan(down, -v);
+      hi = w4_max_nan(hi, v);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      down = w4_max_nan(down, __shfl_xor_sync(0xffffffffu, down, o));
+      hi = w4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    const T st = W4Type<T>::from_f(zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f);
+    const T st = W4Type<T>::from_f(zeros ? (hi + down) / 15.0f : w4_max_nan(hi, down) / 7.0f);
     const float s = static_cast<float>(st);
     const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-    const float z = zeros ? fminf(fmaxf(rintf(-lo * inv), 0.0f), 15.0f) : 8.0f;
+    const float z = zeros ? fminf(fmaxf(rintf(down * inv), 0.0f), 15.0f) : 8.0f;
     if (lane == 0) {
       scales[t] = st;
       if (zeros) zeros[t] = static_cast<uint8_t>(z);

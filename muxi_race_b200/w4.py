@@ -95,7 +95,8 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True, 
     """Quantise 16-bit weights [..., N, K] to 4 bits, rounding to nearest.
 
     Symmetric: scale = amax / 7 of the group, values -8..7. Otherwise scale = (max - min) / 15 with a
-    zero point, over the group's range widened to hold 0.
+    zero point, over the group's range widened to hold 0. A group with NaN or an infinity comes back
+    without finite values.
     """
     _check_group(group_size)
     require(w.is_cuda and w.dtype in HALVES and w.is_contiguous() and w.dim() >= 2,

@@ -266,3 +266,18 @@ def test_out_dtype_is_refused_where_it_has_no_effect(cuda_device, kind):
     out = torch.empty_like(x)
     assert fused(q, *w, ids, tw, out=out, hidden_scale=scale) is out and torch.equal(out, want)  # one route a token
     assert torch.equal(fused(q, *w, ids, tw, hidden_scale=scale, out_dtype=F16), want)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_w4_quantise_shows_spoilt_groups(cuda_device, symmetric, dtype):
+    """NaN or an infinity spoils its group of 32 and leaves the others as they are."""
+    w = randn(80, 6, 200, dtype=dtype)
+    want = m.dequantize_w4(m.quantize_w4(w, 32, symmetric))
+    bad = torch.zeros_like(w, dtype=torch.bool)
+    for r, c, v in ((0, 5, "nan"), (1, 64, "inf"), (2, 199, "-inf"), (4, 40, "nan"), (4, 41, "inf")):
+        w[r, c] = float(v)
+        bad[r, c // 32 * 32:c // 32 * 32 + 32] = True
+    got = m.dequantize_w4(m.quantize_w4(w, 32, symmetric))
+    assert not bool(got[bad].isfinite().any())
+    assert torch.equal(got[~bad], want[~bad])
