@@ -820,18 +820,22 @@ __global__ void w4_quantize_kernel(const T* __restrict__ w, long long rows, int 
       down = w4_max_nan(down, __shfl_xor_sync(0xffffffffu, down, o));
       hi = w4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    const T st = W4Type<T>::from_f(zeros ? (hi + down) / 15.0f : w4_max_nan(hi, down) / 7.0f);
+    float range = (hi + down) / 15.0f;
+    if (range == INFINITY) range = hi / 15.0f + down / 15.0f;  // bf16: the sum may be beyond fp32
+    const T st = W4Type<T>::from_f(zeros ? range : w4_max_nan(hi, down) / 7.0f);
     const float s = static_cast<float>(st);
     const float inv = s > 0.0f ? 1.0f / s : 0.0f;
-    const float z = zeros ? fminf(fmaxf(rintf(down * inv), 0.0f), 15.0f) : 8.0f;
+    // the reciprocal of a scale below 2.9e-39 (bf16) is beyond fp32
+    auto steps = [&](float v) { return rintf(inv == INFINITY ? v / s : v * inv); };
+    const float z = zeros ? fminf(fmaxf(steps(down), 0.0f), 15.0f) : 8.0f;
     if (lane == 0) {
       scales[t] = st;
       if (zeros) zeros[t] = static_cast<uint8_t>(z);
     }
     // groups start on even columns, so each byte belongs to one group
     for (int c = c0 + 2 * lane; c < c1; c += 64) {
-      const float a = fminf(fmaxf(rintf(static_cast<float>(p[c]) * inv) + z, 0.0f), 15.0f);
-      const float b = c + 1 < c1 ? fminf(fmaxf(rintf(static_cast<float>(p[c + 1]) * inv) + z, 0.0f), 15.0f) : 0.0f;
+      const float a = fminf(fmaxf(steps(static_cast<float>(p[c])) + z, 0.0f), 15.0f);
+      const float b = c + 1 < c1 ? fminf(fmaxf(steps(static_cast<float>(p[c + 1])) + z, 0.0f), 15.0f) : 0.0f;
       q[row * row_bytes + c / 2] = static_cast<uint8_t>(static_cast<int>(a) | static_cast<int>(b) << 4);
     }
   }

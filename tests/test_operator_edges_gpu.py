@@ -281,3 +281,19 @@ def test_w4_quantise_shows_spoilt_groups(cuda_device, symmetric, dtype):
     got = m.dequantize_w4(m.quantize_w4(w, 32, symmetric))
     assert not bool(got[bad].isfinite().any())
     assert torch.equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("size", [1e38, 1e-37, 1e-38, 1e-39])
+def test_w4_quantise_the_ends_of_the_range(cuda_device, symmetric, size):
+    """bf16 weights near fp32's largest and least numbers: the bound of test_w4_gpu.py, and where the scale is
+    subnormal half its spacing (2^-134) for each of up to 8 (15) steps."""
+    w = randn(81, 4, 256).clamp(-3, 3)
+    w[:, ::9] = 0
+    w = (w * size).to(BF16)
+    d = m.dequantize_w4(m.quantize_w4(w, 64, symmetric)).double()
+    groups = w.double().view(4, 4, 64)
+    span = groups.abs().amax(-1) / 7 if symmetric else (groups.amax(-1).clamp_min(0) - groups.amin(-1).clamp_max(0)) / 15
+    step = span.repeat_interleave(64, -1)
+    within(d, w.double(), step * (0.5 if symmetric else 1.0) * 1.01 + 16 * U[BF16] * step + 16 * 2.0 ** -134, "weight")
+    assert bool((d[:, ::9] == 0).all())
