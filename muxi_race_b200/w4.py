@@ -113,6 +113,7 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True, 
 
 def dequantize_w4(w: W4Weights) -> torch.Tensor:
     """The weights as a 16-bit tensor of ``w.shape``, each ``scale * (q - zero)`` rounded once."""
+    require(w.packed.is_cuda, "packed weights must be a CUDA tensor")
     *lead, N, K = w.shape
     matrices = 1
     for n in lead:
