@@ -64,15 +64,15 @@ def empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> to
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
-class _OnceDifferentiable(torch.autograd.Function):
+class _NoGraph(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, name, grads, *sources):
-        ctx.name = name
-        return grads
+    def forward(ctx, message, results, *sources):
+        ctx.message = message
+        return results
 
     @staticmethod
     def backward(ctx, *_):
-        raise RuntimeError(f"{ctx.name} can be differentiated once: its gradient comes from a kernel without a graph")
+        raise RuntimeError(ctx.message)
 
 
 def once_differentiable(name: str, grads: tuple, *sources):
@@ -82,7 +82,16 @@ def once_differentiable(name: str, grads: tuple, *sources):
     incoming gradient only, and is passed over by ``torch.autograd.grad``, whose inputs it does not lead to.)"""
     if not torch.is_grad_enabled():
         return grads
-    return _OnceDifferentiable.apply(name, grads, *sources)
+    return _NoGraph.apply(f"{name} can be differentiated once: its gradient comes from a kernel without a graph", grads,
+                          *sources)
+
+
+def without_gradient(name: str, results: tuple, *sources):
+    """The results of an operator that has no gradient. Where `sources` ask for one, going back through the
+    results raises instead of leaving its part out."""
+    if not torch.is_grad_enabled() or not any(s is not None and s.requires_grad for s in sources):
+        return results
+    return _NoGraph.apply(f"{name} is not differentiable", results, *sources)
 
 
 def launch(device: torch.device, name: str, *args) -> None:

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, launch, once_differentiable, overlap, pitch, require, rows
+from ._args import FLOATS, launch, once_differentiable, overlap, pitch, require, rows, without_gradient
 from .fused import _workspace
 
 _Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -126,7 +126,8 @@ def add_rms_norm_quant(
 
     ``scale = max|y| / 127`` and ``q = round(y / scale)`` for ``torch.int8`` (halves away from zero),
     ``/ 448`` and e4m3 rounding for ``torch.float8_e4m3fn``: the scheme of :func:`quantize_rows_int8`
-    / :func:`quantize_rows_fp8`, applied to the unrounded y. x must be fp16 or bf16.
+    / :func:`quantize_rows_fp8`, applied to the unrounded y. x must be fp16 or bf16. Not differentiable: a backward pass that meets the
+    results raises (a ``residual_out`` carries no graph).
     """
     require(q_dtype in _Q_DTYPES, "q_dtype must be torch.int8 or torch.float8_e4m3fn")
     x2 = rows(x, "x")
@@ -138,7 +139,9 @@ def add_rms_norm_quant(
     _, h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x2, residual, residual_out)
     launch(dev, "moe_add_rms_norm", x2.data_ptr(), pitch(x2), r_ptr, r_ld, weight.data_ptr(), wdt, q.data_ptr(), H,
            _Q_DTYPES[q_dtype], scale.data_ptr(), h_ptr, h_ld, T, H, eps, FLOATS[dtype])
-    return q, scale, h
+    if residual_out is not None:
+        return (*without_gradient("add_rms_norm_quant", (q, scale), x, weight, residual), h)
+    return without_gradient("add_rms_norm_quant", (q, scale, h), x, weight, residual)
 
 
 def add_rms_norm_backward(

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, launch, overlap, pitch, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, launch, overlap, pitch, require, rows, without_gradient
 from .fused import _workspace
 
 
@@ -128,7 +128,8 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
     """``x @ W.T`` for a few rows x [..., K] (fp16 / bf16, the dtype of the weight's scales).
 
     Sums in fp32, rounded once. ``out`` must not share memory with x. The weights are read once for up to 16 rows, and again for every 16
-    more: for a prompt, ``torch.matmul`` with :func:`dequantize_w4` is the better call.
+    more: for a prompt, ``torch.matmul`` with :func:`dequantize_w4` is the better call. Not differentiable:
+    a backward pass that meets the result raises (``out`` carries no graph).
     """
     if len(w.shape) != 2 or w.gate_up:
         raise ValueError("w must be one matrix, packed without gate_up")
@@ -138,7 +139,8 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
     if x2.dtype != w.dtype or x2.shape[1] != K:
         raise ValueError(f"x must be {w.dtype} [..., {K}]")
     M = x2.shape[0]
-    if out is None:
+    given = out is not None
+    if not given:
         out = empty2(M, N, w.dtype, dev)
         if x.dim() != 2:
             out = out.view(*x.shape[:-1], N)
@@ -153,7 +155,7 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
     ws = _workspace(nbytes, dev) if nbytes else None  # held until the call has been launched
     launch(dev, "moe_w4_linear", x2.data_ptr(), pitch(x2), w.packed.data_ptr(), out.data_ptr(), ld_out, M, N, K,
            w.group_size, w.has_zeros, FLOATS[w.dtype], None if ws is None else ws.data_ptr(), nbytes)
-    return out
+    return out if given else without_gradient("w4_linear", (out,), x)[0]
 
 
 def fused_moe_w4(
@@ -171,7 +173,8 @@ def fused_moe_w4(
     each chosen expert's weights are read once for up to 8 of its tokens (16 where the experts have
     more than 4 on average). With 8 experts of H = 4096, I = 14336 it is faster than e4m3 experts up to
     16 tokens per expert (275 against 291 us) and than fp16 experts up to 32 (423 against 484 us). The
-    same bits on every run.
+    same bits on every run. Not differentiable: a backward pass that meets the result raises (``out``
+    carries no graph).
     """
     if len(w13.shape) != 3 or not w13.gate_up or len(w2.shape) != 3 or w2.gate_up:
         raise ValueError("w13 must be [E, 2I, H] packed with gate_up, w2 [E, H, I] without")
@@ -191,7 +194,8 @@ def fused_moe_w4(
     if topk_ids.device != dev or topk_weights.device != dev or not topk_ids.is_contiguous() or not topk_weights.is_contiguous():
         raise ValueError(f"topk_ids and topk_weights must be contiguous tensors on {dev}")
     k = topk_ids.shape[1]
-    if out is None:
+    given = out is not None
+    if not given:
         out = empty2(T, H, w13.dtype, dev)
     else:
         require(tuple(out.shape) == (T, H) and out.dtype == w13.dtype and out.is_contiguous() and out.device == dev, "bad out")
@@ -204,4 +208,4 @@ def fused_moe_w4(
            w2.packed.data_ptr(), w2.group_size, w2.has_zeros, topk_ids.data_ptr(), IDS[topk_ids.dtype],
            topk_weights.data_ptr(), FLOATS[topk_weights.dtype], out.data_ptr(), T, H, I, E, k, FLOATS[w13.dtype],
            ws.data_ptr(), ws.numel())
-    return out
+    return out if given else without_gradient("fused_moe_w4", (out,), hidden_states, topk_weights)[0]

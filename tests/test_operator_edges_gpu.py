@@ -297,3 +297,29 @@ def test_w4_quantise_the_ends_of_the_range(cuda_device, symmetric, size):
     step = span.repeat_interleave(64, -1)
     within(d, w.double(), step * (0.5 if symmetric else 1.0) * 1.01 + 16 * U[BF16] * step + 16 * 2.0 ** -134, "weight")
     assert bool((d[:, ::9] == 0).all())
+
+
+def test_operators_without_a_gradient_say_so(cuda_device):
+    """A loss that also has another path to x: the operator's part is not left out in silence."""
+    x, norm = randn(90, 4, 64, dtype=F16), randn(91, 64, dtype=F16)
+    lin, w13, w2 = (m.quantize_w4(randn(s, *shape, dtype=F16), 32, gate_up=g)
+                    for s, shape, g in ((92, (64, 64), False), (93, (4, 64, 64), True), (94, (4, 64, 32), False)))
+    ids, tw = torch.zeros(4, 1, device="cuda", dtype=torch.int32), torch.ones(4, 1, device="cuda")
+    calls = (("w4_linear", lambda x, t: m.w4_linear(x, lin)), ("fused_moe_w4", lambda x, t: m.fused_moe_w4(x, w13, w2, ids, t)),
+             ("add_rms_norm_quant", lambda x, t: m.add_rms_norm_quant(x, norm, x)[1]),
+             ("add_rms_norm_quant", lambda x, t: m.add_rms_norm_quant(x, norm, x)[2]))
+    for name, call in calls:
+        plain = call(x, tw)
+        assert not plain.requires_grad
+        leaf = x.clone().requires_grad_()
+        y = call(leaf, tw)
+        assert torch.equal(y.detach(), plain)
+        with pytest.raises(RuntimeError, match=f"{name} is not differentiable"):
+            (y.float().sum() + leaf.float().sum()).backward()
+        with torch.no_grad():
+            assert not call(leaf, tw).requires_grad
+    t = tw.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="fused_moe_w4 is not differentiable"):
+        (m.fused_moe_w4(x, w13, w2, ids, t).float().sum() + t.sum()).backward()
+    out = torch.empty_like(x)
+    assert m.w4_linear(x.clone().requires_grad_(), lin, out=out) is out and not out.requires_grad
