@@ -69,19 +69,32 @@ __device__ __forceinline__ RowFactor row_factor(float amax) {
   }
   return r;
 }
-// Eight scaled values as bytes.
-template <int Q8>
-__device__ __forceinline__ uint2 enc8(float (&f)[8], const RowFactor& r) {
-  if (r.up != 1.0f) {
+// A lane's share of a row of `vecs` vectors of 8 values, as bytes. UP: the values are moved up first (a form of
+// its own, so that the loop of ordinary rows is free of it).
+template <typename T, int Q8, bool UP>
+__device__ __forceinline__ void encode_row(const uint4* src, uint2* dst, int vecs, int lane, const RowFactor& r) {
+  for (int v = lane; v < vecs; v += 32) {
+    float f[8];
+    unpack8<T>(__ldg(src + v), f);
+    if constexpr (UP) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= r.up;
+      for (int i = 0; i < 8; ++i) f[i] *= r.up;
+    }
+    uint32_t w0 = 0, w1 = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w0 |= QuantKind<Q8>::enc(f[i], r.inv) << (8 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w1 |= QuantKind<Q8>::enc(f[4 + i], r.inv) << (8 * i);
+    dst[v] = make_uint2(w0, w1);
   }
-  uint2 w = make_uint2(0, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w.x |= QuantKind<Q8>::enc(f[i], r.inv) << (8 * i);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w.y |= QuantKind<Q8>::enc(f[4 + i], r.inv) << (8 * i);
-  return w;
+}
+template <typename T, int Q8>
+__device__ __forceinline__ void encode_row(const uint4* src, uint2* dst, int vecs, int lane, float amax) {
+  const RowFactor r = row_factor<Q8>(amax);
+  if (r.up == 1.0f)
+    encode_row<T, Q8, false>(src, dst, vecs, lane, r);
+  else
+    encode_row<T, Q8, true>(src, dst, vecs, lane, r);
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -138,13 +151,7 @@ __global__ void gather_rows_q8_kernel(const T* __restrict__ x, const int32_t* __
         for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
       }
       amax = warp_max(amax);
-      const RowFactor factor = row_factor<Q8>(amax);
-      uint2* dst = reinterpret_cast<uint2*>(xq + static_cast<size_t>(slot) * H);
-      for (int v = lane; v < vecs; v += 32) {
-        float f[8];
-        unpack8<T>(__ldg(src + v), f);
-        dst[v] = enc8<Q8>(f, factor);
-      }
+      encode_row<T, Q8>(src, reinterpret_cast<uint2*>(xq + static_cast<size_t>(slot) * H), vecs, lane, amax);
       if (lane == 0) xscale[slot] = amax / QuantKind<Q8>::kMax;
     } else {
       uint4* dst = reinterpret_cast<uint4*>(zero_out + (item - R) * static_cast<size_t>(H));
@@ -208,13 +215,7 @@ __global__ void quantize_rows_q8_kernel(const T* __restrict__ w, long long rows,
       }
       amax = warp_max(amax);
     }
-    const RowFactor factor = row_factor<Q8>(amax);
-    uint2* dst = reinterpret_cast<uint2*>(q + r * K);
-    for (int v = lane; v < vecs; v += 32) {
-      float f[8];
-      unpack8<T>(__ldg(src + v), f);
-      dst[v] = enc8<Q8>(f, factor);
-    }
+    encode_row<T, Q8>(src, reinterpret_cast<uint2*>(q + r * K), vecs, lane, amax);
     if (lane == 0) scale[r] = amax / QuantKind<Q8>::kMax;
   }
 }
