@@ -509,7 +509,7 @@ MOE_API int moe_route_topk_backward(const float* dweights, const void* logits, i
 /* ------------------------------------------------------------------------------------------
  * 4-bit weights with group scales (weights of 16-bit activations; no reference counterpart, the
  * reference's quantised experiments are 8-bit).
- *   W[n, k] = scales[n, g] * (q[n, k] - zeros[n, g]),  g = k / group,  q in 0..15;
+ *   W[n, k] = scales[n, g] * (q[n, k] - zeros[n, g]),  g = k / group,  q in 0..15, zeros in 0..16;
  *   without zeros (NULL): q - 8. group = 32, 64 or 128.
  * Plain form, for `matrices` matrices [N, K] one after another (experts): q [N, ceil(K / 2)] bytes,
  *   columns 2i in the low half; scales [N, ceil(K / group)] dtype; zeros the same shape, bytes.

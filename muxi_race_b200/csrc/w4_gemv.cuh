@@ -2,7 +2,7 @@
 // around them.
 //
 //   y[m, n] = sum_k x[m, k] * W[n, k],   W[n, k] = s[n, g] * (q[n, k] - z[n, g]),   g = k / group
-// q in 0..15, s in the 16-bit type of x, z in 0..15 (8 where there are no zero points).
+// q in 0..15, s in the 16-bit type of x, z in 0..16 (8 where there are no zero points).
 // Per group the products with the whole numbers q - z (exact in either 16-bit type) are summed in
 // fp32 on the tensor cores, and that sum is scaled and added in fp32.
 //
@@ -745,7 +745,7 @@ __global__ void w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __
       const bool in = row >= 0 && g < G;
       const int at = (rr & 7) * 4 + (rr >> 3);
       reinterpret_cast<uint16_t*>(o + kW4TileBytes + i / kW4TileRows * 64)[at] = in ? scales[(m * N + row) * G + g] : 0;
-      if (zeros) o[kW4TileBytes + groups * 64 + i / kW4TileRows * 32 + at] = in ? zeros[(m * N + row) * G + g] & 15 : 0;
+      if (zeros) o[kW4TileBytes + groups * 64 + i / kW4TileRows * 32 + at] = in ? zeros[(m * N + row) * G + g] : 0;
     }
   }
 }

@@ -1,7 +1,7 @@
 """4-bit weights with group scales: the products of a decode step, dense and per expert.
 
-``W[n, k] = scales[n, g] * (q[n, k] - zeros[n, g])`` with ``g = k // group_size`` and q in 0..15 (8
-where there are no zero points). A weight is laid out once, when the model is loaded
+``W[n, k] = scales[n, g] * (q[n, k] - zeros[n, g])`` with ``g = k // group_size``, q in 0..15 and
+zeros in 0..16 (8 where there are none). A weight is laid out once, when the model is loaded
 (:func:`pack_w4` from a checkpoint's values, :func:`quantize_w4` from 16-bit weights), as the stream
 of tiles that the kernels read.
 """
@@ -63,7 +63,8 @@ def pack_w4(
     gate_up: bool = False,
 ) -> W4Weights:
     """Lay out 4-bit weights: q [..., N, ceil(K / 2)] uint8 (column 2i in the low half of byte i),
-    scales [..., N, ceil(K / group_size)] fp16 / bf16, zeros (optional) uint8 of the scales' shape.
+    scales [..., N, ceil(K / group_size)] fp16 / bf16, zeros (optional) uint8 of the scales' shape, 0..16
+    (16 comes from checkpoints that store z - 1 in 4 bits; the zero points are checked, which waits for the GPU).
 
     ``in_features``: K, where it is odd (default: twice q's last dimension). ``gate_up``: the rows are
     gate rows followed by as many up rows, for :func:`fused_moe_w4`.
@@ -80,6 +81,12 @@ def pack_w4(
     if zeros is not None:
         require(zeros.device == q.device and zeros.dtype == torch.uint8 and zeros.is_contiguous()
                 and tuple(zeros.shape) == want, f"zeros must be a contiguous uint8 tensor {want} on {q.device}")
+        require(not bool((zeros > 16).any()), "zeros must be in 0..16")
+    return _pack(q, scales, zeros, (*lead, N, K), group_size, gate_up)
+
+
+def _pack(q, scales, zeros, shape, group_size, gate_up) -> W4Weights:
+    *lead, N, K = shape
     matrices = 1
     for n in lead:
         matrices *= n
@@ -88,7 +95,7 @@ def pack_w4(
     packed = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     launch(q.device, "moe_w4_pack", q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), matrices, N,
            K, group_size, int(gate_up), packed.data_ptr(), packed.numel())
-    return W4Weights(packed, (*lead, N, K), scales.dtype, group_size, zeros is not None, gate_up)
+    return W4Weights(packed, tuple(shape), scales.dtype, group_size, zeros is not None, gate_up)
 
 
 def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True, gate_up: bool = False) -> W4Weights:
@@ -108,7 +115,7 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True, 
     zeros = None if symmetric else torch.empty(scales.shape, dtype=torch.uint8, device=w.device)
     launch(w.device, "moe_w4_quantize", w.data_ptr(), HALVES[w.dtype], w.numel() // K, K, group_size, q.data_ptr(),
            scales.data_ptr(), None if symmetric else zeros.data_ptr())
-    return pack_w4(q, scales, zeros, K, group_size, gate_up)
+    return _pack(q, scales, zeros, w.shape, group_size, gate_up)
 
 
 def dequantize_w4(w: W4Weights) -> torch.Tensor:

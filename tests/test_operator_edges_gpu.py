@@ -323,3 +323,21 @@ def test_operators_without_a_gradient_say_so(cuda_device):
         (m.fused_moe_w4(x, w13, w2, ids, t).float().sum() + t.sum()).backward()
     out = torch.empty_like(x)
     assert m.w4_linear(x.clone().requires_grad_(), lin, out=out) is out and not out.requires_grad
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_w4_zero_points_of_16(cuda_device, group, dtype):
+    """Checkpoints that store z - 1 in 4 bits have zero points up to 16."""
+    v, s, z = w4_random(95, 70, 300, group, True, dtype)
+    z[::2] = 16
+    w, values = w4_packed(v, s, z, group)
+    assert torch.equal(m.dequantize_w4(w), values.to(dtype))
+    for M in (1, 11):
+        x = randn(96, M, 300).to(dtype)
+        ref, mag = linear_ref(x, values)
+        within(m.w4_linear(x, w), ref, U[dtype] * ref.abs() + F32 * mag + TINY[dtype], "y")
+    z[3, 0] = 17
+    with pytest.raises(ValueError, match="zeros must be in 0..16"):
+        w4_packed(v, s, z, group)
+    assert m.device_status() == 0
