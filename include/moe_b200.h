@@ -521,7 +521,7 @@ MOE_API int moe_route_topk_backward(const float* dweights, const void* logits, i
  * moe_w4_linear: out [M, N] = x [M, K] W^T, row pitches ld_x, ld_out. Sums in fp32. Meant for few rows
  *   (the weights are read once per 16); any M, N, K >= 1.
  * moe_fused_w4: moe_fused with 4-bit w13 (packed with gate_up) and w2; the same sums, h = silu(gate) *
- *   up rounded to dtype in between, the top-k combine in fp32 in route order: the same bits on every
+ *   up rounded to dtype in between (fp16: infinite beyond 65504), the top-k combine in fp32 in route order: the same bits on every
  *   run. Ids outside [0, E) are skipped. Meant for decode batches; any T.
  * Requirements: dtype MOE_F16 / MOE_BF16 (x, out and scales), 1 <= E <= 1024.
  * ---------------------------------------------------------------------------------------- */

@@ -19,11 +19,11 @@
 // One warp per token, its logits in registers. The topk-th largest of the 32 lanes' own maxima is a
 // lower bound of the topk-th largest of all, and few candidates reach it (about 10 for topk = 8 of 256):
 // those go to shared memory, and each counts how many are before it. The
-// next token's logits are loaded meanwhile. T = 32768, E = 256, topk = 8: 21 us (softmax of the chosen;
-// with the softmax of all and counts 23 us, sigmoid with bias and groups 46 us), against 34 us with topk
-// rounds of a warp-wide maximum over all; the 33.5 MB of logits take 5 us, the instructions and the
-// latencies of the steps bound it. The gradient writes (and, softmax of all, reads) those bytes: 18 us for
-// 67 MB, 13 us with the logits in L2.
+// next token's logits are loaded meanwhile. T = 32768, E = 256, topk = 8, one input in a graph
+// (so largely from L2): 20 us (softmax of the chosen; with counts 21 us, sigmoid with bias and groups 44 us), against
+// 34 us with topk rounds of a warp-wide maximum over all. From DRAM, softmax of all with counts: 24.6 us, where
+// the 33.5 MB of logits take 5 us; the instructions and the latencies of the steps bound it. The gradient
+// writes (and, softmax of all, reads) those bytes: 18 us from DRAM for 67 MB, 12 us in a graph.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -13,7 +13,7 @@
 //           four 16-byte loads a lane straight into registers, with no shuffles and no shared memory.
 //   strip   the tiles of 32 rows, one after another along K; an expert's strips follow each other.
 // One CTA per SM. Its warps walk through strips with the loads of the next tiles in flight in
-// registers (w4_ahead tiles a warp: 59 to 89 KB an SM); x (at most 16 rows, one slice of K) stays in
+// registers (w4_ahead tiles a warp: 59 to 89 KB an SM with 14 warps, 43 to 49 KB with 10); x (at most 16 rows, one slice of K) stays in
 // shared memory. Warps that share a strip split K; their sums go through shared memory to the store
 // warps, which add them up, so that no consumer waits for another or for a store.
 // mma.sync and not tcgen05.mma: the weights must pass the registers to be unpacked, a 32-row strip
@@ -33,8 +33,8 @@ constexpr int kW4TileK = 128;
 constexpr int kW4TileRows = 32;
 constexpr int kW4TileBytes = 2048;     // values of one tile
 // Rows of x at a time: two blocks of 8. (Four blocks read the weights half as often, but their sums
-// take the registers of the loads ahead and of the other warps: 32 rows of K = 4096, N = 14336 took
-// 51 us in one pass of 32 and take 41 us in two of 16, the second from L2.)
+// take the registers of the loads ahead and of the other warps: when that was built, 32 rows of K = 4096,
+// N = 14336 took 51 us in one pass of 32 and 41 us in two of 16, the second from L2; the two take 28 us now.)
 constexpr int kW4MaxRows = 16;
 // Consumer warps: with the store warps 16 of 128 registers, or 12 of 168 where two blocks of rows meet
 // small groups, whose scales and zero points fill more registers.
@@ -95,7 +95,7 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 // The differences are formed before the products, exactly: a weight of 0 adds nothing, whatever its x. (As
 // -z sum x + sum q x, with the nibbles as they are, fp16 would take four instructions less per eight
 // values: 128 tokens over 256 experts of 7168 x 2048 1103 us instead of 1240, one token over 8 54 instead of
-// 57, a single row of 14336 x 4096 the same. But the terms of a large x at q = z would cancel only to
+// 57, a single row of 14336 x 4096 11.5 us in a graph instead of 13.4. But the terms of a large x at q = z would cancel only to
 // fp32's rounding of them: with x of 6e4 beside 1e-3 nothing of the small columns' sum is left.)
 template <typename T> struct W4Type;
 __device__ __forceinline__ uint32_t w4_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
@@ -251,10 +251,16 @@ __device__ __forceinline__ void w4_tile(const W4Frag<GROUP, ZEROS>& in, uint32_t
   }
 }
 
+// (__expf: at most about 1e-5 off relatively, where v is -80 and the result nothing; the result is rounded
+// to 16 bits.)
 __device__ __forceinline__ float w4_silu(float v) { return v / (1.0f + __expf(-v)); }
 
 // The sums of block t and fragment rows f of a strip leave: v = {row r: rows 2q, 2q + 1 of x; row
-// r + 8: the same}. `out_row`: the output row of x's row `lane`.
+// r + 8: the same}. `out_row`: the output row of x's row `lane`. kW4GateUp rounds h = silu(gate) * up to the
+// activations' type, since h is the next product's operand: the tensor instruction takes 16 bits, and two
+// halves of an fp32 h would double its steps. This is most of what the experts' result is off by
+// (2.8e-4 of its norm in fp16, 2.3e-3 in bf16; rounded only at the end 2.1e-4 and 1.7e-3); in fp16 an h
+// beyond 65504 is infinite.
 template <typename T>
 __device__ __forceinline__ void w4_store(const W4Args& a, int strip, int slice, int out_row, int rows, int t, int f,
                                          const float4& v) {

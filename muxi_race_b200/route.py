@@ -2,7 +2,10 @@
 selection bias, groups, experts that are switched off, strided logits, tokens per expert.
 
 ``fused_topk`` and ``grouped_topk`` are the two fixed forms of serving (contiguous finite logits, no
-gradient); :func:`route_topk` covers training and masked experts.
+gradient); :func:`route_topk` covers what they do, training and masked experts. On a B200 it is the faster one,
+called by itself (11 against 15 us up to 4096 tokens) and in a graph: 256 experts, top-8, 128 / 32768 tokens 2.8
+/ 20 us (``fused_topk`` 3.6 / 42 us), with sigmoid, bias and groups 4.9 / 44 us (``grouped_topk`` 9.8 / 90 us). Of 8 experts,
+top-2, ``fused_topk`` takes less in a graph (2.1 / 9.6 against 2.3 / 11.7 us).
 """
 from __future__ import annotations
 
@@ -77,7 +80,9 @@ def route_topk(
     ``sigmoid(logits)``; the ``topk`` largest ``score + bias`` are chosen (bias [E] fp32, for balance:
     it moves the choice only) among the experts of the ``topk_groups`` best of ``num_groups`` groups,
     a group counting the sum of its ``group_top`` (1 or 2) best (-inf where fewer are eligible). Ids come in descending order, equal
-    ones by the lower id; weights are the chosen scores, divided by their sum when ``renormalize``,
+    ones by the lower id (without bias and groups the order is that of the logits, which tells experts apart whose
+    scores round to one fp32 value; with a bias, if only of zeros, such experts are equal); weights are the chosen scores,
+    divided by their sum when ``renormalize``,
     times ``scale``. An expert whose logit is -inf is never chosen; slots left without one hold id -1
     (which the expert operators skip) and weight 0. (A sigmoid below -88 is 0 in fp32: a token whose chosen scores are
     all 0 has weights 0, renormalised or not.) The weights are differentiable once in
