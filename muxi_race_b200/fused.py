@@ -15,6 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from ._args import overlap
 
 BLOCK_M = 128
 _DTYPES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
@@ -122,6 +123,22 @@ def _check_fused(hidden_states, w13, w2, topk_ids, topk_weights, int8, q_dtype=t
     return int(T), int(H), int(I), int(E), int(topk_ids.shape[1])
 
 
+def _output(out: Optional[torch.Tensor], x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """`out`, or a new tensor of x's shape in `dtype`. A kernel clears the output while others read x."""
+    if out is None:
+        return torch.empty(x.shape, dtype=dtype, device=x.device)
+    _check(out.shape == x.shape and out.dtype == dtype and out.is_contiguous() and out.device == x.device,
+           f"bad out: it must be a contiguous {dtype} tensor {tuple(x.shape)} on {x.device}")
+    _check(not overlap(out, x), "out must not share memory with hidden_states")
+    return out
+
+
+def _check_scales(w13_scale: torch.Tensor, w2_scale: torch.Tensor, E: int, H: int, I: int, dev: torch.device) -> None:
+    for name, t, n in (("w13_scale", w13_scale, E * 2 * I), ("w2_scale", w2_scale, E * H)):
+        _check(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous() and t.device == dev,
+               f"{name} must be fp32 [E, {n // E}] on {dev}")
+
+
 def fused_moe(
     hidden_states: torch.Tensor,
     w_gate_up: torch.Tensor,
@@ -139,9 +156,7 @@ def fused_moe(
     so repeated calls give identical bits; the default adds them with atomics in Stage2.
     """
     T, H, I, E, k = _check_fused(hidden_states, w_gate_up, w_down, topk_ids, topk_weights, False)
-    if out is None:
-        out = torch.empty((T, H), dtype=hidden_states.dtype, device=hidden_states.device)
-    _check(tuple(out.shape) == (T, H) and out.dtype == hidden_states.dtype and out.is_contiguous(), "bad out")
+    out = _output(out, hidden_states, hidden_states.dtype)
     if T == 0:
         return out
     dev = hidden_states.device
@@ -218,8 +233,8 @@ def grouped_topk(
     bias_ptr = None
     if e_score_correction_bias is not None:
         b = e_score_correction_bias
-        _check(b.is_cuda and b.dtype == torch.float32 and b.is_contiguous() and b.numel() == E,
-               "e_score_correction_bias must be a contiguous fp32 CUDA tensor [E]")
+        _check(b.device == gating_output.device and b.dtype == torch.float32 and b.is_contiguous() and b.numel() == E,
+               "e_score_correction_bias must be a contiguous fp32 tensor [E] on the logits' device")
         bias_ptr = b.data_ptr()
     dev = gating_output.device
     ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
@@ -255,9 +270,7 @@ def fused_moe_router(
     T, H, I, E2, k = _check_fused(hidden_states, w_gate_up, w_down, ids, w, False)
     _check(E2 == E, f"gating_output has {E} experts, the weights {E2}")
     _check(gating_output.device == dev, "gating_output must be on the device of hidden_states")
-    if out is None:
-        out = torch.empty((T, H), dtype=hidden_states.dtype, device=dev)
-    _check(tuple(out.shape) == (T, H) and out.dtype == hidden_states.dtype and out.is_contiguous(), "bad out")
+    out = _output(out, hidden_states, hidden_states.dtype)
     if T:
         dt = _DTYPES[hidden_states.dtype]
         nbytes = _lib.lib().moe_fused_workspace_bytes(T, k, E, H, I, dt)
@@ -298,14 +311,9 @@ def _fused_q8_rows(x_q, x_scale, q_dtype, w13_q, w13_scale, w2_q, w2_scale, topk
     _check(x_scale.dtype == torch.float32 and x_scale.numel() == T and x_scale.is_contiguous() and x_scale.device == x_q.device,
            "hidden_scale must be contiguous fp32 [T]")
     _check(x_q.is_cuda and x_q.is_contiguous(), "hidden_states must be a contiguous CUDA tensor")
-    if out is None:
-        out = torch.empty((T, H), dtype=out_dtype, device=x_q.device)
+    out = _output(out, x_q, out_dtype)
     _, _, I, E, k = _check_fused(out, w13_q, w2_q, topk_ids, topk_weights, True, q_dtype)
-    _check(tuple(out.shape) == (T, H) and out.device == x_q.device, "bad out")
-    _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
-           "w13_scale must be fp32 [E, 2I]")
-    _check(w2_scale.dtype == torch.float32 and w2_scale.numel() == E * H and w2_scale.is_contiguous(),
-           "w2_scale must be fp32 [E, H]")
+    _check_scales(w13_scale, w2_scale, E, H, I, x_q.device)
     if T == 0:
         return out
     dev, dt = x_q.device, _DTYPES[out.dtype]
@@ -343,12 +351,8 @@ def fused_moe_int8(
                               topk_weights, out, out_dtype)
     _check(out_dtype is None, "out_dtype needs hidden_scale: otherwise the output has the dtype of hidden_states")
     T, H, I, E, k = _check_fused(hidden_states, w13_q, w2_q, topk_ids, topk_weights, True)
-    _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
-           "w13_scale must be fp32 [E, 2I]")
-    _check(w2_scale.dtype == torch.float32 and w2_scale.numel() == E * H and w2_scale.is_contiguous(),
-           "w2_scale must be fp32 [E, H]")
-    if out is None:
-        out = torch.empty((T, H), dtype=hidden_states.dtype, device=hidden_states.device)
+    _check_scales(w13_scale, w2_scale, E, H, I, hidden_states.device)
+    out = _output(out, hidden_states, hidden_states.dtype)
     if T == 0:
         return out
     dev = hidden_states.device
@@ -403,12 +407,8 @@ def fused_moe_fp8(
                               topk_weights, out, out_dtype)
     _check(out_dtype is None, "out_dtype needs hidden_scale: otherwise the output has the dtype of hidden_states")
     T, H, I, E, k = _check_fused(hidden_states, w13_q, w2_q, topk_ids, topk_weights, True, torch.float8_e4m3fn)
-    _check(w13_scale.dtype == torch.float32 and w13_scale.numel() == E * 2 * I and w13_scale.is_contiguous(),
-           "w13_scale must be fp32 [E, 2I]")
-    _check(w2_scale.dtype == torch.float32 and w2_scale.numel() == E * H and w2_scale.is_contiguous(),
-           "w2_scale must be fp32 [E, H]")
-    if out is None:
-        out = torch.empty((T, H), dtype=hidden_states.dtype, device=hidden_states.device)
+    _check_scales(w13_scale, w2_scale, E, H, I, hidden_states.device)
+    out = _output(out, hidden_states, hidden_states.dtype)
     if T == 0:
         return out
     dev = hidden_states.device

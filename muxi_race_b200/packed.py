@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .fused import _DTYPES, _ID_DTYPES, _W_DTYPES, _check, _stream, _workspace
+from .fused import _DTYPES, _ID_DTYPES, _W_DTYPES, _check, _output, _stream, _workspace
 
 KINDS = {"fp16": _lib.MOE_F16, "bf16": _lib.MOE_BF16, "int8": _lib.MOE_I8, "fp8": _lib.MOE_F8E4M3}
 _MAGIC = "muxi_race_b200.packed_weights.v1"
@@ -89,8 +89,7 @@ def fused_moe_packed(hidden_states: torch.Tensor, packed: PackedWeights, topk_id
                "all tensors must be contiguous CUDA tensors on one device")
     _check(topk_ids.dtype in _ID_DTYPES and topk_weights.dtype in _W_DTYPES, "bad routing dtypes")
     k = int(topk_ids.shape[1])
-    if out is None:
-        out = torch.empty((T, H), dtype=hidden_states.dtype, device=hidden_states.device)
+    out = _output(out, hidden_states, hidden_states.dtype)
     if T == 0:
         return out
     dev = hidden_states.device
