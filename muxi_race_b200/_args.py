@@ -42,21 +42,23 @@ def pitch(t: torch.Tensor) -> int:
     return t.shape[1] if t.is_contiguous() or t.shape[0] == 1 else t.stride(0)
 
 
-def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two 2-D tensors with contiguous rows share memory. Column ranges of one wider tensor are
-    told apart; rows of different pitches that interleave count as shared."""
-    if a.numel() == 0 or b.numel() == 0:
+def overlap_at(a: int, step_a: int, row_a: int, rows_a: int, b: int, step_b: int, row_b: int, rows_b: int) -> bool:
+    """Whether two blocks of rows share memory: their addresses, and in bytes from row to row and the rows
+    themselves. Column ranges of one wider tensor are told apart; rows of different pitches that interleave
+    count as shared."""
+    if a + (rows_a - 1) * step_a + row_a <= b or b + (rows_b - 1) * step_b + row_b <= a or rows_a == 0 or rows_b == 0:
         return False
-    size_a, size_b = a.element_size(), b.element_size()
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    row_a, row_b = a.shape[1] * size_a, b.shape[1] * size_b
-    step_a, step_b = pitch(a) * size_a, pitch(b) * size_b
-    if a0 + (a.shape[0] - 1) * step_a + row_a <= b0 or b0 + (b.shape[0] - 1) * step_b + row_b <= a0:
-        return False
-    if step_a != step_b or step_a == 0 or a.shape[0] == 1 or b.shape[0] == 1:
+    if step_a != step_b or step_a == 0 or rows_a == 1 or rows_b == 1:
         return True
-    at = (b0 - a0) % step_a  # where a row of b starts from the last start of a row of a
+    at = (b - a) % step_a  # where a row of b starts from the last start of a row of a
     return at < row_a or at + row_b > step_a
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """:func:`overlap_at` of two 2-D tensors with contiguous rows."""
+    size_a, size_b = a.element_size(), b.element_size()
+    return overlap_at(a.data_ptr(), pitch(a) * size_a, a.shape[1] * size_a, a.shape[0],
+                      b.data_ptr(), pitch(b) * size_b, b.shape[1] * size_b, b.shape[0])
 
 
 def empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, launch, once_differentiable, overlap, pitch, require, rows, without_gradient
+from ._args import FLOATS, launch, once_differentiable, overlap_at, pitch, require, rows, without_gradient
 from .fused import _workspace
 
 _Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -27,32 +27,41 @@ def _check_weight(weight: torch.Tensor, H: int, dtype: torch.dtype, dev: torch.d
     return FLOATS[weight.dtype]
 
 
-def _output(t: Optional[torch.Tensor], x: torch.Tensor, name: str, *others: Optional[torch.Tensor]):
+def _output(t: Optional[torch.Tensor], x: torch.Tensor, name: str, T: int, *others: tuple):
     """`t`, or a new tensor of x's shape and dtype, with its address and row pitch. `t` may be one of
-    `others` (2-D), row for row: a row is read before it is written. It may not share memory with them
-    in another way, where a row would be written while another is read from the same place."""
+    `others` (address and pitch of as many rows, T), row for row: a row is read before it is written. It
+    may not share memory with them in another way, where a row would be written while another is read
+    from the same place."""
     if t is None:
         t = torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
         return t, t.data_ptr(), x.shape[-1]
     require(t.shape == x.shape and t.dtype == x.dtype, f"{name} must have the shape and dtype of x")
     t2 = rows(t, name, x.device)
-    ptr, ld = t2.data_ptr(), pitch(t2)
+    here = ptr, ld = t2.data_ptr(), pitch(t2)
     for o in others:
-        if o is not None and not (o.data_ptr() == ptr and pitch(o) == ld) and overlap(t2, o):
+        if o != here and o[0] is not None and _shared(here, o, T, t2):
             raise ValueError(f"{name} must be x or residual itself, or share no memory with them")
     return t, ptr, ld
 
 
-def _sum_args(x, x2, residual, residual_out):
-    """(residual's rows, h, residual's address and pitch, h's address and pitch); no residual: h is None."""
+def _shared(a: tuple, b: tuple, T: int, like: torch.Tensor) -> bool:
+    size = like.element_size()
+    row = like.shape[1] * size
+    return overlap_at(a[0], a[1] * size, row, T, b[0], b[1] * size, row, T)
+
+
+def _sum_args(x, x_at, T, residual, residual_out):
+    """(h, residual's address and pitch, h's address and pitch); no residual: h is None. x_at: x's address
+    and pitch."""
     if residual is None:
         require(residual_out is None, "residual_out needs a residual")
-        return None, None, None, 0, None, 0
+        return None, None, 0, None, 0
     if residual.shape != x.shape or residual.dtype != x.dtype:
         raise ValueError("residual must have the shape and dtype of x")
     r2 = rows(residual, "residual", x.device)
-    h, h_ptr, h_ld = _output(residual_out, x, "residual_out", x2, r2)
-    return r2, h, r2.data_ptr(), pitch(r2), h_ptr, h_ld
+    r_at = r2.data_ptr(), pitch(r2)
+    h, h_ptr, h_ld = _output(residual_out, x, "residual_out", T, x_at, r_at)
+    return h, *r_at, h_ptr, h_ld
 
 
 def _forward(x, weight, residual, eps, out, residual_out):
@@ -60,12 +69,13 @@ def _forward(x, weight, residual, eps, out, residual_out):
     T, H = x2.shape
     dtype, dev = x2.dtype, x2.device
     wdt = _check_weight(weight, H, dtype, dev)
-    r2, h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x2, residual, residual_out)
-    y, y_ptr, y_ld = _output(out, x, "out", x2, r2)
-    if out is not None and residual_out is not None:
-        require(not overlap(rows(out, "out"), rows(residual_out, "residual_out")), "out and residual_out share memory")
+    x_at = x2.data_ptr(), pitch(x2)
+    h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x_at, T, residual, residual_out)
+    y, y_ptr, y_ld = _output(out, x, "out", T, x_at, (r_ptr, r_ld))
+    if out is not None and residual_out is not None and _shared((y_ptr, y_ld), (h_ptr, h_ld), T, x2):
+        raise ValueError("out and residual_out share memory")
     dt = FLOATS[dtype]
-    launch(dev, "moe_add_rms_norm", x2.data_ptr(), pitch(x2), r_ptr, r_ld, weight.data_ptr(), wdt, y_ptr, y_ld, dt, None,
+    launch(dev, "moe_add_rms_norm", *x_at, r_ptr, r_ld, weight.data_ptr(), wdt, y_ptr, y_ld, dt, None,
            h_ptr, h_ld, T, H, eps, dt)
     return y, h
 
@@ -136,8 +146,9 @@ def add_rms_norm_quant(
     wdt = _check_weight(weight, H, dtype, dev)
     q = torch.empty_like(x, dtype=q_dtype, memory_format=torch.contiguous_format)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    _, h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x2, residual, residual_out)
-    launch(dev, "moe_add_rms_norm", x2.data_ptr(), pitch(x2), r_ptr, r_ld, weight.data_ptr(), wdt, q.data_ptr(), H,
+    x_at = x2.data_ptr(), pitch(x2)
+    h, r_ptr, r_ld, h_ptr, h_ld = _sum_args(x, x_at, T, residual, residual_out)
+    launch(dev, "moe_add_rms_norm", *x_at, r_ptr, r_ld, weight.data_ptr(), wdt, q.data_ptr(), H,
            _Q_DTYPES[q_dtype], scale.data_ptr(), h_ptr, h_ld, T, H, eps, FLOATS[dtype])
     if residual_out is not None:
         return (*without_gradient("add_rms_norm_quant", (q, scale), x, weight, residual), h)
