@@ -551,6 +551,78 @@ MOE_API int moe_fused_w4(const void* hidden_states, int64_t ld_hidden, const voi
                          int64_t intermediate, int64_t num_experts, int64_t topk, int dtype, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Products grouped by expert with ragged row counts, and their gradients (training of the experts; no
+ * reference counterpart).
+ *   rows offsets[e] <= r < offsets[e + 1] belong to expert e; offsets [E + 1] int32 / int64, not falling
+ *   moe_grouped_linear:     out[r] = W[e] x[r]        x [R, K], w [E, N, K] contiguous, out [R, N]
+ *   moe_grouped_linear_dx:  dx[r] = W[e]^T dy[r]      dy [R, N], dx [R, K]
+ *   moe_grouped_linear_dw:  dw[e] = sum_r dy[r] x[r]^T over e's rows, 0 without rows; dw [E, N, K] contiguous in
+ *                           dtype or MOE_F32
+ * Rows of no expert (before offsets[0], from offsets[E] on): 0 where zero_rest != 0, else left as they are; what
+ * they hold is never used. Offsets outside [0, R] are clamped. Sums in fp32, one rounding; the same bits on every run.
+ * Requirements: dtype MOE_F16 / MOE_BF16; 1 <= E <= 1024; N and K multiples of 8; x, dy and w on 16-byte boundaries,
+ *   row pitches (in elements) of x and dy multiples of 8; outputs share no memory with inputs.
+ * ---------------------------------------------------------------------------------------- */
+MOE_API int moe_grouped_linear(const void* x, int64_t ld_x, const void* w, const void* offsets, int offsets_dtype, void* out,
+                               int64_t ld_out, int64_t num_rows, int64_t num_experts, int64_t out_features,
+                               int64_t in_features, int dtype, int zero_rest, void* stream);
+
+MOE_API int moe_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, const void* offsets, int offsets_dtype,
+                                  void* dx, int64_t ld_dx, int64_t num_rows, int64_t num_experts, int64_t out_features,
+                                  int64_t in_features, int dtype, int zero_rest, void* stream);
+
+MOE_API int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets,
+                                  int offsets_dtype, void* dw, int dw_dtype, int64_t num_rows, int64_t num_experts,
+                                  int64_t out_features, int64_t in_features, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The activation between the experts' products, and 8-bit copies of rows for the backward pass.
+ * 8-bit rows: fp32 scales [R, parts, ceil(W / parts / 128)], one for each 128 columns of each of a row's `parts`.
+ *   MOE_I8: scale = amax / 127, x / scale to nearest, halves away from zero. MOE_F8E4M3: scale = the smallest
+ *   power of two with 448 scale >= amax. A group with NaN or an infinity: scale NaN.
+ *   moe_save_rows8: x [R, W] (pitch ld) -> q [R, W], scale.
+ *   moe_restore_rows: out[r] = row index[r] / index_div of x (r without an index) in dtype; zeros where that is
+ *     not in [0, src_rows). src_dtype MOE_I8 / MOE_F8E4M3 with scale, or dtype (rows as they are).
+ *   moe_silu_mul: h = w silu(gate) up, gate_up [R, 2 I] (gate, then up), and with q its 8-bit copy (parts = 2).
+ *   moe_silu_mul_backward: dgate_up [R, 2 I], h [R, I] and dweights from dh [R, I] and gate_up, in dtype or as 8-bit rows
+ *     (contiguous, ld = 2 I, src_scale).
+ *     weights (NULL: 1) are taken at weight_at[r] (NULL: r) of num_weights; a row whose place is outside has weight 0.
+ *     dweights (may be NULL) is written at those places in weights_dtype; others are left as they are.
+ *   moe_combine_rows: out[t] = sum of y[slot[t * topk + j]] over j, in that order; slots outside [0, R) are skipped.
+ * valid_rows: on the device, rows from *valid_rows on are left as they are; NULL: none. h, dgate_up, q, out and y contiguous.
+ * Sums in fp32, one rounding; the same bits on every run. dtype MOE_F16 / MOE_BF16, any R, W, I >= 1; outputs share no
+ * memory with inputs.
+ * ---------------------------------------------------------------------------------------- */
+MOE_API int moe_save_rows8(const void* x, int64_t ld, void* q, int q_dtype, float* scale, int64_t num_rows, int64_t width,
+                           int64_t parts, int dtype, void* stream);
+
+MOE_API int moe_restore_rows(const void* x, int64_t ld, int src_dtype, const float* scale, const void* index, int index_dtype,
+                             int64_t index_div, const int32_t* valid_rows, void* out, int64_t num_rows, int64_t src_rows,
+                             int64_t width, int64_t parts, int dtype, void* stream);
+
+MOE_API int moe_silu_mul(const void* gate_up, int64_t ld, const void* weights, int weights_dtype, const int32_t* weight_at,
+                         int64_t num_weights, const int32_t* valid_rows, void* h, void* q, int q_dtype, float* scale,
+                         int64_t num_rows, int64_t intermediate, int dtype, void* stream);
+
+MOE_API int moe_silu_mul_backward(const void* dh, int64_t ld_dh, const void* gate_up, int64_t ld, int src_dtype,
+                                  const float* src_scale, const void* weights, int weights_dtype, const int32_t* weight_at,
+                                  int64_t num_weights, const int32_t* valid_rows, void* dgate_up, void* h, void* dweights,
+                                  int64_t num_rows, int64_t intermediate, int dtype, void* stream);
+
+MOE_API int moe_combine_rows(const void* y, const int32_t* slot, void* out, int64_t num_tokens, int64_t topk, int64_t num_rows,
+                             int64_t hidden, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Dense product of int8 rows: out[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] (+ bias[n]).
+ * x [M, K] (pitch ld_x) and w [N, K] (contiguous) int8 as moe_quantize_rows_int8 or moe_add_rms_norm write them; out [M, N]
+ * (pitch ld_out) MOE_F16, MOE_BF16 or MOE_F32; bias [N] fp32 or NULL. The sum is exact (int32); scales and bias in fp32.
+ * Requirements: K a multiple of 16 below 131072; x and w on 16-byte boundaries, ld_x a multiple of 16.
+ * ---------------------------------------------------------------------------------------- */
+MOE_API int moe_int8_linear(const void* x, int64_t ld_x, const float* x_scale, const void* w, const float* w_scale,
+                            const float* bias, void* out, int64_t ld_out, int out_dtype, int64_t m, int64_t n, int64_t k,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 // capi_host.h — host helpers shared by the translation units of the C ABI: the calling thread's
-// error message, the launch-error macros and the per-device SM count. Defined in moe_capi.cu.
+// error message, the launch-error macros, the per-device SM count and the tensor maps. Defined in moe_capi.cu.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -19,6 +20,11 @@ void clear_error();
 int current_device(int* dev);        // MOE_OK and the current device's ordinal (< kMaxDevices)
 int device_sms(int dev, int* sms);   // MOE_OK and the device's SM count (cached)
 int device_status_ptr(int dev, uint32_t** p);  // MOE_OK and the device's status word
+
+// Tiled map over a tensor of `rank` dimensions (dims[0] innermost, in elements; strides of dims
+// 1..rank-1 in bytes), 128-byte swizzle (matches the kernels' shared-memory descriptors).
+int encode_map(CUtensorMap* map, const void* base, int elt_bytes, int rank, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box, const char* what);
 
 #define MOE_CUDA(call)                                                                        \
   do {                                                                                        \

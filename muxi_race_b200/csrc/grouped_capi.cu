@@ -1,0 +1,175 @@
+// grouped_capi.cu — host side of the products grouped by expert, their gradients, and the dense int8 product
+// (include/moe_b200.h).
+#include "capi_host.h"
+#include "grouped_gemm.cuh"
+
+namespace moe {
+namespace {
+
+constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 1;
+
+
+
+int check_grouped(const void* offsets, int offsets_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype) {
+  if (dtype != MOE_F16 && dtype != MOE_BF16) return fail(MOE_ERR_INVALID_ARG, "dtype must be MOE_F16 or MOE_BF16");
+  if (offsets_dtype != MOE_I32 && offsets_dtype != MOE_I64)
+    return fail(MOE_ERR_INVALID_ARG, "offsets must be int32 or int64");
+  if (!offsets) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  if (E < 1 || E > kGgMaxExperts) return fail(MOE_ERR_INVALID_ARG, "num_experts must be in [1, %d]", kGgMaxExperts);
+  if (N < 8 || K < 8 || N % 8 != 0 || K % 8 != 0 || N > kMaxExtent || K > kMaxExtent)
+    return fail(MOE_ERR_INVALID_ARG, "out_features and in_features must be positive multiples of 8");
+  if (R < 0 || R > kMaxExtent) return fail(MOE_ERR_INVALID_ARG, "bad row count");
+  return MOE_OK;
+}
+
+// Rows [rows, width] of pitch ld (elements), read by boxes of box_width x box_rows.
+int map_rows(CUtensorMap* m, const void* p, int elt, int64_t rows, int64_t width, int64_t ld, int box_width, int box_rows,
+             const char* what) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(rows == 1 ? (width * elt + 15) / 16 * 16 : ld * elt)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_width), static_cast<cuuint32_t>(box_rows)};
+  return encode_map(m, p, elt, 2, dims, strides, box, what);
+}
+
+// Weights [E, N, K], contiguous.
+int map_weights(CUtensorMap* m, const void* p, int elt, int64_t E, int64_t N, int64_t K, int box_width, int box_rows) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(E)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(K * elt), static_cast<cuuint64_t>(N * K * elt)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_width), static_cast<cuuint32_t>(box_rows), 1};
+  return encode_map(m, p, elt, 3, dims, strides, box, "weights");
+}
+
+template <int KIND, typename T, typename OutT>
+int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b32, GroupedArgs args, cudaStream_t s) {
+  int dev, sms;
+  MOE_TRY(current_device(&dev));
+  MOE_TRY(device_sms(dev, &sms));
+  MOE_TRY(device_status_ptr(dev, &args.status));
+  const int64_t lane_tiles = (args.lanes + kGgTile - 1) / kGgTile;
+  const int64_t groups = KIND == kGroupedDw ? static_cast<int64_t>(args.E) * ((args.cols + kGgTile - 1) / kGgTile)
+                                            : (args.rows + kGgTile - 1) / kGgTile + args.E;
+  if (lane_tiles * groups > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
+  int64_t pairs = sms / 2;
+  if (lane_tiles * groups < pairs) pairs = lane_tiles * groups;
+  constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT>;
+  MOE_TRY(allow_smem<kernel>(dev));
+  kernel<<<static_cast<unsigned>(2 * pairs), kGgThreads, kGgSmemBytes, s>>>(a, b, b32, args);
+  MOE_CUDA(cudaGetLastError());
+  return MOE_OK;
+}
+
+// Y and Dx: rows of `red` elements times weights, to rows of `lanes` elements.
+template <int KIND>
+int grouped_rows(const void* in, int64_t ld_in, const void* w, const void* offsets, int offsets_dtype, void* out, int64_t ld_out,
+                 int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, cudaStream_t s) {
+  MOE_TRY(check_grouped(offsets, offsets_dtype, R, E, N, K, dtype));
+  if (R == 0) return MOE_OK;
+  if (!in || !w || !out) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  const int64_t lanes = KIND == kGroupedY ? N : K, red = KIND == kGroupedY ? K : N;
+  if (R > 1 && (ld_in < red || ld_out < lanes)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
+  CUtensorMap a, b, b32;
+  if (KIND == kGroupedY)
+    MOE_TRY(map_weights(&a, w, 2, E, N, K, 64, 128));
+  else
+    MOE_TRY(map_weights(&a, w, 2, E, N, K, 64, 64));
+  MOE_TRY(map_rows(&b, in, 2, R, red, ld_in, 64, 128, "rows"));
+  MOE_TRY(map_rows(&b32, in, 2, R, red, ld_in, 64, 32, "rows"));
+  GroupedArgs g{};
+  g.offsets = offsets;
+  g.offsets64 = offsets_dtype == MOE_I64;
+  g.E = static_cast<int>(E);
+  g.rows = R;
+  g.lanes = static_cast<int>(lanes);
+  g.red = static_cast<int>(red);
+  g.out = out;
+  g.ld_out = ld_out;
+  g.zero_rest = zero_rest;
+  return dtype == MOE_F16 ? launch_grouped<KIND, __half, __half>(a, b, b32, g, s)
+                          : launch_grouped<KIND, __nv_bfloat16, __nv_bfloat16>(a, b, b32, g, s);
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int moe_grouped_linear(const void* x, int64_t ld_x, const void* w, const void* offsets, int offsets_dtype, void* out,
+                       int64_t ld_out, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* stream) {
+  clear_error();
+  return grouped_rows<kGroupedY>(x, ld_x, w, offsets, offsets_dtype, out, ld_out, R, E, N, K, dtype, zero_rest,
+                                 static_cast<cudaStream_t>(stream));
+}
+
+int moe_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, const void* offsets, int offsets_dtype, void* dx,
+                          int64_t ld_dx, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* stream) {
+  clear_error();
+  return grouped_rows<kGroupedDx>(dy, ld_dy, w, offsets, offsets_dtype, dx, ld_dx, R, E, N, K, dtype, zero_rest,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets, int offsets_dtype,
+                          void* dw, int dw_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, void* stream) {
+  clear_error();
+  MOE_TRY(check_grouped(offsets, offsets_dtype, R, E, N, K, dtype));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dw_dtype != dtype && dw_dtype != MOE_F32) return fail(MOE_ERR_INVALID_ARG, "dw_dtype must be dtype or MOE_F32");
+  if (!dw) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  if (R == 0) {
+    MOE_CUDA(cudaMemsetAsync(dw, 0, static_cast<size_t>(E) * N * K * (dw_dtype == MOE_F32 ? 4 : 2), s));
+    return MOE_OK;
+  }
+  if (!dy || !x) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  if (R > 1 && (ld_dy < N || ld_x < K)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
+  CUtensorMap a, b;
+  MOE_TRY(map_rows(&a, x, 2, R, K, ld_x, 64, 64, "x"));
+  MOE_TRY(map_rows(&b, dy, 2, R, N, ld_dy, 64, 64, "dy"));
+  GroupedArgs g{};
+  g.offsets = offsets;
+  g.offsets64 = offsets_dtype == MOE_I64;
+  g.E = static_cast<int>(E);
+  g.rows = R;
+  g.lanes = static_cast<int>(K);
+  g.cols = static_cast<int>(N);
+  g.out = dw;
+  g.ld_out = K;
+  if (dtype == MOE_F16)
+    return dw_dtype == MOE_F32 ? launch_grouped<kGroupedDw, __half, float>(a, b, b, g, s)
+                               : launch_grouped<kGroupedDw, __half, __half>(a, b, b, g, s);
+  return dw_dtype == MOE_F32 ? launch_grouped<kGroupedDw, __nv_bfloat16, float>(a, b, b, g, s)
+                             : launch_grouped<kGroupedDw, __nv_bfloat16, __nv_bfloat16>(a, b, b, g, s);
+}
+
+int moe_int8_linear(const void* x, int64_t ld_x, const float* x_scale, const void* w, const float* w_scale, const float* bias,
+                    void* out, int64_t ld_out, int out_dtype, int64_t M, int64_t N, int64_t K, void* stream) {
+  clear_error();
+  if (out_dtype != MOE_F16 && out_dtype != MOE_BF16 && out_dtype != MOE_F32)
+    return fail(MOE_ERR_INVALID_ARG, "out_dtype must be MOE_F16, MOE_BF16 or MOE_F32");
+  // |sum| <= 2^14 K has to fit 31 bits
+  if (K < 16 || K % 16 != 0 || K >= (1 << 17)) return fail(MOE_ERR_INVALID_ARG, "in_features must be a multiple of 16 below 131072");
+  if (N < 1 || N > kMaxExtent || M < 0 || M > kMaxExtent) return fail(MOE_ERR_INVALID_ARG, "bad row count");
+  if (M == 0) return MOE_OK;
+  if (!x || !x_scale || !w || !w_scale || !out) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  if (M > 1 && (ld_x < K || ld_out < N)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CUtensorMap a, b, b32;
+  MOE_TRY(map_weights(&a, w, 1, 1, N, K, 128, 128));
+  MOE_TRY(map_rows(&b, x, 1, M, K, ld_x, 128, 128, "x"));
+  MOE_TRY(map_rows(&b32, x, 1, M, K, ld_x, 128, 32, "x"));
+  GroupedArgs g{};
+  g.E = 1;
+  g.rows = M;
+  g.lanes = static_cast<int>(N);
+  g.red = static_cast<int>(K);
+  g.out = out;
+  g.ld_out = ld_out;
+  g.lane_scale = w_scale;
+  g.col_scale = x_scale;
+  g.bias = bias;
+  if (out_dtype == MOE_F16) return launch_grouped<kDenseInt8, int8_t, __half>(a, b, b32, g, s);
+  if (out_dtype == MOE_BF16) return launch_grouped<kDenseInt8, int8_t, __nv_bfloat16>(a, b, b32, g, s);
+  return launch_grouped<kDenseInt8, int8_t, float>(a, b, b32, g, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,483 @@
+// grouped_gemm.cuh — matrix products grouped by expert with ragged row counts, and their gradients.
+//
+// Rows offsets[e] <= r < offsets[e + 1] belong to expert e (W [E, N, K] with K contiguous):
+//   kGroupedY    y[r, n]     = sum_k W[e, n, k] x[r, k]
+//   kGroupedDx   dx[r, k]    = sum_n W[e, n, k] dy[r, n]
+//   kGroupedDw   dW[e, n, k] = sum_r x[r, k] dy[r, n]     over e's rows
+//   kDenseInt8   y[m, n]     = xs[m] ws[n] sum_k w[n, k] x[m, k] (+ bias[n]), int8, one group
+// One kernel serves all four. The MMA's M side ("lanes": 256 per CTA pair) is always the dimension that
+// is contiguous in the output (n, k, k, n), its N side ("columns") the output's rows: tokens, or n for
+// dW. So an expert's tokens fill columns in steps of 32, not whole 128-row blocks; the weights are read
+// in full tiles; and a thread, which holds one lane's accumulators, stores elements that its warp's
+// neighbours continue (32 lanes, one segment of 64 or 128 bytes), with any mask or alignment.
+//
+// The reduction runs along k (Y, int8: both operands have it contiguous, "K-major"), along n (Dx: the
+// weights have it outermost, "MN-major") or along the rows (Dw: both operands MN-major). tcgen05 reads
+// either form from 128B-swizzled shared memory: K-major tiles are rows of 128 bytes of reduction, MN-major
+// tiles 64 reduction rows of 128 bytes of lanes or columns, two of them side by side for 128.
+//
+// Bounds: 2 R N K operations at the tensor rate, or the weights' bytes where an expert has fewer than
+// about 250 rows. CTA pairs (cta_group::2) halve each SM's intake of the wider operand: a 256 x 256 tile
+// takes 32 KiB per SM and 64-element step. Six stages of those; two accumulators of 256 columns, so that
+// one tile's stores overlap the next one's MMAs.
+//
+// Dw reduces over rows, so the last block of an expert reaches into the next expert's rows. Those may
+// hold infinities or NaN, which a zero in the other operand would not remove: a warp of its own clears
+// the rows behind the end in both operands (at most 15, up to a multiple of the MMA's 16) after the
+// copy has landed, and only then tells the MMA warp.
+//
+// Roles per CTA (256 threads): warp 0 TMA producer, warp 1 MMA issuer (the pair's leader), warp 2 TMEM
+// and the tile table, warp 3 the clearing of Dw's tails, warps 4-7 epilogue (one TMEM lane quadrant
+// each). Every wait is bounded; the final cluster barrier is reached on every path.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+#include <type_traits>
+
+#include "sm100_ptx.cuh"
+
+namespace moe {
+
+enum GroupedKind : int { kGroupedY = 0, kGroupedDx = 1, kGroupedDw = 2, kDenseInt8 = 3 };
+
+constexpr int kGgStages = 6;
+constexpr int kGgOperandBytes = 128 * 128;  // of one operand, per CTA and stage
+constexpr int kGgStageBytes = 2 * kGgOperandBytes;
+constexpr int kGgTile = 256;                // lanes per pair, columns at most
+constexpr int kGgMaxExperts = 1024;
+constexpr int kGgThreads = 256;
+constexpr int kGgEpiWarps = 4;
+constexpr int kGgBand = 8;  // column tiles that take turns on a weight tile
+constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiples of 32
+constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
+constexpr int kGgSmemBytes = 1024 + kGgStages * kGgStageBytes + 256 + kGgTableInts * 4;
+static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
+
+struct GroupedArgs {
+  const void* offsets;   // [E + 1] int32 / int64; null: one group of all rows
+  int offsets64;
+  int E;
+  int64_t rows;          // R
+  int lanes;             // extent of the lane dimension (contiguous in the output)
+  int cols;              // Dw: extent of the column dimension (N); otherwise unused
+  int red;               // extent of the reduction; Dw: unused
+  void* out;
+  int64_t ld_out;
+  int zero_rest;         // rows of no group are cleared
+  const float* lane_scale;  // int8: ws
+  const float* col_scale;   // int8: xs
+  const float* bias;        // int8, or null
+  uint32_t* status;
+};
+
+template <typename OutT> __device__ __forceinline__ OutT gg_cast(float v);
+template <> __device__ __forceinline__ float gg_cast<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half gg_cast<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 gg_cast<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// MN-major operand: 64 lanes or columns (128 bytes, swizzled) per reduction row, 8 rows per 1024-byte
+// atom (stride SBO), the next 64 lanes 64 rows further (stride LBO).
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(8192u >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+// Arms a barrier of the pair's leader. No data of this thread is published with it, so CTA scope does (a release at
+// cluster scope is a fence, which the producer would wait for in every block).
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr), "r"(bytes)
+               : "memory");
+}
+// 3-D tiled load whose completion is counted on a barrier of the pair's leader; no multicast.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z,
+                                                 uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+
+// One tile: expert, first lane, first column (a row; Dw: an n), columns, and for Dw the rows it reduces.
+struct GroupedTile {
+  int e, lane0, ncols;
+  int64_t row0;
+  int col0, kblocks, tail;  // tail: reduction rows or elements in the last block (0: it is full)
+};
+
+__device__ __forceinline__ int gg_col_step(int rows) {  // columns per tile of a group: even shares of at most 256
+  const int tiles = (rows + kGgTile - 1) / kGgTile;
+  const int share = (rows + tiles - 1) / tiles;
+  return (share + kGgColStep - 1) / kGgColStep * kGgColStep;
+}
+
+template <int KIND>
+struct GroupedSchedule {
+  const int *prefix, *start, *rows;  // tiles before group e, its first row, its rows
+  int E, lane_tiles, red_blocks, red_tail, cols, e;
+
+  __device__ GroupedSchedule(const GroupedArgs& a, const int* table) {
+    prefix = table;
+    start = table + kGgMaxExperts + 1;
+    rows = start + kGgMaxExperts;
+    E = a.E;
+    lane_tiles = (a.lanes + kGgTile - 1) / kGgTile;
+    constexpr int kRed = KIND == kDenseInt8 ? 128 : 64;
+    red_blocks = (a.red + kRed - 1) / kRed;
+    red_tail = a.red % kRed;
+    cols = a.cols;
+    e = 0;
+  }
+  __device__ int tiles() const { return prefix[E]; }
+  // Tiles are asked for in rising order.
+  __device__ GroupedTile get(int tile) {
+    while (tile >= prefix[e + 1]) ++e;
+    GroupedTile t;
+    t.e = e;
+    int i = tile - prefix[e];
+    const int n = rows[e];
+    if (KIND == kGroupedDw) {
+      const int col_tiles = (cols + kGgTile - 1) / kGgTile;
+      t.lane0 = i / col_tiles * kGgTile;
+      t.col0 = i % col_tiles * kGgTile;
+      t.ncols = min(kGgTile, cols - t.col0);
+      t.row0 = start[e];
+      t.kblocks = (n + 63) / 64;
+      t.tail = n % 64;
+    } else {
+      const int step = gg_col_step(n), col_tiles = (n + step - 1) / step;
+      const int band = i / (lane_tiles * kGgBand);
+      i -= band * lane_tiles * kGgBand;
+      const int width = min(kGgBand, col_tiles - band * kGgBand);
+      t.lane0 = i / width * kGgTile;
+      const int c = (band * kGgBand + i % width) * step;
+      t.ncols = min(step, n - c);
+      t.row0 = start[e] + c;
+      t.col0 = 0;
+      t.kblocks = red_blocks;
+      t.tail = red_tail;
+    }
+    return t;
+  }
+};
+
+// Warp-wide: the tile table of all groups. Offsets outside [0, R] are clamped, groups that end before they
+// start are empty, so that no address leaves the tensors whatever the offsets hold.
+template <int KIND>
+__device__ __forceinline__ void gg_build_table(const GroupedArgs& a, int* table, int lane) {
+  int* prefix = table;
+  int* start = table + kGgMaxExperts + 1;
+  int* rows = start + kGgMaxExperts;
+  const int lane_tiles = (a.lanes + kGgTile - 1) / kGgTile;
+  const int dw_tiles = lane_tiles * ((a.cols + kGgTile - 1) / kGgTile);
+  int before = 0;
+  for (int e0 = 0; e0 < a.E; e0 += 32) {
+    const int e = e0 + lane;
+    int n = 0, tiles = 0;
+    if (e < a.E) {
+      int64_t s = 0, t = a.rows;
+      if (a.offsets != nullptr) {
+        s = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[e] : static_cast<const int32_t*>(a.offsets)[e];
+        t = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[e + 1] : static_cast<const int32_t*>(a.offsets)[e + 1];
+      }
+      s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
+      t = t < s ? s : (t > a.rows ? a.rows : t);
+      n = static_cast<int>(t - s);
+      start[e] = static_cast<int>(s);
+      rows[e] = n;
+      if (KIND == kGroupedDw) {
+        tiles = dw_tiles;
+      } else if (n > 0) {
+        const int step = gg_col_step(n);
+        tiles = lane_tiles * ((n + step - 1) / step);
+      }
+    }
+    int incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (e < a.E) prefix[e] = before + incl - tiles;
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) prefix[a.E] = before;
+}
+
+// tmA: the lanes' operand. Y, int8: W as [E][N][K], box 128 bytes x 128 rows. Dx: W, box 64 k x 64 n. Dw: x [R][K],
+// box 64 k x 64 rows. tmB: the columns' operand. Y, Dx, int8: x or dy, box 128 bytes x 128 rows, and the same with 32
+// rows in tmB32. Dw: dy, box 64 n x 64 rows.
+template <int KIND, typename T, typename OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
+    grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                        const __grid_constant__ CUtensorMap tmB32, const GroupedArgs args) {
+  constexpr bool kDw = KIND == kGroupedDw;
+  constexpr bool kInt8 = KIND == kDenseInt8;
+  constexpr bool kMnA = KIND == kGroupedDx || kDw;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kRed = kInt8 ? 128 : 64;   // reduction elements per block
+  constexpr int kMmaRed = kInt8 ? 32 : 16;  // and per MMA
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kGgStages * kGgStageBytes);  // leader's: both CTAs' producers
+  uint64_t* empty = full + kGgStages;
+  uint64_t* landed = empty + kGgStages;  // Dw's tails: this CTA's own copies
+  uint64_t* tfull = landed + kGgStages;
+  uint64_t* tempty = tfull + 2;          // leader's: the epilogue warps of both CTAs
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* table = reinterpret_cast<int*>(smem + kGgStages * kGgStageBytes + 256);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = static_cast<int>(cluster_id_x()), npairs = static_cast<int>(cluster_count_x());
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kGgStages; ++s) {
+      mbar_init(&full[s], 2);
+      mbar_init(&empty[s], 1);
+      mbar_init(&landed[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * kGgEpiWarps);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  if (warp == 2) gg_build_table<KIND>(args, table, lane);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  GroupedSchedule<KIND> sched(args, table);
+  const int tiles = sched.tiles();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      const uint64_t pol = l2_policy_evict_normal();
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += npairs) {
+        const GroupedTile t = sched.get(tile);
+        const int half = (t.ncols + kGgColStep - 1) / kGgColStep * (kGgColStep / 2);  // columns that this CTA brings
+        const int lane0 = t.lane0 + static_cast<int>(rank) * 128;
+        const int boxes = half <= 96 ? (half + 31) / 32 : 0;  // 32-row boxes; 0: one of 128
+        for (int kb = 0; kb < t.kblocks; ++kb) {
+          if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag, args.status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a = smem + st * kGgStageBytes;
+          uint8_t* b = a + kGgOperandBytes;
+          const uint32_t bar = mapa_shared(smem_u32(&full[st]), 0);
+          if constexpr (kDw) {
+            const int row = static_cast<int>(t.row0) + kb * 64;
+            const int col0 = t.col0 + static_cast<int>(rank) * half;
+            if (kb == t.kblocks - 1 && t.tail % 16 != 0) {  // to be cleared behind the end first
+              mbar_arrive_expect_tx(&landed[st], kGgStageBytes);
+              for (int c = 0; c < 2; ++c) {
+                tma_load_2d(a + c * 8192, &tmA, &landed[st], lane0 + c * 64, row, pol);
+                tma_load_2d(b + c * 8192, &tmB, &landed[st], col0 + c * 64, row, pol);
+              }
+            } else {
+              mbar_arrive_expect_tx_cluster(bar, kGgStageBytes);
+              for (int c = 0; c < 2; ++c) {
+                tma_load_2d_pair(a + c * 8192, &tmA, bar, lane0 + c * 64, row, pol);
+                tma_load_2d_pair(b + c * 8192, &tmB, bar, col0 + c * 64, row, pol);
+              }
+            }
+          } else {
+            const int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half;
+            mbar_arrive_expect_tx_cluster(bar, kGgOperandBytes + (boxes ? boxes * 4096 : kGgOperandBytes));
+            if constexpr (kMnA) {
+              for (int c = 0; c < 2; ++c) tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + c * 64, kb * kRed, t.e, pol);
+            } else {
+              tma_load_3d_pair(a, &tmA, bar, kb * kRed, lane0, t.e, pol);
+            }
+            if (boxes == 0) tma_load_2d_pair(b, &tmB, bar, kb * kRed, row, pol);
+            for (int i = 0; i < boxes; ++i) tma_load_2d_pair(b + i * 4096, &tmB32, bar, kb * kRed, row + i * 32, pol);
+          }
+          if (++st == kGgStages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (leader && lane == 0) {
+      int st = 0;
+      uint32_t ph = 0, count = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += npairs) {
+        const GroupedTile t = sched.get(tile);
+        if (t.kblocks == 0) continue;
+        const int slot = count & 1;
+        if (!mbar_wait_cluster(&tempty[slot], ((count >> 1) & 1u) ^ 1u, abort_flag, args.status)) break;
+        ++count;
+        tc_fence_after();
+        const int n = (t.ncols + kGgColStep - 1) / kGgColStep * kGgColStep;
+        uint32_t idesc;
+        if constexpr (kInt8)
+          idesc = idesc_i8(256, n);
+        else
+          idesc = idesc_f16(kBf16, 256, n) | (kMnA ? 1u << 15 : 0u) | (kDw ? 1u << 16 : 0u);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(slot * 256);
+        for (int kb = 0; kb < t.kblocks; ++kb) {
+          const bool cleared = kDw && kb == t.kblocks - 1 && t.tail % 16 != 0;  // with stores of the peer's threads
+          if (!(cleared ? mbar_wait_cluster(&full[st], ph, abort_flag, args.status)
+                        : mbar_wait(&full[st], ph, abort_flag, args.status))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + st * kGgStageBytes), b = a + kGgOperandBytes;
+          const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
+#pragma unroll
+          for (int k = 0; k < kRed / kMmaRed; ++k) {
+            if (k * kMmaRed < left) {
+              const uint64_t ad = kMnA ? smem_desc_sw128_mn(a + k * 2048) : smem_desc_sw128(a + k * 32);
+              const uint64_t bd = kDw ? smem_desc_sw128_mn(b + k * 2048) : smem_desc_sw128(b + k * 32);
+              if constexpr (kInt8)
+                mma_i8_pair(d, ad, bd, idesc, (kb | k) != 0);
+              else
+                mma_f16_pair(d, ad, bd, idesc, (kb | k) != 0);
+            }
+          }
+          tc_commit_pair(&empty[st], 0x3);
+          if (++st == kGgStages) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(&tfull[slot], 0x3);
+      }
+      tc_commit_pair(drain, 0x1);
+      mbar_wait_drain(drain, 0);
+    }
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- Dw: rows behind an expert's end
+    if constexpr (kDw) {
+      uint32_t blocks = 0, phases = 0;  // blocks taken so far; one parity bit per stage
+      for (int tile = pair; tile < tiles; tile += npairs) {
+        const GroupedTile t = sched.get(tile);
+        blocks += static_cast<uint32_t>(t.kblocks);
+        if (t.tail % 16 == 0) continue;
+        const int st = static_cast<int>((blocks - 1) % kGgStages);
+        if (!mbar_wait(&landed[st], (phases >> st) & 1u, abort_flag, args.status)) break;
+        phases ^= 1u << st;
+        const int pieces = (16 - t.tail % 16) * 8;  // 16-byte pieces of the rows to clear, in each of four tiles
+        uint8_t* from = smem + st * kGgStageBytes + t.tail * 128;
+        for (int i = lane; i < pieces * 4; i += 32)
+          *reinterpret_cast<uint4*>(from + i / pieces * 8192 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&full[st]), 0));
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- epilogue
+    const int q = warp & 3;
+    OutT* out = static_cast<OutT*>(args.out);
+    uint32_t count = 0;
+    for (int tile = pair; tile < tiles; tile += npairs) {
+      const GroupedTile t = sched.get(tile);
+      const int f = t.lane0 + static_cast<int>(rank) * 128 + q * 32 + lane;
+      const bool there = f < args.lanes;
+      int64_t at = (t.row0 * args.ld_out);
+      if (kDw) at = (static_cast<int64_t>(t.e) * args.cols + t.col0) * args.ld_out;
+      OutT* p = out + at + f;
+      if (t.kblocks == 0) {  // an expert without rows: dW = 0
+        if (there)
+          for (int c = 0; c < t.ncols; ++c, p += args.ld_out) *p = gg_cast<OutT>(0.0f);
+        continue;
+      }
+      const int slot = count & 1;
+      if (!mbar_wait(&tfull[slot], (count >> 1) & 1u, abort_flag, args.status)) break;
+      ++count;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(slot * 256);
+      float ws = 0.0f, bias = 0.0f;
+      if constexpr (kInt8) {
+        if (there) {
+          ws = args.lane_scale[f];
+          bias = args.bias ? args.bias[f] : 0.0f;
+        }
+      }
+#pragma unroll 1
+      for (int c0 = 0; c0 < t.ncols; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(taddr + c0, r);
+        tmem_ld_wait();
+        if (c0 + 32 >= t.ncols) {  // the last columns: the accumulator is free
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[slot]), 0));
+        }
+        const int left = t.ncols - c0;
+        if (there) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (j < left) {
+              float v;
+              if constexpr (kInt8)
+                v = static_cast<float>(static_cast<int>(r[j])) * args.col_scale[t.row0 + c0 + j] * ws + bias;
+              else
+                v = __uint_as_float(r[j]);
+              *p = gg_cast<OutT>(v);
+            }
+            p += args.ld_out;
+          }
+        }
+        __syncwarp();  // the next read of TMEM is the whole warp's
+      }
+    }
+    if (!kDw && args.zero_rest) {
+      // rows before the first group and behind the last one
+      int64_t s = 0, e = args.rows;
+      if (args.offsets != nullptr) {
+        s = sched.start[0];
+        e = static_cast<int64_t>(sched.start[args.E - 1]) + sched.rows[args.E - 1];
+      }
+      const int64_t n = s + args.rows - e;
+      const int w = (static_cast<int>(blockIdx.x) * kGgEpiWarps) + q;
+      for (int64_t i = w; i < n; i += static_cast<int64_t>(gridDim.x) * kGgEpiWarps) {
+        OutT* p = out + (i < s ? i : e + i - s) * args.ld_out;
+        for (int c = lane; c < args.lanes; c += 32) p[c] = gg_cast<OutT>(0.0f);
+      }
+    }
+  }
+
+  __syncwarp();
+  if (warp == 0 && lane == 0 && *abort_flag) spin_ns(2000000ull);  // copies in flight land before the CTA leaves
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its pair may still touch its shared memory or TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+}  // namespace moe

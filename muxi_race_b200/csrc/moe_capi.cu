@@ -121,8 +121,8 @@ struct TileInfo {
   int kpa = 1;  // k-blocks per A box (one-block units on the TMA A path)
 };
 
-// Tiled map over a tensor of `rank` dimensions (dims[0] innermost, in elements; strides of dims
-// 1..rank-1 in bytes), 128-byte swizzle (matches the kernels' shared-memory descriptors).
+}  // namespace
+
 int encode_map(CUtensorMap* map, const void* base, int elt_bytes, int rank, const cuuint64_t* dims,
                const cuuint64_t* strides, const cuuint32_t* box, const char* what) {
   auto enc = get_encode();
@@ -150,6 +150,8 @@ int encode_map(CUtensorMap* map, const void* base, int elt_bytes, int rank, cons
   if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with %d", what, (int)r);
   return MOE_OK;
 }
+
+namespace {
 
 // Row-major [rows, cols] matrix, box = box_rows x (128 bytes).
 int make_tmap(CUtensorMap* map, const void* base, int elt_bytes, int64_t rows, int64_t cols, int box_rows,
