@@ -104,6 +104,26 @@ __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
+// A whole warp waits for what takes long: one lane polls, with pauses (polling lanes take shared-memory cycles from the
+// MMAs and copies; 128 of them cost a tenth of the rate).
+__device__ __forceinline__ bool gg_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t* status,
+                                             int lane) {
+  int ok = 1;
+  if (lane == 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity)) {
+      __nanosleep(100);
+      if (*abort_flag || globaltimer_ns() - t0 > MOE_WAIT_NS) {
+        if (!*abort_flag && status) atomicOr(status, kStatusWaitTimeout);
+        *abort_flag = 1;
+        ok = 0;
+        break;
+      }
+    }
+  }
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
 // One tile: expert, first lane, first column (a row; Dw: an n), columns, and for Dw the rows it reduces.
 struct GroupedTile {
   int e, lane0, ncols;
@@ -385,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         blocks += static_cast<uint32_t>(t.kblocks);
         if (t.tail % 16 == 0) continue;
         const int st = static_cast<int>((blocks - 1) % kGgStages);
-        if (!mbar_wait(&landed[st], (phases >> st) & 1u, abort_flag, args.status)) break;
+        if (!gg_warp_wait(&landed[st], (phases >> st) & 1u, abort_flag, args.status, lane)) break;
         phases ^= 1u << st;
         const int pieces = (16 - t.tail % 16) * 8;  // 16-byte pieces of the rows to clear, in each of four tiles
         uint8_t* from = smem + st * kGgStageBytes + t.tail * 128;
@@ -414,7 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         continue;
       }
       const int slot = count & 1;
-      if (!mbar_wait(&tfull[slot], (count >> 1) & 1u, abort_flag, args.status)) break;
+      if (!gg_warp_wait(&tfull[slot], (count >> 1) & 1u, abort_flag, args.status, lane)) break;
       ++count;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(slot * 256);

@@ -10,8 +10,12 @@
 //   silu_mul           h = w g s(g) u, s(g) = 1 / (1 + e^-g); gate g and up u are the halves of a row
 //   silu_mul_backward  dg = dh w u s (1 + g (1 - s)), du = dh w g s, dw = sum_j dh g s u, and h again
 //
-// All of it is one pass over the data, bound by HBM. 16 lanes hold a group (8 columns each: one 16-byte
-// access of 16-bit values), so the group's maximum is four shuffles and the copy costs no second read.
+// All of it is one pass over the data, bound by HBM, so instructions per element are kept few. A lane holds
+// 16 columns of a group, 8 in each half of it (an access of 8 lanes covers 128 or 64 bytes without gaps), 8 lanes a
+// group: the group's maximum is taken of the packed 16-bit patterns and three shuffles, and the copy costs no second read. int8 values
+// come out of one multiply-add each: added to 1.5 * 2^23 a number is rounded to a whole one, which stands in
+// the low bits of the result. That rounds halves to even; a factor of 1 + 2^-21 moves them away from zero first
+// (values of 16-bit types are ties, or at least 1.9e-6 of themselves away from one).
 // A row belongs to 1, 2, 4 or 8 warps of a CTA, by its length: short rows do not idle, and dw is a sum
 // within a CTA in a fixed order. Sums and products are fp32; each output is rounded once.
 #pragma once
@@ -24,6 +28,9 @@
 namespace moe {
 
 constexpr int kR8Group = 128;
+constexpr int kR8Lanes = 8;   // of a group, 16 columns each
+constexpr int kR8Cols = 16;
+constexpr int kR8Step = 4;    // groups that a warp takes at a time
 constexpr int kR8Threads = 256;
 constexpr int kR8Warps = kR8Threads / 32;
 
@@ -31,112 +38,216 @@ struct I8 { int8_t v; };
 struct F8 { uint8_t v; };
 struct NoCopy {};
 
-__device__ __forceinline__ float r8_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float r8_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float r8_float(float v) { return v; }
-__device__ __forceinline__ float r8_float(I8 v) { return static_cast<float>(v.v); }
-__device__ __forceinline__ float r8_float(F8 v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v.v, __NV_E4M3)));
-}
-template <typename T> __device__ __forceinline__ T r8_round(float v);
-template <> __device__ __forceinline__ __half r8_round<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 r8_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ float r8_round<float>(float v) { return v; }
-template <> __device__ __forceinline__ I8 r8_round<I8>(float v) {
-  return I8{static_cast<int8_t>(static_cast<int>(v + copysignf(0.5f, v)))};
-}
-template <> __device__ __forceinline__ F8 r8_round<F8>(float v) {
-  return F8{static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3))};
+// How rows are accessed. 8: their starts and lengths are multiples of 8 elements; 1: element by element.
+// The 16 columns of a lane are 8 neighbours in each half of the group, or (1) every 8th of the group.
+template <int VEC> __device__ __forceinline__ int r8_col(int c0, int l8, int i) {
+  return VEC > 1 ? c0 + i / 8 * 64 + l8 * 8 + i % 8 : c0 + l8 + kR8Lanes * i;
 }
 
-template <int N> struct alignas(N) R8Bytes { uint8_t b[N]; };
+// The packed elements of a lane; 0 behind the row's end.
+template <typename S> struct Packed {
+  static constexpr int kWords = kR8Cols * static_cast<int>(sizeof(S)) / 4;
+  uint32_t w[kWords];
+};
 
-// The 8 columns of lane l16 of the group that starts at column c0 of a row of `width`: neighbours where
-// VEC (c0, width and the row's start are multiples of 8 elements), else every 16th.
-template <bool VEC> __device__ __forceinline__ int r8_col(int c0, int l16, int i) {
-  return VEC ? c0 + l16 * 8 + i : c0 + l16 + 16 * i;
-}
-template <bool VEC, typename S>
-__device__ __forceinline__ void r8_load(const S* row, int c0, int l16, int width, float (&v)[8]) {
-  if constexpr (VEC) {
-    alignas(16) S e[8];
-    if (c0 + l16 * 8 < width) {
-      using Piece = typename std::conditional<sizeof(S) == 1, uint2, uint4>::type;
-      *reinterpret_cast<Piece*>(e) = __ldg(reinterpret_cast<const Piece*>(row + c0 + l16 * 8));
+template <int VEC, typename S>
+__device__ __forceinline__ Packed<S> r8_load(const S* row, int c0, int l8, int width) {
+  Packed<S> p;
+  if constexpr (VEC == 1) {
+    using U = typename std::conditional<sizeof(S) == 1, uint8_t, uint16_t>::type;
+    constexpr int kPer = 4 / static_cast<int>(sizeof(S));
+    const U* r = reinterpret_cast<const U*>(row);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = r8_float(e[i]);
-    } else {
+    for (int i = 0; i < Packed<S>::kWords; ++i) {
+      p.w[i] = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      for (int j = 0; j < kPer; ++j) {
+        const int c = r8_col<VEC>(c0, l8, i * kPer + j);
+        if (c < width) p.w[i] |= static_cast<uint32_t>(__ldg(r + c)) << (j * 8 * static_cast<int>(sizeof(S)));
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = r8_col<VEC>(c0, l16, i);
-      v[i] = c < width ? r8_float(row[c]) : 0.0f;
+    for (int i = 0; i < 2; ++i) {
+      const int c = r8_col<VEC>(c0, l8, 8 * i);
+      if constexpr (sizeof(S) == 2) {
+        const uint4 v = c < width ? __ldg(reinterpret_cast<const uint4*>(row + c)) : make_uint4(0, 0, 0, 0);
+        p.w[i * 4] = v.x, p.w[i * 4 + 1] = v.y, p.w[i * 4 + 2] = v.z, p.w[i * 4 + 3] = v.w;
+      } else {
+        const uint2 v = c < width ? __ldg(reinterpret_cast<const uint2*>(row + c)) : make_uint2(0, 0);
+        p.w[i * 2] = v.x, p.w[i * 2 + 1] = v.y;
+      }
     }
   }
+  return p;
 }
-template <bool VEC, typename S>
-__device__ __forceinline__ void r8_store(S* row, int c0, int l16, int width, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c0 + l16 * 8 < width) {
-      using Piece = typename std::conditional<sizeof(S) == 1, uint2, uint4>::type;
-      alignas(16) S e[8];
+
+template <int VEC, typename S>
+__device__ __forceinline__ void r8_store(S* row, int c0, int l8, int width, const Packed<S>& p) {
+  if constexpr (VEC == 1) {
+    using U = typename std::conditional<sizeof(S) == 1, uint8_t, uint16_t>::type;
+    constexpr int kPer = 4 / static_cast<int>(sizeof(S));
+    U* r = reinterpret_cast<U*>(row);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = r8_round<S>(v[i]);
-      *reinterpret_cast<Piece*>(row + c0 + l16 * 8) = *reinterpret_cast<const Piece*>(e);
+    for (int i = 0; i < kR8Cols; ++i) {
+      const int c = r8_col<VEC>(c0, l8, i);
+      if (c < width) r[c] = static_cast<U>(p.w[i / kPer] >> (i % kPer * 8 * static_cast<int>(sizeof(S))));
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = r8_col<VEC>(c0, l16, i);
-      if (c < width) row[c] = r8_round<S>(v[i]);
+    for (int i = 0; i < 2; ++i) {
+      const int c = r8_col<VEC>(c0, l8, 8 * i);
+      if (c < width) {
+        if constexpr (sizeof(S) == 2)
+          *reinterpret_cast<uint4*>(row + c) = make_uint4(p.w[i * 4], p.w[i * 4 + 1], p.w[i * 4 + 2], p.w[i * 4 + 3]);
+        else
+          *reinterpret_cast<uint2*>(row + c) = make_uint2(p.w[i * 2], p.w[i * 2 + 1]);
+      }
     }
   }
 }
 
-// The 8-bit copy of a group: 16 lanes, 8 columns each (those behind the row's end are 0).
-template <bool VEC, typename Q>
-__device__ __forceinline__ void r8_encode(const float (&x)[8], Q* row, float* scale, int c0, int l16, int width) {
-  uint32_t top = 0;  // as bits, so that infinities and NaN stay on top
+// Elements [4 i, 4 i + 4) as fp32.
+__device__ __forceinline__ void r8_unpack4(const Packed<__nv_bfloat16>& p, int i, float (&v)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int j = 0; j < 2; ++j) {
+    v[2 * j] = __uint_as_float(p.w[2 * i + j] << 16);
+    v[2 * j + 1] = __uint_as_float(p.w[2 * i + j] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void r8_unpack4(const Packed<__half>& p, int i, float (&v)[4]) {
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float amax = __uint_as_float(top);
+  for (int j = 0; j < 2; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p.w[2 * i + j]));
+    v[2 * j] = f.x, v[2 * j + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void r8_unpack4(const Packed<I8>& p, int i, float (&v)[4]) {
+  const uint32_t w = p.w[i] ^ 0x80808080u;  // bytes 128 higher, each as the low mantissa of 2^23
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j)) - 8388736.0f;
+}
+__device__ __forceinline__ void r8_unpack4(const Packed<F8>& p, int i, float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(p.w[i] >> (16 * j)), __NV_E4M3);
+    const float2 f = __half22float2(__half2(h));
+    v[2 * j] = f.x, v[2 * j + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void r8_pack4(Packed<__nv_bfloat16>& p, int i, const float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    p.w[2 * i + j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ void r8_pack4(Packed<__half>& p, int i, const float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+    p.w[2 * i + j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Scaled values: to the nearest whole number (halves were moved away from zero), to e4m3.
+__device__ __forceinline__ void r8_code4(Packed<I8>& p, int i, const float (&x)[4], float inv) {
+  uint32_t t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = __float_as_uint(fmaf(x[j], inv, 12582912.0f));
+  p.w[i] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ void r8_code4(Packed<F8>& p, int i, const float (&x)[4], float inv) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);
+  p.w[i] = lo | hi << 16;
+}
+// e4m3 would round what is above 248/256 of the type's last power of two up and out of its range: such values
+// stay at 240/256 of it.
+__device__ __forceinline__ uint32_t r8_near_end(__nv_bfloat16) { return 0x7f78u; }
+__device__ __forceinline__ uint32_t r8_near_end(__half) { return 0x7bc0u; }
+__device__ __forceinline__ float r8_magnitude(uint32_t bits, __nv_bfloat16) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ float r8_magnitude(uint32_t bits, __half) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
+__device__ __forceinline__ float r8_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The 8-bit copy of a group; all lanes of the warp take part.
+template <int VEC, typename Q, typename T>
+__device__ __forceinline__ void r8_encode(const Packed<T>& x, Q* row, float* scale, int c0, int l8, int width) {
+  uint32_t top = 0;  // of the bit patterns without their signs, so that infinities and NaN stay on top
+#pragma unroll
+  for (int i = 0; i < Packed<T>::kWords; ++i) top = __vmaxu2(top, x.w[i] & 0x7fff7fffu);
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int o = kR8Lanes / 2; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float amax = r8_magnitude(top, T());
+  const bool bad = !(amax < INFINITY);  // its codes do not matter
   // groups below 2^-100 are scaled up first, where the reciprocal of their scale would overflow
-  const float up = amax < 0x1p-100f ? 0x1p100f : 1.0f;
-  const float down = amax < 0x1p-100f ? 0x1p-100f : 1.0f;
-  const float a = amax * up;
+  const bool tiny = amax < 0x1p-100f;
+  const float a = tiny ? amax * 0x1p100f : amax;
   float inv, s;
   if constexpr (std::is_same<Q, I8>::value) {
-    inv = __fdiv_rn(127.0f, a);
-    s = __fdiv_rn(amax, 127.0f);
+    // 127 / a by way of a / 16, whose reciprocal is a normal number: 1 unit off, and half a unit for the product and the
+    // factor each, 2.4e-7 in all, against the 4.8e-7 of the factor and 1.9e-6 to the next value that is no tie
+    inv = 7.9375f * r8_reciprocal(a * 0.0625f);
+    inv = fmaf(inv, 0x1p-21f, inv);
+    s = a * (1.0f / 127.0f);  // a / 127: a rounded quotient, and what is left of it
+    s = fmaf(fmaf(-127.0f, s, a), 1.0f / 127.0f, s);
   } else {
     // amax = 1.f * 2^E: 2^(E - 8) holds f up to 1.75, 2^(E - 7) the rest
     const uint32_t bits = __float_as_uint(a);
     const int e = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
     inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    s = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * down;
+    s = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
   }
+  if (tiny) s *= 0x1p-100f;
   if (top == 0) inv = s = 0.0f;
-  const bool bad = top >= 0x7f800000u;
-  if (bad) s = __uint_as_float(0x7fc00000u);
-  float v[8];
+  Packed<Q> q;
+  const bool near_end = std::is_same<Q, F8>::value && top >= r8_near_end(T());
+  if (__any_sync(0xffffffffu, tiny || near_end)) {
+    const float up = tiny ? 0x1p100f : 1.0f;
+    const float most = near_end ? 240.0f * r8_reciprocal(inv) : INFINITY;  // inv is a power of two
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = bad ? 0.0f : x[i] * up * inv;
-  r8_store<VEC>(row, c0, l16, width, v);
-  if (l16 == 0) *scale = s;
+    for (int i = 0; i < kR8Cols / 4; ++i) {
+      float v[4];
+      r8_unpack4(x, i, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fminf(fmaxf(v[j] * up, -most), most);
+      r8_code4(q, i, v, inv);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kR8Cols / 4; ++i) {
+      float v[4];
+      r8_unpack4(x, i, v);
+      r8_code4(q, i, v, inv);
+    }
+  }
+  r8_store<VEC>(row, c0, l8, width, q);
+  if (l8 == 0 && c0 < width) *scale = bad ? __uint_as_float(0x7fc00000u) : s;
 }
 
-// Warps of a row of `groups` groups (two groups a warp at a time), and the rows of a CTA.
-__host__ __device__ inline int r8_row_warps(int groups) { return groups <= 2 ? 1 : groups <= 4 ? 2 : groups <= 8 ? 4 : 8; }
+// Warps of a row of `groups` groups, and so the rows of a CTA.
+__host__ __device__ inline int r8_row_warps(int groups) {
+  return groups <= kR8Step ? 1 : groups <= 2 * kR8Step ? 2 : groups <= 4 * kR8Step ? 4 : 8;
+}
 
 __device__ __forceinline__ float r8_weight(const void* w, int dtype, int64_t i) {  // dtype: MOE_F16 0, MOE_BF16 1, MOE_F32 2
   if (dtype == 2) return static_cast<const float*>(w)[i];
   if (dtype == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
   return __half2float(static_cast<const __half*>(w)[i]);
+}
+
+// s(x) = 1 / (1 + e^-x)
+__device__ __forceinline__ float r8_sigmoid(float x) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  return r8_reciprocal(1.0f + e);
 }
 
 struct SiluArgs {
@@ -166,43 +277,48 @@ __device__ __forceinline__ int64_t r8_weight_at(const SiluArgs& a, int64_t r) {
   return i >= 0 && i < a.num_weights ? i : -1;
 }
 
-template <typename T, typename Q, bool VEC>
+template <typename T, typename Q, int VEC>
 __global__ void __launch_bounds__(kR8Threads) silu_mul_kernel(const SiluArgs a) {
-  const int warp = threadIdx.x >> 5, l16 = threadIdx.x & 15, half = threadIdx.x >> 4 & 1;
+  const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (a.width + kR8Group - 1) / kR8Group;
-  const int row_warps = r8_row_warps(groups), in_row = warp % row_warps;
+  const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
   const int64_t rows = a.valid ? min(a.rows, static_cast<int64_t>(*a.valid)) : a.rows;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kR8Warps / row_warps);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kR8Warps / row_warps) + warp / row_warps; r < rows; r += step) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r < rows; r += step) {
     const T* gate = static_cast<const T*>(a.gate_up) + r * a.ld;
     const int64_t at = r8_weight_at(a, r);
     const float w = at >= 0 ? r8_weight(a.weights, a.weights_dtype, at) : (a.weights ? 0.0f : 1.0f);
-    for (int g0 = in_row * 2; g0 < groups; g0 += row_warps * 2) {
-      const int grp = g0 + half, c0 = grp * kR8Group;  // the second half may be behind the row: it loads zeros
-      float g[8], u[8], h[8];
-      r8_load<VEC>(gate, c0, l16, a.width, g);
-      r8_load<VEC>(gate + a.width, c0, l16, a.width, u);
+    for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
+      const int c0 = (g0 + sub) * kR8Group;  // behind the row's end the lanes hold zeros and store nothing
+      const Packed<T> g = r8_load<VEC>(gate, c0, l8, a.width), u = r8_load<VEC>(gate + a.width, c0, l8, a.width);
+      Packed<T> h;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = w * (__fdividef(g[i], 1.0f + __expf(-g[i])) * u[i]);
-      r8_store<VEC>(static_cast<T*>(a.h) + r * a.width, c0, l16, a.width, h);
+      for (int i = 0; i < kR8Cols / 4; ++i) {
+        float gv[4], uv[4];
+        r8_unpack4(g, i, gv);
+        r8_unpack4(u, i, uv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) gv[j] = w * (gv[j] * r8_sigmoid(gv[j]) * uv[j]);
+        r8_pack4(h, i, gv);
+      }
+      r8_store<VEC>(static_cast<T*>(a.h) + r * a.width, c0, l8, a.width, h);
       if constexpr (!std::is_same<Q, NoCopy>::value) {
         Q* q = static_cast<Q*>(a.q) + r * 2 * a.width;
-        float* s = a.scale + r * 2 * groups + grp;
-        float none;  // a group behind the row has no scale
-        r8_encode<VEC>(g, q, grp < groups ? s : &none, c0, l16, a.width);
-        r8_encode<VEC>(u, q + a.width, grp < groups ? s + groups : &none, c0, l16, a.width);
+        float* s = a.scale + r * 2 * groups + g0 + sub;
+        r8_encode<VEC>(g, q, s, c0, l8, a.width);
+        r8_encode<VEC>(u, q + a.width, s + groups, c0, l8, a.width);
       }
     }
   }
 }
 
 // S: T (gate_up as it was), I8 or F8.
-template <typename T, typename S, bool VEC>
+template <typename T, typename S, int VEC>
 __global__ void __launch_bounds__(kR8Threads) silu_mul_backward_kernel(const SiluArgs a) {
   __shared__ float sums[kR8Warps];
-  const int warp = threadIdx.x >> 5, l16 = threadIdx.x & 15, half = threadIdx.x >> 4 & 1;
+  const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (a.width + kR8Group - 1) / kR8Group;
-  const int row_warps = r8_row_warps(groups), in_row = warp % row_warps, cta_rows = kR8Warps / row_warps;
+  const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
   const int64_t rows = a.valid ? min(a.rows, static_cast<int64_t>(*a.valid)) : a.rows;
   const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * cta_rows; r0 < rows; r0 += step) {
@@ -215,35 +331,41 @@ __global__ void __launch_bounds__(kR8Threads) silu_mul_backward_kernel(const Sil
       const S* gate = static_cast<const S*>(a.gate_up) + r * a.ld;
       const T* dh_row = static_cast<const T*>(a.dh) + r * a.ld_dh;
       T* d = static_cast<T*>(a.q) + r * 2 * a.width;
-      for (int g0 = in_row * 2; g0 < groups; g0 += row_warps * 2) {
-        const int grp = g0 + half, c0 = grp * kR8Group;
-        float g[8], u[8], dh[8], dg[8], du[8], h[8];
-        r8_load<VEC>(gate, c0, l16, a.width, g);
-        r8_load<VEC>(gate + a.width, c0, l16, a.width, u);
-        r8_load<VEC>(dh_row, c0, l16, a.width, dh);
+      for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
+        const int c0 = (g0 + sub) * kR8Group;
+        const Packed<T> dh = r8_load<VEC>(dh_row, c0, l8, a.width);
+        const Packed<S> g = r8_load<VEC>(gate, c0, l8, a.width), u = r8_load<VEC>(gate + a.width, c0, l8, a.width);
+        float sg = 0.0f, su = 0.0f;
         if constexpr (!std::is_same<S, T>::value) {
-          if (grp < groups) {
-            const float* s = a.src_scale + r * 2 * groups + grp;
-            const float sg = s[0], su = s[groups];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              g[i] *= sg;
-              u[i] *= su;
-            }
+          if (c0 < a.width) {
+            const float* s = a.src_scale + r * 2 * groups + g0 + sub;
+            sg = __ldg(s), su = __ldg(s + groups);
           }
         }
+        Packed<T> dg, du, h;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float sig = __fdividef(1.0f, 1.0f + __expf(-g[i]));
-          const float act = g[i] * sig, t = dh[i] * w;
-          du[i] = t * act;
-          dg[i] = t * u[i] * (sig * (1.0f + g[i] * (1.0f - sig)));
-          h[i] = w * act * u[i];
-          if (VEC ? c0 + l16 * 8 < a.width : r8_col<VEC>(c0, l16, i) < a.width) sum += dh[i] * act * u[i];
+        for (int i = 0; i < kR8Cols / 4; ++i) {
+          float dhv[4], gv[4], uv[4], dgv[4], duv[4], hv[4];
+          r8_unpack4(dh, i, dhv);
+          r8_unpack4(g, i, gv);
+          r8_unpack4(u, i, uv);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float gj = std::is_same<S, T>::value ? gv[j] : gv[j] * sg;
+            const float uj = std::is_same<S, T>::value ? uv[j] : uv[j] * su;
+            const float sig = r8_sigmoid(gj), act = gj * sig, t = dhv[j] * w, au = act * uj;
+            duv[j] = t * act;
+            dgv[j] = t * uj * fmaf(act, 1.0f - sig, sig);
+            hv[j] = w * au;
+            if (r8_col<VEC>(c0, l8, 4 * i + j) < a.width) sum = fmaf(dhv[j], au, sum);
+          }
+          r8_pack4(dg, i, dgv);
+          r8_pack4(du, i, duv);
+          r8_pack4(h, i, hv);
         }
-        r8_store<VEC>(d, c0, l16, a.width, dg);
-        r8_store<VEC>(d + a.width, c0, l16, a.width, du);
-        r8_store<VEC>(static_cast<T*>(a.h) + r * a.width, c0, l16, a.width, h);
+        r8_store<VEC>(d, c0, l8, a.width, dg);
+        r8_store<VEC>(d + a.width, c0, l8, a.width, du);
+        r8_store<VEC>(static_cast<T*>(a.h) + r * a.width, c0, l8, a.width, h);
       }
     }
     if (a.dweights != nullptr) {
@@ -280,84 +402,128 @@ struct Rows8Args {
   int width, parts;
 };
 
-// 16-bit rows to 8 bits.
-template <typename T, typename Q, bool VEC>
+// 16-bit rows to 8 bits. A warp takes its part of two rows at a time, so that enough loads are in flight.
+template <typename T, typename Q, int VEC>
 __global__ void __launch_bounds__(kR8Threads) save_rows8_kernel(const Rows8Args a) {
-  const int warp = threadIdx.x >> 5, l16 = threadIdx.x & 15, half = threadIdx.x >> 4 & 1;
+  const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (a.width + kR8Group - 1) / kR8Group;
-  const int row_warps = r8_row_warps(groups), in_row = warp % row_warps;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kR8Warps / row_warps);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kR8Warps / row_warps) + warp / row_warps; r < a.rows; r += step) {
+  const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r < a.rows; r += 2 * step) {
+    const int64_t r2 = r + step;
+    const int width2 = r2 < a.rows ? a.width : 0;
     for (int p = 0; p < a.parts; ++p) {
       const T* x = static_cast<const T*>(a.x) + r * a.ld + static_cast<int64_t>(p) * a.width;
-      Q* q = static_cast<Q*>(a.out) + (r * a.parts + p) * a.width;
-      for (int g0 = in_row * 2; g0 < groups; g0 += row_warps * 2) {
-        const int grp = g0 + half;
-        float v[8], none;
-        r8_load<VEC>(x, grp * kR8Group, l16, a.width, v);
-        r8_encode<VEC>(v, q, grp < groups ? a.scale + (r * a.parts + p) * groups + grp : &none, grp * kR8Group, l16, a.width);
+      const T* x2 = x + (width2 ? step * a.ld : 0);
+      const int64_t at = r * a.parts + p, at2 = r2 * a.parts + p;
+      for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
+        const int grp = g0 + sub, c0 = grp * kR8Group;
+        const Packed<T> v = r8_load<VEC>(x, c0, l8, a.width), v2 = r8_load<VEC>(x2, c0, l8, width2);
+        r8_encode<VEC>(v, static_cast<Q*>(a.out) + at * a.width, a.scale + at * groups + grp, c0, l8, a.width);
+        r8_encode<VEC>(v2, static_cast<Q*>(a.out) + at2 * a.width, a.scale + at2 * groups + grp, c0, l8, width2);
       }
     }
   }
 }
 
+// Where row r comes from; -1: from nowhere.
+__device__ __forceinline__ int64_t r8_from(const Rows8Args& a, int64_t r) {
+  int64_t from = r;
+  if (a.index != nullptr)
+    from = a.index64 ? static_cast<const int64_t*>(a.index)[r] : static_cast<const int32_t*>(a.index)[r];
+  if (a.index_div > 1 && from >= 0)
+    from = from < (int64_t(1) << 31) ? static_cast<uint32_t>(from) / static_cast<uint32_t>(a.index_div) : a.src_rows;
+  return from >= 0 && from < a.src_rows ? from : -1;
+}
+
 // Rows of type S (T itself, I8 or F8) back to T, in the order of an index; a source row that is not there: zeros.
-template <typename T, typename S, bool VEC>
+// Several rows at a time, as in save_rows8_kernel.
+template <typename T, typename S, int VEC>
 __global__ void __launch_bounds__(kR8Threads) restore_rows_kernel(const Rows8Args a) {
-  const int warp = threadIdx.x >> 5, l16 = threadIdx.x & 15, half = threadIdx.x >> 4 & 1;
+  constexpr int kRows = sizeof(S) == 1 ? 4 : 2;
+  const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (a.width + kR8Group - 1) / kR8Group;
-  const int row_warps = r8_row_warps(groups), in_row = warp % row_warps;
+  const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
   const int64_t rows = a.valid ? min(a.rows, static_cast<int64_t>(*a.valid)) : a.rows;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kR8Warps / row_warps);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kR8Warps / row_warps) + warp / row_warps; r < rows; r += step) {
-    int64_t from = r;
-    if (a.index != nullptr)
-      from = a.index64 ? static_cast<const int64_t*>(a.index)[r] : static_cast<const int32_t*>(a.index)[r];
-    const bool there = from >= 0 && (from /= a.index_div) < a.src_rows;
-    for (int p = 0; p < a.parts; ++p) {
-      const S* x = static_cast<const S*>(a.x) + from * a.ld + static_cast<int64_t>(p) * a.width;
-      T* out = static_cast<T*>(a.out) + (r * a.parts + p) * a.width;
-      for (int g0 = in_row * 2; g0 < groups; g0 += row_warps * 2) {
-        const int grp = g0 + half;
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (there) {
-          r8_load<VEC>(x, grp * kR8Group, l16, a.width, v);
-          if constexpr (!std::is_same<S, T>::value) {
-            if (grp < groups) {
-              const float s = a.scale[(from * a.parts + p) * groups + grp];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r0 < rows; r0 += kRows * step) {
+    const S* src[kRows];
+    const float* src_scale[kRows];
+    int width[kRows];  // to be read: 0 where a row comes from nowhere
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] *= s;
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t f = r0 + i * step < rows ? r8_from(a, r0 + i * step) : -1;
+      width[i] = f < 0 ? 0 : a.width;
+      src[i] = static_cast<const S*>(a.x) + (f < 0 ? 0 : f) * a.ld;
+      src_scale[i] = a.scale + (f < 0 ? 0 : f) * a.parts * groups;
+    }
+    for (int p = 0; p < a.parts; ++p) {
+      for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
+        const int grp = g0 + sub, c0 = grp * kR8Group;
+        Packed<S> q[kRows];
+        float s[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          q[i] = r8_load<VEC>(src[i] + static_cast<int64_t>(p) * a.width, c0, l8, width[i]);
+          s[i] = !std::is_same<S, T>::value && c0 < width[i] ? __ldg(src_scale[i] + p * groups + grp) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          if (r0 + i * step >= rows) break;
+          T* out = static_cast<T*>(a.out) + ((r0 + i * step) * a.parts + p) * a.width;
+          if constexpr (std::is_same<S, T>::value) {
+            r8_store<VEC>(out, c0, l8, a.width, q[i]);
+          } else {
+            Packed<T> y;
+#pragma unroll
+            for (int k = 0; k < kR8Cols / 4; ++k) {
+              float v[4];
+              r8_unpack4(q[i], k, v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] *= s[i];
+              r8_pack4(y, k, v);
             }
+            r8_store<VEC>(out, c0, l8, a.width, y);
           }
         }
-        r8_store<VEC>(out, grp * kR8Group, l16, a.width, v);
       }
     }
   }
 }
 
 // out[t] = sum over j of y[slot[t * k + j]] in fp32, in that order; slots outside [0, rows) are skipped.
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kR8Threads)
     combine_rows_kernel(const T* __restrict__ y, const int32_t* __restrict__ slot, int64_t tokens, int k, int64_t rows, int width,
                         T* __restrict__ out) {
-  const int warp = threadIdx.x >> 5, l16 = threadIdx.x & 15, half = threadIdx.x >> 4 & 1;
+  const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (width + kR8Group - 1) / kR8Group;
-  const int row_warps = r8_row_warps(groups), in_row = warp % row_warps;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kR8Warps / row_warps);
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kR8Warps / row_warps) + warp / row_warps; t < tokens; t += step) {
-    for (int g0 = in_row * 2; g0 < groups; g0 += row_warps * 2) {
-      const int c0 = (g0 + half) * kR8Group;
-      float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; t < tokens; t += step) {
+    for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
+      const int c0 = (g0 + sub) * kR8Group;
+      float sum[kR8Cols] = {};
+#pragma unroll 4
       for (int j = 0; j < k; ++j) {
         const int s = slot[t * k + j];
-        if (s < 0 || s >= rows) continue;
-        float v[8];
-        r8_load<VEC>(y + static_cast<int64_t>(s) * width, c0, l16, width, v);
+        const bool there = s >= 0 && s < rows;
+        const Packed<T> p = r8_load<VEC>(y + static_cast<int64_t>(there ? s : 0) * width, c0, l8, there ? width : 0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] += v[i];
+        for (int i = 0; i < kR8Cols / 4; ++i) {
+          float v[4];
+          r8_unpack4(p, i, v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[4 * i + c] += v[c];
+        }
       }
-      r8_store<VEC>(out + t * width, c0, l16, width, sum);
+      Packed<T> o;
+#pragma unroll
+      for (int i = 0; i < kR8Cols / 4; ++i) {
+        const float v[4] = {sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]};
+        r8_pack4(o, i, v);
+      }
+      r8_store<VEC>(out + t * width, c0, l8, width, o);
     }
   }
 }

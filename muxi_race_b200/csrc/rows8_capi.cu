@@ -8,10 +8,11 @@ namespace {
 
 constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 1;
 
-// Whether rows of `width` elements from p on, ld apart, can be taken 8 elements at a time.
-bool by_8(const void* p, int64_t ld, int64_t width, int elt) {
-  return reinterpret_cast<uintptr_t>(p) % (8 * elt) == 0 && ld % 8 == 0 && width % 8 == 0;
+// How many elements rows of `width` elements from p on, ld apart, can be taken at a time: 8 or 1.
+int at_a_time(const void* p, int64_t ld, int64_t width, int elt) {
+  return reinterpret_cast<uintptr_t>(p) % (8 * elt) == 0 && ld % 8 == 0 && width % 8 == 0 ? 8 : 1;
 }
+int least(int a, int b) { return a < b ? a : b; }
 
 int check_rows(int64_t R, int64_t W, int dtype) {
   if (dtype != MOE_F16 && dtype != MOE_BF16) return fail(MOE_ERR_INVALID_ARG, "dtype must be MOE_F16 or MOE_BF16");
@@ -38,49 +39,49 @@ int row_grid(int64_t rows, int64_t width, unsigned* grid) {
 }
 
 template <typename T, typename Q>
-int launch_silu(const SiluArgs& a, bool vec, cudaStream_t s) {
+int launch_silu(const SiluArgs& a, int vec, cudaStream_t s) {
   unsigned grid;
   MOE_TRY(row_grid(a.rows, a.width, &grid));
-  if (vec)
-    silu_mul_kernel<T, Q, true><<<grid, kR8Threads, 0, s>>>(a);
+  if (vec == 8)
+    silu_mul_kernel<T, Q, 8><<<grid, kR8Threads, 0, s>>>(a);
   else
-    silu_mul_kernel<T, Q, false><<<grid, kR8Threads, 0, s>>>(a);
+    silu_mul_kernel<T, Q, 1><<<grid, kR8Threads, 0, s>>>(a);
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
 
 template <typename T, typename S>
-int launch_silu_backward(const SiluArgs& a, bool vec, cudaStream_t s) {
+int launch_silu_backward(const SiluArgs& a, int vec, cudaStream_t s) {
   unsigned grid;
   MOE_TRY(row_grid(a.rows, a.width, &grid));
-  if (vec)
-    silu_mul_backward_kernel<T, S, true><<<grid, kR8Threads, 0, s>>>(a);
+  if (vec == 8)
+    silu_mul_backward_kernel<T, S, 8><<<grid, kR8Threads, 0, s>>>(a);
   else
-    silu_mul_backward_kernel<T, S, false><<<grid, kR8Threads, 0, s>>>(a);
+    silu_mul_backward_kernel<T, S, 1><<<grid, kR8Threads, 0, s>>>(a);
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
 
 template <typename T, typename Q>
-int launch_save(const Rows8Args& a, bool vec, cudaStream_t s) {
+int launch_save(const Rows8Args& a, int vec, cudaStream_t s) {
   unsigned grid;
   MOE_TRY(row_grid(a.rows, a.width, &grid));
-  if (vec)
-    save_rows8_kernel<T, Q, true><<<grid, kR8Threads, 0, s>>>(a);
+  if (vec == 8)
+    save_rows8_kernel<T, Q, 8><<<grid, kR8Threads, 0, s>>>(a);
   else
-    save_rows8_kernel<T, Q, false><<<grid, kR8Threads, 0, s>>>(a);
+    save_rows8_kernel<T, Q, 1><<<grid, kR8Threads, 0, s>>>(a);
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
 
 template <typename T, typename S>
-int launch_restore(const Rows8Args& a, bool vec, cudaStream_t s) {
+int launch_restore(const Rows8Args& a, int vec, cudaStream_t s) {
   unsigned grid;
   MOE_TRY(row_grid(a.rows, a.width, &grid));
-  if (vec)
-    restore_rows_kernel<T, S, true><<<grid, kR8Threads, 0, s>>>(a);
+  if (vec == 8)
+    restore_rows_kernel<T, S, 8><<<grid, kR8Threads, 0, s>>>(a);
   else
-    restore_rows_kernel<T, S, false><<<grid, kR8Threads, 0, s>>>(a);
+    restore_rows_kernel<T, S, 1><<<grid, kR8Threads, 0, s>>>(a);
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
@@ -91,10 +92,10 @@ int launch_combine(const void* y, const int32_t* slot, int64_t T_, int64_t k, in
   MOE_TRY(row_grid(T_, H, &grid));
   const T* src = static_cast<const T*>(y);
   T* dst = static_cast<T*>(out);
-  if (by_8(y, H, H, 2) && by_8(out, H, H, 2))
-    combine_rows_kernel<T, true><<<grid, kR8Threads, 0, s>>>(src, slot, T_, (int)k, R, (int)H, dst);
+  if (least(at_a_time(y, H, H, 2), at_a_time(out, H, H, 2)) >= 8)
+    combine_rows_kernel<T, 8><<<grid, kR8Threads, 0, s>>>(src, slot, T_, (int)k, R, (int)H, dst);
   else
-    combine_rows_kernel<T, false><<<grid, kR8Threads, 0, s>>>(src, slot, T_, (int)k, R, (int)H, dst);
+    combine_rows_kernel<T, 1><<<grid, kR8Threads, 0, s>>>(src, slot, T_, (int)k, R, (int)H, dst);
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
@@ -129,7 +130,7 @@ int moe_silu_mul(const void* gate_up, int64_t ld, const void* weights, int weigh
   a.scale = scale;
   a.rows = R;
   a.width = static_cast<int>(I);
-  const bool vec = by_8(gate_up, ld, I, 2) && by_8(h, I, I, 2) && by_8(q, I, I, 1);
+  const int vec = least(least(at_a_time(gate_up, ld, I, 2), at_a_time(h, I, I, 2)), at_a_time(q, I, I, 1));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MOE_F16)
     return !q ? launch_silu<__half, NoCopy>(a, vec, s)
@@ -167,7 +168,8 @@ int moe_silu_mul_backward(const void* dh, int64_t ld_dh, const void* gate_up, in
   a.dweights = dweights;
   a.rows = R;
   a.width = static_cast<int>(I);
-  const bool vec = by_8(gate_up, ld, I, q8 ? 1 : 2) && by_8(dh, ld_dh, I, 2) && by_8(h, I, I, 2) && by_8(dgate_up, I, I, 2);
+  const int vec = least(least(at_a_time(gate_up, ld, I, q8 ? 1 : 2), at_a_time(dh, ld_dh, I, 2)),
+                        least(at_a_time(h, I, I, 2), at_a_time(dgate_up, I, I, 2)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MOE_F16)
     return !q8 ? launch_silu_backward<__half, __half>(a, vec, s)
@@ -194,7 +196,7 @@ int moe_save_rows8(const void* x, int64_t ld, void* q, int q_dtype, float* scale
   a.rows = a.src_rows = R;
   a.width = static_cast<int>(W / parts);
   a.parts = static_cast<int>(parts);
-  const bool vec = by_8(x, ld, a.width, 2) && by_8(q, a.width, a.width, 1);
+  const int vec = least(at_a_time(x, ld, a.width, 2), at_a_time(q, a.width, a.width, 1));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MOE_F16) return q_dtype == MOE_I8 ? launch_save<__half, I8>(a, vec, s) : launch_save<__half, F8>(a, vec, s);
   return q_dtype == MOE_I8 ? launch_save<__nv_bfloat16, I8>(a, vec, s) : launch_save<__nv_bfloat16, F8>(a, vec, s);
@@ -227,7 +229,7 @@ int moe_restore_rows(const void* x, int64_t ld, int src_dtype, const float* scal
   a.src_rows = src_rows;
   a.width = static_cast<int>(W / parts);
   a.parts = static_cast<int>(parts);
-  const bool vec = by_8(x, ld, a.width, q8 ? 1 : 2) && by_8(out, a.width, a.width, 2);
+  const int vec = least(at_a_time(x, ld, a.width, q8 ? 1 : 2), at_a_time(out, a.width, a.width, 2));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MOE_F16)
     return !q8 ? launch_restore<__half, __half>(a, vec, s)
