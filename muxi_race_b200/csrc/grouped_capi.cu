@@ -42,6 +42,8 @@ int map_weights(CUtensorMap* m, const void* p, int elt, int64_t E, int64_t N, in
 template <int KIND, typename T, typename OutT>
 int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b32, GroupedArgs args, cudaStream_t s) {
   int dev, sms;
+  constexpr int elt = static_cast<int>(sizeof(OutT));
+  args.out16 = reinterpret_cast<uintptr_t>(args.out) % 16 == 0 && args.ld_out * elt % 16 == 0 && args.lanes * elt % 16 == 0;
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &args.status));

@@ -26,9 +26,13 @@
 // the rows behind the end in both operands (at most 15, up to a multiple of the MMA's 16) after the
 // copy has landed, and only then tells the MMA warp.
 //
-// Roles per CTA (256 threads): warp 0 TMA producer, warp 1 MMA issuer (the pair's leader), warp 2 TMEM
-// and the tile table, warp 3 the clearing of Dw's tails, warps 4-7 epilogue (one TMEM lane quadrant
-// each). Every wait is bounded; the final cluster barrier is reached on every path.
+// Epilogue: a warp alone on its scheduler issues an instruction every four to five cycles, so what counts is how few there
+// are. 16-bit results are read from TMEM as 8 x 8 fragments, packed in pairs of columns, stored transposed to shared
+// memory by stmatrix (4 packs and one store for 256 elements) and copied from there 16 bytes at a time.
+//
+// Roles per CTA (384 threads): warp 0 TMA producer, warp 1 MMA issuer (the pair's leader), warp 2 the tile table,
+// warp 3 the clearing of Dw's tails, warps 4-11 epilogue. Every wait is bounded; the final cluster barrier is
+// reached on every path.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,12 +50,14 @@ constexpr int kGgOperandBytes = 128 * 128;  // of one operand, per CTA and stage
 constexpr int kGgStageBytes = 2 * kGgOperandBytes;
 constexpr int kGgTile = 256;                // lanes per pair, columns at most
 constexpr int kGgMaxExperts = 1024;
-constexpr int kGgThreads = 256;
-constexpr int kGgEpiWarps = 4;
+constexpr int kGgEpiWarps = 8;              // two per TMEM lane quadrant, each with half of the columns
+constexpr int kGgThreads = 128 + 32 * kGgEpiWarps;
 constexpr int kGgBand = 8;  // column tiles that take turns on a weight tile
 constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiples of 32
 constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
-constexpr int kGgSmemBytes = 1024 + kGgStages * kGgStageBytes + 256 + kGgTableInts * 4;
+constexpr int kGgPiece = 2048;  // an epilogue warp's staging: 32 lanes of 32 columns (16 bits) or of 16 (32 bits)
+constexpr int kGgOutBytes = kGgEpiWarps * kGgPiece;
+constexpr int kGgSmemBytes = 1024 + kGgStages * kGgStageBytes + kGgOutBytes + 256 + kGgTableInts * 4;
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
 struct GroupedArgs {
@@ -65,6 +71,7 @@ struct GroupedArgs {
   void* out;
   int64_t ld_out;
   int zero_rest;         // rows of no group are cleared
+  int out16;             // out's rows start on 16 bytes, and lanes come in whole 16 bytes
   const float* lane_scale;  // int8: ws
   const float* col_scale;   // int8: xs
   const float* bias;        // int8, or null
@@ -94,6 +101,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_a
   asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr), "r"(bytes)
                : "memory");
 }
+// Arrives on a barrier of the pair's leader; what this warp did with TMEM before is ordered by tcgen05's own fence. (A release
+// at cluster scope would wait for the warp's global stores, a microsecond in each tile.)
+__device__ __forceinline__ void gg_arrive(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // 3-D tiled load whose completion is counted on a barrier of the pair's leader; no multicast.
 __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z,
                                                  uint64_t policy) {
@@ -112,7 +124,7 @@ __device__ __forceinline__ bool gg_warp_wait(uint64_t* bar, uint32_t parity, vol
   if (lane == 0) {
     const uint64_t t0 = globaltimer_ns();
     while (!mbar_try_wait(bar, parity)) {
-      __nanosleep(100);
+      __nanosleep(20);
       if (*abort_flag || globaltimer_ns() - t0 > MOE_WAIT_NS) {
         if (!*abort_flag && status) atomicOr(status, kStatusWaitTimeout);
         *abort_flag = 1;
@@ -187,6 +199,31 @@ struct GroupedSchedule {
   }
 };
 
+// 16 TMEM lanes x 32 columns as fragments: registers 4 i + {0, 1} hold columns 8 i + 2 (t % 4) + {0, 1} of lane t / 4 for
+// thread t, registers 4 i + {2, 3} those of lane t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// Four 8 x 8 matrices of 16-bit elements, transposed: thread t gives the address of row t % 8 of matrix t / 8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+template <typename OutT> __device__ __forceinline__ uint32_t gg_pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t gg_pack<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t gg_pack<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // Warp-wide: the tile table of all groups. Offsets outside [0, R] are clamped, groups that end before they
 // start are empty, so that no address leaves the tensors whatever the offsets hold.
 template <int KIND>
@@ -245,7 +282,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   constexpr int kMmaRed = kInt8 ? 32 : 16;  // and per MMA
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kGgStages * kGgStageBytes);  // leader's: both CTAs' producers
+  uint8_t* pieces_out = smem + kGgStages * kGgStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(pieces_out + kGgOutBytes);  // leader's: both CTAs' producers
   uint64_t* empty = full + kGgStages;
   uint64_t* landed = empty + kGgStages;  // Dw's tails: this CTA's own copies
   uint64_t* tfull = landed + kGgStages;
@@ -253,7 +291,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* table = reinterpret_cast<int*>(smem + kGgStages * kGgStageBytes + 256);
+  int* table = reinterpret_cast<int*>(pieces_out + kGgOutBytes + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -353,7 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         const GroupedTile t = sched.get(tile);
         if (t.kblocks == 0) continue;
         const int slot = count & 1;
-        if (!mbar_wait_cluster(&tempty[slot], ((count >> 1) & 1u) ^ 1u, abort_flag, args.status)) break;
+        if (!mbar_wait(&tempty[slot], ((count >> 1) & 1u) ^ 1u, abort_flag, args.status)) break;
         ++count;
         tc_fence_after();
         const int n = (t.ncols + kGgColStep - 1) / kGgColStep * kGgColStep;
@@ -418,19 +456,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- epilogue
-    const int q = warp & 3;
+    const int q = warp & 3, part = (warp - 4) >> 2;  // lane quadrant, half of the columns
+    constexpr bool kWide = sizeof(OutT) == 4;
+    constexpr int kPieceCols = kGgPiece / (32 * static_cast<int>(sizeof(OutT)));
+    constexpr int kPieceRow = 32 * static_cast<int>(sizeof(OutT));  // bytes of a column's 32 lanes
     OutT* out = static_cast<OutT*>(args.out);
+    uint8_t* piece = pieces_out + (warp - 4) * kGgPiece;
     uint32_t count = 0;
+    // where this thread's row of a matrix starts (stmatrix), and its element of a row (lane): the 16-byte chunks of
+    // 64-byte rows are swizzled
+    const uint32_t st_row = lane & 7, st_at = st_row * 64 + ((lane >> 3) ^ (st_row >> 1 & 3)) * 16;
     for (int tile = pair; tile < tiles; tile += npairs) {
       const GroupedTile t = sched.get(tile);
-      const int f = t.lane0 + static_cast<int>(rank) * 128 + q * 32 + lane;
+      const int f0 = t.lane0 + static_cast<int>(rank) * 128 + q * 32, f = f0 + lane;
       const bool there = f < args.lanes;
       int64_t at = (t.row0 * args.ld_out);
       if (kDw) at = (static_cast<int64_t>(t.e) * args.cols + t.col0) * args.ld_out;
+      // this warp's columns: even shares of what there is, in whole pieces of 32
+      const int share = (t.ncols + 63) / 64 * 32;
+      const int from = part * share, to = part ? t.ncols : min(share, t.ncols);
       OutT* p = out + at + f;
       if (t.kblocks == 0) {  // an expert without rows: dW = 0
         if (there)
-          for (int c = 0; c < t.ncols; ++c, p += args.ld_out) *p = gg_cast<OutT>(0.0f);
+          for (int c = from; c < to; ++c) p[c * args.ld_out] = gg_cast<OutT>(0.0f);
         continue;
       }
       const int slot = count & 1;
@@ -438,36 +486,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
       ++count;
       tc_fence_after();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(slot * 256);
-      float ws = 0.0f, bias = 0.0f;
+      auto release = [&]() {  // this warp's part of the accumulator is read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) gg_arrive(mapa_shared(smem_u32(&tempty[slot]), 0));
+      };
+      float ws[4], bias[4];
       if constexpr (kInt8) {
-        if (there) {
-          ws = args.lane_scale[f];
-          bias = args.bias ? args.bias[f] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int fi = kWide ? f : f0 + i * 8 + lane / 4;
+          ws[i] = fi < args.lanes ? args.lane_scale[fi] : 0.0f;
+          bias[i] = fi < args.lanes && args.bias ? args.bias[fi] : 0.0f;
         }
       }
+      if (from >= to) release();
 #pragma unroll 1
-      for (int c0 = 0; c0 < t.ncols; c0 += 32) {
+      for (int c0 = from; c0 < to; c0 += 32) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(taddr + c0, r);
-        tmem_ld_wait();
-        if (c0 + 32 >= t.ncols) {  // the last columns: the accumulator is free
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[slot]), 0));
+        if constexpr (kWide) {
+          tmem_ld_32x32b_x32(taddr + c0, r);
+        } else {
+          tmem_ld_16x256b_x4(taddr + c0, r);
+          tmem_ld_16x256b_x4(taddr + (16u << 16) + c0, r + 16);
         }
-        const int left = t.ncols - c0;
-        if (there) {
+        tmem_ld_wait();
+        if (c0 + 32 >= to) release();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j < left) {
-              float v;
-              if constexpr (kInt8)
-                v = static_cast<float>(static_cast<int>(r[j])) * args.col_scale[t.row0 + c0 + j] * ws + bias;
-              else
-                v = __uint_as_float(r[j]);
-              *p = gg_cast<OutT>(v);
+        for (int k = 0; k < 32 / kPieceCols; ++k) {
+          const int c1 = c0 + k * kPieceCols;
+          if (c1 >= to) break;
+          __syncwarp();  // the last piece has been copied
+          if constexpr (kWide) {
+#pragma unroll
+            for (int j = 0; j < kPieceCols; ++j) {
+              float v = __uint_as_float(r[k * kPieceCols + j]);
+              if constexpr (kInt8) {
+                const float xs = c1 + j < t.ncols ? __ldg(args.col_scale + t.row0 + c1 + j) : 0.0f;
+                v = static_cast<float>(static_cast<int>(r[k * kPieceCols + j])) * xs * ws[0] + bias[0];
+              }
+              reinterpret_cast<float*>(piece)[j * 32 + lane] = v;
             }
-            p += args.ld_out;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // 8 columns
+              uint32_t m[4];               // matrices of 8 lanes
+              float xs[2];
+              if constexpr (kInt8) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const int c = c1 + i * 8 + lane % 4 * 2 + j;
+                  xs[j] = c < t.ncols ? __ldg(args.col_scale + t.row0 + c) : 0.0f;
+                }
+              }
+#pragma unroll
+              for (int l = 0; l < 4; ++l) {
+                const uint32_t* v = r + (l >> 1) * 16 + i * 4 + (l & 1) * 2;
+                if constexpr (kInt8)
+                  m[l] = gg_pack<OutT>(static_cast<float>(static_cast<int>(v[0])) * xs[0] * ws[l] + bias[l],
+                                       static_cast<float>(static_cast<int>(v[1])) * xs[1] * ws[l] + bias[l]);
+                else
+                  m[l] = gg_pack<OutT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
+              }
+              stmatrix_x4_trans(smem_u32(piece) + i * 512 + st_at, m[0], m[1], m[2], m[3]);
+            }
+          }
+          __syncwarp();
+          const int n = min(kPieceCols, to - c1);
+          if (args.out16) {
+            constexpr int kRowLanes = kPieceRow / 16, kPer = 32 / kRowLanes;  // threads of a row, rows at a time
+            constexpr int kElts = 16 / static_cast<int>(sizeof(OutT));
+            const int row = lane / kRowLanes, chunk = lane % kRowLanes;
+            if (f0 + chunk * kElts < args.lanes) {
+              OutT* o = out + at + f0 + chunk * kElts + (c1 + row) * args.ld_out;
+#pragma unroll
+              for (int j = 0; j < kPieceCols / kPer; ++j) {
+                const int rj = row + j * kPer;
+                const int byte = rj * kPieceRow + (kWide ? chunk : chunk ^ (rj >> 1 & 3)) * 16;
+                if (rj < n) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(piece + byte);
+                o += kPer * args.ld_out;
+              }
+            }
+          } else {
+            OutT* o = p + c1 * args.ld_out;
+            for (int j = 0; j < n; ++j, o += args.ld_out) {
+              const int byte = kWide ? j * 128 + lane * 4 : j * 64 + ((lane >> 3) ^ (j >> 1 & 3)) * 16 + (lane & 7) * 2;
+              if (there) *o = *reinterpret_cast<const OutT*>(piece + byte);
+            }
           }
         }
         __syncwarp();  // the next read of TMEM is the whole warp's
@@ -481,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         e = static_cast<int64_t>(sched.start[args.E - 1]) + sched.rows[args.E - 1];
       }
       const int64_t n = s + args.rows - e;
-      const int w = (static_cast<int>(blockIdx.x) * kGgEpiWarps) + q;
+      const int w = static_cast<int>(blockIdx.x) * kGgEpiWarps + warp - 4;
       for (int64_t i = w; i < n; i += static_cast<int64_t>(gridDim.x) * kGgEpiWarps) {
         OutT* p = out + (i < s ? i : e + i - s) * args.ld_out;
         for (int c = lane; c < args.lanes; c += 32) p[c] = gg_cast<OutT>(0.0f);

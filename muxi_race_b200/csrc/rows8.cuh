@@ -82,7 +82,8 @@ __device__ __forceinline__ Packed<S> r8_load(const S* row, int c0, int l8, int w
   return p;
 }
 
-template <int VEC, typename S>
+// STREAM: rows that are written once and not read soon, which should leave the L2 to what is.
+template <int VEC, bool STREAM = false, typename S>
 __device__ __forceinline__ void r8_store(S* row, int c0, int l8, int width, const Packed<S>& p) {
   if constexpr (VEC == 1) {
     using U = typename std::conditional<sizeof(S) == 1, uint8_t, uint16_t>::type;
@@ -98,7 +99,9 @@ __device__ __forceinline__ void r8_store(S* row, int c0, int l8, int width, cons
     for (int i = 0; i < 2; ++i) {
       const int c = r8_col<VEC>(c0, l8, 8 * i);
       if (c < width) {
-        if constexpr (sizeof(S) == 2)
+        if constexpr (sizeof(S) == 2 && STREAM)
+          __stcs(reinterpret_cast<uint4*>(row + c), make_uint4(p.w[i * 4], p.w[i * 4 + 1], p.w[i * 4 + 2], p.w[i * 4 + 3]));
+        else if constexpr (sizeof(S) == 2)
           *reinterpret_cast<uint4*>(row + c) = make_uint4(p.w[i * 4], p.w[i * 4 + 1], p.w[i * 4 + 2], p.w[i * 4 + 3]);
         else
           *reinterpret_cast<uint2*>(row + c) = make_uint2(p.w[i * 2], p.w[i * 2 + 1]);
@@ -402,26 +405,25 @@ struct Rows8Args {
   int width, parts;
 };
 
-// 16-bit rows to 8 bits. A warp takes its part of two rows at a time, so that enough loads are in flight.
+// 16-bit rows to 8 bits.
 template <typename T, typename Q, int VEC>
 __global__ void __launch_bounds__(kR8Threads) save_rows8_kernel(const Rows8Args a) {
   const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (a.width + kR8Group - 1) / kR8Group;
   const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
   const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r < a.rows; r += 2 * step) {
-    const int64_t r2 = r + step;
-    const int width2 = r2 < a.rows ? a.width : 0;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r < a.rows; r += step) {
+    const T* x = static_cast<const T*>(a.x) + r * a.ld;
+    Q* q = static_cast<Q*>(a.out) + r * a.parts * a.width;
+    float* scale = a.scale + r * a.parts * groups;
     for (int p = 0; p < a.parts; ++p) {
-      const T* x = static_cast<const T*>(a.x) + r * a.ld + static_cast<int64_t>(p) * a.width;
-      const T* x2 = x + (width2 ? step * a.ld : 0);
-      const int64_t at = r * a.parts + p, at2 = r2 * a.parts + p;
       for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
-        const int grp = g0 + sub, c0 = grp * kR8Group;
-        const Packed<T> v = r8_load<VEC>(x, c0, l8, a.width), v2 = r8_load<VEC>(x2, c0, l8, width2);
-        r8_encode<VEC>(v, static_cast<Q*>(a.out) + at * a.width, a.scale + at * groups + grp, c0, l8, a.width);
-        r8_encode<VEC>(v2, static_cast<Q*>(a.out) + at2 * a.width, a.scale + at2 * groups + grp, c0, l8, width2);
+        const int c0 = (g0 + sub) * kR8Group;
+        r8_encode<VEC>(r8_load<VEC>(x, c0, l8, a.width), q, scale + g0 + sub, c0, l8, a.width);
       }
+      x += a.width;
+      q += a.width;
+      scale += groups;
     }
   }
 }
@@ -437,56 +439,45 @@ __device__ __forceinline__ int64_t r8_from(const Rows8Args& a, int64_t r) {
 }
 
 // Rows of type S (T itself, I8 or F8) back to T, in the order of an index; a source row that is not there: zeros.
-// Several rows at a time, as in save_rows8_kernel.
+// The rows that are written pass the L2 by, so that a source row that several take stays there (4096 int8 rows of 7168,
+// each taken 8 times: 88 us, 118 us without). One row at a time: with two or four in flight the registers cost more warps than
+// the loads gain (93 and 119 us).
 template <typename T, typename S, int VEC>
 __global__ void __launch_bounds__(kR8Threads) restore_rows_kernel(const Rows8Args a) {
-  constexpr int kRows = sizeof(S) == 1 ? 4 : 2;
   const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;
   const int groups = (a.width + kR8Group - 1) / kR8Group;
   const int row_warps = r8_row_warps(groups), in_row = warp & (row_warps - 1), cta_rows = kR8Warps / row_warps;
   const int64_t rows = a.valid ? min(a.rows, static_cast<int64_t>(*a.valid)) : a.rows;
   const int64_t step = static_cast<int64_t>(gridDim.x) * cta_rows;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r0 < rows; r0 += kRows * step) {
-    const S* src[kRows];
-    const float* src_scale[kRows];
-    int width[kRows];  // to be read: 0 where a row comes from nowhere
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int64_t f = r0 + i * step < rows ? r8_from(a, r0 + i * step) : -1;
-      width[i] = f < 0 ? 0 : a.width;
-      src[i] = static_cast<const S*>(a.x) + (f < 0 ? 0 : f) * a.ld;
-      src_scale[i] = a.scale + (f < 0 ? 0 : f) * a.parts * groups;
-    }
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * cta_rows + warp / row_warps; r < rows; r += step) {
+    const int64_t from = r8_from(a, r);
+    const int width = from < 0 ? 0 : a.width;  // nothing to read: zeros
+    const S* src = static_cast<const S*>(a.x) + (from < 0 ? 0 : from) * a.ld;
+    const float* src_scale = a.scale + (from < 0 ? 0 : from) * a.parts * groups;
+    T* out = static_cast<T*>(a.out) + r * a.parts * a.width;
     for (int p = 0; p < a.parts; ++p) {
       for (int g0 = in_row * kR8Step; g0 < groups; g0 += row_warps * kR8Step) {
         const int grp = g0 + sub, c0 = grp * kR8Group;
-        Packed<S> q[kRows];
-        float s[kRows];
+        const Packed<S> q = r8_load<VEC>(src, c0, l8, width);
+        if constexpr (std::is_same<S, T>::value) {
+          r8_store<VEC, true>(out, c0, l8, a.width, q);
+        } else {
+          const float s = c0 < width ? __ldg(src_scale + grp) : 0.0f;
+          Packed<T> y;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          q[i] = r8_load<VEC>(src[i] + static_cast<int64_t>(p) * a.width, c0, l8, width[i]);
-          s[i] = !std::is_same<S, T>::value && c0 < width[i] ? __ldg(src_scale[i] + p * groups + grp) : 0.0f;
-        }
+          for (int k = 0; k < kR8Cols / 4; ++k) {
+            float v[4];
+            r8_unpack4(q, k, v);
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          if (r0 + i * step >= rows) break;
-          T* out = static_cast<T*>(a.out) + ((r0 + i * step) * a.parts + p) * a.width;
-          if constexpr (std::is_same<S, T>::value) {
-            r8_store<VEC>(out, c0, l8, a.width, q[i]);
-          } else {
-            Packed<T> y;
-#pragma unroll
-            for (int k = 0; k < kR8Cols / 4; ++k) {
-              float v[4];
-              r8_unpack4(q[i], k, v);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) v[j] *= s[i];
-              r8_pack4(y, k, v);
-            }
-            r8_store<VEC>(out, c0, l8, a.width, y);
+            for (int j = 0; j < 4; ++j) v[j] *= s;
+            r8_pack4(y, k, v);
           }
+          r8_store<VEC, true>(out, c0, l8, a.width, y);
         }
       }
+      src += a.width;
+      src_scale += groups;
+      out += a.width;
     }
   }
 }
