@@ -47,12 +47,17 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   MOE_TRY(current_device(&dev));
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &args.status));
-  const int64_t lane_tiles = (args.lanes + kGgTile - 1) / kGgTile;
-  const int64_t groups = KIND == kGroupedDw ? static_cast<int64_t>(args.E) * ((args.cols + kGgTile - 1) / kGgTile)
-                                            : (args.rows + kGgTile - 1) / kGgTile + args.E;
-  if (lane_tiles * groups > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
+  // Groups of columns: about R / 256 and half a one more for each expert (where they begin and end is not known here).
+  const int64_t most = KIND == kGroupedDw ? static_cast<int64_t>(args.E) * ((args.cols + kGgTile - 1) / kGgTile)
+                                          : (args.rows + kGgTile - 1) / kGgTile + args.E;
+  const int64_t usual = KIND == kGroupedDw ? most : (args.rows + kGgTile - 1) / kGgTile + (args.E < args.rows ? args.E : args.rows) / 2;
   int64_t pairs = sms / 2;
-  if (lane_tiles * groups < pairs) pairs = lane_tiles * groups;
+  auto lane_tiles = [&](int halves) { return (args.lanes + halves * kGgHalf - 1) / (halves * kGgHalf); };
+  auto rounds = [&](int halves) { return (lane_tiles(halves) * usual + pairs - 1) / pairs; };
+  // A tile of 512 lanes takes as long as 1.5 of 256 (8192^3: %PERF%); fewer rounds of the smaller ones win where there are few tiles.
+  args.halves = args.lanes > kGgHalf && 3 * rounds(2) <= 2 * rounds(1) ? 2 : 1;
+  if (lane_tiles(args.halves) * most > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
+  if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;
   constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT>;
   MOE_TRY(allow_smem<kernel>(dev));
   kernel<<<static_cast<unsigned>(2 * pairs), kGgThreads, kGgSmemBytes, s>>>(a, b, b32, args);

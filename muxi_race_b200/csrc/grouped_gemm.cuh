@@ -5,21 +5,22 @@
 //   kGroupedDx   dx[r, k]    = sum_n W[e, n, k] dy[r, n]
 //   kGroupedDw   dW[e, n, k] = sum_r x[r, k] dy[r, n]     over e's rows
 //   kDenseInt8   y[m, n]     = xs[m] ws[n] sum_k w[n, k] x[m, k] (+ bias[n]), int8, one group
-// One kernel serves all four. The MMA's M side ("lanes": 256 per CTA pair) is always the dimension that
-// is contiguous in the output (n, k, k, n), its N side ("columns") the output's rows: tokens, or n for
-// dW. So an expert's tokens fill columns in steps of 32, not whole 128-row blocks; the weights are read
-// in full tiles; and a thread, which holds one lane's accumulators, stores elements that its warp's
-// neighbours continue (32 lanes, one segment of 64 or 128 bytes), with any mask or alignment.
+// One kernel serves all four. The MMA's M side ("lanes") is always the dimension that is contiguous in the output (n, k, k,
+// n), its N side ("columns") the output's rows: tokens, or n for dW. So an expert's tokens fill columns in steps of 32, not
+// whole 128-row blocks, the weights are read in full tiles, and a warp's stores are 64 or 128 bytes of a row, with any mask.
 //
 // The reduction runs along k (Y, int8: both operands have it contiguous, "K-major"), along n (Dx: the
 // weights have it outermost, "MN-major") or along the rows (Dw: both operands MN-major). tcgen05 reads
 // either form from 128B-swizzled shared memory: K-major tiles are rows of 128 bytes of reduction, MN-major
 // tiles 64 reduction rows of 128 bytes of lanes or columns, two of them side by side for 128.
 //
-// Bounds: 2 R N K operations at the tensor rate, or the weights' bytes where an expert has fewer than
-// about 250 rows. CTA pairs (cta_group::2) halve each SM's intake of the wider operand: a 256 x 256 tile
-// takes 32 KiB per SM and 64-element step. Six stages of those; two accumulators of 256 columns, so that
-// one tile's stores overlap the next one's MMAs.
+// Bounds: 2 R N K operations at the tensor rate, or the weights' bytes where an expert has fewer than about 250 rows. What
+// the copies write into shared memory and what the MMAs read from it share its 128 bytes a cycle: with a tile of 256 lanes x 256
+// columns per CTA pair (cta_group::2) every byte written is read once, both together take as long as the MMAs themselves,
+// and 8192^3 runs at 0.70 of the tensor pipe's cycles. A tile is therefore 512 lanes x 256 columns, two MMAs of 256 lanes that
+// share the columns' operand: 48 KiB per SM and 64-element step instead of 64 (or of 32 for half as much). Its two halves fill all 512
+// TMEM columns. They are handed to the epilogue and back one by one: the MMA warp runs the first half of the next tile ahead while the
+// second is still being stored. Where 512 lanes would leave SMs without work, tiles have 256.
 //
 // Dw reduces over rows, so the last block of an expert reaches into the next expert's rows. Those may
 // hold infinities or NaN, which a zero in the other operand would not remove: a warp of its own clears
@@ -45,10 +46,12 @@ namespace moe {
 
 enum GroupedKind : int { kGroupedY = 0, kGroupedDx = 1, kGroupedDw = 2, kDenseInt8 = 3 };
 
-constexpr int kGgStages = 6;
-constexpr int kGgOperandBytes = 128 * 128;  // of one operand, per CTA and stage
-constexpr int kGgStageBytes = 2 * kGgOperandBytes;
-constexpr int kGgTile = 256;                // lanes per pair, columns at most
+constexpr int kGgStages = 4;
+constexpr int kGgOperandBytes = 128 * 128;  // 128 lanes or columns of an operand, per CTA and stage
+constexpr int kGgStageBytes = 3 * kGgOperandBytes;  // two halves of lanes, columns
+constexpr int kGgHalf = 256;                // lanes of a pair's MMA
+constexpr int kGgTile = 256;                // columns at most
+constexpr int kGgAhead = 3;                 // blocks that one half may be ahead of the other
 constexpr int kGgMaxExperts = 1024;
 constexpr int kGgEpiWarps = 8;              // two per TMEM lane quadrant, each with half of the columns
 constexpr int kGgThreads = 128 + 32 * kGgEpiWarps;
@@ -65,6 +68,7 @@ struct GroupedArgs {
   int offsets64;
   int E;
   int64_t rows;          // R
+  int halves;            // of a tile: 1 or 2 times 256 lanes
   int lanes;             // extent of the lane dimension (contiguous in the output)
   int cols;              // Dw: extent of the column dimension (N); otherwise unused
   int red;               // extent of the reduction; Dw: unused
@@ -136,9 +140,23 @@ __device__ __forceinline__ bool gg_warp_wait(uint64_t* bar, uint32_t parity, vol
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// Lanes that waited each for themselves go on together: a wait given up by one is given up by all.
+__device__ __forceinline__ bool gg_all(bool ok) { return __all_sync(0xffffffffu, ok) != 0; }
+
+// True in one thread of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok));
+  return ok != 0;
+}
+
 // One tile: expert, first lane, first column (a row; Dw: an n), columns, and for Dw the rows it reduces.
 struct GroupedTile {
-  int e, lane0, ncols;
+  int e, lane0, halves, ncols;
   int64_t row0;
   int col0, kblocks, tail;  // tail: reduction rows or elements in the last block (0: it is full)
 };
@@ -152,14 +170,16 @@ __device__ __forceinline__ int gg_col_step(int rows) {  // columns per tile of a
 template <int KIND>
 struct GroupedSchedule {
   const int *prefix, *start, *rows;  // tiles before group e, its first row, its rows
-  int E, lane_tiles, red_blocks, red_tail, cols, e;
+  int E, lanes, tile_lanes, lane_tiles, red_blocks, red_tail, cols, e;
 
   __device__ GroupedSchedule(const GroupedArgs& a, const int* table) {
     prefix = table;
     start = table + kGgMaxExperts + 1;
     rows = start + kGgMaxExperts;
     E = a.E;
-    lane_tiles = (a.lanes + kGgTile - 1) / kGgTile;
+    lanes = a.lanes;
+    tile_lanes = a.halves * kGgHalf;
+    lane_tiles = (lanes + tile_lanes - 1) / tile_lanes;
     constexpr int kRed = KIND == kDenseInt8 ? 128 : 64;
     red_blocks = (a.red + kRed - 1) / kRed;
     red_tail = a.red % kRed;
@@ -176,7 +196,7 @@ struct GroupedSchedule {
     const int n = rows[e];
     if (KIND == kGroupedDw) {
       const int col_tiles = (cols + kGgTile - 1) / kGgTile;
-      t.lane0 = i / col_tiles * kGgTile;
+      t.lane0 = i / col_tiles * tile_lanes;
       t.col0 = i % col_tiles * kGgTile;
       t.ncols = min(kGgTile, cols - t.col0);
       t.row0 = start[e];
@@ -187,7 +207,7 @@ struct GroupedSchedule {
       const int band = i / (lane_tiles * kGgBand);
       i -= band * lane_tiles * kGgBand;
       const int width = min(kGgBand, col_tiles - band * kGgBand);
-      t.lane0 = i / width * kGgTile;
+      t.lane0 = i / width * tile_lanes;
       const int c = (band * kGgBand + i % width) * step;
       t.ncols = min(step, n - c);
       t.row0 = start[e] + c;
@@ -195,6 +215,7 @@ struct GroupedSchedule {
       t.kblocks = red_blocks;
       t.tail = red_tail;
     }
+    t.halves = min(tile_lanes, lanes - t.lane0) > kGgHalf ? 2 : 1;
     return t;
   }
 };
@@ -231,7 +252,7 @@ __device__ __forceinline__ void gg_build_table(const GroupedArgs& a, int* table,
   int* prefix = table;
   int* start = table + kGgMaxExperts + 1;
   int* rows = start + kGgMaxExperts;
-  const int lane_tiles = (a.lanes + kGgTile - 1) / kGgTile;
+  const int lane_tiles = (a.lanes + a.halves * kGgHalf - 1) / (a.halves * kGgHalf);
   const int dw_tiles = lane_tiles * ((a.cols + kGgTile - 1) / kGgTile);
   int before = 0;
   for (int e0 = 0; e0 < a.E; e0 += 32) {
@@ -329,7 +350,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
-    if (lane == 0) {
+    // All lanes go through the loop and one of them issues, here and in the MMA warp: addresses and descriptors are then
+    // computed in uniform registers, which these instructions read. From a loop of lane 0 alone an MMA took about 200 cycles to
+    // issue, more than it runs.
+    {
       const uint64_t pol = l2_policy_evict_normal();
       int st = 0;
       uint32_t ph = 0;
@@ -340,40 +364,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         const int lane0 = t.lane0 + static_cast<int>(rank) * 128;
         const int boxes = half <= 96 ? (half + 31) / 32 : 0;  // 32-row boxes; 0: one of 128
         for (int kb = 0; kb < t.kblocks; ++kb) {
-          if (!mbar_wait(&empty[st], ph ^ 1u, abort_flag, args.status)) {
+          if (!gg_all(mbar_wait(&empty[st], ph ^ 1u, abort_flag, args.status))) {
             ok = false;
             break;
           }
           uint8_t* a = smem + st * kGgStageBytes;
-          uint8_t* b = a + kGgOperandBytes;
+          uint8_t* b = a + 2 * kGgOperandBytes;
           const uint32_t bar = mapa_shared(smem_u32(&full[st]), 0);
-          if constexpr (kDw) {
-            const int row = static_cast<int>(t.row0) + kb * 64;
-            const int col0 = t.col0 + static_cast<int>(rank) * half;
-            if (kb == t.kblocks - 1 && t.tail % 16 != 0) {  // to be cleared behind the end first
-              mbar_arrive_expect_tx(&landed[st], kGgStageBytes);
-              for (int c = 0; c < 2; ++c) {
-                tma_load_2d(a + c * 8192, &tmA, &landed[st], lane0 + c * 64, row, pol);
-                tma_load_2d(b + c * 8192, &tmB, &landed[st], col0 + c * 64, row, pol);
+          if (elect_one()) {
+            if constexpr (kDw) {
+              const int row = static_cast<int>(t.row0) + kb * 64;
+              const int col0 = t.col0 + static_cast<int>(rank) * half;
+              const uint32_t bytes = (t.halves + 1) * kGgOperandBytes;
+              if (kb == t.kblocks - 1 && t.tail % 16 != 0) {  // to be cleared behind the end first
+                mbar_arrive_expect_tx(&landed[st], bytes);
+                for (int c = 0; c < 2; ++c) tma_load_2d(b + c * 8192, &tmB, &landed[st], col0 + c * 64, row, pol);
+                for (int c = 0; c < 2 * t.halves; ++c)
+                  tma_load_2d(a + c * 8192, &tmA, &landed[st], lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, row, pol);
+              } else {
+                mbar_arrive_expect_tx_cluster(bar, bytes);
+                for (int c = 0; c < 2; ++c) tma_load_2d_pair(b + c * 8192, &tmB, bar, col0 + c * 64, row, pol);
+                for (int c = 0; c < 2 * t.halves; ++c)
+                  tma_load_2d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, row, pol);
               }
             } else {
-              mbar_arrive_expect_tx_cluster(bar, kGgStageBytes);
-              for (int c = 0; c < 2; ++c) {
-                tma_load_2d_pair(a + c * 8192, &tmA, bar, lane0 + c * 64, row, pol);
-                tma_load_2d_pair(b + c * 8192, &tmB, bar, col0 + c * 64, row, pol);
+              const int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half;
+              mbar_arrive_expect_tx_cluster(bar, t.halves * kGgOperandBytes + (boxes ? boxes * 4096 : kGgOperandBytes));
+              if constexpr (kMnA) {
+                for (int c = 0; c < 2 * t.halves; ++c)
+                  tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, kb * kRed, t.e, pol);
+              } else {
+                for (int h = 0; h < t.halves; ++h)
+                  tma_load_3d_pair(a + h * kGgOperandBytes, &tmA, bar, kb * kRed, lane0 + h * kGgHalf, t.e, pol);
               }
+              if (boxes == 0) tma_load_2d_pair(b, &tmB, bar, kb * kRed, row, pol);
+              for (int i = 0; i < boxes; ++i) tma_load_2d_pair(b + i * 4096, &tmB32, bar, kb * kRed, row + i * 32, pol);
             }
-          } else {
-            const int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half;
-            mbar_arrive_expect_tx_cluster(bar, kGgOperandBytes + (boxes ? boxes * 4096 : kGgOperandBytes));
-            if constexpr (kMnA) {
-              for (int c = 0; c < 2; ++c) tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + c * 64, kb * kRed, t.e, pol);
-            } else {
-              tma_load_3d_pair(a, &tmA, bar, kb * kRed, lane0, t.e, pol);
-            }
-            if (boxes == 0) tma_load_2d_pair(b, &tmB, bar, kb * kRed, row, pol);
-            for (int i = 0; i < boxes; ++i) tma_load_2d_pair(b + i * 4096, &tmB32, bar, kb * kRed, row + i * 32, pol);
           }
+          __syncwarp();
           if (++st == kGgStages) {
             st = 0;
             ph ^= 1u;
@@ -383,16 +411,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (leader && lane == 0) {
-      int st = 0;
-      uint32_t ph = 0, count = 0;
+    if (leader) {
+      int st = 0, held = 0;  // next stage; stages whose second half is to come
+      uint32_t ph = 0;
+      uint32_t uses[2] = {0, 0};
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += npairs) {
         const GroupedTile t = sched.get(tile);
         if (t.kblocks == 0) continue;
-        const int slot = count & 1;
-        if (!mbar_wait(&tempty[slot], ((count >> 1) & 1u) ^ 1u, abort_flag, args.status)) break;
-        ++count;
+        if (!gg_all(mbar_wait(&tempty[0], (uses[0] & 1u) ^ 1u, abort_flag, args.status))) break;
+        ++uses[0];
         tc_fence_after();
         const int n = (t.ncols + kGgColStep - 1) / kGgColStep * kGgColStep;
         uint32_t idesc;
@@ -400,38 +428,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           idesc = idesc_i8(256, n);
         else
           idesc = idesc_f16(kBf16, 256, n) | (kMnA ? 1u << 15 : 0u) | (kDw ? 1u << 16 : 0u);
-        const uint32_t d = tmem_base + static_cast<uint32_t>(slot * 256);
+        auto mmas = [&](int stage, int half, int kb) {
+          const uint32_t a = smem_u32(smem + stage * kGgStageBytes) + half * kGgOperandBytes;
+          const uint32_t b = smem_u32(smem + stage * kGgStageBytes) + 2 * kGgOperandBytes;
+          const uint32_t d = tmem_base + static_cast<uint32_t>(half * 256);
+          const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kRed / kMmaRed; ++k) {
+              if (k * kMmaRed < left) {
+                const uint64_t ad = kMnA ? smem_desc_sw128_mn(a + k * 2048) : smem_desc_sw128(a + k * 32);
+                const uint64_t bd = kDw ? smem_desc_sw128_mn(b + k * 2048) : smem_desc_sw128(b + k * 32);
+                if constexpr (kInt8)
+                  mma_i8_pair(d, ad, bd, idesc, (kb | k) != 0);
+                else
+                  mma_f16_pair(d, ad, bd, idesc, (kb | k) != 0);
+              }
+            }
+          }
+          __syncwarp();
+        };
+        bool second = false;  // the second half's accumulator is free
         for (int kb = 0; kb < t.kblocks; ++kb) {
           const bool cleared = kDw && kb == t.kblocks - 1 && t.tail % 16 != 0;  // with stores of the peer's threads
-          if (!(cleared ? mbar_wait_cluster(&full[st], ph, abort_flag, args.status)
-                        : mbar_wait(&full[st], ph, abort_flag, args.status))) {
+          if (!gg_all(cleared ? mbar_wait_cluster(&full[st], ph, abort_flag, args.status)
+                              : mbar_wait(&full[st], ph, abort_flag, args.status))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + st * kGgStageBytes), b = a + kGgOperandBytes;
-          const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
-#pragma unroll
-          for (int k = 0; k < kRed / kMmaRed; ++k) {
-            if (k * kMmaRed < left) {
-              const uint64_t ad = kMnA ? smem_desc_sw128_mn(a + k * 2048) : smem_desc_sw128(a + k * 32);
-              const uint64_t bd = kDw ? smem_desc_sw128_mn(b + k * 2048) : smem_desc_sw128(b + k * 32);
-              if constexpr (kInt8)
-                mma_i8_pair(d, ad, bd, idesc, (kb | k) != 0);
-              else
-                mma_f16_pair(d, ad, bd, idesc, (kb | k) != 0);
+          mmas(st, 0, kb);
+          const int last = kb == t.kblocks - 1;
+          if (last && elect_one()) tc_commit_pair(&tfull[0], 0x3);
+          __syncwarp();
+          ++held;
+          if (t.halves == 2 && !second) {
+            second = __all_sync(0xffffffffu, mbar_try_wait(&tempty[1], (uses[1] & 1u) ^ 1u));
+            if (!second && (last || held == kGgAhead)) {
+              if (!gg_all(mbar_wait(&tempty[1], (uses[1] & 1u) ^ 1u, abort_flag, args.status))) {
+                ok = false;
+                break;
+              }
+              second = true;
+            }
+            if (second) tc_fence_after();
+          }
+          // the second half follows at once, but at the tile's end after the first, whose stores can then begin
+          if (t.halves == 1 || (second && (last || kb < t.kblocks - kGgAhead || held == kGgAhead))) {
+            for (; held > 0; --held) {
+              const int back = held - 1, stage = st >= back ? st - back : st - back + kGgStages;
+              if (t.halves == 2) mmas(stage, 1, kb - back);
+              if (elect_one()) tc_commit_pair(&empty[stage], 0x3);
+              __syncwarp();
             }
           }
-          tc_commit_pair(&empty[st], 0x3);
           if (++st == kGgStages) {
             st = 0;
             ph ^= 1u;
           }
         }
         if (!ok) break;
-        tc_commit_pair(&tfull[slot], 0x3);
+        if (t.halves == 2) {
+          ++uses[1];
+          if (elect_one()) tc_commit_pair(&tfull[1], 0x3);
+          __syncwarp();
+        }
       }
-      tc_commit_pair(drain, 0x1);
+      if (elect_one()) tc_commit_pair(drain, 0x1);
+      __syncwarp();
       mbar_wait_drain(drain, 0);
     }
   } else if (warp == 3) {
@@ -445,10 +509,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         const int st = static_cast<int>((blocks - 1) % kGgStages);
         if (!gg_warp_wait(&landed[st], (phases >> st) & 1u, abort_flag, args.status, lane)) break;
         phases ^= 1u << st;
-        const int pieces = (16 - t.tail % 16) * 8;  // 16-byte pieces of the rows to clear, in each of four tiles
-        uint8_t* from = smem + st * kGgStageBytes + t.tail * 128;
-        for (int i = lane; i < pieces * 4; i += 32)
-          *reinterpret_cast<uint4*>(from + i / pieces * 8192 + i % pieces * 16) = make_uint4(0, 0, 0, 0);
+        const int rows = 16 - t.tail % 16;  // to clear, in each of the stage's six boxes of 64 rows
+        uint8_t* from = smem + st * kGgStageBytes + t.tail * 128 + lane % 8 * 16;
+        for (int i = lane / 8; i < rows * 6; i += 4) {
+          const int box = i / rows;
+          *reinterpret_cast<uint4*>(from + box * 8192 + (i - box * rows) * 128) = make_uint4(0, 0, 0, 0);
+        }
         asm volatile("fence.proxy.async;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&full[st]), 0));
@@ -462,120 +528,126 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     constexpr int kPieceRow = 32 * static_cast<int>(sizeof(OutT));  // bytes of a column's 32 lanes
     OutT* out = static_cast<OutT*>(args.out);
     uint8_t* piece = pieces_out + (warp - 4) * kGgPiece;
-    uint32_t count = 0;
+    uint32_t uses[2] = {0, 0};
+    bool ok = true;
     // where this thread's row of a matrix starts (stmatrix), and its element of a row (lane): the 16-byte chunks of
     // 64-byte rows are swizzled
     const uint32_t st_row = lane & 7, st_at = st_row * 64 + ((lane >> 3) ^ (st_row >> 1 & 3)) * 16;
-    for (int tile = pair; tile < tiles; tile += npairs) {
+    for (int tile = pair; tile < tiles && ok; tile += npairs) {
       const GroupedTile t = sched.get(tile);
-      const int f0 = t.lane0 + static_cast<int>(rank) * 128 + q * 32, f = f0 + lane;
-      const bool there = f < args.lanes;
       int64_t at = (t.row0 * args.ld_out);
       if (kDw) at = (static_cast<int64_t>(t.e) * args.cols + t.col0) * args.ld_out;
       // this warp's columns: even shares of what there is, in whole pieces of 32
       const int share = (t.ncols + 63) / 64 * 32;
       const int from = part * share, to = part ? t.ncols : min(share, t.ncols);
-      OutT* p = out + at + f;
-      if (t.kblocks == 0) {  // an expert without rows: dW = 0
-        if (there)
-          for (int c = from; c < to; ++c) p[c * args.ld_out] = gg_cast<OutT>(0.0f);
-        continue;
-      }
-      const int slot = count & 1;
-      if (!gg_warp_wait(&tfull[slot], (count >> 1) & 1u, abort_flag, args.status, lane)) break;
-      ++count;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(slot * 256);
-      auto release = [&]() {  // this warp's part of the accumulator is read
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) gg_arrive(mapa_shared(smem_u32(&tempty[slot]), 0));
-      };
-      float ws[4], bias[4];
-      if constexpr (kInt8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int fi = kWide ? f : f0 + i * 8 + lane / 4;
-          ws[i] = fi < args.lanes ? args.lane_scale[fi] : 0.0f;
-          bias[i] = fi < args.lanes && args.bias ? args.bias[fi] : 0.0f;
-        }
-      }
-      if (from >= to) release();
 #pragma unroll 1
-      for (int c0 = from; c0 < to; c0 += 32) {
-        uint32_t r[32];
-        if constexpr (kWide) {
-          tmem_ld_32x32b_x32(taddr + c0, r);
-        } else {
-          tmem_ld_16x256b_x4(taddr + c0, r);
-          tmem_ld_16x256b_x4(taddr + (16u << 16) + c0, r + 16);
+      for (int half = 0; half < t.halves; ++half) {
+        const int f0 = t.lane0 + half * kGgHalf + static_cast<int>(rank) * 128 + q * 32, f = f0 + lane;
+        const bool there = f < args.lanes;
+        OutT* p = out + at + f;
+        if (t.kblocks == 0) {  // an expert without rows: dW = 0
+          if (there)
+            for (int c = from; c < to; ++c) p[c * args.ld_out] = gg_cast<OutT>(0.0f);
+          continue;
         }
-        tmem_ld_wait();
-        if (c0 + 32 >= to) release();
+        if (!gg_warp_wait(&tfull[half], uses[half] & 1u, abort_flag, args.status, lane)) {
+          ok = false;
+          break;
+        }
+        ++uses[half];
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * 256);
+        auto release = [&]() {  // this warp's part of the accumulator is read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) gg_arrive(mapa_shared(smem_u32(&tempty[half]), 0));
+        };
+        float ws[4], bias[4];
+        if constexpr (kInt8) {
 #pragma unroll
-        for (int k = 0; k < 32 / kPieceCols; ++k) {
-          const int c1 = c0 + k * kPieceCols;
-          if (c1 >= to) break;
-          __syncwarp();  // the last piece has been copied
+          for (int i = 0; i < 4; ++i) {
+            const int fi = kWide ? f : f0 + i * 8 + lane / 4;
+            ws[i] = fi < args.lanes ? args.lane_scale[fi] : 0.0f;
+            bias[i] = fi < args.lanes && args.bias ? args.bias[fi] : 0.0f;
+          }
+        }
+        if (from >= to) release();
+#pragma unroll 1
+        for (int c0 = from; c0 < to; c0 += 32) {
+          uint32_t r[32];
           if constexpr (kWide) {
-#pragma unroll
-            for (int j = 0; j < kPieceCols; ++j) {
-              float v = __uint_as_float(r[k * kPieceCols + j]);
-              if constexpr (kInt8) {
-                const float xs = c1 + j < t.ncols ? __ldg(args.col_scale + t.row0 + c1 + j) : 0.0f;
-                v = static_cast<float>(static_cast<int>(r[k * kPieceCols + j])) * xs * ws[0] + bias[0];
-              }
-              reinterpret_cast<float*>(piece)[j * 32 + lane] = v;
-            }
+            tmem_ld_32x32b_x32(taddr + c0, r);
           } else {
+            tmem_ld_16x256b_x4(taddr + c0, r);
+            tmem_ld_16x256b_x4(taddr + (16u << 16) + c0, r + 16);
+          }
+          tmem_ld_wait();
+          if (c0 + 32 >= to) release();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // 8 columns
-              uint32_t m[4];               // matrices of 8 lanes
-              float xs[2];
-              if constexpr (kInt8) {
+          for (int k = 0; k < 32 / kPieceCols; ++k) {
+            const int c1 = c0 + k * kPieceCols;
+            if (c1 >= to) break;
+            __syncwarp();  // the last piece has been copied
+            if constexpr (kWide) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  const int c = c1 + i * 8 + lane % 4 * 2 + j;
-                  xs[j] = c < t.ncols ? __ldg(args.col_scale + t.row0 + c) : 0.0f;
+              for (int j = 0; j < kPieceCols; ++j) {
+                float v = __uint_as_float(r[k * kPieceCols + j]);
+                if constexpr (kInt8) {
+                  const float xs = c1 + j < t.ncols ? __ldg(args.col_scale + t.row0 + c1 + j) : 0.0f;
+                  v = static_cast<float>(static_cast<int>(r[k * kPieceCols + j])) * xs * ws[0] + bias[0];
+                }
+                reinterpret_cast<float*>(piece)[j * 32 + lane] = v;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {  // 8 columns
+                uint32_t m[4];               // matrices of 8 lanes
+                float xs[2];
+                if constexpr (kInt8) {
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) {
+                    const int c = c1 + i * 8 + lane % 4 * 2 + j;
+                    xs[j] = c < t.ncols ? __ldg(args.col_scale + t.row0 + c) : 0.0f;
+                  }
+                }
+#pragma unroll
+                for (int l = 0; l < 4; ++l) {
+                  const uint32_t* v = r + (l >> 1) * 16 + i * 4 + (l & 1) * 2;
+                  if constexpr (kInt8)
+                    m[l] = gg_pack<OutT>(static_cast<float>(static_cast<int>(v[0])) * xs[0] * ws[l] + bias[l],
+                                         static_cast<float>(static_cast<int>(v[1])) * xs[1] * ws[l] + bias[l]);
+                  else
+                    m[l] = gg_pack<OutT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
+                }
+                stmatrix_x4_trans(smem_u32(piece) + i * 512 + st_at, m[0], m[1], m[2], m[3]);
+              }
+            }
+            __syncwarp();
+            const int n = min(kPieceCols, to - c1);
+            if (args.out16) {
+              constexpr int kRowLanes = kPieceRow / 16, kPer = 32 / kRowLanes;  // threads of a row, rows at a time
+              constexpr int kElts = 16 / static_cast<int>(sizeof(OutT));
+              const int row = lane / kRowLanes, chunk = lane % kRowLanes;
+              if (f0 + chunk * kElts < args.lanes) {
+                OutT* o = out + at + f0 + chunk * kElts + (c1 + row) * args.ld_out;
+#pragma unroll
+                for (int j = 0; j < kPieceCols / kPer; ++j) {
+                  const int rj = row + j * kPer;
+                  const int byte = rj * kPieceRow + (kWide ? chunk : chunk ^ (rj >> 1 & 3)) * 16;
+                  if (rj < n) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(piece + byte);
+                  o += kPer * args.ld_out;
                 }
               }
-#pragma unroll
-              for (int l = 0; l < 4; ++l) {
-                const uint32_t* v = r + (l >> 1) * 16 + i * 4 + (l & 1) * 2;
-                if constexpr (kInt8)
-                  m[l] = gg_pack<OutT>(static_cast<float>(static_cast<int>(v[0])) * xs[0] * ws[l] + bias[l],
-                                       static_cast<float>(static_cast<int>(v[1])) * xs[1] * ws[l] + bias[l]);
-                else
-                  m[l] = gg_pack<OutT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
-              }
-              stmatrix_x4_trans(smem_u32(piece) + i * 512 + st_at, m[0], m[1], m[2], m[3]);
-            }
-          }
-          __syncwarp();
-          const int n = min(kPieceCols, to - c1);
-          if (args.out16) {
-            constexpr int kRowLanes = kPieceRow / 16, kPer = 32 / kRowLanes;  // threads of a row, rows at a time
-            constexpr int kElts = 16 / static_cast<int>(sizeof(OutT));
-            const int row = lane / kRowLanes, chunk = lane % kRowLanes;
-            if (f0 + chunk * kElts < args.lanes) {
-              OutT* o = out + at + f0 + chunk * kElts + (c1 + row) * args.ld_out;
-#pragma unroll
-              for (int j = 0; j < kPieceCols / kPer; ++j) {
-                const int rj = row + j * kPer;
-                const int byte = rj * kPieceRow + (kWide ? chunk : chunk ^ (rj >> 1 & 3)) * 16;
-                if (rj < n) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(piece + byte);
-                o += kPer * args.ld_out;
+            } else {
+              OutT* o = p + c1 * args.ld_out;
+              for (int j = 0; j < n; ++j, o += args.ld_out) {
+                const int byte = kWide ? j * 128 + lane * 4 : j * 64 + ((lane >> 3) ^ (j >> 1 & 3)) * 16 + (lane & 7) * 2;
+                if (there) *o = *reinterpret_cast<const OutT*>(piece + byte);
               }
             }
-          } else {
-            OutT* o = p + c1 * args.ld_out;
-            for (int j = 0; j < n; ++j, o += args.ld_out) {
-              const int byte = kWide ? j * 128 + lane * 4 : j * 64 + ((lane >> 3) ^ (j >> 1 & 3)) * 16 + (lane & 7) * 2;
-              if (there) *o = *reinterpret_cast<const OutT*>(piece + byte);
-            }
           }
+          __syncwarp();  // the next read of TMEM is the whole warp's
         }
-        __syncwarp();  // the next read of TMEM is the whole warp's
       }
     }
     if (!kDw && args.zero_rest) {
