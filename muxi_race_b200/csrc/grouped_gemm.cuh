@@ -29,7 +29,8 @@
 //
 // Epilogue: a warp alone on its scheduler issues an instruction every four to five cycles, so what counts is how few there
 // are. 16-bit results are read from TMEM as 8 x 8 fragments, packed in pairs of columns, stored transposed to shared
-// memory by stmatrix (4 packs and one store for 256 elements) and copied from there 16 bytes at a time.
+// memory by stmatrix (4 packs and one store for 256 elements) and copied from there 16 bytes at a time. dW of 256 experts with
+// 128 rows (7168 x 2048 bf16), where nothing hides the stores: 3090 us with an element of each lane at a time.
 //
 // Roles per CTA (384 threads): warp 0 TMA producer, warp 1 MMA issuer (the pair's leader), warp 2 the tile table,
 // warp 3 the clearing of Dw's tails, warps 4-11 epilogue. Every wait is bounded; the final cluster barrier is
@@ -58,8 +59,7 @@ constexpr int kGgThreads = 128 + 32 * kGgEpiWarps;
 constexpr int kGgBand = 8;  // column tiles that take turns on a weight tile
 constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiples of 32
 constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
-constexpr int kGgPiece = 2048;  // an epilogue warp's staging: 32 lanes of 32 columns (16 bits) or of 16 (32 bits)
-constexpr int kGgOutBytes = kGgEpiWarps * kGgPiece;
+constexpr int kGgOutBytes = kGgEpiWarps * 2048;  // the epilogue's staging
 constexpr int kGgSmemBytes = 1024 + kGgStages * kGgStageBytes + kGgOutBytes + 256 + kGgTableInts * 4;
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
@@ -229,6 +229,28 @@ __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* r) 
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
+// Two warps meet, and learn whether all of their threads say yes.
+__device__ __forceinline__ bool gg_pair_and(int id, bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(all)
+      : "r"(id), "r"(static_cast<uint32_t>(yes))
+      : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ void gg_pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+// 16 bytes; STREAM: of a result that is not read soon.
+template <bool STREAM> __device__ __forceinline__ void gg_store16(void* to, uint4 v) {
+  if constexpr (STREAM)
+    __stcs(reinterpret_cast<uint4*>(to), v);
+  else
+    *reinterpret_cast<uint4*>(to) = v;
+}
+
 // Four 8 x 8 matrices of 16-bit elements, transposed: thread t gives the address of row t % 8 of matrix t / 8.
 __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
@@ -524,15 +546,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     // ---------------------------------------------------------------- epilogue
     const int q = warp & 3, part = (warp - 4) >> 2;  // lane quadrant, half of the columns
     constexpr bool kWide = sizeof(OutT) == 4;
-    constexpr int kPieceCols = kGgPiece / (32 * static_cast<int>(sizeof(OutT)));
-    constexpr int kPieceRow = 32 * static_cast<int>(sizeof(OutT));  // bytes of a column's 32 lanes
+    constexpr int kPieceCols = kWide ? 16 : 32;
+    // Staging of a piece, rows of 128 bytes: a warp's 32 lanes of 32 bits, or the 64 lanes of 16 bits of two neighbouring
+    // warps, which write and copy it together (stores of whole 128-byte lines: dW of 256 experts with 128 rows 1870 us in
+    // half lines). 16-byte chunk c of row j is at c ^ (j % 8) for the 64-lane rows.
     OutT* out = static_cast<OutT*>(args.out);
-    uint8_t* piece = pieces_out + (warp - 4) * kGgPiece;
-    uint32_t uses[2] = {0, 0};
+    uint8_t* piece = pieces_out + (kWide ? warp - 4 : (warp - 4) >> 1) * (kWide ? 2048 : 4096);
+    const int pair_id = 1 + ((warp - 4) >> 1), side = q & 1;
+    uint32_t uses = 0;  // parity of each half's next wait
     bool ok = true;
-    // where this thread's row of a matrix starts (stmatrix), and its element of a row (lane): the 16-byte chunks of
-    // 64-byte rows are swizzled
-    const uint32_t st_row = lane & 7, st_at = st_row * 64 + ((lane >> 3) ^ (st_row >> 1 & 3)) * 16;
+    const uint32_t st_row = lane & 7;  // where this thread's row of a matrix starts (stmatrix)
+    const uint32_t st_at = st_row * 128 + (((side * 4 + (lane >> 3)) ^ st_row) << 4);
     for (int tile = pair; tile < tiles && ok; tile += npairs) {
       const GroupedTile t = sched.get(tile);
       int64_t at = (t.row0 * args.ld_out);
@@ -550,11 +574,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
             for (int c = from; c < to; ++c) p[c * args.ld_out] = gg_cast<OutT>(0.0f);
           continue;
         }
-        if (!gg_warp_wait(&tfull[half], uses[half] & 1u, abort_flag, args.status, lane)) {
-          ok = false;
-          break;
-        }
-        ++uses[half];
+        ok = gg_warp_wait(&tfull[half], uses >> half & 1u, abort_flag, args.status, lane);
+        if constexpr (!kWide) ok = gg_pair_and(pair_id, ok);  // both or none: they meet again below
+        if (!ok) break;
+        uses ^= 1u << half;
         tc_fence_after();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * 256);
         auto release = [&]() {  // this warp's part of the accumulator is read
@@ -587,7 +610,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           for (int k = 0; k < 32 / kPieceCols; ++k) {
             const int c1 = c0 + k * kPieceCols;
             if (c1 >= to) break;
-            __syncwarp();  // the last piece has been copied
+            // the last piece has been copied
+            if constexpr (kWide)
+              __syncwarp();
+            else
+              gg_pair_sync(pair_id);
             if constexpr (kWide) {
 #pragma unroll
               for (int j = 0; j < kPieceCols; ++j) {
@@ -619,30 +646,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
                   else
                     m[l] = gg_pack<OutT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
                 }
-                stmatrix_x4_trans(smem_u32(piece) + i * 512 + st_at, m[0], m[1], m[2], m[3]);
+                stmatrix_x4_trans(smem_u32(piece) + i * 1024 + st_at, m[0], m[1], m[2], m[3]);
               }
             }
-            __syncwarp();
             const int n = min(kPieceCols, to - c1);
-            if (args.out16) {
-              constexpr int kRowLanes = kPieceRow / 16, kPer = 32 / kRowLanes;  // threads of a row, rows at a time
-              constexpr int kElts = 16 / static_cast<int>(sizeof(OutT));
-              const int row = lane / kRowLanes, chunk = lane % kRowLanes;
-              if (f0 + chunk * kElts < args.lanes) {
-                OutT* o = out + at + f0 + chunk * kElts + (c1 + row) * args.ld_out;
+            if constexpr (kWide)
+              __syncwarp();
+            else
+              gg_pair_sync(pair_id);
+            constexpr int kElts = 16 / static_cast<int>(sizeof(OutT));
+            const int p0 = kWide ? f0 : f0 - side * 32;  // the piece's first lane
+            if (args.out16) {  // 8 threads a row, 4 rows at a time
+              const int row = (kWide ? 0 : side * 16) + lane / 8, chunk = lane % 8;
+              if (p0 + chunk * kElts < args.lanes) {
+                OutT* o = out + at + p0 + chunk * kElts + (c1 + row) * args.ld_out;
 #pragma unroll
-                for (int j = 0; j < kPieceCols / kPer; ++j) {
-                  const int rj = row + j * kPer;
-                  const int byte = rj * kPieceRow + (kWide ? chunk : chunk ^ (rj >> 1 & 3)) * 16;
-                  if (rj < n) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(piece + byte);
-                  o += kPer * args.ld_out;
+                for (int j = 0; j < 4; ++j) {
+                  const int rj = row + j * 4;
+                  const int byte = rj * 128 + (kWide ? chunk : chunk ^ (rj & 7)) * 16;
+                  if (rj < n) gg_store16<kDw>(o, *reinterpret_cast<const uint4*>(piece + byte));
+                  o += 4 * args.ld_out;
                 }
               }
             } else {
-              OutT* o = p + c1 * args.ld_out;
-              for (int j = 0; j < n; ++j, o += args.ld_out) {
-                const int byte = kWide ? j * 128 + lane * 4 : j * 64 + ((lane >> 3) ^ (j >> 1 & 3)) * 16 + (lane & 7) * 2;
-                if (there) *o = *reinterpret_cast<const OutT*>(piece + byte);
+              for (int j = kWide ? 0 : side * 16; j < min(n, kWide ? 16 : side * 16 + 16); ++j) {
+                for (int l = lane; l < (kWide ? 32 : 64); l += 32) {
+                  const int byte = j * 128 + (kWide ? l * 4 : ((l >> 3) ^ (j & 7)) * 16 + (l & 7) * 2);
+                  if (p0 + l < args.lanes)
+                    out[at + p0 + l + (c1 + j) * args.ld_out] = *reinterpret_cast<const OutT*>(piece + byte);
+                }
               }
             }
           }
