@@ -147,6 +147,13 @@ int encode_map(CUtensorMap* map, const void* base, int elt_bytes, int rank, cons
   }();
   CUresult r = enc(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread's first CUDA call, as in a backward pass: bind the device's context
+    int dev;
+    MOE_CUDA(cudaGetDevice(&dev));
+    MOE_CUDA(cudaSetDevice(dev));
+    r = enc(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
   if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with %d", what, (int)r);
   return MOE_OK;
 }
