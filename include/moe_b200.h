@@ -619,9 +619,11 @@ MOE_API int moe_combine_rows(const void* y, const int32_t* slot, void* out, int6
  * (pitch ld_out) MOE_F16, MOE_BF16 or MOE_F32; bias [N] fp32 or NULL. The sum is exact (int32); scales and bias in fp32.
  * Requirements: K a multiple of 16 below 131072; x and w on 16-byte boundaries, ld_x a multiple of 16.
  * ---------------------------------------------------------------------------------------- */
+MOE_API size_t moe_int8_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
 MOE_API int moe_int8_linear(const void* x, int64_t ld_x, const float* x_scale, const void* w, const float* w_scale,
                             const float* bias, void* out, int64_t ld_out, int out_dtype, int64_t m, int64_t n, int64_t k,
-                            void* stream);
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -66,7 +66,9 @@ SIGNATURES = {
         + [_i64, _i64, _int, _c_void_p],
     ),
     "moe_combine_rows": (_int, [_c_void_p] * 3 + [_i64] * 4 + [_int, _c_void_p]),
-    "moe_int8_linear": (_int, [_c_void_p, _i64] + [_c_void_p] * 5 + [_i64, _int] + [_i64] * 3 + [_c_void_p]),
+    "moe_int8_linear_workspace_bytes": (_size, [_i64] * 3),
+    "moe_int8_linear": (
+        _int, [_c_void_p, _i64] + [_c_void_p] * 5 + [_i64, _int] + [_i64] * 3 + [_c_void_p, _size, _c_void_p]),
     "moe_w4_quantize": (_int, [_c_void_p, _int, _i64, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "moe_w4_packed_bytes": (_size, [_i64, _i64, _i64, _int, _int, _int]),
     "moe_w4_pack": (_int, [_c_void_p] * 3 + [_i64] * 3 + [_int, _int, _c_void_p, _size, _c_void_p]),

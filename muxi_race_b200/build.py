@@ -26,7 +26,7 @@ SOURCES = {
     "norm_capi.cu": ["rms_norm.cuh"],
     "route_capi.cu": ["route_topk.cuh", "sm100_ptx.cuh"],
     "w4_capi.cu": ["w4_gemv.cuh", "sm100_ptx.cuh"],
-    "grouped_capi.cu": ["grouped_gemm.cuh", "sm100_ptx.cuh"],
+    "grouped_capi.cu": ["grouped_gemm.cuh", "int8_stream.cuh", "sm100_ptx.cuh"],
     "rows8_capi.cu": ["rows8.cuh"],
 }
 GENCODE = "arch=compute_100a,code=sm_100a"

@@ -47,9 +47,9 @@ namespace moe {
 
 enum GroupedKind : int { kGroupedY = 0, kGroupedDx = 1, kGroupedDw = 2, kDenseInt8 = 3 };
 
-constexpr int kGgStages = 4;
 constexpr int kGgOperandBytes = 128 * 128;  // 128 lanes or columns of an operand, per CTA and stage
-constexpr int kGgStageBytes = 3 * kGgOperandBytes;  // two halves of lanes, columns
+constexpr int kGgRingBytes = 12 * kGgOperandBytes;  // 4 stages of two halves of lanes and the columns, 6 of one half
+constexpr int kGgMaxStages = 6;
 constexpr int kGgHalf = 256;                // lanes of a pair's MMA
 constexpr int kGgTile = 256;                // columns at most
 constexpr int kGgAhead = 3;                 // blocks that one half may be ahead of the other
@@ -60,11 +60,11 @@ constexpr int kGgBand = 8;  // column tiles that take turns on a weight tile
 constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiples of 32
 constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
 constexpr int kGgOutBytes = kGgEpiWarps * 2048;  // the epilogue's staging
-constexpr int kGgSmemBytes = 1024 + kGgStages * kGgStageBytes + kGgOutBytes + 256 + kGgTableInts * 4;
+constexpr int kGgSmemBytes = 1024 + kGgRingBytes + kGgOutBytes + 256 + kGgTableInts * 4;
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
 struct GroupedArgs {
-  const void* offsets;   // [E + 1] int32 / int64; null: one group of all rows
+  const void* offsets;   // [E + 1] int32 / int64; int8: unused
   int offsets64;
   int E;
   int64_t rows;          // R
@@ -76,6 +76,7 @@ struct GroupedArgs {
   int64_t ld_out;
   int zero_rest;         // rows of no group are cleared
   int out16;             // out's rows start on 16 bytes, and lanes come in whole 16 bytes
+  int split, split_blocks;  // int8: slices of the reduction, blocks of each; slice i writes rows [i rows, (i + 1) rows)
   const float* lane_scale;  // int8: ws
   const float* col_scale;   // int8: xs
   const float* bias;        // int8, or null
@@ -83,6 +84,7 @@ struct GroupedArgs {
 };
 
 template <typename OutT> __device__ __forceinline__ OutT gg_cast(float v);
+template <> __device__ __forceinline__ int gg_cast<int>(float v) { return __float_as_int(v); }  // a sum's bits
 template <> __device__ __forceinline__ float gg_cast<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half gg_cast<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 gg_cast<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
@@ -139,7 +141,7 @@ __device__ __forceinline__ bool elect_one() {
 struct GroupedTile {
   int e, lane0, halves, ncols;
   int64_t row0;
-  int col0, kblocks, tail;  // tail: reduction rows or elements in the last block (0: it is full)
+  int col0, kb0, kblocks, tail;  // tail: reduction rows or elements in the last block (0: it is full)
 };
 
 __device__ __forceinline__ int gg_col_step(int rows) {  // columns per tile of a group: even shares of at most 256
@@ -148,12 +150,15 @@ __device__ __forceinline__ int gg_col_step(int rows) {  // columns per tile of a
   return (share + kGgColStep - 1) / kGgColStep * kGgColStep;
 }
 
+// Tiles go round the pairs. What is left for a last round that would not fill them is cut into halves of the lanes and
+// shares of the columns, as many as there are pairs for.
 template <int KIND>
 struct GroupedSchedule {
   const int *prefix, *start, *rows;  // tiles before group e, its first row, its rows
-  int E, lanes, tile_lanes, lane_tiles, red_blocks, red_tail, cols, e;
+  int E, lanes, tile_lanes, lane_tiles, red_blocks, red_tail, cols, split_blocks, e;
+  int whole, left, lane_parts, col_parts;  // tiles of whole rounds; the others, and what each is cut into
 
-  __device__ GroupedSchedule(const GroupedArgs& a, const int* table) {
+  __device__ GroupedSchedule(const GroupedArgs& a, const int* table, int npairs) {
     prefix = table;
     start = table + kGgMaxExperts + 1;
     rows = start + kGgMaxExperts;
@@ -164,17 +169,29 @@ struct GroupedSchedule {
     constexpr int kRed = KIND == kDenseInt8 ? 128 : 64;
     red_blocks = (a.red + kRed - 1) / kRed;
     red_tail = a.red % kRed;
+    split_blocks = KIND == kDenseInt8 ? a.split_blocks : red_blocks;
     cols = a.cols;
     e = 0;
+    left = prefix[E] % npairs;
+    whole = prefix[E] - left;
+    lane_parts = col_parts = 1;
+    if (a.halves == 2 && left * 2 <= npairs) lane_parts = 2;
+    while (col_parts < 4 && left * lane_parts * col_parts * 2 <= npairs) col_parts *= 2;
   }
-  __device__ int tiles() const { return prefix[E]; }
-  // Tiles are asked for in rising order.
-  __device__ GroupedTile get(int tile) {
-    while (tile >= prefix[e + 1]) ++e;
+  __device__ int tiles() const { return whole + left * lane_parts * col_parts; }
+  // Tiles are asked for in rising order. One without columns is to be passed over.
+  __device__ GroupedTile get(int i) {
+    int part = -1;
+    if (i >= whole && lane_parts * col_parts > 1) {
+      part = (i - whole) % (lane_parts * col_parts);
+      i = whole + (i - whole) / (lane_parts * col_parts);
+    }
+    while (i >= prefix[e + 1]) ++e;
     GroupedTile t;
     t.e = e;
-    int i = tile - prefix[e];
+    i -= prefix[e];
     const int n = rows[e];
+    t.kb0 = 0;
     if (KIND == kGroupedDw) {
       const int col_tiles = (cols + kGgTile - 1) / kGgTile;
       t.lane0 = i / col_tiles * tile_lanes;
@@ -195,8 +212,27 @@ struct GroupedSchedule {
       t.col0 = 0;
       t.kblocks = red_blocks;
       t.tail = red_tail;
+      if (KIND == kDenseInt8) {  // group e is a slice of the reduction
+        t.kb0 = e * split_blocks;
+        t.kblocks = min(split_blocks, red_blocks - t.kb0);
+        if (e < E - 1) t.tail = 0;
+      }
     }
     t.halves = min(tile_lanes, lanes - t.lane0) > kGgHalf ? 2 : 1;
+    if (part >= 0) {
+      if (lane_parts == 2) {
+        if (part % 2 == 1 && t.halves == 1) t.ncols = 0;
+        t.lane0 += part % 2 * kGgHalf;
+        t.halves = 1;
+      }
+      const int share = ((t.ncols + col_parts - 1) / col_parts + kGgColStep - 1) / kGgColStep * kGgColStep;
+      const int c = part / lane_parts * share;
+      t.ncols = max(0, min(share, t.ncols - c));
+      if (KIND == kGroupedDw)
+        t.col0 += c;
+      else
+        t.row0 += c;
+    }
     return t;
   }
 };
@@ -263,12 +299,17 @@ __device__ __forceinline__ void gg_build_table(const GroupedArgs& a, int* table,
     int n = 0, tiles = 0;
     if (e < a.E) {
       int64_t s = 0, t = a.rows;
-      if (a.offsets != nullptr) {
+      if (KIND == kDenseInt8) {  // the slices' rows, one after another
+        s = e * a.rows;
+        t = s + a.rows;
+      } else {
         s = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[e] : static_cast<const int32_t*>(a.offsets)[e];
         t = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[e + 1] : static_cast<const int32_t*>(a.offsets)[e + 1];
       }
-      s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
-      t = t < s ? s : (t > a.rows ? a.rows : t);
+      if (KIND != kDenseInt8) {
+        s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
+        t = t < s ? s : (t > a.rows ? a.rows : t);
+      }
       n = static_cast<int>(t - s);
       start[e] = static_cast<int>(s);
       rows[e] = n;
@@ -300,17 +341,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
                         const __grid_constant__ CUtensorMap tmB32, const GroupedArgs args) {
   constexpr bool kDw = KIND == kGroupedDw;
   constexpr bool kInt8 = KIND == kDenseInt8;
+  constexpr bool kScaled = kInt8 && !std::is_same<OutT, int>::value;  // int: a slice's sums as they are
   constexpr bool kMnA = KIND == kGroupedDx || kDw;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kRed = kInt8 ? 128 : 64;   // reduction elements per block
   constexpr int kMmaRed = kInt8 ? 32 : 16;  // and per MMA
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* pieces_out = smem + kGgStages * kGgStageBytes;
+  uint8_t* pieces_out = smem + kGgRingBytes;
+  const int stages = args.halves == 2 ? 4 : 6, stage_bytes = (args.halves + 1) * kGgOperandBytes;
+  const int b_at = args.halves * kGgOperandBytes;  // of a stage: the columns
   uint64_t* full = reinterpret_cast<uint64_t*>(pieces_out + kGgOutBytes);  // leader's: both CTAs' producers
-  uint64_t* empty = full + kGgStages;
-  uint64_t* landed = empty + kGgStages;  // Dw's tails: this CTA's own copies
-  uint64_t* tfull = landed + kGgStages;
+  uint64_t* empty = full + kGgMaxStages;
+  uint64_t* landed = empty + kGgMaxStages;  // Dw's tails: this CTA's own copies
+  uint64_t* tfull = landed + kGgMaxStages;
   uint64_t* tempty = tfull + 2;          // leader's: the epilogue warps of both CTAs
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -323,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   const int pair = static_cast<int>(cluster_id_x()), npairs = static_cast<int>(cluster_count_x());
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kGgStages; ++s) {
+    for (int s = 0; s < kGgMaxStages; ++s) {
       mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
       mbar_init(&landed[s], 1);
@@ -348,7 +392,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  GroupedSchedule<KIND> sched(args, table);
+  GroupedSchedule<KIND> sched(args, table, npairs);
   const int tiles = sched.tiles();
 
   if (warp == 0) {
@@ -363,6 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += npairs) {
         const GroupedTile t = sched.get(tile);
+        if (t.ncols == 0) continue;
         const int half = (t.ncols + kGgColStep - 1) / kGgColStep * (kGgColStep / 2);  // columns that this CTA brings
         const int lane0 = t.lane0 + static_cast<int>(rank) * 128;
         const int boxes = half <= 96 ? (half + 31) / 32 : 0;  // 32-row boxes; 0: one of 128
@@ -371,8 +416,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
             ok = false;
             break;
           }
-          uint8_t* a = smem + st * kGgStageBytes;
-          uint8_t* b = a + 2 * kGgOperandBytes;
+          uint8_t* a = smem + st * stage_bytes;
+          uint8_t* b = a + b_at;
           const uint32_t bar = mapa_shared(smem_u32(&full[st]), 0);
           if (elect_one()) {
             if constexpr (kDw) {
@@ -391,21 +436,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
                   tma_load_2d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, row, pol);
               }
             } else {
-              const int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half;
+              int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half, z = t.e;
+            const int k0 = (t.kb0 + kb) * kRed;
+            if constexpr (kInt8) {
+              row -= t.e * static_cast<int>(args.rows);
+              z = 0;
+            }
               mbar_arrive_expect_tx_cluster(bar, t.halves * kGgOperandBytes + (boxes ? boxes * 4096 : kGgOperandBytes));
               if constexpr (kMnA) {
                 for (int c = 0; c < 2 * t.halves; ++c)
-                  tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, kb * kRed, t.e, pol);
+                  tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, k0, z, pol);
               } else {
                 for (int h = 0; h < t.halves; ++h)
-                  tma_load_3d_pair(a + h * kGgOperandBytes, &tmA, bar, kb * kRed, lane0 + h * kGgHalf, t.e, pol);
+                  tma_load_3d_pair(a + h * kGgOperandBytes, &tmA, bar, k0, lane0 + h * kGgHalf, z, pol);
               }
-              if (boxes == 0) tma_load_2d_pair(b, &tmB, bar, kb * kRed, row, pol);
-              for (int i = 0; i < boxes; ++i) tma_load_2d_pair(b + i * 4096, &tmB32, bar, kb * kRed, row + i * 32, pol);
+              if (boxes == 0) tma_load_2d_pair(b, &tmB, bar, k0, row, pol);
+              for (int i = 0; i < boxes; ++i) tma_load_2d_pair(b + i * 4096, &tmB32, bar, k0, row + i * 32, pol);
             }
           }
           __syncwarp();
-          if (++st == kGgStages) {
+          if (++st == stages) {
             st = 0;
             ph ^= 1u;
           }
@@ -421,7 +471,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += npairs) {
         const GroupedTile t = sched.get(tile);
-        if (t.kblocks == 0) continue;
+        if (t.kblocks == 0 || t.ncols == 0) continue;
         if (!gg_all(mbar_wait(&tempty[0], (uses[0] & 1u) ^ 1u, abort_flag, args.status))) break;
         ++uses[0];
         tc_fence_after();
@@ -432,8 +482,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         else
           idesc = idesc_f16(kBf16, 256, n) | (kMnA ? 1u << 15 : 0u) | (kDw ? 1u << 16 : 0u);
         auto mmas = [&](int stage, int half, int kb) {
-          const uint32_t a = smem_u32(smem + stage * kGgStageBytes) + half * kGgOperandBytes;
-          const uint32_t b = smem_u32(smem + stage * kGgStageBytes) + 2 * kGgOperandBytes;
+          const uint32_t a = smem_u32(smem + stage * stage_bytes) + half * kGgOperandBytes;
+          const uint32_t b = smem_u32(smem + stage * stage_bytes) + b_at;
           const uint32_t d = tmem_base + static_cast<uint32_t>(half * 256);
           const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
           if (elect_one()) {
@@ -479,13 +529,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           // the second half follows at once, but at the tile's end after the first, whose stores can then begin
           if (t.halves == 1 || (second && (last || kb < t.kblocks - kGgAhead || held == kGgAhead))) {
             for (; held > 0; --held) {
-              const int back = held - 1, stage = st >= back ? st - back : st - back + kGgStages;
+              const int back = held - 1, stage = st >= back ? st - back : st - back + stages;
               if (t.halves == 2) mmas(stage, 1, kb - back);
               if (elect_one()) tc_commit_pair(&empty[stage], 0x3);
               __syncwarp();
             }
           }
-          if (++st == kGgStages) {
+          if (++st == stages) {
             st = 0;
             ph ^= 1u;
           }
@@ -507,14 +557,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
       uint32_t blocks = 0, phases = 0;  // blocks taken so far; one parity bit per stage
       for (int tile = pair; tile < tiles; tile += npairs) {
         const GroupedTile t = sched.get(tile);
+        if (t.ncols == 0) continue;
         blocks += static_cast<uint32_t>(t.kblocks);
         if (t.tail % 16 == 0) continue;
-        const int st = static_cast<int>((blocks - 1) % kGgStages);
+        const int st = static_cast<int>((blocks - 1) % stages);
         if (!gg_all(mbar_wait(&landed[st], (phases >> st) & 1u, abort_flag, args.status))) break;
         phases ^= 1u << st;
-        const int rows = 16 - t.tail % 16;  // to clear, in each of the stage's six boxes of 64 rows
-        uint8_t* from = smem + st * kGgStageBytes + t.tail * 128 + lane % 8 * 16;
-        for (int i = lane / 8; i < rows * 6; i += 4) {
+        const int rows = 16 - t.tail % 16;  // to clear, in each of the stage's boxes of 64 rows
+        uint8_t* from = smem + st * stage_bytes + t.tail * 128 + lane % 8 * 16;
+        for (int i = lane / 8; i < rows * (args.halves + 1) * 2; i += 4) {
           const int box = i / rows;
           *reinterpret_cast<uint4*>(from + box * 8192 + (i - box * rows) * 128) = make_uint4(0, 0, 0, 0);
         }
@@ -540,6 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     const uint32_t st_at = st_row * 128 + (((side * 4 + (lane >> 3)) ^ st_row) << 4);
     for (int tile = pair; tile < tiles && ok; tile += npairs) {
       const GroupedTile t = sched.get(tile);
+      if (t.ncols == 0) continue;
       int64_t at = (t.row0 * args.ld_out);
       if (kDw) at = (static_cast<int64_t>(t.e) * args.cols + t.col0) * args.ld_out;
       // this warp's columns: even shares of what there is, in whole pieces of 32
@@ -567,7 +619,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           if (lane == 0) gg_arrive(mapa_shared(smem_u32(&tempty[half]), 0));
         };
         float ws[4], bias[4];
-        if constexpr (kInt8) {
+        if constexpr (kScaled) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int fi = kWide ? f : f0 + i * 8 + lane / 4;
@@ -600,18 +652,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
 #pragma unroll
               for (int j = 0; j < kPieceCols; ++j) {
                 float v = __uint_as_float(r[k * kPieceCols + j]);
-                if constexpr (kInt8) {
+                if constexpr (kScaled) {
                   const float xs = c1 + j < t.ncols ? __ldg(args.col_scale + t.row0 + c1 + j) : 0.0f;
                   v = static_cast<float>(static_cast<int>(r[k * kPieceCols + j])) * xs * ws[0] + bias[0];
                 }
-                reinterpret_cast<float*>(piece)[j * 32 + lane] = v;
+                reinterpret_cast<OutT*>(piece)[j * 32 + lane] = gg_cast<OutT>(v);
               }
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {  // 8 columns
                 uint32_t m[4];               // matrices of 8 lanes
                 float xs[2];
-                if constexpr (kInt8) {
+                if constexpr (kScaled) {
 #pragma unroll
                   for (int j = 0; j < 2; ++j) {
                     const int c = c1 + i * 8 + lane % 4 * 2 + j;
@@ -621,7 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
 #pragma unroll
                 for (int l = 0; l < 4; ++l) {
                   const uint32_t* v = r + (l >> 1) * 16 + i * 4 + (l & 1) * 2;
-                  if constexpr (kInt8)
+                  if constexpr (kScaled)
                     m[l] = gg_pack<OutT>(static_cast<float>(static_cast<int>(v[0])) * xs[0] * ws[l] + bias[l],
                                          static_cast<float>(static_cast<int>(v[1])) * xs[1] * ws[l] + bias[l]);
                   else
@@ -665,11 +717,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     }
     if (!kDw && args.zero_rest) {
       // rows before the first group and behind the last one
-      int64_t s = 0, e = args.rows;
-      if (args.offsets != nullptr) {
-        s = sched.start[0];
-        e = static_cast<int64_t>(sched.start[args.E - 1]) + sched.rows[args.E - 1];
-      }
+      const int64_t s = sched.start[0], e = static_cast<int64_t>(sched.start[args.E - 1]) + sched.rows[args.E - 1];
       const int64_t n = s + args.rows - e;
       const int w = static_cast<int>(blockIdx.x) * kGgEpiWarps + warp - 4;
       for (int64_t i = w; i < n; i += static_cast<int64_t>(gridDim.x) * kGgEpiWarps) {

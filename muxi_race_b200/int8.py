@@ -9,8 +9,9 @@ from typing import Optional
 
 import torch
 
-from . import _lib
 from ._args import FLOATS, empty2, launch, overlap, pitch, require, rows, without_gradient
+from .fused import _workspace
+from .w4 import _workspace_bytes as workspace_bytes
 
 
 def int8_linear(
@@ -62,6 +63,9 @@ def int8_linear(
         require(M < 2 or ld_out >= N, "rows of out must not overlap")
         for t in (x2, w, x_scale.view(1, -1), w_scale.view(1, -1), bias if bias is None else bias.view(1, -1)):
             require(t is None or not overlap(out2, t), "out must not share memory with the inputs")
+    nbytes = workspace_bytes("moe_int8_linear_workspace_bytes", M, N, K) if M > 16 else 0
+    ws = _workspace(nbytes, dev) if nbytes else None  # held until the call has been launched
     launch(dev, "moe_int8_linear", x2.data_ptr(), ld, x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-           None if bias is None else bias.data_ptr(), out.data_ptr(), ld_out, FLOATS[out.dtype], M, N, K)
+           None if bias is None else bias.data_ptr(), out.data_ptr(), ld_out, FLOATS[out.dtype], M, N, K,
+           None if ws is None else ws.data_ptr(), nbytes)
     return out if given else without_gradient("int8_linear", (out,), x_scale, w_scale, bias)[0]
