@@ -399,7 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     // ---------------------------------------------------------------- TMA producer
     // All lanes go through the loop and one of them issues, here and in the MMA warp: addresses and descriptors are then
     // computed in uniform registers, which these instructions read. From a loop of lane 0 alone an MMA took about 200 cycles to
-    // issue, more than it runs.
+    // issue, more than it runs. A block's MMAs and commits stand in one elected section: each section takes some 50 cycles more.
     {
       const uint64_t pol = l2_policy_evict_normal();
       int st = 0;
@@ -486,20 +486,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           const uint32_t b = smem_u32(smem + stage * stage_bytes) + b_at;
           const uint32_t d = tmem_base + static_cast<uint32_t>(half * 256);
           const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
-          if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kRed / kMmaRed; ++k) {
-              if (k * kMmaRed < left) {
-                const uint64_t ad = kMnA ? smem_desc_sw128_mn(a + k * 2048) : smem_desc_sw128(a + k * 32);
-                const uint64_t bd = kDw ? smem_desc_sw128_mn(b + k * 2048) : smem_desc_sw128(b + k * 32);
-                if constexpr (kInt8)
-                  mma_i8_pair(d, ad, bd, idesc, (kb | k) != 0);
-                else
-                  mma_f16_pair(d, ad, bd, idesc, (kb | k) != 0);
-              }
+          for (int k = 0; k < kRed / kMmaRed; ++k) {
+            if (k * kMmaRed < left) {
+              const uint64_t ad = kMnA ? smem_desc_sw128_mn(a + k * 2048) : smem_desc_sw128(a + k * 32);
+              const uint64_t bd = kDw ? smem_desc_sw128_mn(b + k * 2048) : smem_desc_sw128(b + k * 32);
+              if constexpr (kInt8)
+                mma_i8_pair(d, ad, bd, idesc, (kb | k) != 0);
+              else
+                mma_f16_pair(d, ad, bd, idesc, (kb | k) != 0);
             }
           }
-          __syncwarp();
         };
         bool second = false;  // the second half's accumulator is free
         for (int kb = 0; kb < t.kblocks; ++kb) {
@@ -510,30 +507,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
             break;
           }
           tc_fence_after();
-          mmas(st, 0, kb);
           const int last = kb == t.kblocks - 1;
-          if (last && elect_one()) tc_commit_pair(&tfull[0], 0x3);
-          __syncwarp();
-          ++held;
-          if (t.halves == 2 && !second) {
-            second = __all_sync(0xffffffffu, mbar_try_wait(&tempty[1], (uses[1] & 1u) ^ 1u));
-            if (!second && (last || held == kGgAhead)) {
-              if (!gg_all(mbar_wait(&tempty[1], (uses[1] & 1u) ^ 1u, abort_flag, args.status))) {
-                ok = false;
-                break;
+          if (t.halves == 1) {
+            if (elect_one()) {
+              mmas(st, 0, kb);
+              tc_commit_pair(&empty[st], 0x3);
+              if (last) tc_commit_pair(&tfull[0], 0x3);
+            }
+            __syncwarp();
+          } else {
+            ++held;
+            // The second half follows at once, but at the tile's end after the first, whose stores can then begin; and at its
+            // start as soon as its accumulator is free, at the latest when kGgAhead stages are held.
+            bool now = last || held == kGgAhead, issued = false;
+            if (!second) {
+              second = __all_sync(0xffffffffu, mbar_try_wait(&tempty[1], (uses[1] & 1u) ^ 1u));
+              if (!second && now) {
+                if (elect_one()) {
+                  mmas(st, 0, kb);
+                  if (last) tc_commit_pair(&tfull[0], 0x3);
+                }
+                __syncwarp();
+                issued = second = true;
+                if (!gg_all(mbar_wait(&tempty[1], (uses[1] & 1u) ^ 1u, abort_flag, args.status))) {
+                  ok = false;
+                  break;
+                }
               }
-              second = true;
+              if (second) tc_fence_after();
             }
-            if (second) tc_fence_after();
-          }
-          // the second half follows at once, but at the tile's end after the first, whose stores can then begin
-          if (t.halves == 1 || (second && (last || kb < t.kblocks - kGgAhead || held == kGgAhead))) {
-            for (; held > 0; --held) {
-              const int back = held - 1, stage = st >= back ? st - back : st - back + stages;
-              if (t.halves == 2) mmas(stage, 1, kb - back);
-              if (elect_one()) tc_commit_pair(&empty[stage], 0x3);
-              __syncwarp();
+            now = now || (second && kb < t.kblocks - kGgAhead);
+            if (elect_one()) {
+              if (!issued) {
+                mmas(st, 0, kb);
+                if (last) tc_commit_pair(&tfull[0], 0x3);
+              }
+              if (now) {
+                for (int back = held - 1; back >= 0; --back) {
+                  const int stage = st >= back ? st - back : st - back + stages;
+                  mmas(stage, 1, kb - back);
+                  tc_commit_pair(&empty[stage], 0x3);
+                }
+                if (last) tc_commit_pair(&tfull[1], 0x3);
+              }
             }
+            __syncwarp();
+            if (now) held = 0;
           }
           if (++st == stages) {
             st = 0;
@@ -541,11 +560,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           }
         }
         if (!ok) break;
-        if (t.halves == 2) {
-          ++uses[1];
-          if (elect_one()) tc_commit_pair(&tfull[1], 0x3);
-          __syncwarp();
-        }
+        if (t.halves == 2) ++uses[1];
       }
       if (elect_one()) tc_commit_pair(drain, 0x1);
       __syncwarp();
