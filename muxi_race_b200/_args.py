@@ -42,6 +42,18 @@ def pitch(t: torch.Tensor) -> int:
     return t.shape[1] if t.is_contiguous() or t.shape[0] == 1 else t.stride(0)
 
 
+def matrix(t: torch.Tensor, name: str, index: int | None = None) -> tuple:
+    """(rows, columns, row pitch in elements, address) of `t` [..., W] as :func:`rows` takes it, the shortest way to them;
+    index: the device's ordinal."""
+    if t.dim() == 2 and t.is_cuda and (index is None or t.get_device() == index):
+        R, W = t.shape
+        ld, step = t.stride()
+        if step == 1 or W <= 1:
+            return R, W, (W if R == 1 else ld), t.data_ptr()
+    t = rows(t, name, None if index is None else torch.device("cuda", index))
+    return t.shape[0], t.shape[1], pitch(t), t.data_ptr()
+
+
 def overlap_at(a: int, step_a: int, row_a: int, rows_a: int, b: int, step_b: int, row_b: int, rows_b: int) -> bool:
     """Whether two blocks of rows share memory: their addresses, and in bytes from row to row and the rows
     themselves. Column ranges of one wider tensor are told apart; rows of different pitches that interleave

@@ -13,64 +13,65 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, launch, once_differentiable, overlap, pitch, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, launch, matrix, once_differentiable, overlap, pitch, require, rows
 from .fused import moe_align
 from .rows8 import Q_DTYPES, Rows8, restore_rows8, save_rows8, silu_backward, silu_forward
 
 
-def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, width: int, R: Optional[int] = None) -> int:
-    """Row pitch of an operand [R, width] that is read in 16-byte pieces."""
+def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, index: int, width: int, R: Optional[int] = None) -> tuple:
+    """(rows, row pitch, address) of an operand [R, width] that is read in 16-byte pieces."""
     if t.dim() != 2 or t.shape[1] != width or (R is not None and t.shape[0] != R) or t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype} [{'R' if R is None else R}, {width}]")
-    rows(t, name, dev)
-    ld = pitch(t)
-    if t.data_ptr() % 16 or (ld % 8 and t.shape[0] > 1):
+    R, _, ld, ptr = matrix(t, name, index)
+    if ptr % 16 or (ld % 8 and R > 1):
         raise ValueError(f"{name} must start on 16 bytes, with a row pitch that is a multiple of 8")
-    return ld
+    return R, ld, ptr
 
 
 def _check(w: torch.Tensor, offsets: torch.Tensor):
+    """(E, N, K, address of w, its device)"""
     if w.dim() != 3 or w.dtype not in HALVES:
         raise ValueError("w must be fp16 or bf16 [E, N, K]")
-    dev = w.device
-    if not w.is_cuda or not w.is_contiguous() or w.data_ptr() % 16:
+    ptr, dev = w.data_ptr(), w.device
+    if not w.is_cuda or not w.is_contiguous() or ptr % 16:
         raise ValueError("w must be a contiguous CUDA tensor that starts on 16 bytes")
     E, N, K = w.shape
     if E < 1 or N < 8 or K < 8 or N % 8 or K % 8:
         raise ValueError("w needs at least one expert, and N and K positive multiples of 8")
-    if offsets.shape != (E + 1,) or offsets.dtype not in IDS or offsets.device != dev or not offsets.is_contiguous():
+    if (offsets.dim() != 1 or offsets.shape[0] != E + 1 or offsets.dtype not in IDS or offsets.get_device() != dev.index
+            or not offsets.is_contiguous()):
         raise ValueError(f"offsets must be a contiguous int32 or int64 tensor [{E + 1}] on {dev}")
-    return E, N, K, dev
+    return E, N, K, ptr, dev
 
 
 def _rows_product(name: str, x: torch.Tensor, x_name: str, w: torch.Tensor, offsets: torch.Tensor, transposed: bool,
                   out: Optional[torch.Tensor] = None, zero_rest: bool = True) -> torch.Tensor:
-    E, N, K, dev = _check(w, offsets)
+    E, N, K, w_ptr, dev = _check(w, offsets)
     red, width = (N, K) if transposed else (K, N)
-    ld = _operand(x, x_name, w.dtype, dev, red)
-    R = x.shape[0]
+    dtype = w.dtype
+    R, ld, ptr = _operand(x, x_name, dtype, dev.index, red)
     if out is None:
-        out, ld_out = empty2(R, width, w.dtype, dev), width
+        out, ld_out = empty2(R, width, dtype, dev), width
     else:
-        require(tuple(out.shape) == (R, width) and out.dtype == w.dtype, f"out must be {w.dtype} [{R}, {width}]")
+        require(tuple(out.shape) == (R, width) and out.dtype == dtype, f"out must be {dtype} [{R}, {width}]")
         rows(out, "out", dev)
         ld_out = pitch(out)
         require(R < 2 or ld_out >= width, "rows of out must not overlap")
         for t in (x, w.view(1, -1), offsets.view(1, -1)):
             require(not overlap(out, t), "out must not share memory with the inputs")
-    launch(dev, name, x.data_ptr(), ld, w.data_ptr(), offsets.data_ptr(), IDS[offsets.dtype], out.data_ptr(), ld_out, R, E, N, K,
-           HALVES[w.dtype], int(zero_rest))
+    launch(dev, name, ptr, ld, w_ptr, offsets.data_ptr(), IDS[offsets.dtype], out.data_ptr(), ld_out, R, E, N, K, HALVES[dtype],
+           zero_rest)
     return out
 
 
 def _grouped_dw(dy, x, w_shape, offsets, dw_dtype) -> torch.Tensor:
     E, N, K = w_shape
     dev, dtype = dy.device, dy.dtype
-    ld_dy = _operand(dy, "dy", dtype, dev, N)
-    ld_x = _operand(x, "x", dtype, dev, K, dy.shape[0])
+    R, ld_dy, dy_ptr = _operand(dy, "dy", dtype, dev.index, N)
+    _, ld_x, x_ptr = _operand(x, "x", dtype, dev.index, K, R)
     dw = torch.empty((E, N, K), dtype=dw_dtype, device=dev)
-    launch(dev, "moe_grouped_linear_dw", dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, offsets.data_ptr(), IDS[offsets.dtype],
-           dw.data_ptr(), FLOATS[dw_dtype], dy.shape[0], E, N, K, HALVES[dtype])
+    launch(dev, "moe_grouped_linear_dw", dy_ptr, ld_dy, x_ptr, ld_x, offsets.data_ptr(), IDS[offsets.dtype], dw.data_ptr(),
+           FLOATS[dw_dtype], R, E, N, K, HALVES[dtype])
     return dw
 
 
@@ -141,10 +142,12 @@ def grouped_linear_backward(
     Returns ``(dx, dw)``, None for what is not asked for. x [R, K] or its :class:`Rows8` (not needed without dw); dw in
     w's dtype or ``torch.float32``, 0 for an expert without rows. Rows of no expert take no part, and their dx is 0.
     """
-    E, N, K, dev = _check(w, offsets)
-    dw_dtype = w.dtype if dw_dtype is None else dw_dtype
-    require(dw_dtype in (w.dtype, torch.float32), "dw_dtype must be the dtype of w or torch.float32")
-    _operand(dy, "dy", w.dtype, dev, N)
+    E, N, K, _, dev = _check(w, offsets)
+    if dw_dtype is None:
+        dw_dtype = w.dtype
+    elif dw_dtype != w.dtype and dw_dtype != torch.float32:
+        raise ValueError("dw_dtype must be the dtype of w or torch.float32")
+    _operand(dy, "dy", w.dtype, dev.index, N)
     dx = _rows_product("moe_grouped_linear_dx", dy, "dy", w, offsets, True) if need_dx else None
     dw = None
     if need_dw:

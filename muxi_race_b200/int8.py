@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 
-from ._args import FLOATS, empty2, launch, overlap, pitch, require, rows, without_gradient
+from ._args import FLOATS, empty2, launch, matrix, overlap, pitch, require, rows, without_gradient
 from .fused import _workspace
 from .w4 import _workspace_bytes as workspace_bytes
 
@@ -36,15 +36,14 @@ def int8_linear(
     dev = w.device
     if N < 1 or K < 16 or K % 16 or K >= 1 << 17:
         raise ValueError("w needs at least one row, and K a multiple of 16 below 131072")
-    x2 = rows(x, "x", dev)
-    if x2.dtype != torch.int8 or x2.shape[1] != K:
+    M, width, ld, ptr = matrix(x, "x", dev.index)
+    if x.dtype != torch.int8 or width != K:
         raise ValueError(f"x must be int8 [..., {K}]")
-    M, ld = x2.shape[0], pitch(x2)
-    if x2.data_ptr() % 16 or (ld % 16 and M > 1):
+    if ptr % 16 or (ld % 16 and M > 1):
         raise ValueError("x must start on 16 bytes, with a row pitch that is a multiple of 16")
-    if x_scale.dtype != torch.float32 or x_scale.numel() != M or x_scale.device != dev or not x_scale.is_contiguous():
+    if x_scale.dtype != torch.float32 or x_scale.numel() != M or x_scale.get_device() != dev.index or not x_scale.is_contiguous():
         raise ValueError(f"x_scale must be a contiguous fp32 tensor of {M} scales on {dev}")
-    if w_scale.dtype != torch.float32 or w_scale.numel() != N or w_scale.device != dev or not w_scale.is_contiguous():
+    if w_scale.dtype != torch.float32 or w_scale.numel() != N or w_scale.get_device() != dev.index or not w_scale.is_contiguous():
         raise ValueError(f"w_scale must be a contiguous fp32 tensor of {N} scales on {dev}")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or bias.device != dev or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous fp32 tensor [{N}] on {dev}")
@@ -61,11 +60,11 @@ def int8_linear(
         out2 = rows(out, "out", dev)
         ld_out = pitch(out2)
         require(M < 2 or ld_out >= N, "rows of out must not overlap")
-        for t in (x2, w, x_scale.view(1, -1), w_scale.view(1, -1), bias if bias is None else bias.view(1, -1)):
+        for t in (rows(x, "x"), w, x_scale.view(1, -1), w_scale.view(1, -1), bias if bias is None else bias.view(1, -1)):
             require(t is None or not overlap(out2, t), "out must not share memory with the inputs")
     nbytes = workspace_bytes("moe_int8_linear_workspace_bytes", M, N, K) if M > 16 else 0
     ws = _workspace(nbytes, dev) if nbytes else None  # held until the call has been launched
-    launch(dev, "moe_int8_linear", x2.data_ptr(), ld, x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+    launch(dev, "moe_int8_linear", ptr, ld, x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
            None if bias is None else bias.data_ptr(), out.data_ptr(), ld_out, FLOATS[out.dtype], M, N, K,
            None if ws is None else ws.data_ptr(), nbytes)
     return out if given else without_gradient("int8_linear", (out,), x_scale, w_scale, bias)[0]

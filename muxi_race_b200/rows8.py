@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, launch, once_differentiable, overlap, pitch, require, rows, without_gradient
+from ._args import FLOATS, HALVES, IDS, launch, matrix, once_differentiable, overlap, require, without_gradient
 
 GROUP = 128
 Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -64,10 +64,12 @@ def _check_half(t: torch.Tensor, name: str) -> int:
 
 
 def _empty_rows8(shape, parts: int, q_dtype: torch.dtype, dtype: torch.dtype, dev: torch.device) -> Rows8:
-    require(q_dtype in Q_DTYPES, "q_dtype must be torch.int8 or torch.float8_e4m3fn")
-    *lead, W = shape
-    return Rows8(torch.empty(shape, dtype=q_dtype, device=dev),
-                 torch.empty((*lead, groups_of(W, parts)), dtype=torch.float32, device=dev), dtype, parts)
+    W = shape[-1]
+    r = Rows8.__new__(Rows8)  # what __post_init__ checks holds
+    r.q = torch.empty(shape, dtype=q_dtype, device=dev)
+    r.scale = torch.empty((*shape[:-1], groups_of(W, parts)), dtype=torch.float32, device=dev)
+    r.dtype, r.parts = dtype, parts
+    return r
 
 
 def save_rows8(x: torch.Tensor, q_dtype: torch.dtype = torch.int8, parts: int = 1) -> Rows8:
@@ -77,14 +79,15 @@ def save_rows8(x: torch.Tensor, q_dtype: torch.dtype = torch.int8, parts: int = 
     ``torch.float8_e4m3fn``: the scale is the smallest power of two with 448 scale >= amax. A group that holds NaN
     or an infinity comes back as NaN. Not differentiable: a backward pass that meets the result raises.
     """
-    x2 = rows(x, "x")
+    R, W, ld, ptr = matrix(x, "x")
     dt = _check_half(x, "x")
-    R, W = x2.shape
-    require(W >= 1, "x must have at least one column")
-    require(parts >= 1 and W % parts == 0, "parts must divide the row length")
-    r = _empty_rows8(x.shape, parts, q_dtype, x.dtype, x.device)
-    launch(x.device, "moe_save_rows8", x2.data_ptr(), pitch(x2), r.q.data_ptr(), Q_DTYPES[q_dtype], r.scale.data_ptr(), R, W,
-           parts, dt)
+    if W < 1 or parts < 1 or W % parts:
+        raise ValueError("x must have at least one column, and parts must divide the row length")
+    if q_dtype not in Q_DTYPES:
+        raise ValueError("q_dtype must be torch.int8 or torch.float8_e4m3fn")
+    dev = x.device
+    r = _empty_rows8(x.shape, parts, q_dtype, x.dtype, dev)
+    launch(dev, "moe_save_rows8", ptr, ld, r.q.data_ptr(), Q_DTYPES[q_dtype], r.scale.data_ptr(), R, W, parts, dt)
     if torch.is_grad_enabled() and x.requires_grad:
         # the scales carry the node: every use of the copy reads them
         r.scale, = without_gradient("save_rows8", (r.scale,), x)
@@ -94,29 +97,32 @@ def save_rows8(x: torch.Tensor, q_dtype: torch.dtype = torch.int8, parts: int = 
 def restore_rows8(saved: Rows8, index: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The 16-bit rows that `saved` stands for; with ``index`` [R] int32 / int64, rows ``index[r]`` of a 2-D copy
     (zeros where that is no row). Not differentiable."""
-    require(saved.q.is_cuda, "saved rows must be CUDA tensors")
-    dev, W = saved.device, saved.shape[-1]
-    q = saved.q
-    src_rows = q.numel() // W if W else 0
-    if index is None:
-        shape, R, idx = q.shape, src_rows, (None, _lib.MOE_I32)
-    else:
-        if q.dim() != 2:
+    q, scale, dtype = saved.q, saved.scale, saved.dtype
+    if not q.is_cuda:
+        raise ValueError("saved rows must be CUDA tensors")
+    dev, shape = q.device, q.shape
+    W = shape[-1]
+    R = src_rows = q.numel() // W if W else 0
+    index_ptr, index_dt = None, 0
+    if index is not None:
+        if len(shape) != 2:
             raise ValueError("index needs rows [T, W]")
         if index.dim() != 1 or index.dtype not in IDS or index.device != dev or not index.is_contiguous():
             raise ValueError(f"index must be a contiguous int32 or int64 tensor [R] on {dev}")
         R = index.shape[0]
-        shape, idx = (R, W), (index.data_ptr(), IDS[index.dtype])
+        shape, index_ptr, index_dt = (R, W), index.data_ptr(), IDS[index.dtype]
     if out is None:
-        out = torch.empty(shape, dtype=saved.dtype, device=dev)
+        out = torch.empty(shape, dtype=dtype, device=dev)
     else:
-        require(tuple(out.shape) == tuple(shape) and out.dtype == saved.dtype and out.is_contiguous() and out.device == dev,
-                f"out must be a contiguous {saved.dtype} tensor {tuple(shape)} on {dev}")
+        require(tuple(out.shape) == tuple(shape) and out.dtype == dtype and out.is_contiguous() and out.device == dev,
+                f"out must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
         flat = out.view(1, -1)
-        for t in (q, saved.scale, index):
+        for t in (q, scale, index):
             require(t is None or not overlap(flat, t.view(1, -1)), "out must not share memory with the saved rows or the index")
-    launch(dev, "moe_restore_rows", q.data_ptr(), W, Q_DTYPES[q.dtype], saved.scale.data_ptr(), *idx, 1, None, out.data_ptr(),
-           R, src_rows, W, saved.parts, HALVES[saved.dtype])
+    launch(dev, "moe_restore_rows", q.data_ptr(), W, Q_DTYPES[q.dtype], scale.data_ptr(), index_ptr, index_dt, 1, None,
+           out.data_ptr(), R, src_rows, W, saved.parts, HALVES[dtype])
+    if not scale.requires_grad:
+        return out
     return without_gradient("restore_rows8", (out,), saved.scale)[0]
 
 
@@ -129,50 +135,46 @@ def _weights_args(weights: Optional[torch.Tensor], R: int, dev: torch.device):
     return weights.data_ptr(), FLOATS[weights.dtype]
 
 
-def _check_gate_up(gate_up: torch.Tensor) -> int:
-    I = gate_up.shape[-1] // 2
-    require(I >= 1 and gate_up.shape[-1] == 2 * I, "gate_up must be [..., 2 I]")
-    return I
-
-
 def silu_forward(gate_up, weights, q_dtype, at=None, valid=None):
     """(h, Rows8 or None) of gate_up [..., 2 I]. at: weights are taken at at[r], valid: pointer to the number of
     rows (rows behind it stay uninitialised)."""
-    g2 = rows(gate_up, "gate_up")
+    R, W, ld, ptr = matrix(gate_up, "gate_up")
     dt = _check_half(gate_up, "gate_up")
-    I = _check_gate_up(gate_up)
-    R, dev = g2.shape[0], gate_up.device
+    I = W // 2
+    if I < 1 or W != 2 * I:
+        raise ValueError("gate_up must be [..., 2 I]")
+    dev, shape = gate_up.device, gate_up.shape
     w_ptr, w_dt = _weights_args(weights, R, dev) if at is None else (weights.data_ptr(), FLOATS[weights.dtype])
-    h = torch.empty((*gate_up.shape[:-1], I), dtype=gate_up.dtype, device=dev)
-    saved = None if q_dtype is None else _empty_rows8(gate_up.shape, 2, q_dtype, gate_up.dtype, dev)
-    q_args = (None, 0, None) if saved is None else (saved.q.data_ptr(), Q_DTYPES[q_dtype], saved.scale.data_ptr())
-    launch(dev, "moe_silu_mul", g2.data_ptr(), pitch(g2), w_ptr, w_dt, None if at is None else at.data_ptr(),
+    h = torch.empty((*shape[:-1], I), dtype=gate_up.dtype, device=dev)
+    saved, q_args = None, (None, 0, None)
+    if q_dtype is not None:
+        saved = _empty_rows8(shape, 2, q_dtype, gate_up.dtype, dev)
+        q_args = (saved.q.data_ptr(), Q_DTYPES[q_dtype], saved.scale.data_ptr())
+    launch(dev, "moe_silu_mul", ptr, ld, w_ptr, w_dt, None if at is None else at.data_ptr(),
            0 if weights is None else weights.numel(), valid, h.data_ptr(), *q_args, R, I, dt)
     return h, saved
 
 
 def silu_backward(dh, gate_up, weights, dweights, at=None, valid=None):
     """(dgate_up, h); dweights, if any, is filled in."""
-    d2 = rows(dh, "dh")
+    R, I, ld_dh, dh_ptr = matrix(dh, "dh")
     dt = _check_half(dh, "dh")
-    dev = dh.device
+    dev, dtype, shape = dh.device, dh.dtype, gate_up.shape
     if isinstance(gate_up, Rows8):
-        require(gate_up.parts == 2 and gate_up.dtype == dh.dtype, "saved gate_up must have parts = 2 and the dtype of dh")
-        g_args = (gate_up.q.data_ptr(), gate_up.shape[-1], Q_DTYPES[gate_up.q.dtype], gate_up.scale.data_ptr())
+        if gate_up.parts != 2 or gate_up.dtype != dtype or gate_up.q.get_device() != dev.index:
+            raise ValueError(f"saved gate_up must have parts = 2 and the dtype of dh, and be on {dev}")
+        g_args = (gate_up.q.data_ptr(), 2 * I, Q_DTYPES[gate_up.q.dtype], gate_up.scale.data_ptr())
     else:
-        g2 = rows(gate_up, "gate_up", dev)
-        require(gate_up.dtype == dh.dtype, "gate_up must have the dtype of dh")
-        g_args = (g2.data_ptr(), pitch(g2), dt, None)
-    if gate_up.device != dev:
-        raise ValueError(f"gate_up must be on {dev}")
-    I = dh.shape[-1]
-    if I < 1 or tuple(gate_up.shape) != (*dh.shape[:-1], 2 * I):
+        _, _, ld, ptr = matrix(gate_up, "gate_up", dev.index)
+        if gate_up.dtype != dtype:
+            raise ValueError("gate_up must have the dtype of dh")
+        g_args = (ptr, ld, dt, None)
+    if I < 1 or shape[-1] != 2 * I or shape[:-1] != dh.shape[:-1]:
         raise ValueError(f"gate_up must be {(*dh.shape[:-1], 2 * I)}, twice as wide as dh")
-    R = d2.shape[0]
     w_ptr, w_dt = _weights_args(weights, R, dev) if at is None else (weights.data_ptr(), FLOATS[weights.dtype])
-    dgate_up = torch.empty(gate_up.shape, dtype=dh.dtype, device=dev)
-    h = torch.empty(dh.shape, dtype=dh.dtype, device=dev)
-    launch(dev, "moe_silu_mul_backward", d2.data_ptr(), pitch(d2), *g_args, w_ptr, w_dt, None if at is None else at.data_ptr(),
+    dgate_up = torch.empty(shape, dtype=dtype, device=dev)
+    h = torch.empty(dh.shape, dtype=dtype, device=dev)
+    launch(dev, "moe_silu_mul_backward", dh_ptr, ld_dh, *g_args, w_ptr, w_dt, None if at is None else at.data_ptr(),
            0 if weights is None else weights.numel(), valid, dgate_up.data_ptr(), h.data_ptr(),
            None if dweights is None else dweights.data_ptr(), R, I, dt)
     return dgate_up, h
@@ -213,9 +215,10 @@ def silu_mul(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = None, 
 def silu_mul_rows8(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = None, q_dtype: torch.dtype = torch.int8):
     """:func:`silu_mul` and the 8-bit copy of gate_up that :func:`silu_mul_backward` takes, in one pass: ``(h, Rows8)``.
     Not differentiable (``silu_mul(..., save=)`` is)."""
-    require(q_dtype in Q_DTYPES, "q_dtype must be torch.int8 or torch.float8_e4m3fn")
+    if q_dtype not in Q_DTYPES:
+        raise ValueError("q_dtype must be torch.int8 or torch.float8_e4m3fn")
     h, saved = silu_forward(gate_up, row_weights, q_dtype)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (gate_up.requires_grad or (row_weights is not None and row_weights.requires_grad)):
         h, saved.scale = without_gradient("silu_mul_rows8", (h, saved.scale), gate_up, row_weights)
     return h, saved
 

@@ -16,8 +16,11 @@ import torch
 from torch import Tensor
 
 from . import fused as _fused
+from . import grouped as _grouped
+from . import int8 as _int8
 from . import norm as _norm
 from . import route as _route
+from . import rows8 as _rows8
 from . import submission as _submission
 from . import w4 as _w4
 
@@ -152,3 +155,43 @@ def fused_moe_w4(hidden_states: Tensor, w13: Tensor, w2: Tensor, num_experts: in
 def _fused_moe_w4_fake(hidden_states, w13, w2, num_experts, intermediate, group_size13, has_zeros13, group_size2,
                        has_zeros2, topk_ids, topk_weights):
     return hidden_states.new_empty(hidden_states.shape)
+
+
+@torch.library.custom_op("muxi_race_b200::grouped_linear", mutates_args=())
+def grouped_linear(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
+    return _grouped._rows_product("moe_grouped_linear", x, "x", w, offsets, False)
+
+
+@grouped_linear.register_fake
+def _grouped_linear_fake(x, w, offsets):
+    return x.new_empty((x.shape[0], w.shape[1]))
+
+
+@torch.library.custom_op("muxi_race_b200::grouped_linear_backward", mutates_args=())
+def grouped_linear_backward(dy: Tensor, x: Tensor, w: Tensor, offsets: Tensor) -> tuple[Tensor, Tensor]:
+    return _grouped.grouped_linear_backward(dy, x, w, offsets)
+
+
+@grouped_linear_backward.register_fake
+def _grouped_linear_backward_fake(dy, x, w, offsets):
+    return x.new_empty(x.shape), w.new_empty(w.shape)
+
+
+@torch.library.custom_op("muxi_race_b200::silu_mul", mutates_args=())
+def silu_mul(gate_up: Tensor, row_weights: Optional[Tensor]) -> Tensor:
+    return _rows8.silu_forward(gate_up, row_weights, None)[0]
+
+
+@silu_mul.register_fake
+def _silu_mul_fake(gate_up, row_weights):
+    return gate_up.new_empty((*gate_up.shape[:-1], gate_up.shape[-1] // 2))
+
+
+@torch.library.custom_op("muxi_race_b200::int8_linear", mutates_args=())
+def int8_linear(x: Tensor, x_scale: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor], out_dtype: torch.dtype) -> Tensor:
+    return _int8.int8_linear(x, x_scale, w, w_scale, bias, out_dtype)
+
+
+@int8_linear.register_fake
+def _int8_linear_fake(x, x_scale, w, w_scale, bias, out_dtype):
+    return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=out_dtype)
