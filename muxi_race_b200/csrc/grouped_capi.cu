@@ -56,7 +56,8 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   int64_t pairs = sms / 2;
   auto lane_tiles = [&](int halves) { return (args.lanes + halves * kGgHalf - 1) / (halves * kGgHalf); };
   auto rounds = [&](int halves) { return (lane_tiles(halves) * usual + pairs - 1) / pairs; };
-  // A tile of 512 lanes takes as long as 1.5 of 256 where both are bound by shared memory; fewer rounds of the smaller ones win where there are few tiles.
+  // A tile of 512 lanes takes about 1.5 times as long as one of 256, which shared memory bounds; fewer rounds of the smaller ones win
+  // where there are few tiles.
   args.halves = args.lanes > kGgHalf && 3 * rounds(2) <= 2 * rounds(1) ? 2 : 1;
   if (lane_tiles(args.halves) * most > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
   if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;

@@ -20,7 +20,8 @@
 // and 8192^3 runs at 0.70 of the tensor pipe's cycles. A tile is therefore 512 lanes x 256 columns, two MMAs of 256 lanes that
 // share the columns' operand: 48 KiB per SM and 64-element step instead of 64 (or of 32 for half as much). Its two halves fill all 512
 // TMEM columns. They are handed to the epilogue and back one by one: the MMA warp runs the first half of the next tile ahead while the
-// second is still being stored. Where 512 lanes would leave SMs without work, tiles have 256.
+// second is still being stored. Tiles of 256 lanes take turns with the two accumulators: where 512 would leave SMs without work, or
+// where a tile's stores take as long as its MMAs (dW of few rows), which then run beside each other.
 //
 // Dw reduces over rows, so the last block of an expert reaches into the next expert's rows. Those may
 // hold infinities or NaN, which a zero in the other operand would not remove: a warp of its own clears
@@ -59,7 +60,7 @@ constexpr int kGgThreads = 128 + 32 * kGgEpiWarps;
 constexpr int kGgBand = 8;  // column tiles that take turns on a weight tile
 constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiples of 32
 constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
-constexpr int kGgOutBytes = kGgEpiWarps * 2048;  // the epilogue's staging
+constexpr int kGgOutBytes = kGgEpiWarps / 2 * 4096;  // the epilogue's staging
 constexpr int kGgSmemBytes = 1024 + kGgRingBytes + kGgOutBytes + 256 + kGgTableInts * 4;
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
@@ -467,13 +468,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     if (leader) {
       int st = 0, held = 0;  // next stage; stages whose second half is to come
       uint32_t ph = 0;
-      uint32_t uses[2] = {0, 0};
+      int slot = args.halves == 1 ? 1 : 0;
+      uint32_t uses = 0;  // parity of each accumulator's next wait
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += npairs) {
         const GroupedTile t = sched.get(tile);
         if (t.kblocks == 0 || t.ncols == 0) continue;
-        if (!gg_all(mbar_wait(&tempty[0], (uses[0] & 1u) ^ 1u, abort_flag, args.status))) break;
-        ++uses[0];
+        if (args.halves == 1) slot ^= 1;  // tiles of 256 lanes take the two accumulators in turn
+        if (!gg_all(mbar_wait(&tempty[slot], (uses >> slot & 1u) ^ 1u, abort_flag, args.status))) break;
+        uses ^= 1u << slot;
         tc_fence_after();
         const int n = (t.ncols + kGgColStep - 1) / kGgColStep * kGgColStep;
         uint32_t idesc;
@@ -481,10 +484,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           idesc = idesc_i8(256, n);
         else
           idesc = idesc_f16(kBf16, 256, n) | (kMnA ? 1u << 15 : 0u) | (kDw ? 1u << 16 : 0u);
-        auto mmas = [&](int stage, int half, int kb) {
+        auto mmas = [&](int stage, int half, int acc, int kb) {
           const uint32_t a = smem_u32(smem + stage * stage_bytes) + half * kGgOperandBytes;
           const uint32_t b = smem_u32(smem + stage * stage_bytes) + b_at;
-          const uint32_t d = tmem_base + static_cast<uint32_t>(half * 256);
+          const uint32_t d = tmem_base + static_cast<uint32_t>(acc * 256);
           const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
 #pragma unroll
           for (int k = 0; k < kRed / kMmaRed; ++k) {
@@ -510,9 +513,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           const int last = kb == t.kblocks - 1;
           if (t.halves == 1) {
             if (elect_one()) {
-              mmas(st, 0, kb);
+              mmas(st, 0, slot, kb);
               tc_commit_pair(&empty[st], 0x3);
-              if (last) tc_commit_pair(&tfull[0], 0x3);
+              if (last) tc_commit_pair(&tfull[slot], 0x3);
             }
             __syncwarp();
           } else {
@@ -521,15 +524,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
             // start as soon as its accumulator is free, at the latest when kGgAhead stages are held.
             bool now = last || held == kGgAhead, issued = false;
             if (!second) {
-              second = __all_sync(0xffffffffu, mbar_try_wait(&tempty[1], (uses[1] & 1u) ^ 1u));
+              second = __all_sync(0xffffffffu, mbar_try_wait(&tempty[1], (uses >> 1 & 1u) ^ 1u));
               if (!second && now) {
                 if (elect_one()) {
-                  mmas(st, 0, kb);
+                  mmas(st, 0, 0, kb);
                   if (last) tc_commit_pair(&tfull[0], 0x3);
                 }
                 __syncwarp();
                 issued = second = true;
-                if (!gg_all(mbar_wait(&tempty[1], (uses[1] & 1u) ^ 1u, abort_flag, args.status))) {
+                if (!gg_all(mbar_wait(&tempty[1], (uses >> 1 & 1u) ^ 1u, abort_flag, args.status))) {
                   ok = false;
                   break;
                 }
@@ -539,13 +542,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
             now = now || (second && kb < t.kblocks - kGgAhead);
             if (elect_one()) {
               if (!issued) {
-                mmas(st, 0, kb);
+                mmas(st, 0, 0, kb);
                 if (last) tc_commit_pair(&tfull[0], 0x3);
               }
               if (now) {
                 for (int back = held - 1; back >= 0; --back) {
                   const int stage = st >= back ? st - back : st - back + stages;
-                  mmas(stage, 1, kb - back);
+                  mmas(stage, 1, 1, kb - back);
                   tc_commit_pair(&empty[stage], 0x3);
                 }
                 if (last) tc_commit_pair(&tfull[1], 0x3);
@@ -560,7 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           }
         }
         if (!ok) break;
-        if (t.halves == 2) ++uses[1];
+        if (t.halves == 2) uses ^= 2u;
       }
       if (elect_one()) tc_commit_pair(drain, 0x1);
       __syncwarp();
@@ -593,14 +596,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     // ---------------------------------------------------------------- epilogue
     const int q = warp & 3, part = (warp - 4) >> 2;  // lane quadrant, half of the columns
     constexpr bool kWide = sizeof(OutT) == 4;
-    constexpr int kPieceCols = kWide ? 16 : 32;
-    // Staging of a piece, rows of 128 bytes: a warp's 32 lanes of 32 bits, or the 64 lanes of 16 bits of two neighbouring
-    // warps, which write and copy it together (stores of whole 128-byte lines: dW of 256 experts with 128 rows 1870 us in
-    // half lines). 16-byte chunk c of row j is at c ^ (j % 8) for the 64-lane rows.
+    // 16-bit results are staged in pieces of 32 columns and the 64 lanes of two neighbouring warps, which write and copy them
+    // together in whole lines of 128 bytes (dW of 256 experts with 128 rows: 1870 us in half lines, 1650 in whole ones).
+    // 16-byte chunk c of row j is at c ^ (j % 8).
     OutT* out = static_cast<OutT*>(args.out);
-    uint8_t* piece = pieces_out + (kWide ? warp - 4 : (warp - 4) >> 1) * (kWide ? 2048 : 4096);
+    uint8_t* piece = pieces_out + ((warp - 4) >> 1) * 4096;
     const int pair_id = 1 + ((warp - 4) >> 1), side = q & 1;
-    uint32_t uses = 0;  // parity of each half's next wait
+    int slot = args.halves == 1 ? 1 : 0;
+    uint32_t uses = 0;  // parity of each accumulator's next wait
     bool ok = true;
     const uint32_t st_row = lane & 7;  // where this thread's row of a matrix starts (stmatrix)
     const uint32_t st_at = st_row * 128 + (((side * 4 + (lane >> 3)) ^ st_row) << 4);
@@ -622,16 +625,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
             for (int c = from; c < to; ++c) p[c * args.ld_out] = gg_cast<OutT>(0.0f);
           continue;
         }
-        ok = gg_all(mbar_wait(&tfull[half], uses >> half & 1u, abort_flag, args.status));
+        if (args.halves == 1)
+          slot ^= 1;
+        else
+          slot = half;
+        ok = gg_all(mbar_wait(&tfull[slot], uses >> slot & 1u, abort_flag, args.status));
         if constexpr (!kWide) ok = gg_pair_and(pair_id, ok);  // both or none: they meet again below
         if (!ok) break;
-        uses ^= 1u << half;
+        uses ^= 1u << slot;
         tc_fence_after();
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * 256);
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(slot * 256);
         auto release = [&]() {  // this warp's part of the accumulator is read
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) gg_arrive(mapa_shared(smem_u32(&tempty[half]), 0));
+          if (lane == 0) gg_arrive(mapa_shared(smem_u32(&tempty[slot]), 0));
         };
         float ws[4], bias[4];
         if constexpr (kScaled) {
@@ -654,76 +661,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           }
           tmem_ld_wait();
           if (c0 + 32 >= to) release();
+          const int n = min(32, to - c0);
+          if constexpr (kWide) {
+            // a column's 32 lanes are a line of 128 bytes: straight from the registers
+            OutT* o = out + at + f + c0 * args.ld_out;
+            if (there) {
 #pragma unroll
-          for (int k = 0; k < 32 / kPieceCols; ++k) {
-            const int c1 = c0 + k * kPieceCols;
-            if (c1 >= to) break;
-            // the last piece has been copied
-            if constexpr (kWide)
-              __syncwarp();
-            else
-              gg_pair_sync(pair_id);
-            if constexpr (kWide) {
-#pragma unroll
-              for (int j = 0; j < kPieceCols; ++j) {
-                float v = __uint_as_float(r[k * kPieceCols + j]);
-                if constexpr (kScaled) {
-                  const float xs = c1 + j < t.ncols ? __ldg(args.col_scale + t.row0 + c1 + j) : 0.0f;
-                  v = static_cast<float>(static_cast<int>(r[k * kPieceCols + j])) * xs * ws[0] + bias[0];
-                }
-                reinterpret_cast<OutT*>(piece)[j * 32 + lane] = gg_cast<OutT>(v);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {  // 8 columns
-                uint32_t m[4];               // matrices of 8 lanes
-                float xs[2];
-                if constexpr (kScaled) {
-#pragma unroll
-                  for (int j = 0; j < 2; ++j) {
-                    const int c = c1 + i * 8 + lane % 4 * 2 + j;
-                    xs[j] = c < t.ncols ? __ldg(args.col_scale + t.row0 + c) : 0.0f;
-                  }
-                }
-#pragma unroll
-                for (int l = 0; l < 4; ++l) {
-                  const uint32_t* v = r + (l >> 1) * 16 + i * 4 + (l & 1) * 2;
+              for (int j = 0; j < 32; ++j) {
+                if (j < n) {
+                  float v = __uint_as_float(r[j]);
                   if constexpr (kScaled)
-                    m[l] = gg_pack<OutT>(static_cast<float>(static_cast<int>(v[0])) * xs[0] * ws[l] + bias[l],
-                                         static_cast<float>(static_cast<int>(v[1])) * xs[1] * ws[l] + bias[l]);
+                    v = static_cast<float>(static_cast<int>(r[j])) * __ldg(args.col_scale + t.row0 + c0 + j) * ws[0] + bias[0];
+                  if constexpr (kDw)
+                    __stcs(o, gg_cast<OutT>(v));
                   else
-                    m[l] = gg_pack<OutT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
+                    *o = gg_cast<OutT>(v);
                 }
-                stmatrix_x4_trans(smem_u32(piece) + i * 1024 + st_at, m[0], m[1], m[2], m[3]);
+                o += args.ld_out;
               }
             }
-            const int n = min(kPieceCols, to - c1);
-            if constexpr (kWide)
-              __syncwarp();
-            else
-              gg_pair_sync(pair_id);
-            constexpr int kElts = 16 / static_cast<int>(sizeof(OutT));
-            const int p0 = kWide ? f0 : f0 - side * 32;  // the piece's first lane
+          } else {
+            gg_pair_sync(pair_id);  // the last piece has been copied
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // 8 columns
+              uint32_t m[4];               // matrices of 8 lanes
+              float xs[2];
+              if constexpr (kScaled) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const int c = c0 + i * 8 + lane % 4 * 2 + j;
+                  xs[j] = c < t.ncols ? __ldg(args.col_scale + t.row0 + c) : 0.0f;
+                }
+              }
+#pragma unroll
+              for (int l = 0; l < 4; ++l) {
+                const uint32_t* v = r + (l >> 1) * 16 + i * 4 + (l & 1) * 2;
+                if constexpr (kScaled)
+                  m[l] = gg_pack<OutT>(static_cast<float>(static_cast<int>(v[0])) * xs[0] * ws[l] + bias[l],
+                                       static_cast<float>(static_cast<int>(v[1])) * xs[1] * ws[l] + bias[l]);
+                else
+                  m[l] = gg_pack<OutT>(__uint_as_float(v[0]), __uint_as_float(v[1]));
+              }
+              stmatrix_x4_trans(smem_u32(piece) + i * 1024 + st_at, m[0], m[1], m[2], m[3]);
+            }
+            gg_pair_sync(pair_id);
+            const int p0 = f0 - side * 32;  // the piece's first lane
             if (args.out16) {  // 8 threads a row, 4 rows at a time
-              const int row = (kWide ? 0 : side * 16) + lane / 8, chunk = lane % 8;
-              if (p0 + chunk * kElts < args.lanes) {
-                OutT* o = out + at + p0 + chunk * kElts + (c1 + row) * args.ld_out;
+              const int row = side * 16 + lane / 8, chunk = lane % 8;
+              if (p0 + chunk * 8 < args.lanes) {
+                OutT* o = out + at + p0 + chunk * 8 + (c0 + row) * args.ld_out;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const int rj = row + j * 4;
-                  const int byte = rj * 128 + (kWide ? chunk : chunk ^ (rj & 7)) * 16;
-                  if (rj < n) gg_store16<kDw>(o, *reinterpret_cast<const uint4*>(piece + byte));
+                  if (rj < n) gg_store16<kDw>(o, *reinterpret_cast<const uint4*>(piece + rj * 128 + (chunk ^ (rj & 7)) * 16));
                   o += 4 * args.ld_out;
                 }
               }
             } else {
-              for (int j = kWide ? 0 : side * 16; j < min(n, kWide ? 16 : side * 16 + 16); ++j) {
-                for (int l = lane; l < (kWide ? 32 : 64); l += 32) {
-                  const int byte = j * 128 + (kWide ? l * 4 : ((l >> 3) ^ (j & 7)) * 16 + (l & 7) * 2);
+              for (int j = side * 16; j < min(n, side * 16 + 16); ++j)
+                for (int l = lane; l < 64; l += 32)
                   if (p0 + l < args.lanes)
-                    out[at + p0 + l + (c1 + j) * args.ld_out] = *reinterpret_cast<const OutT*>(piece + byte);
-                }
-              }
+                    out[at + p0 + l + (c0 + j) * args.ld_out] =
+                        *reinterpret_cast<const OutT*>(piece + j * 128 + ((l >> 3) ^ (j & 7)) * 16 + (l & 7) * 2);
             }
           }
           __syncwarp();  // the next read of TMEM is the whole warp's
