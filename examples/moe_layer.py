@@ -6,6 +6,9 @@
   int8     the same with 8-bit rows from the norm straight into int8 experts
   train    norm and router with their gradients: one step towards a target distribution of the
            routing weights, and the balance bias moved by the tokens per expert
+  experts  a training step of the whole layer, norm, router and 16-bit experts, towards a target output;
+           what the experts' backward pass reads again is kept in 8 bits
+  dense    an int8 projection beside the experts, fed by the norm's rows
 """
 from __future__ import annotations
 
@@ -25,7 +28,7 @@ class Layer:
     norm: torch.Tensor   # [H]
     gate: torch.Tensor   # [E, H] router weight
     bias: torch.Tensor   # [E] fp32, for balance
-    w13: object          # experts' gate and up: W4Weights, or (int8 values, scales)
+    w13: object          # experts' gate and up: W4Weights, (int8 values, scales) or bf16
     w2: object
     topk: int
 
@@ -44,7 +47,7 @@ def make_layer(H=1024, I=512, E=32, topk=4, kind="w4", seed=0, device="cuda") ->
     w13, w2 = (randn(E, 2 * I, H) * H ** -0.5).bfloat16(), (randn(E, H, I) * I ** -0.5).bfloat16()
     if kind == "w4":
         w13, w2 = m.quantize_w4(w13, gate_up=True), m.quantize_w4(w2)
-    else:
+    elif kind == "int8":
         w13, w2 = m.quantize_rows_int8(w13), m.quantize_rows_int8(w2)
     return Layer((1 + 0.1 * randn(H)).bfloat16(), (randn(E, H) * H ** -0.5).bfloat16(),
                  torch.zeros(E, device=device), w13, w2, topk)
@@ -80,6 +83,31 @@ def train_step(layer: Layer, x: torch.Tensor, residual: torch.Tensor, target: to
     return float(loss.detach())
 
 
+def layer_loss(x, residual, norm, gate, w13, w2, topk: int, target, save=None):
+    """Mean square of what the layer's output, added to the residual stream, is off `target` [T, H]."""
+    y, stream = m.add_rms_norm(x, norm, residual)
+    weights, ids = m.route_topk(y.float() @ gate.T, topk, scoring="sigmoid")
+    return (stream.float() + m.moe_mlp(y, w13, w2, ids, weights, save=save).float() - target.float()).square().mean()
+
+
+def train_experts(layer: Layer, x: torch.Tensor, residual: torch.Tensor, target: torch.Tensor, lr=2.0, save=torch.int8) -> float:
+    """One step of all of the layer's weights (bf16 experts) towards `target`."""
+    leaves = [layer.norm.float().requires_grad_(), layer.gate.float().requires_grad_(), layer.w13.detach().requires_grad_(),
+              layer.w2.detach().requires_grad_()]
+    loss = layer_loss(x, residual, *leaves, layer.topk, target, save)
+    loss.backward()
+    with torch.no_grad():
+        for t, leaf in zip((layer.norm, layer.gate, layer.w13, layer.w2), leaves):
+            t.copy_(leaf.detach() - lr * leaf.grad)
+    return float(loss.detach())
+
+
+def dense_int8(layer: Layer, x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor):
+    """A projection (int8 weights [N, H] of quantize_rows_int8) of the normalised rows, which leave the norm in 8 bits."""
+    q, scale, _ = m.add_rms_norm_quant(x, layer.norm, residual)
+    return m.int8_linear(q, scale, w, w_scale, out_dtype=x.dtype)
+
+
 def main() -> None:
     g = torch.Generator(device="cuda").manual_seed(1)
     x, residual = (torch.randn((16, 1024), generator=g, device="cuda").bfloat16() for _ in range(2))
@@ -92,6 +120,11 @@ def main() -> None:
     target = torch.softmax(torch.randn((16, 32), generator=g, device="cuda") * 3, -1)
     losses = [train_step(layer, x, residual, target) for _ in range(20)]
     print(f"train    loss {losses[0]:.4f} -> {losses[-1]:.4f}")
+    layer, target = make_layer(kind="bf16"), torch.randn((16, 1024), generator=g, device="cuda").bfloat16()
+    losses = [train_experts(layer, x, residual, target) for _ in range(20)]
+    print(f"experts  loss {losses[0]:.4f} -> {losses[-1]:.4f}")
+    w = m.quantize_rows_int8((torch.randn((2048, 1024), generator=g, device="cuda") * 1024 ** -0.5).bfloat16())
+    print(f"dense    T=16  |out| = {float(dense_int8(layer, x, residual, *w).float().norm()):.3f}")
     assert m.device_status() == 0
 
 

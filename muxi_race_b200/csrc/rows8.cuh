@@ -192,7 +192,7 @@ __device__ __forceinline__ void r8_encode(const Packed<T>& x, Q* row, float* sca
   const float amax = r8_magnitude(top, T());
   const bool bad = !(amax < INFINITY);  // its codes do not matter
   // groups below 2^-100 are scaled up first, where the reciprocal of their scale would overflow
-  const bool tiny = amax < 0x1p-100f;
+  const bool tiny = top != 0 && amax < 0x1p-100f;
   const float a = tiny ? amax * 0x1p100f : amax;
   float inv, s;
   if constexpr (std::is_same<Q, I8>::value) {

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._args import FLOATS, HALVES, IDS, empty2, launch, matrix, once_differentiable, overlap, pitch, require, rows
-from .fused import moe_align
+from .fused import _workspace
 from .rows8 import Q_DTYPES, Rows8, restore_rows8, save_rows8, silu_backward, silu_forward
 
 
@@ -168,7 +168,7 @@ def _gather(x, order, topk: int, valid: int, R: int) -> torch.Tensor:
     else:
         src = (x.data_ptr(), pitch(x), HALVES[x.dtype], None)
     out = empty2(R, H, x.dtype, x.device)
-    launch(x.device, "moe_restore_rows", *src, order.data_ptr(), _lib.MOE_I32, topk, valid, out.data_ptr(), R, T, H, 1,
+    launch(x.device, "moe_restore_rows", *src, order.data_ptr(), _lib.MOE_I32, max(topk, 1), valid, out.data_ptr(), R, T, H, 1,
            HALVES[x.dtype])
     return out
 
@@ -180,12 +180,24 @@ def _combine(y: torch.Tensor, slot: torch.Tensor, T: int, topk: int) -> torch.Te
     return out
 
 
+def _sort_routes(ids: torch.Tensor, E: int) -> tuple:
+    """(offsets [E + 1], the routes in the experts' order, each route's place there or -1): ``moe_align`` without padding."""
+    R, dev = ids.numel(), ids.device
+    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
+    rest = torch.empty(2 * E + 1 + 4, dtype=torch.int32, device=dev)  # sizes, padded offsets (the same), totals
+    order, slot = (torch.empty(max(R, 1), dtype=torch.int32, device=dev) for _ in range(2))
+    ws = _workspace(_lib.lib().moe_align_workspace_bytes(R, E), dev)
+    at = rest.data_ptr()
+    launch(dev, "moe_align", ids.data_ptr(), IDS[ids.dtype], R, E, 1, at, offsets.data_ptr(), at + 4 * E, None, order.data_ptr(),
+           slot.data_ptr(), at + 4 * (2 * E + 1), ws.data_ptr(), ws.numel())
+    return offsets, order, slot
+
+
 def _mlp_forward(x, w13, w2, ids, weights, save):
     """(out, offsets, order, slot, gate_up or its Rows8)."""
     T, topk = ids.shape
     R, E = T * topk, w13.shape[0]
-    al = moe_align(ids, E, 1)
-    offsets, order, slot = al.group_offsets, al.sorted_route_ids, al.route_slot
+    offsets, order, slot = _sort_routes(ids, E)
     valid = offsets.data_ptr() + 4 * E
     xs = _gather(x, order, topk, valid, R)
     gate_up = _rows_product("moe_grouped_linear", xs, "x", w13, offsets, False, None, False)

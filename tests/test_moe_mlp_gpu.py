@@ -118,6 +118,8 @@ def test_no_route_and_no_token(cuda_device):
     assert all(bool((t == 0).all()) for t in (out, dx, dw13, dw2, dweights))
     out, dx, dw13, dw2, dweights = run(x[:0], w13, w2, ids[:0], weights[:0], dout[:0], None)
     assert out.shape == (0, 64) and bool((dw13 == 0).all()) and bool((dw2 == 0).all()) and dweights.shape == (0, 2)
+    out, dx, dw13, dw2, dweights = run(x, w13, w2, ids[:, :0].contiguous(), weights[:, :0].contiguous(), dout, None)
+    assert all(bool((t == 0).all()) for t in (out, dx, dw13, dw2)) and dweights.shape == (6, 0)
 
 
 def test_only_some_gradients(cuda_device):
@@ -172,6 +174,43 @@ def test_stream_and_graph(cuda_device):
     x.copy_(new[0] * 0.5), ids.copy_(new[3]), weights.copy_(new[4])
     graph.replay()
     assert torch.equal(out, m.moe_mlp(x, args[1], args[2], ids, weights))
+
+
+def test_backward_in_a_graph(cuda_device):
+    """Forward and backward captured as one graph (leaves without an eager graph that still lives), and replayed on new
+    values."""
+    args = make(40, 128, 64, 4, 2, BF16)
+    static = [t.clone() for t in (*args[:3], args[4], args[5])]
+    ids = args[3].clone()
+
+    def step(leaves):
+        out = m.moe_mlp(leaves[0], leaves[1], leaves[2], ids, leaves[3], save=I8)
+        return torch.autograd.grad(out, leaves, static[4])
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step([t.detach().requires_grad_() for t in static[:4]])
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step([t.detach().requires_grad_() for t in static[:4]])
+    new = make(40, 128, 64, 4, 2, BF16, seed=9)
+    ids.copy_(new[3]), static[3].copy_(new[4]), static[0].mul_(-0.5)
+    for _ in range(2):
+        graph.replay()
+    want = run(*static[:3], ids, static[3], static[4], I8)[1:]
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_many_routes_to_one_expert(cuda_device):
+    """All 40000 routes to the last of 3 experts, and one row longer than the sorted part of a lane."""
+    x, w13, w2, _, _, dout = make(20000, 64, 32, 3, 2, BF16)
+    ids = torch.full((20000, 2), 2, dtype=torch.int32, device="cuda")
+    ids[777, 1] = 0
+    weights = torch.full((20000, 2), 0.5, device="cuda")
+    got, want = run(x, w13, w2, ids, weights, dout, None), chain(x, w13, w2, ids, weights, dout, None)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_with_the_router_and_the_norm(cuda_device):
