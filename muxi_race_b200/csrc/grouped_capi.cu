@@ -55,10 +55,20 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   const int64_t usual = KIND == kGroupedDw || KIND == kDenseInt8 ? most : (args.rows + kGgTile - 1) / kGgTile + (args.E < args.rows ? args.E : args.rows) / 2;
   int64_t pairs = sms / 2;
   auto lane_tiles = [&](int halves) { return (args.lanes + halves * kGgHalf - 1) / (halves * kGgHalf); };
-  auto rounds = [&](int halves) { return (lane_tiles(halves) * usual + pairs - 1) / pairs; };
-  // A tile of 512 lanes takes about 1.5 times as long as one of 256, which shared memory bounds; fewer rounds of the smaller ones win
-  // where there are few tiles.
-  args.halves = args.lanes > kGgHalf && 3 * rounds(2) <= 2 * rounds(1) ? 2 : 1;
+  // Rounds of the SM pairs, the last one cut as GroupedSchedule does, a quarter longer for the small tiles. A tile of 512 lanes takes
+  // 1.8 times as long as one of 256 (8192^3 bf16: 725 us in 7 rounds of those, 760 us in 14 of these; 4096^3: 99 us in 2, 103 us in 3.5),
+  // and more where the reduction has few blocks, as its stores are hidden less (int8, 4095 rows, 7168 x 2048: 56 us, with 256 lanes 49 us);
+  // not for dW, whose stores bound either form (64 experts of 128 rows, 7168 x 2048: 409 us, with 256 lanes 582 us).
+  const int64_t blocks = KIND == kDenseInt8 ? args.split_blocks : (args.red + 63) / 64;
+  const double unit = KIND == kGroupedDw ? 1.8 : 1.76 + 5.6 / static_cast<double>(blocks);
+  auto cost = [&](int halves) {
+    const int64_t n = lane_tiles(halves) * usual, left = n % pairs;
+    int64_t parts = 1;
+    while (parts < 4 * halves && left * parts * 2 <= pairs) parts *= 2;
+    return (halves == 2 ? unit : 1.0) *
+           (static_cast<double>(n / pairs) + (left == 0 ? 0.0 : parts == 1 ? 1.0 : 1.25 / static_cast<double>(parts)));
+  };
+  args.halves = lane_tiles(1) * usual > pairs && cost(2) <= cost(1) ? 2 : 1;
   if (lane_tiles(args.halves) * most > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
   if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;
   constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT>;
