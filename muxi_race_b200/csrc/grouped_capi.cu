@@ -69,6 +69,9 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
            (static_cast<double>(n / pairs) + (left == 0 ? 0.0 : parts == 1 ? 1.0 : 1.25 / static_cast<double>(parts)));
   };
   args.halves = lane_tiles(1) * usual > pairs && cost(2) <= cost(1) ? 2 : 1;
+  // A dW in parts: with the two accumulators in turn a part's sums are added while the next one's MMAs run (4096^3:
+  // 158 us, with 512 lanes 188 us).
+  if (KIND == kGroupedDw && sizeof(OutT) == 4 && args.rows / args.E > 64 * kGgChunk) args.halves = 1;
   if (lane_tiles(args.halves) * most > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
   if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;
   constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT>;
