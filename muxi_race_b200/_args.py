@@ -78,6 +78,15 @@ def empty2(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> to
     return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
+def empty_of(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """An uninitialised contiguous tensor, by :func:`empty2` where that does."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
 class _NoGraph(torch.autograd.Function):
     @staticmethod
     def forward(ctx, message, results, *sources):

@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, launch, matrix, once_differentiable, overlap, require, without_gradient
+from ._args import FLOATS, HALVES, IDS, empty_of, launch, matrix, once_differentiable, overlap, require, without_gradient
 
 GROUP = 128
 Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -66,8 +66,8 @@ def _check_half(t: torch.Tensor, name: str) -> int:
 def _empty_rows8(shape, parts: int, q_dtype: torch.dtype, dtype: torch.dtype, dev: torch.device) -> Rows8:
     W = shape[-1]
     r = Rows8.__new__(Rows8)  # what __post_init__ checks holds
-    r.q = torch.empty(shape, dtype=q_dtype, device=dev)
-    r.scale = torch.empty((*shape[:-1], groups_of(W, parts)), dtype=torch.float32, device=dev)
+    r.q = empty_of(shape, q_dtype, dev)
+    r.scale = empty_of((*shape[:-1], groups_of(W, parts)), torch.float32, dev)
     r.dtype, r.parts = dtype, parts
     return r
 
@@ -112,7 +112,7 @@ def restore_rows8(saved: Rows8, index: Optional[torch.Tensor] = None, out: Optio
         R = index.shape[0]
         shape, index_ptr, index_dt = (R, W), index.data_ptr(), IDS[index.dtype]
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = empty_of(shape, dtype, dev)
     else:
         require(tuple(out.shape) == tuple(shape) and out.dtype == dtype and out.is_contiguous() and out.device == dev,
                 f"out must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
@@ -145,7 +145,7 @@ def silu_forward(gate_up, weights, q_dtype, at=None, valid=None):
         raise ValueError("gate_up must be [..., 2 I]")
     dev, shape = gate_up.device, gate_up.shape
     w_ptr, w_dt = _weights_args(weights, R, dev) if at is None else (weights.data_ptr(), FLOATS[weights.dtype])
-    h = torch.empty((*shape[:-1], I), dtype=gate_up.dtype, device=dev)
+    h = empty_of((*shape[:-1], I), gate_up.dtype, dev)
     saved, q_args = None, (None, 0, None)
     if q_dtype is not None:
         saved = _empty_rows8(shape, 2, q_dtype, gate_up.dtype, dev)
@@ -172,8 +172,8 @@ def silu_backward(dh, gate_up, weights, dweights, at=None, valid=None):
     if I < 1 or shape[-1] != 2 * I or shape[:-1] != dh.shape[:-1]:
         raise ValueError(f"gate_up must be {(*dh.shape[:-1], 2 * I)}, twice as wide as dh")
     w_ptr, w_dt = _weights_args(weights, R, dev) if at is None else (weights.data_ptr(), FLOATS[weights.dtype])
-    dgate_up = torch.empty(shape, dtype=dtype, device=dev)
-    h = torch.empty(dh.shape, dtype=dtype, device=dev)
+    dgate_up = empty_of(shape, dtype, dev)
+    h = empty_of(dh.shape, dtype, dev)
     launch(dev, "moe_silu_mul_backward", dh_ptr, ld_dh, *g_args, w_ptr, w_dt, None if at is None else at.data_ptr(),
            0 if weights is None else weights.numel(), valid, dgate_up.data_ptr(), h.data_ptr(),
            None if dweights is None else dweights.data_ptr(), R, I, dt)
@@ -229,6 +229,6 @@ def silu_mul_backward(dh: torch.Tensor, gate_up, row_weights: Optional[torch.Ten
 
     drow_weights has the dtype and shape of row_weights and a fixed summation order.
     """
-    dweights = None if row_weights is None else torch.empty_like(row_weights)
+    dweights = None if row_weights is None else empty_of(row_weights.shape, row_weights.dtype, row_weights.device)
     dgate_up, h = silu_backward(dh, gate_up, row_weights, dweights)
     return dgate_up, dweights, h

@@ -238,3 +238,21 @@ def test_refusals(cuda_device):
     many = torch.zeros(1026, dtype=torch.int32, device="cuda")
     with pytest.raises(m._lib.MoeError, match="1024"):
         m.grouped_linear(torch.zeros(8, 8, dtype=BF16, device="cuda"), torch.zeros(1025, 8, 8, dtype=BF16, device="cuda"), many)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_long_sums_in_32_bits(cuda_device, dtype):
+    """A 32-bit dW of many rows: parts of at most 768 rows are 48 steps of the tensor core, each off by at most 2^-23 of the sum so
+    far and towards zero, and their sums are added with rounding. Of normal data the sum so far is on average two thirds of
+    sqrt(rows of the part) and the parts' errors add up like their values: below 48 * 2^-24 * 2 / 3 = 1.9e-6 of dW's norm, for any
+    number of rows; in one piece 6000 rows would have 1.5e-5."""
+    R, N, K = 6001, 264, 512
+    x, dy = randn(20, R, K, dtype=dtype), randn(21, R, N, dtype=dtype)
+    offsets = torch.tensor([0, 770, 770, R], dtype=torch.int32, device="cuda")
+    _, dw = m.grouped_linear_backward(dy, x, torch.empty(3, N, K, dtype=dtype, device="cuda"), offsets, dw_dtype=F32, need_dx=False)
+    ref, mag = grouped_dw_ref(dy, x, offsets)
+    for e in (0, 2):
+        assert float((dw[e].double() - ref[e]).norm() / ref[e].norm()) < 1.9e-6
+    assert bool((dw[1] == 0).all())
+    again = m.grouped_linear_backward(dy, x, torch.empty(3, N, K, dtype=dtype, device="cuda"), offsets, dw_dtype=F32, need_dx=False)[1]
+    assert torch.equal(dw, again)
