@@ -497,6 +497,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
       int slot = args.halves == 1 ? 1 : 0;
       uint32_t uses = 0;  // parity of each accumulator's next wait
       bool ok = true;
+      const uint64_t a_desc = kMnA ? smem_desc_sw128_mn(smem_u32(smem)) : smem_desc_sw128(smem_u32(smem));
+      const uint64_t b_desc = kDw ? smem_desc_sw128_mn(smem_u32(smem) + b_at) : smem_desc_sw128(smem_u32(smem) + b_at);
       for (int tile = pair, row_part = 0; tile < tiles && ok; sched.next(tile, row_part, npairs)) {
         const GroupedTile t = sched.get(tile, row_part);
         if (t.kblocks == 0 || t.ncols == 0) continue;
@@ -511,15 +513,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         else
           idesc = idesc_f16(kBf16, 256, n) | (kMnA ? 1u << 15 : 0u) | (kDw ? 1u << 16 : 0u);
         auto mmas = [&](int stage, int half, int acc, int kb) {
-          const uint32_t a = smem_u32(smem + stage * stage_bytes) + half * kGgOperandBytes;
-          const uint32_t b = smem_u32(smem + stage * stage_bytes) + b_at;
+          // a descriptor's address field counts 16 bytes, and no sum leaves its 14 bits
+          const uint32_t at = static_cast<uint32_t>(stage * stage_bytes) >> 4;
+          const uint64_t a = a_desc + at + static_cast<uint32_t>(half * kGgOperandBytes >> 4), b = b_desc + at;
           const uint32_t d = tmem_base + static_cast<uint32_t>(acc * 256);
           const int left = kb == t.kblocks - 1 && t.tail ? t.tail : kRed;
 #pragma unroll
           for (int k = 0; k < kRed / kMmaRed; ++k) {
             if (k * kMmaRed < left) {
-              const uint64_t ad = kMnA ? smem_desc_sw128_mn(a + k * 2048) : smem_desc_sw128(a + k * 32);
-              const uint64_t bd = kDw ? smem_desc_sw128_mn(b + k * 2048) : smem_desc_sw128(b + k * 32);
+              const uint64_t ad = a + k * ((kMnA ? 2048 : 32) >> 4), bd = b + k * ((kDw ? 2048 : 32) >> 4);
               if constexpr (kInt8)
                 mma_i8_pair(d, ad, bd, idesc, (kb | k) != 0);
               else
