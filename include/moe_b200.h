@@ -586,7 +586,8 @@ MOE_API int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, 
  * The activation between the experts' products, and 8-bit copies of rows for the backward pass.
  * 8-bit rows: fp32 scales [R, parts, ceil(W / parts / 128)], one for each 128 columns of each of a row's `parts`.
  *   MOE_I8: scale = amax / 127, x / scale to nearest, halves away from zero. MOE_F8E4M3: scale = the smallest
- *   power of two with 448 scale >= amax. A group with NaN or an infinity: scale NaN.
+ *   power of two with 448 scale >= amax; values that would round beyond dtype stay at 240 scale. A group with NaN or an
+ *   infinity: scale NaN.
  *   moe_save_rows8: x [R, W] (pitch ld) -> q [R, W], scale.
  *   moe_restore_rows: out[r] = row index[r] / index_div of x (r without an index) in dtype; zeros where that is
  *     not in [0, src_rows). src_dtype MOE_I8 / MOE_F8E4M3 with scale, or dtype (rows as they are).

@@ -76,8 +76,9 @@ def save_rows8(x: torch.Tensor, q_dtype: torch.dtype = torch.int8, parts: int = 
     """8-bit copy of rows x [..., W] fp16 / bf16 (of any one pitch).
 
     ``torch.int8``: scale = amax / 127 of each 128 columns, values rounded to nearest, halves away from zero.
-    ``torch.float8_e4m3fn``: the scale is the smallest power of two with 448 scale >= amax. A group that holds NaN
-    or an infinity comes back as NaN. Not differentiable: a backward pass that meets the result raises.
+    ``torch.float8_e4m3fn``: the scale is the smallest power of two with 448 scale >= amax; values that would round
+    beyond x's type stay at 240 scale. A group that holds NaN or an infinity comes back as NaN.
+    Not differentiable: a backward pass that meets the result raises.
     """
     R, W, ld, ptr = matrix(x, "x")
     dt = _check_half(x, "x")
