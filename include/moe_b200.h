@@ -562,21 +562,15 @@ MOE_API int moe_fused_w4(const void* hidden_states, int64_t ld_hidden, const voi
  * Rows of no expert (before offsets[0], from offsets[E] on): 0 where zero_rest != 0, else left as they are; what
  * they hold is never used. Offsets outside [0, R] are clamped. Sums in fp32, one rounding; the same bits on every run.
  * Requirements: dtype MOE_F16 / MOE_BF16; 1 <= E <= 1024; N and K multiples of 8; x, dy and w on 16-byte boundaries,
- *   row pitches (in elements) of x and dy multiples of 8; outputs share no memory with inputs. The rows' products of few
- *   rows take a 16-byte aligned workspace of moe_grouped_linear_workspace_bytes (dx != 0: for moe_grouped_linear_dx).
+ *   row pitches (in elements) of x and dy multiples of 8; outputs share no memory with inputs.
  * ---------------------------------------------------------------------------------------- */
-MOE_API size_t moe_grouped_linear_workspace_bytes(int64_t num_rows, int64_t num_experts, int64_t out_features,
-                                                  int64_t in_features, int dx);
-
 MOE_API int moe_grouped_linear(const void* x, int64_t ld_x, const void* w, const void* offsets, int offsets_dtype, void* out,
                                int64_t ld_out, int64_t num_rows, int64_t num_experts, int64_t out_features,
-                               int64_t in_features, int dtype, int zero_rest, void* workspace, size_t workspace_bytes,
-                               void* stream);
+                               int64_t in_features, int dtype, int zero_rest, void* stream);
 
 MOE_API int moe_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, const void* offsets, int offsets_dtype,
                                   void* dx, int64_t ld_dx, int64_t num_rows, int64_t num_experts, int64_t out_features,
-                                  int64_t in_features, int dtype, int zero_rest, void* workspace, size_t workspace_bytes,
-                                  void* stream);
+                                  int64_t in_features, int dtype, int zero_rest, void* stream);
 
 MOE_API int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets,
                                   int offsets_dtype, void* dw, int dw_dtype, int64_t num_rows, int64_t num_experts,

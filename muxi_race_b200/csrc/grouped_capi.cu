@@ -40,21 +40,6 @@ int map_weights(CUtensorMap* m, const void* p, int elt, int64_t E, int64_t N, in
   return encode_map(m, p, elt, 3, dims, strides, box, "weights");
 }
 
-// Slices of the reduction for rows' products whose tiles leave half of the 74 CTA pairs or more without work. Each has at least 8
-// blocks of 64, and they save at least 24 blocks of the time, of 0.2 us each: joining them takes 4 us (7 rows of 3 experts,
-// N = 64, K = 13000: 19 us, in one 60; 4096 rows of one, N = 256, K = 4096: 28 us, in one 31; 8192 rows of one, N = 64, K = 1024
-// would take 26 us in two, 18 in one).
-int64_t grouped_split(int64_t R, int64_t E, int64_t lanes, int64_t red) {
-  if (R <= 0 || E <= 0 || lanes <= 0 || red <= 0) return 1;
-  const int64_t tiles = (lanes + kGgHalf - 1) / kGgHalf * (R / kGgTile + (E < R ? E : R)), blocks = (red + 63) / 64;
-  int64_t split = 74 / tiles;
-  if (split > blocks / 8) split = blocks / 8;
-  if (split > 16) split = 16;
-  if (split < 2) return 1;
-  const int64_t per = (blocks + split - 1) / split;
-  return blocks - per < 24 ? 1 : (blocks + per - 1) / per;  // no empty slices
-}
-
 template <int KIND, typename T, typename OutT>
 int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b32, GroupedArgs args, cudaStream_t s) {
   int dev, sms;
@@ -64,18 +49,17 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   MOE_TRY(device_sms(dev, &sms));
   MOE_TRY(device_status_ptr(dev, &args.status));
   // Groups of columns: about R / 256 and half a one more for each expert (where they begin and end is not known here).
-  const int64_t row_tiles = (args.rows + kGgTile - 1) / kGgTile;
   const int64_t most = KIND == kGroupedDw   ? static_cast<int64_t>(args.E) * ((args.cols + kGgTile - 1) / kGgTile)
-                       : KIND == kDenseInt8 ? row_tiles * args.split
-                                            : (row_tiles + args.E) * args.split;
-  const int64_t usual = KIND == kGroupedDw || KIND == kDenseInt8 ? most : (row_tiles + (args.E < args.rows ? args.E : args.rows) / 2) * args.split;
+                       : KIND == kDenseInt8 ? static_cast<int64_t>(args.E) * ((args.rows + kGgTile - 1) / kGgTile)
+                                          : (args.rows + kGgTile - 1) / kGgTile + args.E;
+  const int64_t usual = KIND == kGroupedDw || KIND == kDenseInt8 ? most : (args.rows + kGgTile - 1) / kGgTile + (args.E < args.rows ? args.E : args.rows) / 2;
   int64_t pairs = sms / 2;
   auto lane_tiles = [&](int halves) { return (args.lanes + halves * kGgHalf - 1) / (halves * kGgHalf); };
   // Rounds of the SM pairs, the last one cut as GroupedSchedule does, a quarter longer for the small tiles. A tile of 512 lanes takes
   // 1.8 times as long as one of 256 (8192^3 bf16: 725 us in 7 rounds of those, 760 us in 14 of these; 4096^3: 99 us in 2, 103 us in 3.5),
   // and more where the reduction has few blocks, as its stores are hidden less (int8, 4095 rows, 7168 x 2048: 56 us, with 256 lanes 49 us);
   // not for dW, whose stores bound either form (64 experts of 128 rows, 7168 x 2048: 409 us, with 256 lanes 582 us).
-  const int64_t blocks = KIND == kGroupedDw ? 1 : args.split_blocks;
+  const int64_t blocks = KIND == kDenseInt8 ? args.split_blocks : (args.red + 63) / 64;
   const double unit = KIND == kGroupedDw ? 1.8 : 1.76 + 5.6 / static_cast<double>(blocks);
   auto cost = [&](int halves) {
     const int64_t n = lane_tiles(halves) * usual, left = n % pairs;
@@ -97,42 +81,15 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   return MOE_OK;
 }
 
-template <int KIND, typename T>
-int grouped_rows_of(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b32, const GroupedArgs& g, void* workspace,
-                    cudaStream_t s) {
-  if (g.split == 1) return launch_grouped<KIND, T, T>(a, b, b32, g, s);
-  GroupedArgs part = g;
-  part.out = workspace;
-  part.ld_out = g.lanes;
-  part.zero_rest = 0;
-  MOE_TRY((launch_grouped<KIND, T, float>(a, b, b32, part, s)));
-  const dim3 grid((g.lanes + 1023) / 1024, static_cast<unsigned>(g.rows < 32768 ? g.rows : 32768));
-  const float* sums = static_cast<const float*>(workspace);
-  T* out = static_cast<T*>(g.out);
-  if (reinterpret_cast<uintptr_t>(out) % 8 == 0 && g.ld_out % 4 == 0)
-    grouped_join_kernel<true, T><<<grid, 256, 0, s>>>(sums, g.split, g.offsets, g.offsets64, g.E, g.rows, g.lanes, out, g.ld_out,
-                                                      g.zero_rest);
-  else
-    grouped_join_kernel<false, T><<<grid, 256, 0, s>>>(sums, g.split, g.offsets, g.offsets64, g.E, g.rows, g.lanes, out, g.ld_out,
-                                                       g.zero_rest);
-  MOE_CUDA(cudaGetLastError());
-  return MOE_OK;
-}
-
 // Y and Dx: rows of `red` elements times weights, to rows of `lanes` elements.
 template <int KIND>
 int grouped_rows(const void* in, int64_t ld_in, const void* w, const void* offsets, int offsets_dtype, void* out, int64_t ld_out,
-                 int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* workspace, size_t workspace_bytes,
-                 cudaStream_t s) {
+                 int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, cudaStream_t s) {
   MOE_TRY(check_grouped(offsets, offsets_dtype, R, E, N, K, dtype));
   if (R == 0) return MOE_OK;
   if (!in || !w || !out) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
   const int64_t lanes = KIND == kGroupedY ? N : K, red = KIND == kGroupedY ? K : N;
   if (R > 1 && (ld_in < red || ld_out < lanes)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
-  const int64_t split = grouped_split(R, E, lanes, red), blocks = (red + 63) / 64;
-  const size_t need = split == 1 ? 0 : static_cast<size_t>(split) * R * lanes * sizeof(float);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", need);
-  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(MOE_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
   CUtensorMap a, b, b32;
   if (KIND == kGroupedY)
     MOE_TRY(map_weights(&a, w, 2, E, N, K, 64, 128));
@@ -150,10 +107,8 @@ int grouped_rows(const void* in, int64_t ld_in, const void* w, const void* offse
   g.out = out;
   g.ld_out = ld_out;
   g.zero_rest = zero_rest;
-  g.split = static_cast<int>(split);
-  g.split_blocks = static_cast<int>((blocks + split - 1) / split);
-  return dtype == MOE_F16 ? grouped_rows_of<KIND, __half>(a, b, b32, g, workspace, s)
-                          : grouped_rows_of<KIND, __nv_bfloat16>(a, b, b32, g, workspace, s);
+  return dtype == MOE_F16 ? launch_grouped<KIND, __half, __half>(a, b, b32, g, s)
+                          : launch_grouped<KIND, __nv_bfloat16, __nv_bfloat16>(a, b, b32, g, s);
 }
 
 template <int NT, int WARPS, int AHEAD, typename OutT>
@@ -198,7 +153,7 @@ int64_t int8_split(int64_t M, int64_t N, int64_t K) {
 template <typename OutT>
 int int8_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b32, GroupedArgs g, void* workspace,
                cudaStream_t s) {
-  if (g.split == 1) return launch_grouped<kDenseInt8, int8_t, OutT>(a, b, b32, g, s);
+  if (g.E == 1) return launch_grouped<kDenseInt8, int8_t, OutT>(a, b, b32, g, s);
   GroupedArgs part = g;
   part.out = workspace;
   part.ld_out = g.lanes;
@@ -209,9 +164,9 @@ int int8_tiles(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b3
   const int* sums = static_cast<const int*>(workspace);
   OutT* out = static_cast<OutT*>(g.out);
   if (vec)
-    int8_join_kernel<4, OutT><<<grid, 256, 0, s>>>(sums, g.split, (int)g.rows, g.lanes, g.col_scale, g.lane_scale, g.bias, out, g.ld_out);
+    int8_join_kernel<4, OutT><<<grid, 256, 0, s>>>(sums, g.E, (int)g.rows, g.lanes, g.col_scale, g.lane_scale, g.bias, out, g.ld_out);
   else
-    int8_join_kernel<1, OutT><<<grid, 256, 0, s>>>(sums, g.split, (int)g.rows, g.lanes, g.col_scale, g.lane_scale, g.bias, out, g.ld_out);
+    int8_join_kernel<1, OutT><<<grid, 256, 0, s>>>(sums, g.E, (int)g.rows, g.lanes, g.col_scale, g.lane_scale, g.bias, out, g.ld_out);
   MOE_CUDA(cudaGetLastError());
   return MOE_OK;
 }
@@ -225,25 +180,18 @@ using namespace moe;
 
 extern "C" {
 
-size_t moe_grouped_linear_workspace_bytes(int64_t R, int64_t E, int64_t N, int64_t K, int dx) {
-  const int64_t lanes = dx ? K : N, split = grouped_split(R, E, lanes, dx ? N : K);
-  return split == 1 ? 0 : static_cast<size_t>(split) * R * lanes * sizeof(float);
-}
-
 int moe_grouped_linear(const void* x, int64_t ld_x, const void* w, const void* offsets, int offsets_dtype, void* out,
-                       int64_t ld_out, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* workspace,
-                       size_t workspace_bytes, void* stream) {
+                       int64_t ld_out, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* stream) {
   clear_error();
-  return grouped_rows<kGroupedY>(x, ld_x, w, offsets, offsets_dtype, out, ld_out, R, E, N, K, dtype, zero_rest, workspace,
-                                 workspace_bytes, static_cast<cudaStream_t>(stream));
+  return grouped_rows<kGroupedY>(x, ld_x, w, offsets, offsets_dtype, out, ld_out, R, E, N, K, dtype, zero_rest,
+                                 static_cast<cudaStream_t>(stream));
 }
 
 int moe_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, const void* offsets, int offsets_dtype, void* dx,
-                          int64_t ld_dx, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* workspace,
-                          size_t workspace_bytes, void* stream) {
+                          int64_t ld_dx, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, int zero_rest, void* stream) {
   clear_error();
-  return grouped_rows<kGroupedDx>(dy, ld_dy, w, offsets, offsets_dtype, dx, ld_dx, R, E, N, K, dtype, zero_rest, workspace,
-                                  workspace_bytes, static_cast<cudaStream_t>(stream));
+  return grouped_rows<kGroupedDx>(dy, ld_dy, w, offsets, offsets_dtype, dx, ld_dx, R, E, N, K, dtype, zero_rest,
+                                  static_cast<cudaStream_t>(stream));
 }
 
 int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets, int offsets_dtype,
@@ -269,7 +217,6 @@ int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t 
   g.rows = R;
   g.lanes = static_cast<int>(K);
   g.cols = static_cast<int>(N);
-  g.split = 1;
   g.out = dw;
   g.ld_out = K;
   if (dtype == MOE_F16)
@@ -317,8 +264,7 @@ int moe_int8_linear(const void* x, int64_t ld_x, const float* x_scale, const voi
   const int64_t blocks = (K + 127) / 128, split = int8_split(M, N, K);
   GroupedArgs g{};
   g.split_blocks = static_cast<int>((blocks + split - 1) / split);
-  g.split = static_cast<int>((blocks + g.split_blocks - 1) / g.split_blocks);  // no empty slices
-  g.E = 1;
+  g.E = g.split = static_cast<int>((blocks + g.split_blocks - 1) / g.split_blocks);  // no empty slices
   g.rows = M;
   g.lanes = static_cast<int>(N);
   g.red = static_cast<int>(K);

@@ -64,7 +64,7 @@ constexpr int kGgSmemBytes = 1024 + kGgRingBytes + kGgOutBytes + 256 + kGgTableI
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
 struct GroupedArgs {
-  const void* offsets;   // [E + 1] int32 / int64; int8: unused, all rows are one group
+  const void* offsets;   // [E + 1] int32 / int64; int8: unused
   int offsets64;
   int E;
   int64_t rows;          // R
@@ -76,7 +76,7 @@ struct GroupedArgs {
   int64_t ld_out;
   int zero_rest;         // rows of no group are cleared
   int out16;             // out's rows start on 16 bytes, and lanes come in whole 16 bytes
-  int split, split_blocks;  // not Dw: slices of the reduction, blocks of each; slice i writes rows [i rows, (i + 1) rows) of out
+  int split, split_blocks;  // int8: slices of the reduction, blocks of each; slice i writes rows [i rows, (i + 1) rows)
   const float* lane_scale;  // int8: ws
   const float* col_scale;   // int8: xs
   const float* bias;        // int8, or null
@@ -141,7 +141,6 @@ __device__ __forceinline__ bool elect_one() {
 struct GroupedTile {
   int e, lane0, halves, ncols;
   int64_t row0;
-  int slice;       // of the reduction
   int part, more;  // of a 32-bit dW: its number, and whether others follow
   int col0, kb0, kblocks, tail;  // tail: reduction rows or elements in the last block (0: it is full)
 };
@@ -160,12 +159,10 @@ __device__ __forceinline__ int gg_col_step(int rows) {  // columns per tile of a
 // beside a rounding to 16 bits. For a 32-bit dW (PARTS) a tile's rows are taken in equal parts of at most 768, whose sums the epilogue
 // adds to those before, rounding; the same thread reads what it wrote, while the next MMAs run. The error then stays below 1e-6 for any
 // number of rows (4064 rows of 8 experts, 4096 x 14336: 565 -> 619 us; 8192 rows of one, 8192 x 8192: 780 -> 1220 us).
-//
-// SLICED: the reduction is cut into slices of whole blocks, each a tile of its own.
-template <int KIND, bool PARTS, bool SLICED>
+template <int KIND, bool PARTS>
 struct GroupedSchedule {
   const int *prefix, *start, *rows;  // tiles before group e, its first row, its rows
-  int E, lanes, tile_lanes, lane_tiles, red_blocks, red_tail, cols, split, split_blocks, e;
+  int E, lanes, tile_lanes, lane_tiles, red_blocks, red_tail, cols, split_blocks, e;
   int whole, left, lane_parts, col_parts;  // tiles of whole rounds; the others, and what each is cut into
   int parts = 1;                           // of the rows of the last tile that was asked for
 
@@ -180,8 +177,7 @@ struct GroupedSchedule {
     constexpr int kRed = KIND == kDenseInt8 ? 128 : 64;
     red_blocks = (a.red + kRed - 1) / kRed;
     red_tail = a.red % kRed;
-    split = a.split;
-    split_blocks = a.split_blocks;
+    split_blocks = KIND == kDenseInt8 ? a.split_blocks : red_blocks;
     cols = a.cols;
     e = 0;
     left = prefix[E] % npairs;
@@ -209,7 +205,7 @@ struct GroupedSchedule {
     t.e = e;
     i -= prefix[e];
     const int n = rows[e];
-    t.kb0 = t.slice = 0;
+    t.kb0 = 0;
     if (KIND == kGroupedDw) {
       const int col_tiles = (cols + kGgTile - 1) / kGgTile;
       t.lane0 = i / col_tiles * tile_lanes;
@@ -219,10 +215,6 @@ struct GroupedSchedule {
       t.kblocks = (n + 63) / 64;
       t.tail = n % 64;
     } else {
-      if (SLICED) {
-        t.slice = i % split;
-        i /= split;
-      }
       const int step = gg_col_step(n), col_tiles = (n + step - 1) / step;
       const int band = i / (lane_tiles * kGgBand);
       i -= band * lane_tiles * kGgBand;
@@ -234,10 +226,10 @@ struct GroupedSchedule {
       t.col0 = 0;
       t.kblocks = red_blocks;
       t.tail = red_tail;
-      if (SLICED) {
-        t.kb0 = t.slice * split_blocks;
+      if (KIND == kDenseInt8) {  // group e is a slice of the reduction
+        t.kb0 = e * split_blocks;
         t.kblocks = min(split_blocks, red_blocks - t.kb0);
-        if (t.slice < split - 1) t.tail = 0;
+        if (e < E - 1) t.tail = 0;
       }
     }
     t.halves = min(tile_lanes, lanes - t.lane0) > kGgHalf ? 2 : 1;
@@ -334,12 +326,17 @@ __device__ __forceinline__ void gg_build_table(const GroupedArgs& a, int* table,
     int n = 0, tiles = 0;
     if (e < a.E) {
       int64_t s = 0, t = a.rows;
-      if (KIND != kDenseInt8) {
+      if (KIND == kDenseInt8) {  // the slices' rows, one after another
+        s = e * a.rows;
+        t = s + a.rows;
+      } else {
         s = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[e] : static_cast<const int32_t*>(a.offsets)[e];
         t = a.offsets64 ? static_cast<const int64_t*>(a.offsets)[e + 1] : static_cast<const int32_t*>(a.offsets)[e + 1];
       }
-      s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
-      t = t < s ? s : (t > a.rows ? a.rows : t);
+      if (KIND != kDenseInt8) {
+        s = s < 0 ? 0 : (s > a.rows ? a.rows : s);
+        t = t < s ? s : (t > a.rows ? a.rows : t);
+      }
       n = static_cast<int>(t - s);
       start[e] = static_cast<int>(s);
       rows[e] = n;
@@ -347,7 +344,7 @@ __device__ __forceinline__ void gg_build_table(const GroupedArgs& a, int* table,
         tiles = dw_tiles;
       } else if (n > 0) {
         const int step = gg_col_step(n);
-        tiles = lane_tiles * ((n + step - 1) / step) * a.split;
+        tiles = lane_tiles * ((n + step - 1) / step);
       }
     }
     int incl = tiles;
@@ -372,7 +369,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   constexpr bool kDw = KIND == kGroupedDw;
   constexpr bool kInt8 = KIND == kDenseInt8;
   constexpr bool kScaled = kInt8 && !std::is_same<OutT, int>::value;  // int: a slice's sums as they are
-  constexpr bool kSliced = kInt8 ? std::is_same<OutT, int>::value : !kDw && sizeof(OutT) == 4;
   constexpr bool kMnA = KIND == kGroupedDx || kDw;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kRed = kInt8 ? 128 : 64;   // reduction elements per block
@@ -423,7 +419,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  GroupedSchedule<KIND, kDw && sizeof(OutT) == 4, kSliced> sched(args, table, npairs);
+  GroupedSchedule<KIND, kDw && sizeof(OutT) == 4> sched(args, table, npairs);
   const int tiles = sched.tiles();
 
   if (warp == 0) {
@@ -467,14 +463,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
                   tma_load_2d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, row, pol);
               }
             } else {
-              const int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half, k0 = (t.kb0 + kb) * kRed;
+              int row = static_cast<int>(t.row0) + static_cast<int>(rank) * half, z = t.e;
+              const int k0 = (t.kb0 + kb) * kRed;
+              if constexpr (kInt8) {
+                row -= t.e * static_cast<int>(args.rows);
+                z = 0;
+              }
               mbar_arrive_expect_tx_cluster(bar, t.halves * kGgOperandBytes + (boxes ? boxes * 4096 : kGgOperandBytes));
               if constexpr (kMnA) {
                 for (int c = 0; c < 2 * t.halves; ++c)
-                  tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, k0, t.e, pol);
+                  tma_load_3d_pair(a + c * 8192, &tmA, bar, lane0 + (c >> 1) * kGgHalf + (c & 1) * 64, k0, z, pol);
               } else {
                 for (int h = 0; h < t.halves; ++h)
-                  tma_load_3d_pair(a + h * kGgOperandBytes, &tmA, bar, k0, lane0 + h * kGgHalf, t.e, pol);
+                  tma_load_3d_pair(a + h * kGgOperandBytes, &tmA, bar, k0, lane0 + h * kGgHalf, z, pol);
               }
               if (boxes == 0) tma_load_2d_pair(b, &tmB, bar, k0, row, pol);
               for (int i = 0; i < boxes; ++i) tma_load_2d_pair(b + i * 4096, &tmB32, bar, k0, row + i * 32, pol);
@@ -637,7 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     for (int tile = pair, row_part = 0; tile < tiles && ok; sched.next(tile, row_part, npairs)) {
       const GroupedTile t = sched.get(tile, row_part);
       if (t.ncols == 0) continue;
-      int64_t at = ((kSliced ? t.slice * args.rows : 0) + t.row0) * args.ld_out;
+      int64_t at = (t.row0 * args.ld_out);
       if (kDw) at = (static_cast<int64_t>(t.e) * args.cols + t.col0) * args.ld_out;
       // this warp's columns: even shares of what there is, in whole pieces of 32
       const int share = (t.ncols + 63) / 64 * 32;
@@ -793,37 +794,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
-  }
-}
-
-// The slices' fp32 sums [split][R][width] of rows of experts, added in order and rounded; rows of no expert as the products
-// leave them. 4 columns a thread (width is a multiple of 8); VEC: out can be stored 8 bytes at a time.
-template <bool VEC, typename OutT>
-__global__ void __launch_bounds__(256) grouped_join_kernel(const float* __restrict__ sums, int split, const void* offsets,
-                                                           int offsets64, int E, int64_t rows, int width, OutT* __restrict__ out,
-                                                           int64_t ld_out, int zero_rest) {
-  const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
-  if (c >= width) return;
-  int64_t s = offsets64 ? static_cast<const int64_t*>(offsets)[0] : static_cast<const int32_t*>(offsets)[0];
-  int64_t e = offsets64 ? static_cast<const int64_t*>(offsets)[E] : static_cast<const int32_t*>(offsets)[E];
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const bool inside = r >= s && r < e;
-    if (!inside && !zero_rest) continue;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (inside) {
-      const float* p = sums + r * width + c;
-      for (int i = 0; i < split; ++i, p += rows * width) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(p));
-        v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-      }
-    }
-    OutT* o = out + r * ld_out + c;
-    if constexpr (VEC) {
-      *reinterpret_cast<uint2*>(o) = make_uint2(gg_pack<OutT>(v[0], v[1]), gg_pack<OutT>(v[2], v[3]));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = gg_cast<OutT>(v[j]);
-    }
   }
 }
 

@@ -16,7 +16,6 @@ from . import _lib
 from ._args import FLOATS, HALVES, IDS, empty2, launch, matrix, once_differentiable, overlap, pitch, require, rows
 from .fused import _workspace
 from .rows8 import Q_DTYPES, Rows8, restore_rows8, save_rows8, silu_backward, silu_forward
-from .w4 import _workspace_bytes
 
 
 def _operand(t: torch.Tensor, name: str, dtype: torch.dtype, index: int, width: int, R: Optional[int] = None) -> tuple:
@@ -60,10 +59,8 @@ def _rows_product(name: str, x: torch.Tensor, x_name: str, w: torch.Tensor, offs
         require(R < 2 or ld_out >= width, "rows of out must not overlap")
         for t in (x, w.view(1, -1), offsets.view(1, -1)):
             require(not overlap(out, t), "out must not share memory with the inputs")
-    nbytes = _workspace_bytes("moe_grouped_linear_workspace_bytes", R, E, N, K, int(transposed))
-    ws = _workspace(nbytes, dev) if nbytes else None  # held until the call has been launched
     launch(dev, name, ptr, ld, w_ptr, offsets.data_ptr(), IDS[offsets.dtype], out.data_ptr(), ld_out, R, E, N, K, HALVES[dtype],
-           zero_rest, None if ws is None else ws.data_ptr(), nbytes)
+           zero_rest)
     return out
 
 

@@ -256,43 +256,3 @@ def test_long_sums_in_32_bits(cuda_device, dtype):
     assert bool((dw[1] == 0).all())
     again = m.grouped_linear_backward(dy, x, torch.empty(3, N, K, dtype=dtype, device="cuda"), offsets, dw_dtype=F32, need_dx=False)[1]
     assert torch.equal(dw, again)
-
-
-# rows of the experts, N, K: few rows, and sums long enough to be taken in slices (of y, of dx, of both)
-@pytest.mark.parametrize("sizes,N,K", [([1], 8, 2048), ([0, 2, 1], 64, 13000), ([3, 0, 4], 13000, 64), ([1, 1], 4104, 4104),
-                                       ([8000], 64, 3208), ([9000], 3400, 72), ([300, 0, 17], 264, 2056), ([5] * 3, 1032, 4104)])
-@pytest.mark.parametrize("dtype", [F16, BF16])
-def test_sums_in_slices(cuda_device, sizes, N, K, dtype):
-    """At most 16 slices: each has one short step at most (16 of the tolerance's steps), and 15 additions with a rounding of 2^-24 of S
-    join them (less than 4 steps): 20 steps, as 320 terms more would have."""
-    x, w, dy, offsets = make(sizes, N, K, dtype)
-    ends = offsets.tolist()
-    inside = torch.zeros(x.shape[0], 1, dtype=torch.bool, device="cuda")
-    inside[ends[0]:ends[-1]] = True
-    ref_y, ref_dx = grouped_ref(torch.where(inside, x, 0), w, offsets), grouped_ref(torch.where(inside, dy, 0), w.mT, offsets)
-    y = m.grouped_linear(x, w, offsets)
-    dx, _ = m.grouped_linear_backward(dy, x, w, offsets, need_dw=False)
-    within(y, *ref_y, K + 320, "y")
-    within(dx, *ref_dx, N + 320, "dx")
-    assert not bool(y[~inside[:, 0]].any()) and not bool(dx[~inside[:, 0]].any())
-    assert torch.equal(y, m.grouped_linear(x, w, offsets))
-    for start, pitch in ((0, N + 8), (3, N + 5), (2, N + 2)):  # rows that are given keep what is not an expert's
-        out = torch.full((x.shape[0], pitch + 8), 7.0, dtype=dtype, device="cuda")
-        view = out[:, start:start + N]
-        assert m.grouped_linear(x, w, offsets, out=view) is view
-        assert torch.equal(view[ends[0]:ends[-1]], y[ends[0]:ends[-1]])
-        view[ends[0]:ends[-1]] = 7.0
-        assert bool((out == 7.0).all())
-    x2, w2 = x.clone(), w.clone()
-    with torch.no_grad():  # captured: the slices' sums belong to the graph
-        s = torch.cuda.Stream()
-        s.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(s):
-            m.grouped_linear(x2, w2, offsets)
-        torch.cuda.current_stream().wait_stream(s)
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
-            z = m.grouped_linear(x2, w2, offsets)
-    graph.replay()
-    assert torch.equal(z, y)
-    assert m.device_status() == 0
