@@ -560,7 +560,8 @@ MOE_API int moe_fused_w4(const void* hidden_states, int64_t ld_hidden, const voi
  *   moe_grouped_linear_dw:  dw[e] = sum_r dy[r] x[r]^T over e's rows, 0 without rows; dw [E, N, K] contiguous in
  *                           dtype or MOE_F32
  * Rows of no expert (before offsets[0], from offsets[E] on): 0 where zero_rest != 0, else left as they are; what
- * they hold is never used. Offsets outside [0, R] are clamped. Sums in fp32, one rounding; the same bits on every run.
+ * they hold is never used. Offsets outside [0, R] are clamped. Sums in fp32, one rounding; the same bits on every run,
+ * and for a row of y or dx whatever the other rows are and however many.
  * Requirements: dtype MOE_F16 / MOE_BF16; 1 <= E <= 1024; N and K multiples of 8; x, dy and w on 16-byte boundaries,
  *   row pitches (in elements) of x and dy multiples of 8; outputs share no memory with inputs.
  * ---------------------------------------------------------------------------------------- */

@@ -116,7 +116,8 @@ def grouped_linear(
     x [R, K] fp16 / bf16 with rows of any pitch that is a multiple of 8, w [E, N, K] (N and K multiples of 8,
     E <= 1024), offsets [E + 1] int32 / int64, not falling (``moe_align(ids, E, 1).group_offsets``). Rows of no
     expert, before offsets[0] or from offsets[E] on, are 0 in a new result and left as they are in ``out``; what they
-    hold in x is not used. Sums in fp32, rounded once; the same bits on every run.
+    hold in x is not used. Sums in fp32, rounded once; the same bits on every run, and for a row whatever the others are
+    and however many.
 
     Differentiable once in x and w (``out`` is not). ``save=torch.int8`` or ``torch.float8_e4m3fn``: x is kept for the
     gradient of w as an 8-bit copy (:func:`save_rows8`).

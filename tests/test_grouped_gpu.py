@@ -256,3 +256,22 @@ def test_long_sums_in_32_bits(cuda_device, dtype):
     assert bool((dw[1] == 0).all())
     again = m.grouped_linear_backward(dy, x, torch.empty(3, N, K, dtype=dtype, device="cuda"), offsets, dw_dtype=F32, need_dx=False)[1]
     assert torch.equal(dw, again)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("N,K", [(64, 13000), (4104, 1544), (264, 4096)])
+def test_a_row_does_not_depend_on_the_others(cuda_device, N, K, dtype):
+    """The same bits of y and dx for one row, a few and thousands, which take tiles of other sizes and cuts."""
+    x, w, dy, _ = make([0, 4700], N, K, dtype, 0, 0)
+
+    def products(rows):
+        offsets = torch.tensor([0, 0, rows], dtype=torch.int32).cuda()
+        return m.grouped_linear(x[:rows], w, offsets), m.grouped_linear_backward(dy[:rows], None, w, offsets, need_dw=False)[0]
+
+    y, dx = products(4700)
+    for rows in (1, 2, 33, 300, 1100, 2600):
+        y2, dx2 = products(rows)
+        assert torch.equal(y[:rows], y2) and torch.equal(dx[:rows], dx2), rows
+    first = torch.tensor([0, 1000, 4700], dtype=torch.int64).cuda()
+    y2 = m.grouped_linear(x, w[1:].expand(2, N, K).contiguous(), first)
+    assert torch.equal(y, y2)
