@@ -648,9 +648,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
         const int f0 = t.lane0 + half * kGgHalf + static_cast<int>(rank) * 128 + q * 32, f = f0 + lane;
         const bool there = f < args.lanes;
         OutT* p = out + at + f;
-        if (t.kblocks == 0) {  // an expert without rows: dW = 0
-          if (there)
+        if (t.kblocks == 0) {  // an expert without rows: dW = 0, in whole rows of this CTA's 128 lanes (64 experts, 7168 x 2048 in
+                               // 16 bits, none with rows: 312 us; 570 in a warp's 32 lanes)
+          constexpr int kRow = 8 * sizeof(OutT);  // threads a row
+          const int thread = q * 32 + lane, l = f0 - q * 32 + thread % kRow * (16 / static_cast<int>(sizeof(OutT)));
+          if (args.out16) {
+            if (l < args.lanes)
+              for (int c = from + thread / kRow; c < to; c += 128 / kRow)
+                gg_store16<kDw>(out + at + l + c * args.ld_out, make_uint4(0, 0, 0, 0));
+          } else if (there) {
             for (int c = from; c < to; ++c) p[c * args.ld_out] = gg_cast<OutT>(0.0f);
+          }
           continue;
         }
         // the sums of the parts before, written by this thread: asked for one step of columns ahead
