@@ -109,6 +109,12 @@ def once_differentiable(name: str, grads: tuple, *sources):
                           *sources)
 
 
+def graph_link(t: torch.Tensor) -> torch.Tensor:
+    """A tensor without elements that leads to `t` in the graph and holds nothing of its memory: the source that an operator
+    gives :func:`once_differentiable` in place of an input that it does not keep as it is."""
+    return t[:0].clone()
+
+
 def without_gradient(name: str, results: tuple, *sources):
     """The results of an operator that has no gradient. Where `sources` ask for one, going back through the
     results raises instead of leaving its part out."""

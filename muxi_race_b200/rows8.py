@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty_of, launch, matrix, once_differentiable, overlap, require, without_gradient
+from ._args import FLOATS, HALVES, IDS, empty_of, graph_link, launch, matrix, once_differentiable, overlap, require, without_gradient
 
 GROUP = 128
 Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -183,21 +183,21 @@ def silu_backward(dh, gate_up, weights, dweights, at=None, valid=None):
 
 class _SiluMul(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gate_up, row_weights, q_dtype):
+    def forward(ctx, gate_up, row_weights, q_dtype, link):
         h, saved = silu_forward(gate_up, row_weights, q_dtype)
         if saved is None:
-            ctx.save_for_backward(gate_up, None, row_weights)
+            ctx.save_for_backward(gate_up, None, row_weights, None)
         else:
-            ctx.save_for_backward(saved.q, saved.scale, row_weights)
+            ctx.save_for_backward(saved.q, saved.scale, row_weights, link)
         return h
 
     @staticmethod
     def backward(ctx, dh):
-        a, scale, row_weights = ctx.saved_tensors
+        a, scale, row_weights, link = ctx.saved_tensors
         gate_up = a if scale is None else Rows8(a, scale, dh.dtype, 2)
         dgate_up, dweights, _ = silu_mul_backward(dh.contiguous(), gate_up, row_weights)
-        grads = once_differentiable("silu_mul", (dgate_up,) if dweights is None else (dgate_up, dweights), dh, a, row_weights)
-        return grads[0], (grads[1] if dweights is not None else None), None
+        grads = once_differentiable("silu_mul", (dgate_up,) if dweights is None else (dgate_up, dweights), dh, a, row_weights, link)
+        return grads[0], (grads[1] if dweights is not None else None), None, None
 
 
 def silu_mul(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = None, save: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -209,7 +209,7 @@ def silu_mul(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = None, 
     """
     require(save is None or save in Q_DTYPES, "save must be None, torch.int8 or torch.float8_e4m3fn")
     if torch.is_grad_enabled() and (gate_up.requires_grad or (row_weights is not None and row_weights.requires_grad)):
-        return _SiluMul.apply(gate_up, row_weights, save)
+        return _SiluMul.apply(gate_up, row_weights, save, None if save is None else graph_link(gate_up))
     return silu_forward(gate_up, row_weights, None)[0]
 
 
