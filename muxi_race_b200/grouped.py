@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, launch, matrix, once_differentiable, overlap, pitch, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, graph_link, launch, matrix, once_differentiable, overlap, pitch, require, rows
 from .fused import _workspace
 from .rows8 import Q_DTYPES, Rows8, restore_rows8, save_rows8, silu_backward, silu_forward
 
@@ -83,25 +83,25 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, offsets, save):
+    def forward(ctx, x, w, offsets, save, link):
         y = _rows_product("moe_grouped_linear", x, "x", w, offsets, False)
         if save is None or not ctx.needs_input_grad[1]:
-            ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, None, w, offsets)
+            ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, None, w, offsets, None)
         else:
             with torch.no_grad():
                 saved = save_rows8(x, save)
-            ctx.save_for_backward(saved.q, saved.scale, w, offsets)
+            ctx.save_for_backward(saved.q, saved.scale, w, offsets, link)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        a, scale, w, offsets = ctx.saved_tensors
+        a, scale, w, offsets, link = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
         with torch.no_grad():
             x = a if scale is None else Rows8(a, scale, w.dtype)
             grads = grouped_linear_backward(_aligned(dy), x, w, offsets, need_dx=need_dx, need_dw=need_dw)
-        done = iter(once_differentiable("grouped_linear", tuple(g for g in grads if g is not None), dy, a, w))
-        return tuple(None if g is None else next(done) for g in grads) + (None, None)
+        done = iter(once_differentiable("grouped_linear", tuple(g for g in grads if g is not None), dy, a, w, link))
+        return tuple(None if g is None else next(done) for g in grads) + (None, None, None)
 
 
 def grouped_linear(
@@ -125,7 +125,7 @@ def grouped_linear(
     require(save is None or save in Q_DTYPES, "save must be None, torch.int8 or torch.float8_e4m3fn")
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         require(out is None, "out is not differentiable")
-        return _GroupedLinear.apply(x, w, offsets, save)
+        return _GroupedLinear.apply(x, w, offsets, save, None if save is None else graph_link(x))
     return _rows_product("moe_grouped_linear", x, "x", w, offsets, False, out, out is None)
 
 

@@ -3,7 +3,7 @@ else needs a gradient. The kernels are replaced by CPU functions that, like them
 import pytest
 import torch
 
-from muxi_race_b200 import rows8
+from muxi_race_b200 import grouped, rows8
 
 SAVES = (None, torch.int8, torch.float8_e4m3fn)
 
@@ -42,3 +42,34 @@ def test_silu_mul(monkeypatch, save, square, weights):
     h = rows8.silu_mul(gate_up, w, save=save)
     h.float().sum().backward()
     assert bool((gate_up.grad == 1).all())
+
+
+@pytest.mark.parametrize("save", SAVES)
+@pytest.mark.parametrize("square", [False, True])
+@pytest.mark.parametrize("frozen", [False, True])  # x itself
+def test_grouped_linear(monkeypatch, save, square, frozen):
+    def product(name, x, x_name, w, offsets, transposed, out=None, zero_rest=True):
+        with torch.no_grad():
+            return x @ w[0].T
+
+    def backward(dy, x, w, offsets, need_dx=True, need_dw=True):
+        with torch.no_grad():
+            return dy @ w[0] if need_dx else None, torch.ones_like(w) if need_dw else None
+
+    monkeypatch.setattr(grouped, "_rows_product", product)
+    monkeypatch.setattr(grouped, "grouped_linear_backward", backward)
+    monkeypatch.setattr(grouped, "save_rows8",
+                        lambda x, q_dtype: rows8.Rows8(torch.zeros(x.shape, dtype=q_dtype), torch.ones(x.shape[0], 1), x.dtype))
+    source = torch.randn(3, 8, requires_grad=True)  # what x comes from
+    w, offsets = torch.randn(1, 8, 8).bfloat16().requires_grad_(), torch.tensor([0, 3])
+    for leaf in (w,) if frozen else (source, w):
+        x = source.bfloat16().detach() if frozen else source.bfloat16()
+        y = grouped.grouped_linear(x, w, offsets, save=save)
+        # dw depends on x, dx on w: each derivative through the other one has to be noticed
+        g, = torch.autograd.grad((y.float().square() if square else y.float()).sum(), w, create_graph=True)
+        if not frozen or square:
+            with pytest.raises(RuntimeError, match="grouped_linear can be differentiated once"):
+                torch.autograd.grad(g.float().square().sum(), leaf, allow_unused=True)
+    x = source.bfloat16()
+    grouped.grouped_linear(x, w, offsets, save=save).float().sum().backward()
+    assert bool((w.grad == 1).all()) and source.grad is not None
