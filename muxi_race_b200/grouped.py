@@ -209,7 +209,7 @@ def _mlp_forward(x, w13, w2, ids, weights, save):
 
 class _MoeMlp(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w13, w2, ids, weights, save):
+    def forward(ctx, x, w13, w2, ids, weights, save, link):
         out, offsets, order, slot, gate_up = _mlp_forward(x, w13, w2, ids, weights, save)
         if save is None:
             kept = (x, None, gate_up, None)
@@ -217,15 +217,15 @@ class _MoeMlp(torch.autograd.Function):
             with torch.no_grad():
                 x8 = save_rows8(x, save)
             kept = (x8.q, x8.scale, gate_up.q, gate_up.scale)
-        ctx.save_for_backward(*kept, w13, w2, weights, offsets, order, slot)
+        ctx.save_for_backward(*kept, w13, w2, weights, offsets, order, slot, link)
         ctx.topk = ids.shape[1]
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        x, x_scale, gate_up, scale, w13, w2, weights, offsets, order, slot = ctx.saved_tensors
-        need_x, need_w13, need_w2, _, need_weights, _ = ctx.needs_input_grad
-        grads = [None] * 6
+        x, x_scale, gate_up, scale, w13, w2, weights, offsets, order, slot, link = ctx.saved_tensors
+        need_x, need_w13, need_w2, _, need_weights, *_ = ctx.needs_input_grad
+        grads = [None] * 7
         with torch.no_grad():
             kept = x
             if scale is not None:
@@ -246,8 +246,12 @@ class _MoeMlp(torch.autograd.Function):
             if need_w13:
                 grads[1] = _grouped_dw(dgate_up, _gather(x, order, topk, valid, R), w13.shape, offsets, w13.dtype)
             grads[4] = dweights
-        done = iter(once_differentiable("moe_mlp", tuple(g for g in grads if g is not None), dout, kept, w13, w2, weights))
+        done = iter(once_differentiable("moe_mlp", tuple(g for g in grads if g is not None), dout, kept, w13, w2, weights, link))
         return tuple(None if g is None else next(done) for g in grads)
+
+
+def _moe_mlp_graph(x, w13, w2, ids, weights, save):
+    return _MoeMlp.apply(x, w13, w2, ids, weights, save, None if save is None else graph_link(x))
 
 
 def moe_mlp(
@@ -294,5 +298,5 @@ def moe_mlp(
         raise ValueError("w_gate_up and w_down must start on 16 bytes")
     tensors = (hidden_states, w_gate_up, w_down, topk_weights)
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return _MoeMlp.apply(hidden_states, w_gate_up, w_down, topk_ids, topk_weights, save)
+        return _moe_mlp_graph(hidden_states, w_gate_up, w_down, topk_ids, topk_weights, save)
     return _mlp_forward(hidden_states, w_gate_up, w_down, topk_ids, topk_weights, None)[0]

@@ -73,3 +73,50 @@ def test_grouped_linear(monkeypatch, save, square, frozen):
     x = source.bfloat16()
     grouped.grouped_linear(x, w, offsets, save=save).float().sum().backward()
     assert bool((w.grad == 1).all()) and source.grad is not None
+
+
+class CpuMlp:
+    """The kernels of moe_mlp as CPU functions; one token is one route of one expert."""
+
+    def __init__(self, monkeypatch, T=3, H=8, I=4):
+        def half(*shape):
+            return torch.randn(shape).bfloat16()
+
+        self.sizes = T, H, I
+        self.args = [half(T, H), half(1, 2 * I, H), half(1, H, I), torch.zeros(T, 1, dtype=torch.int32), torch.rand(T, 1)]
+
+        def forward(x, w13, w2, ids, weights, save):
+            with torch.no_grad():
+                g, u = (x @ w13[0].T).chunk(2, -1)
+                out = weights.to(x.dtype) * (torch.nn.functional.silu(g) * u) @ w2[0].T
+                gate_up = torch.cat((g, u), -1)
+                if save is not None:
+                    gate_up = rows8.Rows8(torch.zeros(T, 2 * I, dtype=save), torch.ones(T, 2), x.dtype, 2)
+                return out, torch.tensor([0, T], dtype=torch.int32), torch.arange(T), torch.arange(T), gate_up
+
+        def silu_backward(dh, gate_up, weights, dweights, at=None, valid=None):
+            if dweights is not None:
+                dweights.fill_(1)
+            return half(T, 2 * I), half(T, I)
+
+        monkeypatch.setattr(grouped, "_mlp_forward", forward)
+        monkeypatch.setattr(grouped, "silu_backward", silu_backward)
+        monkeypatch.setattr(grouped, "_gather", lambda x, *a: half(T, H))
+        monkeypatch.setattr(grouped, "_combine", lambda y, *a: half(T, H))
+        monkeypatch.setattr(grouped, "_rows_product", lambda name, dy, n, w, *a: half(T, w.shape[2]))
+        monkeypatch.setattr(grouped, "_grouped_dw", lambda dy, x, shape, offsets, dt: torch.ones(shape, dtype=dt))
+        monkeypatch.setattr(grouped, "save_rows8",
+                            lambda x, q_dtype: rows8.Rows8(torch.zeros(x.shape, dtype=q_dtype), torch.ones(x.shape[0], 1), x.dtype))
+
+
+@pytest.mark.parametrize("save", SAVES)
+@pytest.mark.parametrize("square", [False, True])
+@pytest.mark.parametrize("trained", [(0,), (0, 1), (0, 2), (0, 4), (1, 4), (0, 1, 2, 4)])  # x, w13, w2, weights
+def test_moe_mlp(monkeypatch, save, square, trained):
+    cpu = CpuMlp(monkeypatch)
+    for leaf in trained:
+        args = [t.clone().requires_grad_() if i in trained else t for i, t in enumerate(cpu.args)]
+        with pytest.raises(RuntimeError, match="moe_mlp can be differentiated once"):
+            second(grouped._moe_mlp_graph(*args, save), args[leaf], square)
+    grouped._moe_mlp_graph(*args, save).float().sum().backward()
+    assert all(args[i].grad is not None for i in trained)
