@@ -211,12 +211,15 @@ class _MoeMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, w2, ids, weights, save, link):
         out, offsets, order, slot, gate_up = _mlp_forward(x, w13, w2, ids, weights, save)
-        if save is None:
-            kept = (x, None, gate_up, None)
-        else:
-            with torch.no_grad():
-                x8 = save_rows8(x, save)
-            kept = (x8.q, x8.scale, gate_up.q, gate_up.scale)
+        kept = None, None  # x is read for w13's gradient only
+        if ctx.needs_input_grad[1]:
+            if save is None:
+                kept = x, None
+            else:
+                with torch.no_grad():
+                    x8 = save_rows8(x, save)
+                kept = x8.q, x8.scale
+        kept += (gate_up, None) if save is None else (gate_up.q, gate_up.scale)
         ctx.save_for_backward(*kept, w13, w2, weights, offsets, order, slot, link)
         ctx.topk = ids.shape[1]
         return out
@@ -228,8 +231,10 @@ class _MoeMlp(torch.autograd.Function):
         grads = [None] * 7
         with torch.no_grad():
             kept = x
+            if x_scale is not None:
+                x = Rows8(x, x_scale, w13.dtype)
             if scale is not None:
-                x, gate_up = Rows8(x, x_scale, w13.dtype), Rows8(gate_up, scale, w13.dtype, 2)
+                gate_up = Rows8(gate_up, scale, w13.dtype, 2)
             T, topk, E = dout.shape[0], ctx.topk, w13.shape[0]
             R, valid = T * topk, offsets.data_ptr() + 4 * E
             dy = _gather(_aligned(dout), order, topk, valid, R)
@@ -251,7 +256,8 @@ class _MoeMlp(torch.autograd.Function):
 
 
 def _moe_mlp_graph(x, w13, w2, ids, weights, save):
-    return _MoeMlp.apply(x, w13, w2, ids, weights, save, None if save is None else graph_link(x))
+    link = None if save is None and w13.requires_grad else graph_link(x)  # None: x itself is kept
+    return _MoeMlp.apply(x, w13, w2, ids, weights, save, link)
 
 
 def moe_mlp(
@@ -269,7 +275,7 @@ def moe_mlp(
     first), w_down [E, H, I], H and I multiples of 8, E <= 1024; topk_ids [T, k] int32 / int64, topk_weights [T, k] fp32 / fp16 /
     bf16. The same bits on every run, forward and backward.
 
-    For the backward pass the call keeps hidden_states and gate_up [T k, 2 I]; with ``save=torch.int8`` or
+    For the backward pass the call keeps gate_up [T k, 2 I] and, for w_gate_up's gradient, hidden_states; with ``save=torch.int8`` or
     ``torch.float8_e4m3fn`` as 8-bit copies (half the memory), from which the gradients of the weights and of the activation
     are then taken. The rows between the products are rounded to the dtype (in fp16 values beyond 65504 become
     infinite); the routing weight is applied in front of the down product.

@@ -120,3 +120,19 @@ def test_moe_mlp(monkeypatch, save, square, trained):
             second(grouped._moe_mlp_graph(*args, save), args[leaf], square)
     grouped._moe_mlp_graph(*args, save).float().sum().backward()
     assert all(args[i].grad is not None for i in trained)
+
+
+@pytest.mark.parametrize("save", SAVES)
+@pytest.mark.parametrize("trained", [(0,), (2,), (4,), (0, 2, 4), (1,), (0, 1)])
+def test_moe_mlp_keeps_tokens_for_their_gradient_only(monkeypatch, save, trained):
+    """The tokens, or their copy, are read for the gradient of w_gate_up: without that nothing of their size is kept for them."""
+    cpu = CpuMlp(monkeypatch, T=5, H=24, I=4)
+    copies = []
+    copy = grouped.save_rows8
+    monkeypatch.setattr(grouped, "save_rows8", lambda x, q_dtype: copies.append(x) or copy(x, q_dtype))
+    args = [t.clone().requires_grad_() if i in trained else t for i, t in enumerate(cpu.args)]
+    out = grouped._moe_mlp_graph(*args, save)
+    tokens = [t for t in out.grad_fn.saved_tensors if t is not None and t.shape == (5, 24)]
+    assert len(tokens) == (1 in trained) and len(copies) == (1 in trained and save is not None)
+    out.float().sum().backward()
+    assert all(args[i].grad is not None for i in trained)
