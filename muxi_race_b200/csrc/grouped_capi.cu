@@ -7,9 +7,10 @@
 namespace moe {
 namespace {
 
-constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 1;
-
-
+constexpr int64_t kMaxTiles = (int64_t(1) << 31) - 1;
+// Of rows, lanes and the reduction: the kernels round them up to whole tiles and blocks in 32 bits.
+constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 2 * kGgHalf;
+static_assert(kMaxExtent + kGgTile <= kMaxTiles && kMaxExtent + 2 * kGgHalf - 1 <= kMaxTiles, "a rounded extent has to fit an int");
 
 int check_grouped(const void* offsets, int offsets_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype) {
   if (dtype != MOE_F16 && dtype != MOE_BF16) return fail(MOE_ERR_INVALID_ARG, "dtype must be MOE_F16 or MOE_BF16");
@@ -18,7 +19,7 @@ int check_grouped(const void* offsets, int offsets_dtype, int64_t R, int64_t E, 
   if (!offsets) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
   if (E < 1 || E > kGgMaxExperts) return fail(MOE_ERR_INVALID_ARG, "num_experts must be in [1, %d]", kGgMaxExperts);
   if (N < 8 || K < 8 || N % 8 != 0 || K % 8 != 0 || N > kMaxExtent || K > kMaxExtent)
-    return fail(MOE_ERR_INVALID_ARG, "out_features and in_features must be positive multiples of 8");
+    return fail(MOE_ERR_INVALID_ARG, "out_features and in_features must be positive multiples of 8 up to 2^31 - 512");
   if (R < 0 || R > kMaxExtent) return fail(MOE_ERR_INVALID_ARG, "bad row count");
   return MOE_OK;
 }
@@ -72,7 +73,7 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   // A dW in parts: with the two accumulators in turn a part's sums are added while the next one's MMAs run (4096^3:
   // 158 us, with 512 lanes 188 us).
   if (KIND == kGroupedDw && sizeof(OutT) == 4 && args.rows / args.E > 64 * kGgChunk) args.halves = 1;
-  if (lane_tiles(args.halves) * most > kMaxExtent) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
+  if (lane_tiles(args.halves) * most > kMaxTiles) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
   if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;
   constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT>;
   MOE_TRY(allow_smem<kernel>(dev));
