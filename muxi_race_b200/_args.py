@@ -3,6 +3,7 @@ host time of a call counts)."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -107,6 +108,16 @@ def once_differentiable(name: str, grads: tuple, *sources):
         return grads
     return _NoGraph.apply(f"{name} can be differentiated once: its gradient comes from a kernel without a graph", grads,
                           *sources)
+
+
+def no_tangents(name: str, *tensors) -> None:
+    """Raises where one of `tensors` carries a forward-mode tangent: it has requires_grad False and the address of its values, so
+    the kernel would pass for a constant what depends on it."""
+    if forward_ad._current_level < 0:  # no level is open
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def graph_link(t: torch.Tensor) -> torch.Tensor:

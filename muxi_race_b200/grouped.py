@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, graph_link, launch, matrix, once_differentiable, overlap, pitch, require, rows
+from ._args import FLOATS, HALVES, IDS, empty2, graph_link, launch, matrix, no_tangents, once_differentiable, overlap, pitch, require, rows
 from .fused import _workspace
 from .rows8 import Q_DTYPES, Rows8, restore_rows8, save_rows8, silu_backward, silu_forward
 
@@ -123,6 +123,7 @@ def grouped_linear(
     gradient of w as an 8-bit copy (:func:`save_rows8`).
     """
     require(save is None or save in Q_DTYPES, "save must be None, torch.int8 or torch.float8_e4m3fn")
+    no_tangents("grouped_linear", x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         require(out is None, "out is not differentiable")
         return _GroupedLinear.apply(x, w, offsets, save, None if save is None else graph_link(x))
@@ -143,6 +144,7 @@ def grouped_linear_backward(
     Returns ``(dx, dw)``, None for what is not asked for. x [R, K] or its :class:`Rows8` (not needed without dw); dw in
     w's dtype or ``torch.float32``, 0 for an expert without rows. Rows of no expert take no part, and their dx is 0.
     """
+    no_tangents("grouped_linear_backward", dy, x.scale if isinstance(x, Rows8) else x, w)
     E, N, K, _, dev = _check(w, offsets)
     if dw_dtype is None:
         dw_dtype = w.dtype
@@ -281,6 +283,7 @@ def moe_mlp(
     infinite); the routing weight is applied in front of the down product.
     """
     require(save is None or save in Q_DTYPES, "save must be None, torch.int8 or torch.float8_e4m3fn")
+    no_tangents("moe_mlp", hidden_states, w_gate_up, w_down, topk_weights)
     if w_gate_up.dim() != 3 or w_down.dim() != 3 or hidden_states.dim() != 2:
         raise ValueError("hidden_states must be [T, H], w_gate_up [E, 2I, H] and w_down [E, H, I]")
     E, two_i, H = w_gate_up.shape

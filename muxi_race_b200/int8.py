@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 
-from ._args import FLOATS, empty2, launch, matrix, overlap, pitch, require, rows, without_gradient
+from ._args import FLOATS, empty2, launch, matrix, no_tangents, overlap, pitch, require, rows, without_gradient
 from .fused import _workspace
 from .w4 import _workspace_bytes as workspace_bytes
 
@@ -30,6 +30,7 @@ def int8_linear(
     bias are applied in fp32, one rounding. ``out`` (rows of any pitch) must not share memory with x. Not differentiable: a
     backward pass that meets the result raises (``out`` carries no graph).
     """
+    no_tangents("int8_linear", x_scale, w_scale, bias)
     if w.dim() != 2 or w.dtype != torch.int8 or not w.is_cuda or not w.is_contiguous() or w.data_ptr() % 16:
         raise ValueError("w must be a contiguous int8 CUDA tensor [N, K] that starts on 16 bytes")
     N, K = w.shape

@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty_of, graph_link, launch, matrix, once_differentiable, overlap, require, without_gradient
+from ._args import FLOATS, HALVES, IDS, empty_of, graph_link, launch, matrix, no_tangents, once_differentiable, overlap, require, without_gradient
 
 GROUP = 128
 Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -80,6 +80,7 @@ def save_rows8(x: torch.Tensor, q_dtype: torch.dtype = torch.int8, parts: int = 
     beyond x's type stay at 240 scale. A group that holds NaN or an infinity comes back as NaN.
     Not differentiable: a backward pass that meets the result raises.
     """
+    no_tangents("save_rows8", x)
     R, W, ld, ptr = matrix(x, "x")
     dt = _check_half(x, "x")
     if W < 1 or parts < 1 or W % parts:
@@ -99,6 +100,7 @@ def restore_rows8(saved: Rows8, index: Optional[torch.Tensor] = None, out: Optio
     """The 16-bit rows that `saved` stands for; with ``index`` [R] int32 / int64, rows ``index[r]`` of a 2-D copy
     (zeros where that is no row). Not differentiable."""
     q, scale, dtype = saved.q, saved.scale, saved.dtype
+    no_tangents("restore_rows8", scale)
     if not q.is_cuda:
         raise ValueError("saved rows must be CUDA tensors")
     dev, shape = q.device, q.shape
@@ -208,6 +210,7 @@ def silu_mul(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = None, 
     works from an 8-bit copy (:func:`save_rows8`, made in the same pass) instead of gate_up itself.
     """
     require(save is None or save in Q_DTYPES, "save must be None, torch.int8 or torch.float8_e4m3fn")
+    no_tangents("silu_mul", gate_up, row_weights)
     if torch.is_grad_enabled() and (gate_up.requires_grad or (row_weights is not None and row_weights.requires_grad)):
         return _SiluMul.apply(gate_up, row_weights, save, None if save is None else graph_link(gate_up))
     return silu_forward(gate_up, row_weights, None)[0]
@@ -218,6 +221,7 @@ def silu_mul_rows8(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = 
     Not differentiable (``silu_mul(..., save=)`` is)."""
     if q_dtype not in Q_DTYPES:
         raise ValueError("q_dtype must be torch.int8 or torch.float8_e4m3fn")
+    no_tangents("silu_mul_rows8", gate_up, row_weights)
     h, saved = silu_forward(gate_up, row_weights, q_dtype)
     if torch.is_grad_enabled() and (gate_up.requires_grad or (row_weights is not None and row_weights.requires_grad)):
         h, saved.scale = without_gradient("silu_mul_rows8", (h, saved.scale), gate_up, row_weights)
@@ -230,6 +234,7 @@ def silu_mul_backward(dh: torch.Tensor, gate_up, row_weights: Optional[torch.Ten
 
     drow_weights has the dtype and shape of row_weights and a fixed summation order.
     """
+    no_tangents("silu_mul_backward", dh, gate_up.scale if isinstance(gate_up, Rows8) else gate_up, row_weights)
     dweights = None if row_weights is None else empty_of(row_weights.shape, row_weights.dtype, row_weights.device)
     dgate_up, h = silu_backward(dh, gate_up, row_weights, dweights)
     return dgate_up, dweights, h

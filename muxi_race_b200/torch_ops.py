@@ -23,6 +23,7 @@ from . import route as _route
 from . import rows8 as _rows8
 from . import submission as _submission
 from . import w4 as _w4
+from ._args import no_tangents as _no_tangents
 
 
 @torch.library.custom_op("muxi_race_b200::fused_moe", mutates_args=())
@@ -159,6 +160,7 @@ def _fused_moe_w4_fake(hidden_states, w13, w2, num_experts, intermediate, group_
 
 @torch.library.custom_op("muxi_race_b200::grouped_linear", mutates_args=())
 def grouped_linear(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
+    _no_tangents("grouped_linear", x, w)
     return _grouped._rows_product("moe_grouped_linear", x, "x", w, offsets, False)
 
 
@@ -179,6 +181,7 @@ def _grouped_linear_backward_fake(dy, x, w, offsets):
 
 @torch.library.custom_op("muxi_race_b200::silu_mul", mutates_args=())
 def silu_mul(gate_up: Tensor, row_weights: Optional[Tensor]) -> Tensor:
+    _no_tangents("silu_mul", gate_up, row_weights)
     return _rows8.silu_forward(gate_up, row_weights, None)[0]
 
 
