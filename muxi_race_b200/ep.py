@@ -32,6 +32,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib
+from ._args import no_tangents
 from ._lib import _c_void_p
 from .fused import _DTYPES, _ID_DTYPES, _W_DTYPES, _stream, _workspace, fused_moe
 
@@ -207,6 +208,7 @@ class ExpertParallelMoE:
         local MoE. Every rank takes part in all ``chunks`` rounds of exchanges, with empty sends for
         chunks it does not have, so the collectives match across ranks whatever their token
         counts."""
+        no_tangents("ExpertParallelMoE", hidden_states, topk_weights)
         x = hidden_states
         T, H = x.shape
         k = topk_ids.shape[1]
@@ -384,6 +386,7 @@ class PeerMemoryEP:
     def forward(self, hidden_states: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
         if self._closed:
             raise RuntimeError("module closed")
+        no_tangents("PeerMemoryEP", hidden_states, topk_weights)
         x, ids, w = hidden_states.contiguous(), topk_ids.contiguous(), topk_weights.contiguous()
         T = int(x.shape[0])
         if T > self.T_max or x.shape[1] != self.H or ids.shape != (T, self.k) or w.shape != (T, self.k):

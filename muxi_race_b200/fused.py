@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import overlap
+from ._args import no_tangents, overlap
 
 BLOCK_M = 128
 _DTYPES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
@@ -155,6 +155,7 @@ def fused_moe(
     ``deterministic``: sum each token's k rows in route order in fp32 (``moe_fused_ordered``),
     so repeated calls give identical bits; the default adds them with atomics in Stage2.
     """
+    no_tangents("fused_moe", hidden_states, w_gate_up, w_down, topk_weights)
     T, H, I, E, k = _check_fused(hidden_states, w_gate_up, w_down, topk_ids, topk_weights, False)
     out = _output(out, hidden_states, hidden_states.dtype)
     if T == 0:
@@ -197,6 +198,7 @@ def fused_topk(
     ``renormalize``; ids in descending logit order, equal logits by ascending expert id.
     ``hidden_states`` only fixes T (the argument order of the usual fused-MoE router helper).
     """
+    no_tangents("fused_topk", gating_output)
     T = int(hidden_states.shape[0])
     E = _check_logits(gating_output, T, topk)
     dev = gating_output.device
@@ -226,6 +228,7 @@ def grouped_topk(
     at the chosen ids, renormalised when ``renormalize``, times ``routed_scaling_factor``.
     """
     T = int(hidden_states.shape[0])
+    no_tangents("grouped_topk", gating_output, e_score_correction_bias)
     _check(gating_output.dim() == 2 and gating_output.shape[0] == T, "gating_output must be [T, E]")
     _check(gating_output.is_cuda and gating_output.is_contiguous(), "gating_output must be a contiguous CUDA tensor")
     _check(gating_output.dtype in _LOGIT_DTYPES, "gating_output must be fp32, fp16 or bf16")
@@ -262,6 +265,7 @@ def fused_moe_router(
     kernel also builds the alignment's expert histogram. Returns ``out`` or, with
     ``return_routing``, ``(out, topk_weights, topk_ids)``.
     """
+    no_tangents("fused_moe_router", hidden_states, w_gate_up, w_down, gating_output)
     T = int(hidden_states.shape[0])
     E = _check_logits(gating_output, T, topk)
     dev = hidden_states.device
@@ -290,6 +294,7 @@ def quantize_rows_int8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``w`` [..., K] fp16/bf16 (e.g. stacked weights [E, N, K], one scale per output row).
     Returns (q int8 of w's shape, scale fp32 of shape w.shape[:-1]).
     """
+    no_tangents("quantize_rows_int8", w)
     _check(w.is_cuda and w.is_contiguous() and w.dtype in _DTYPES, "w must be a contiguous fp16/bf16 CUDA tensor")
     K = w.shape[-1]
     rows = w.numel() // K if K else 0
@@ -346,6 +351,7 @@ def fused_moe_int8(
 
     With ``hidden_scale`` [T] fp32 the rows are int8 already (:func:`add_rms_norm_quant`) and the output
     is in ``out_dtype`` (default: that of ``out``, or bf16), which is for this form only."""
+    no_tangents("fused_moe_int8", hidden_states, hidden_scale, w13_scale, w2_scale, topk_weights)
     if hidden_scale is not None:
         return _fused_q8_rows(hidden_states, hidden_scale, torch.int8, w13_q, w13_scale, w2_q, w2_scale, topk_ids,
                               topk_weights, out, out_dtype)
@@ -374,6 +380,7 @@ def quantize_rows_fp8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``w`` [..., K] fp16/bf16. Returns (q torch.float8_e4m3fn of w's shape, scale fp32 of shape
     w.shape[:-1]).
     """
+    no_tangents("quantize_rows_fp8", w)
     _check(w.is_cuda and w.is_contiguous() and w.dtype in _DTYPES, "w must be a contiguous fp16/bf16 CUDA tensor")
     K = w.shape[-1]
     rows = w.numel() // K if K else 0
@@ -402,6 +409,7 @@ def fused_moe_fp8(
 
     With ``hidden_scale`` [T] fp32 the rows are e4m3 already (:func:`add_rms_norm_quant`) and the output
     is in ``out_dtype`` (default: that of ``out``, or bf16), which is for this form only."""
+    no_tangents("fused_moe_fp8", hidden_states, hidden_scale, w13_scale, w2_scale, topk_weights)
     if hidden_scale is not None:
         return _fused_q8_rows(hidden_states, hidden_scale, torch.float8_e4m3fn, w13_q, w13_scale, w2_q, w2_scale, topk_ids,
                               topk_weights, out, out_dtype)

@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, launch, once_differentiable, overlap_at, pitch, require, rows, without_gradient
+from ._args import FLOATS, launch, no_tangents, once_differentiable, overlap_at, pitch, require, rows, without_gradient
 from .fused import _workspace
 
 _Q_DTYPES = {torch.int8: _lib.MOE_I8, torch.float8_e4m3fn: _lib.MOE_F8E4M3}
@@ -65,6 +65,7 @@ def _sum_args(x, x_at, T, residual, residual_out):
 
 
 def _forward(x, weight, residual, eps, out, residual_out):
+    no_tangents("add_rms_norm", x, weight, residual)
     x2 = rows(x, "x")
     T, H = x2.shape
     dtype, dev = x2.dtype, x2.device
@@ -140,6 +141,7 @@ def add_rms_norm_quant(
     results raises (a ``residual_out`` carries no graph).
     """
     require(q_dtype in _Q_DTYPES, "q_dtype must be torch.int8 or torch.float8_e4m3fn")
+    no_tangents("add_rms_norm_quant", x, weight, residual)
     x2 = rows(x, "x")
     T, H = x2.shape
     dtype, dev = x2.dtype, x2.device
@@ -167,6 +169,7 @@ def add_rms_norm_backward(
     ``h`` is the sum that the forward returned (x itself without a residual), ``dh`` the gradient that
     reaches it from its other uses. dweight has the weight's dtype and a fixed summation order.
     """
+    no_tangents("add_rms_norm_backward", dy, h, weight, dh)
     y2 = rows(dy, "dy")
     h2 = rows(h, "h", y2.device)
     require(dy.shape == h.shape and dy.dtype == h.dtype, "dy and h must have one shape and dtype")

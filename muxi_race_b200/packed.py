@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from ._args import no_tangents
 from .fused import _DTYPES, _ID_DTYPES, _W_DTYPES, _check, _output, _stream, _workspace
 
 KINDS = {"fp16": _lib.MOE_F16, "bf16": _lib.MOE_BF16, "int8": _lib.MOE_I8, "fp8": _lib.MOE_F8E4M3}
@@ -62,6 +63,7 @@ class PackedWeights:
 def pack_weights(gate_w: torch.Tensor, up_w: torch.Tensor, down_w: torch.Tensor, kind: Optional[str] = None
                  ) -> PackedWeights:
     """Pack reference-layout weights (fp16/bf16 CUDA tensors); kind defaults to their dtype."""
+    no_tangents("pack_weights", gate_w, up_w, down_w)
     for t in (gate_w, up_w, down_w):
         _check(t.is_cuda and t.is_contiguous() and t.dtype in _DTYPES, "weights must be contiguous fp16/bf16 CUDA")
     _check(gate_w.dim() == 3 and gate_w.shape == up_w.shape, "gate_w and up_w must both be [E, I, H]")
@@ -79,6 +81,7 @@ def pack_weights(gate_w: torch.Tensor, up_w: torch.Tensor, down_w: torch.Tensor,
 def fused_moe_packed(hidden_states: torch.Tensor, packed: PackedWeights, topk_ids: torch.Tensor,
                      topk_weights: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``fused_moe`` (or its int8 / fp8 route, by the packed kind) on packed weights."""
+    no_tangents("fused_moe_packed", hidden_states, topk_weights)
     _check(hidden_states.dim() == 2 and hidden_states.dtype in _DTYPES, "hidden_states must be fp16/bf16 [T, H]")
     T, H = hidden_states.shape
     _check(H == packed.H, f"hidden size {H} != packed {packed.H}")

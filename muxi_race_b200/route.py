@@ -13,12 +13,13 @@ from typing import Optional
 
 import torch
 
-from ._args import FLOATS, empty2, launch, once_differentiable, pitch, require, rows
+from ._args import FLOATS, empty2, launch, no_tangents, once_differentiable, pitch, require, rows
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
 
 
 def _forward(logits, topk, scoring, bias, num_groups, topk_groups, group_top, renormalize, scale, counts):
+    no_tangents("route_topk", logits, bias)
     l2 = rows(logits, "logits")
     T, E = l2.shape
     dev, dtype = l2.device, l2.dtype
@@ -106,6 +107,7 @@ def route_topk_backward(
 ) -> torch.Tensor:
     """Gradient of :func:`route_topk`'s weights for the logits ([T, E], the logits' dtype), given the
     ids that it chose (each expert at most once per token)."""
+    no_tangents("route_topk_backward", dweights, logits)
     l2 = rows(logits, "logits")
     require(logits.dim() == 2 and l2.dtype in FLOATS, "logits must be fp32, fp16 or bf16 [T, E]")
     require(scoring in _SCORING, "scoring must be 'softmax' or 'sigmoid'")

@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from ._args import no_tangents
 
 _DTYPES = {torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
 _ROUTED_DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16}
@@ -53,6 +54,7 @@ def run_kernel(
     Same arguments as the reference ``run_kernel``. Tensors must be contiguous CUDA tensors on one
     device; token/weight/output dtype fp16 or bf16 (the reference is fp16 only); metadata int32.
     """
+    no_tangents("run_kernel", stacked_expert_tokens, gate_w, up_w, down_w, routed_expert_weights)
     x = stacked_expert_tokens
     hidden = int(x.shape[1])
     intermediate = int(gate_w.shape[1])

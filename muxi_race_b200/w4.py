@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._args import FLOATS, HALVES, IDS, empty2, launch, overlap, pitch, require, rows, without_gradient
+from ._args import FLOATS, HALVES, IDS, empty2, launch, no_tangents, overlap, pitch, require, rows, without_gradient
 from .fused import _workspace
 
 
@@ -69,6 +69,7 @@ def pack_w4(
     ``in_features``: K, where it is odd (default: twice q's last dimension). ``gate_up``: the rows are
     gate rows followed by as many up rows, for :func:`fused_moe_w4`.
     """
+    no_tangents("pack_w4", scales)
     _check_group(group_size)
     require(q.is_cuda and q.dtype == torch.uint8 and q.is_contiguous() and q.dim() >= 2,
             "q must be a contiguous uint8 CUDA tensor [..., N, ceil(K / 2)]")
@@ -105,6 +106,7 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, symmetric: bool = True, 
     zero point, over the group's range widened to hold 0. A group with NaN or an infinity comes back
     without finite values.
     """
+    no_tangents("quantize_w4", w)
     _check_group(group_size)
     require(w.is_cuda and w.dtype in HALVES and w.is_contiguous() and w.dim() >= 2,
             "w must be a contiguous fp16 or bf16 CUDA tensor [..., N, K]")
@@ -138,6 +140,7 @@ def w4_linear(x: torch.Tensor, w: W4Weights, out: Optional[torch.Tensor] = None)
     more: for a prompt, ``torch.matmul`` with :func:`dequantize_w4` is the better call. Not differentiable:
     a backward pass that meets the result raises (``out`` carries no graph).
     """
+    no_tangents("w4_linear", x)
     if len(w.shape) != 2 or w.gate_up:
         raise ValueError("w must be one matrix, packed without gate_up")
     N, K = w.shape
@@ -190,6 +193,7 @@ def fused_moe_w4(
     Not differentiable: a backward pass that meets the result raises (``out``
     carries no graph).
     """
+    no_tangents("fused_moe_w4", hidden_states, topk_weights)
     if len(w13.shape) != 3 or not w13.gate_up or len(w2.shape) != 3 or w2.gate_up:
         raise ValueError("w13 must be [E, 2I, H] packed with gate_up, w2 [E, H, I] without")
     E, N13, H = w13.shape

@@ -6,6 +6,9 @@ from torch.autograd import forward_ad
 
 import muxi_race_b200 as m
 import muxi_race_b200.torch_ops  # noqa: F401
+from muxi_race_b200 import _lib
+from muxi_race_b200.ep import ExpertParallelMoE, PeerMemoryEP
+from muxi_race_b200.packed import packed_layout
 
 OPS = torch.ops.muxi_race_b200
 BF16, I8 = torch.bfloat16, torch.int8
@@ -61,3 +64,68 @@ def check(call, args):
 def test_training(name):
     call, *args = TRAINING[name]
     check(call, args)
+
+
+def w4(*shape, gate_up=False):
+    """4-bit weights [..., N, K] on the CPU."""
+    matrices = 1
+    for n in shape[:-2]:
+        matrices *= n
+    nbytes = _lib.lib().moe_w4_packed_bytes(matrices, *shape[-2:], 128, 0, int(gate_up))
+    return m.W4Weights(torch.zeros(nbytes, dtype=torch.uint8), shape, BF16, 128, False, gate_up)
+
+
+def packed():
+    _, total = packed_layout(2, 8, 8, "bf16")
+    return m.PackedWeights(torch.zeros(total, dtype=torch.uint8), 2, 8, 8, "bf16")
+
+
+Q13, Q2 = torch.zeros(2, 16, 8, dtype=I8), torch.zeros(2, 8, 8, dtype=I8)
+S13, S2 = torch.ones(2, 16), torch.ones(2, 8)
+ROWS8 = torch.zeros(4, 8, dtype=I8)
+LOGITS = torch.zeros(4, 2)
+META = [torch.zeros(n, dtype=torch.int32) for n in (2, 3, 3, 1)]
+OTHERS = {
+    "fused_moe": (lambda x, w13, w2, w: m.fused_moe(x, w13, w2, IDS, w), half(4, 8), W13, W2, WEIGHTS),
+    "fused_moe_router": (lambda x, w13, w2, g: m.fused_moe_router(x, w13, w2, g, 1), half(4, 8), W13, W2, LOGITS),
+    "fused_moe_int8": (lambda x, s13, s2, w: m.fused_moe_int8(x, Q13, s13, Q2, s2, IDS, w), half(4, 8), S13, S2, WEIGHTS),
+    "fused_moe_int8, 8-bit rows": (lambda s, s13, s2, w: m.fused_moe_int8(ROWS8, Q13, s13, Q2, s2, IDS, w, hidden_scale=s),
+                                   SCALE, S13, S2, WEIGHTS),
+    "fused_moe_fp8": (lambda x, s13, s2, w: m.fused_moe_fp8(x, Q13, s13, Q2, s2, IDS, w), half(4, 8), S13, S2, WEIGHTS),
+    "fused_moe_packed": (lambda x, w: m.fused_moe_packed(x, packed(), IDS, w), half(4, 8), WEIGHTS),
+    "fused_moe_w4": (lambda x, w: m.fused_moe_w4(x, w4(2, 16, 8, gate_up=True), w4(2, 8, 8), IDS, w), half(4, 8), WEIGHTS),
+    "pack_weights": (m.pack_weights, half(2, 8, 8), half(2, 8, 8), half(2, 8, 8)),
+    "quantize_rows_int8": (m.quantize_rows_int8, half(4, 8)),
+    "quantize_rows_fp8": (m.quantize_rows_fp8, half(4, 8)),
+    "quantize_w4": (m.quantize_w4, half(4, 8)),
+    "pack_w4": (lambda s: m.pack_w4(torch.zeros(4, 4, dtype=torch.uint8), s), half(4, 1)),
+    "w4_linear": (lambda x: m.w4_linear(x, w4(3, 8)), half(4, 8)),
+    "fused_topk": (lambda g: m.fused_topk(half(4, 8), g, 1), LOGITS),
+    "grouped_topk": (lambda g, b: m.grouped_topk(half(4, 8), g, 1, True, 1, 1, b), LOGITS, torch.zeros(2)),
+    "route_topk": (lambda g, b: m.route_topk(g, 1, bias=b), LOGITS, torch.zeros(2)),
+    "route_topk_backward": (lambda d, g: m.route_topk_backward(d, g, IDS), WEIGHTS, LOGITS),
+    "add_rms_norm": (m.add_rms_norm, half(4, 8), half(8), half(4, 8)),
+    "add_rms_norm_quant": (m.add_rms_norm_quant, half(4, 8), half(8), half(4, 8)),
+    "add_rms_norm_backward": (m.add_rms_norm_backward, half(4, 8), half(4, 8), half(8), half(4, 8)),
+    "run_kernel": (lambda x, g, u, d, w: m.run_kernel(x, g, u, d, w, *META, half(4, 8)), half(4, 8), half(2, 8, 8), half(2, 8, 8),
+                   half(2, 8, 8), torch.ones(4)),
+    "torch.ops add_rms_norm": (lambda x, w, r: OPS.add_rms_norm(x, w, r, 1e-6), half(4, 8), half(8), half(4, 8)),
+    "torch.ops route_topk": (lambda g, b: OPS.route_topk(g, 1, "softmax", b, 1, 1, 2, True, 1.0), LOGITS, torch.zeros(2)),
+    "torch.ops fused_moe": (lambda x, w13, w2, w: OPS.fused_moe(x, w13, w2, IDS, w), half(4, 8), W13, W2, WEIGHTS),
+}
+
+
+@pytest.mark.parametrize("name", OTHERS)
+def test_others(name):
+    call, *args = OTHERS[name]
+    check(call, args)
+
+
+@pytest.mark.parametrize("kind", [ExpertParallelMoE, PeerMemoryEP])
+def test_expert_parallel(kind):
+    layer = kind.__new__(kind)  # a rank without a group: the check comes first
+    layer._closed = False
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(half(4, 8), half(4, 8))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            layer.forward(x, IDS, WEIGHTS)
