@@ -586,7 +586,8 @@ MOE_API int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, 
  *   moe_save_rows8: x [R, W] (pitch ld) -> q [R, W], scale.
  *   moe_restore_rows: out[r] = row index[r] / index_div of x (r without an index) in dtype; zeros where that is
  *     not in [0, src_rows). src_dtype MOE_I8 / MOE_F8E4M3 with scale, or dtype (rows as they are).
- *   moe_silu_mul: h = w silu(gate) up, gate_up [R, 2 I] (gate, then up), and with q its 8-bit copy (parts = 2).
+ *   moe_silu_mul: h = w silu(gate) up, gate_up [R, 2 I] (gate, then up), and with q its 8-bit copy (parts = 2). silu of a
+ *     gate below -88.7, where e^-gate is infinite in fp32, is 0.
  *   moe_silu_mul_backward: dgate_up [R, 2 I], h [R, I] and dweights from dh [R, I] and gate_up, in dtype or as 8-bit rows
  *     (contiguous, ld = 2 I, src_scale).
  *     weights (NULL: 1) are taken at weight_at[r] (NULL: r) of num_weights; a row whose place is outside has weight 0.

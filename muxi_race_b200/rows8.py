@@ -205,7 +205,8 @@ class _SiluMul(torch.autograd.Function):
 def silu_mul(gate_up: torch.Tensor, row_weights: Optional[torch.Tensor] = None, save: Optional[torch.dtype] = None) -> torch.Tensor:
     """``h = row_weight * silu(gate) * up`` of gate_up [..., 2 I] fp16 / bf16 (gate columns first; rows of any one pitch).
 
-    row_weights: one per row, fp32 / fp16 / bf16 (the routing weights of the experts' rows), 1 without.
+    row_weights: one per row, fp32 / fp16 / bf16 (the routing weights of the experts' rows), 1 without. fp32 in between: silu
+    of a gate below -88.7, where e^-gate is infinite, is 0.
     Differentiable once in gate_up and row_weights. ``save=torch.int8`` or ``torch.float8_e4m3fn``: the backward pass
     works from an 8-bit copy (:func:`save_rows8`, made in the same pass) instead of gate_up itself.
     """
