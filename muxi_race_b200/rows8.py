@@ -91,14 +91,15 @@ def save_rows8(x: torch.Tensor, q_dtype: torch.dtype = torch.int8, parts: int = 
     r = _empty_rows8(x.shape, parts, q_dtype, x.dtype, dev)
     launch(dev, "moe_save_rows8", ptr, ld, r.q.data_ptr(), Q_DTYPES[q_dtype], r.scale.data_ptr(), R, W, parts, dt)
     if torch.is_grad_enabled() and x.requires_grad:
-        # the scales carry the node: every use of the copy reads them
+        # the scales carry the node, and restore_rows8 hands it on
         r.scale, = without_gradient("save_rows8", (r.scale,), x)
     return r
 
 
 def restore_rows8(saved: Rows8, index: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The 16-bit rows that `saved` stands for; with ``index`` [R] int32 / int64, rows ``index[r]`` of a 2-D copy
-    (zeros where that is no row). Not differentiable."""
+    (zeros where that is no row). Not differentiable: a backward pass that meets the result of a copy of rows that need a
+    gradient raises (``out`` carries no graph)."""
     q, scale, dtype = saved.q, saved.scale, saved.dtype
     no_tangents("restore_rows8", scale)
     if not q.is_cuda:
@@ -114,7 +115,8 @@ def restore_rows8(saved: Rows8, index: Optional[torch.Tensor] = None, out: Optio
             raise ValueError(f"index must be a contiguous int32 or int64 tensor [R] on {dev}")
         R = index.shape[0]
         shape, index_ptr, index_dt = (R, W), index.data_ptr(), IDS[index.dtype]
-    if out is None:
+    given = out is not None
+    if not given:
         out = empty_of(shape, dtype, dev)
     else:
         require(tuple(out.shape) == tuple(shape) and out.dtype == dtype and out.is_contiguous() and out.device == dev,
@@ -124,9 +126,9 @@ def restore_rows8(saved: Rows8, index: Optional[torch.Tensor] = None, out: Optio
             require(t is None or not overlap(flat, t.view(1, -1)), "out must not share memory with the saved rows or the index")
     launch(dev, "moe_restore_rows", q.data_ptr(), W, Q_DTYPES[q.dtype], scale.data_ptr(), index_ptr, index_dt, 1, None,
            out.data_ptr(), R, src_rows, W, saved.parts, HALVES[dtype])
-    if not scale.requires_grad:
+    if given or not scale.requires_grad:
         return out
-    return without_gradient("restore_rows8", (out,), saved.scale)[0]
+    return without_gradient("restore_rows8", (out,), scale)[0]
 
 
 # ----------------------------------------------------------------------------- silu(gate) * up
