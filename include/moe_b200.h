@@ -577,6 +577,17 @@ MOE_API int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, 
                                   int offsets_dtype, void* dw, int dw_dtype, int64_t num_rows, int64_t num_experts,
                                   int64_t out_features, int64_t in_features, int dtype, void* stream);
 
+/* moe_grouped_linear_dw with a workspace, for experts of very many rows. The tensor core cuts each sum of 16 products and what it
+ * has so far towards zero, off by up to 2^-23 of it; a 32-bit dw adds parts of at most 768 rows with rounding. With a 16-bit dw
+ * the call without a workspace takes an expert's rows in one sum (of 2^20 rows of one sign 0.7 % is lost), this one in parts of at
+ * most 32768. No workspace is needed, and the two are the same, with MOE_F32 or up to 32768 rows in all. */
+MOE_API size_t moe_grouped_linear_dw_workspace_bytes(int64_t num_rows, int dw_dtype);
+
+MOE_API int moe_grouped_linear_dw_long(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets,
+                                       int offsets_dtype, void* dw, int dw_dtype, int64_t num_rows, int64_t num_experts,
+                                       int64_t out_features, int64_t in_features, int dtype, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * The activation between the experts' products, and 8-bit copies of rows for the backward pass.
  * 8-bit rows: fp32 scales [R, parts, ceil(W / parts / 128)], one for each 128 columns of each of a row's `parts`.

@@ -50,6 +50,9 @@ SIGNATURES = {
         _int, [_c_void_p, _i64, _c_void_p, _c_void_p, _int, _c_void_p] + [_i64] * 5 + [_int, _int, _c_void_p]),
     "moe_grouped_linear_dw": (
         _int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _int] + [_i64] * 4 + [_int, _c_void_p]),
+    "moe_grouped_linear_dw_workspace_bytes": (_size, [_i64, _int]),
+    "moe_grouped_linear_dw_long": (
+        _int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _int] + [_i64] * 4 + [_int, _c_void_p, _size, _c_void_p]),
     "moe_save_rows8": (_int, [_c_void_p, _i64, _c_void_p, _int, _c_void_p] + [_i64] * 3 + [_int, _c_void_p]),
     "moe_restore_rows": (
         _int,

@@ -41,7 +41,7 @@ int map_weights(CUtensorMap* m, const void* p, int elt, int64_t E, int64_t N, in
   return encode_map(m, p, elt, 3, dims, strides, box, "weights");
 }
 
-template <int KIND, typename T, typename OutT>
+template <int KIND, typename T, typename OutT, bool LONG = false>
 int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& b32, GroupedArgs args, cudaStream_t s) {
   int dev, sms;
   constexpr int elt = static_cast<int>(sizeof(OutT));
@@ -75,7 +75,8 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   if (KIND == kGroupedDw && sizeof(OutT) == 4 && args.rows / args.E > 64 * kGgChunk) args.halves = 1;
   if (lane_tiles(args.halves) * most > kMaxTiles) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
   if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;
-  constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT>;
+  if (LONG && pairs > kGgSumPairs) pairs = kGgSumPairs;
+  constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT, LONG>;
   MOE_TRY(allow_smem<kernel>(dev));
   kernel<<<static_cast<unsigned>(2 * pairs), kGgThreads, kGgSmemBytes, s>>>(a, b, b32, args);
   MOE_CUDA(cudaGetLastError());
@@ -110,6 +111,45 @@ int grouped_rows(const void* in, int64_t ld_in, const void* w, const void* offse
   g.zero_rest = zero_rest;
   return dtype == MOE_F16 ? launch_grouped<KIND, __half, __half>(a, b, b32, g, s)
                           : launch_grouped<KIND, __nv_bfloat16, __nv_bfloat16>(a, b, b32, g, s);
+}
+
+// What a 16-bit dW of R rows needs for the sums of its parts: nothing where no expert can have more rows than a part.
+size_t dw_workspace(int64_t R, int dw_dtype) {
+  return dw_dtype == MOE_F32 || R <= 64 * kGgChunk16 ? 0 : static_cast<size_t>(2 * kGgSumPairs) * kGgSumBytes;
+}
+
+int grouped_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets, int offsets_dtype, void* dw,
+               int dw_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, void* workspace, cudaStream_t s) {
+  MOE_TRY(check_grouped(offsets, offsets_dtype, R, E, N, K, dtype));
+  if (dw_dtype != dtype && dw_dtype != MOE_F32) return fail(MOE_ERR_INVALID_ARG, "dw_dtype must be dtype or MOE_F32");
+  if (!dw) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  if (R == 0) {
+    MOE_CUDA(cudaMemsetAsync(dw, 0, static_cast<size_t>(E) * N * K * (dw_dtype == MOE_F32 ? 4 : 2), s));
+    return MOE_OK;
+  }
+  if (!dy || !x) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  if (R > 1 && (ld_dy < N || ld_x < K)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
+  CUtensorMap a, b;
+  MOE_TRY(map_rows(&a, x, 2, R, K, ld_x, 64, 64, "x"));
+  MOE_TRY(map_rows(&b, dy, 2, R, N, ld_dy, 64, 64, "dy"));
+  GroupedArgs g{};
+  g.offsets = offsets;
+  g.offsets64 = offsets_dtype == MOE_I64;
+  g.E = static_cast<int>(E);
+  g.rows = R;
+  g.lanes = static_cast<int>(K);
+  g.cols = static_cast<int>(N);
+  g.out = dw;
+  g.ld_out = K;
+  g.sums = static_cast<uint4*>(workspace);
+  if (workspace && dw_workspace(R, dw_dtype) > 0)
+    return dtype == MOE_F16 ? launch_grouped<kGroupedDw, __half, __half, true>(a, b, b, g, s)
+                            : launch_grouped<kGroupedDw, __nv_bfloat16, __nv_bfloat16, true>(a, b, b, g, s);
+  if (dtype == MOE_F16)
+    return dw_dtype == MOE_F32 ? launch_grouped<kGroupedDw, __half, float>(a, b, b, g, s)
+                               : launch_grouped<kGroupedDw, __half, __half>(a, b, b, g, s);
+  return dw_dtype == MOE_F32 ? launch_grouped<kGroupedDw, __nv_bfloat16, float>(a, b, b, g, s)
+                             : launch_grouped<kGroupedDw, __nv_bfloat16, __nv_bfloat16>(a, b, b, g, s);
 }
 
 template <int NT, int WARPS, int AHEAD, typename OutT>
@@ -198,33 +238,21 @@ int moe_grouped_linear_dx(const void* dy, int64_t ld_dy, const void* w, const vo
 int moe_grouped_linear_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets, int offsets_dtype,
                           void* dw, int dw_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, void* stream) {
   clear_error();
-  MOE_TRY(check_grouped(offsets, offsets_dtype, R, E, N, K, dtype));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dw_dtype != dtype && dw_dtype != MOE_F32) return fail(MOE_ERR_INVALID_ARG, "dw_dtype must be dtype or MOE_F32");
-  if (!dw) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
-  if (R == 0) {
-    MOE_CUDA(cudaMemsetAsync(dw, 0, static_cast<size_t>(E) * N * K * (dw_dtype == MOE_F32 ? 4 : 2), s));
-    return MOE_OK;
-  }
-  if (!dy || !x) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
-  if (R > 1 && (ld_dy < N || ld_x < K)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
-  CUtensorMap a, b;
-  MOE_TRY(map_rows(&a, x, 2, R, K, ld_x, 64, 64, "x"));
-  MOE_TRY(map_rows(&b, dy, 2, R, N, ld_dy, 64, 64, "dy"));
-  GroupedArgs g{};
-  g.offsets = offsets;
-  g.offsets64 = offsets_dtype == MOE_I64;
-  g.E = static_cast<int>(E);
-  g.rows = R;
-  g.lanes = static_cast<int>(K);
-  g.cols = static_cast<int>(N);
-  g.out = dw;
-  g.ld_out = K;
-  if (dtype == MOE_F16)
-    return dw_dtype == MOE_F32 ? launch_grouped<kGroupedDw, __half, float>(a, b, b, g, s)
-                               : launch_grouped<kGroupedDw, __half, __half>(a, b, b, g, s);
-  return dw_dtype == MOE_F32 ? launch_grouped<kGroupedDw, __nv_bfloat16, float>(a, b, b, g, s)
-                             : launch_grouped<kGroupedDw, __nv_bfloat16, __nv_bfloat16>(a, b, b, g, s);
+  return grouped_dw(dy, ld_dy, x, ld_x, offsets, offsets_dtype, dw, dw_dtype, R, E, N, K, dtype, nullptr,
+                    static_cast<cudaStream_t>(stream));
+}
+
+size_t moe_grouped_linear_dw_workspace_bytes(int64_t R, int dw_dtype) { return dw_workspace(R, dw_dtype); }
+
+int moe_grouped_linear_dw_long(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets, int offsets_dtype,
+                               void* dw, int dw_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  clear_error();
+  const size_t need = dw_workspace(R, dw_dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return fail(MOE_ERR_WORKSPACE, "workspace must hold %zu bytes", need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(MOE_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  return grouped_dw(dy, ld_dy, x, ld_x, offsets, offsets_dtype, dw, dw_dtype, R, E, N, K, dtype, workspace,
+                    static_cast<cudaStream_t>(stream));
 }
 
 size_t moe_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {

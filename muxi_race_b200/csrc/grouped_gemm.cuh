@@ -55,11 +55,14 @@ constexpr int kGgAhead = 3;                 // blocks that one half may be ahead
 constexpr int kGgMaxExperts = 1024;
 constexpr int kGgEpiWarps = 8;              // two per TMEM lane quadrant, each with half of the columns
 constexpr int kGgThreads = 128 + 32 * kGgEpiWarps;
-constexpr int kGgChunk = 12;  // blocks of rows that are added up in TMEM at a time for a 32-bit dW
+constexpr int kGgChunk = 12;     // blocks of rows that are added up in TMEM at a time for a 32-bit dW
+constexpr int kGgChunk16 = 512;  // and for a 16-bit one
 constexpr int kGgBand = 8;  // column tiles that take turns on a weight tile
 constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiples of 32
 constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
 constexpr int kGgOutBytes = kGgEpiWarps / 2 * 4096;  // the epilogue's staging
+constexpr int kGgSumBytes = 2 * 256 * 128 * 4;  // of a CTA: the sums of a 16-bit dW's parts, 128 lanes x 256 columns of two halves
+constexpr int kGgSumPairs = 74;                 // pairs that there is room for (all of a B200)
 constexpr int kGgSmemBytes = 1024 + kGgRingBytes + kGgOutBytes + 256 + kGgTableInts * 4;
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
@@ -74,6 +77,7 @@ struct GroupedArgs {
   int red;               // extent of the reduction; Dw: unused
   void* out;
   int64_t ld_out;
+  uint4* sums;           // Dw, 16 bits in parts: kGgSumBytes for each CTA
   int zero_rest;         // rows of no group are cleared
   int out16;             // out's rows start on 16 bytes, and lanes come in whole 16 bytes
   int split, split_blocks;  // int8: slices of the reduction, blocks of each; slice i writes rows [i rows, (i + 1) rows)
@@ -141,7 +145,7 @@ __device__ __forceinline__ bool elect_one() {
 struct GroupedTile {
   int e, lane0, halves, ncols;
   int64_t row0;
-  int part, more;  // of a 32-bit dW: its number, and whether others follow
+  int part, more;  // of dW's rows: its number, and whether others follow
   int col0, kb0, kblocks, tail;  // tail: reduction rows or elements in the last block (0: it is full)
 };
 
@@ -155,11 +159,14 @@ __device__ __forceinline__ int gg_col_step(int rows) {  // columns per tile of a
 // shares of the columns, as many as there are pairs for.
 //
 // The tensor core cuts each sum of an accumulator and 16 products to the accumulator's last place, always towards zero, so its
-// error grows with the number of MMAs: 1.3e-6 of dW's norm at 1255 rows, where fp32 sums that round have 2e-7. That is nothing
-// beside a rounding to 16 bits. For a 32-bit dW (PARTS) a tile's rows are taken in equal parts of at most 768, whose sums the epilogue
-// adds to those before, rounding; the same thread reads what it wrote, while the next MMAs run. The error then stays below 1e-6 for any
-// number of rows (4064 rows of 8 experts, 4096 x 14336: 565 -> 619 us; 8192 rows of one, 8192 x 8192: 780 -> 1220 us).
-template <int KIND, bool PARTS>
+// error grows with the number of MMAs: 1.3e-6 of dW's norm at 1255 rows of normal data, where fp32 sums that round have 2e-7; 1.2e-3
+// at 2^20 rows, and 7e-3 where all terms have one sign. So dW's rows are taken in equal parts of at most PART blocks, whose sums the epilogue
+// adds to those before, rounding; the same thread reads what it wrote, while the next MMAs run.
+//   32 bits: 768 rows, 48 MMAs, sums in dW itself. 4e-7 to 7e-7 of its norm for normal data up to 9000 rows; what grows with the rows
+//   is the rounding of the parts' sum (4064 rows of 8 experts, 4096 x 14336: 565 -> 619 us; 8192 rows of one, 8192 x 8192: 780 -> 1220 us).
+//   16 bits: 32768 rows, 2048 MMAs: at most 1.6e-4 of dW's norm, 1.2e-4 of a sum of one sign, beside a rounding of 2^-11 (fp16) or 2^-8;
+//   sums in a workspace. Calls of at most 32768 rows have a kernel of their own, without parts (9088 rows: 466 us, 470 with).
+template <int KIND, int PART>
 struct GroupedSchedule {
   const int *prefix, *start, *rows;  // tiles before group e, its first row, its rows
   int E, lanes, tile_lanes, lane_tiles, red_blocks, red_tail, cols, split_blocks, e;
@@ -189,7 +196,7 @@ struct GroupedSchedule {
   __device__ int tiles() const { return whole + left * lane_parts * col_parts; }
   // The next part of a tile, or the next of this pair's tiles.
   __device__ void next(int& tile, int& row_part, int npairs) const {
-    if (PARTS && ++row_part < parts) return;
+    if (PART > 0 && ++row_part < parts) return;
     row_part = 0;
     tile += npairs;
   }
@@ -248,10 +255,10 @@ struct GroupedSchedule {
         t.row0 += c;
     }
     t.part = t.more = 0;
-    if (PARTS) {
+    if (PART > 0) {
       parts = 1;
-      if (t.kblocks > kGgChunk && t.ncols > 0) {
-        const int most = (t.kblocks + kGgChunk - 1) / kGgChunk, per = (t.kblocks + most - 1) / most;
+      if (t.kblocks > PART && t.ncols > 0) {
+        const int most = (t.kblocks + PART - 1) / PART, per = (t.kblocks + most - 1) / most;
         parts = (t.kblocks + per - 1) / per;
         t.part = row_part;
         t.more = row_part + 1 < parts;
@@ -361,8 +368,8 @@ __device__ __forceinline__ void gg_build_table(const GroupedArgs& a, int* table,
 
 // tmA: the lanes' operand. Y, int8: W as [E][N][K], box 128 bytes x 128 rows. Dx: W, box 64 k x 64 n. Dw: x [R][K],
 // box 64 k x 64 rows. tmB: the columns' operand. Y, Dx, int8: x or dy, box 128 bytes x 128 rows, and the same with 32
-// rows in tmB32. Dw: dy, box 64 n x 64 rows.
-template <int KIND, typename T, typename OutT>
+// rows in tmB32. Dw: dy, box 64 n x 64 rows. LONG: a 16-bit dW in parts.
+template <int KIND, typename T, typename OutT, bool LONG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmB32, const GroupedArgs args) {
@@ -419,7 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  GroupedSchedule<KIND, kDw && sizeof(OutT) == 4> sched(args, table, npairs);
+  GroupedSchedule<KIND, LONG ? kGgChunk16 : kDw && sizeof(OutT) == 4 ? kGgChunk : 0> sched(args, table, npairs);
   const int tiles = sched.tiles();
 
   if (warp == 0) {
@@ -707,6 +714,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGgThreads, 1)
           tmem_ld_wait();
           if (c0 + 32 >= to) release();
           const int n = min(32, to - c0);
+          if constexpr (LONG) {
+            if (t.part > 0 || t.more) {  // the sums of the parts before, written by this thread
+              uint4* s = args.sums + static_cast<int64_t>(blockIdx.x) * (kGgSumBytes / 16) +
+                         ((half * kGgEpiWarps + warp - 4) * 4 + (c0 - from) / 32) * 256 + lane;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                uint32_t* v = r + 4 * j;
+                if (t.part > 0) {
+                  const uint4 b = s[j * 32];
+                  v[0] = __float_as_uint(__uint_as_float(b.x) + __uint_as_float(v[0]));
+                  v[1] = __float_as_uint(__uint_as_float(b.y) + __uint_as_float(v[1]));
+                  v[2] = __float_as_uint(__uint_as_float(b.z) + __uint_as_float(v[2]));
+                  v[3] = __float_as_uint(__uint_as_float(b.w) + __uint_as_float(v[3]));
+                }
+                if (t.more) s[j * 32] = make_uint4(v[0], v[1], v[2], v[3]);
+              }
+              if (t.more) {
+                __syncwarp();
+                continue;
+              }
+            }
+          }
           if constexpr (kWide) {
             // a column's 32 lanes are a line of 128 bytes: straight from the registers
             OutT* o = out + at + f + c0 * args.ld_out;
