@@ -10,6 +10,8 @@ namespace {
 constexpr int64_t kMaxTiles = (int64_t(1) << 31) - 1;
 // Of rows, lanes and the reduction: the kernels round them up to whole tiles and blocks in 32 bits.
 constexpr int64_t kMaxExtent = (int64_t(1) << 31) - 2 * kGgHalf;
+// Of a sum that the tensor core takes as one: its tile is waited for, 0.35 us for each 64 terms, and waits give up after 2 s.
+constexpr int64_t kMaxReduction = int64_t(1) << 27;
 static_assert(kMaxExtent + kGgTile <= kMaxTiles && kMaxExtent + 2 * kGgHalf - 1 <= kMaxTiles, "a rounded extent has to fit an int");
 
 int check_grouped(const void* offsets, int offsets_dtype, int64_t R, int64_t E, int64_t N, int64_t K, int dtype) {
@@ -91,6 +93,7 @@ int grouped_rows(const void* in, int64_t ld_in, const void* w, const void* offse
   if (R == 0) return MOE_OK;
   if (!in || !w || !out) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
   const int64_t lanes = KIND == kGroupedY ? N : K, red = KIND == kGroupedY ? K : N;
+  if (red > kMaxReduction) return fail(MOE_ERR_UNSUPPORTED, "sums of more than 2^27 terms");
   if (R > 1 && (ld_in < red || ld_out < lanes)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
   CUtensorMap a, b, b32;
   if (KIND == kGroupedY)
@@ -128,6 +131,9 @@ int grouped_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const
     return MOE_OK;
   }
   if (!dy || !x) return fail(MOE_ERR_INVALID_ARG, "null tensor argument");
+  const bool parts = workspace && dw_workspace(R, dw_dtype) > 0;  // of a 16-bit dW; those of a 32-bit one need nothing
+  if (R > kMaxReduction && dw_dtype != MOE_F32 && !parts)
+    return fail(MOE_ERR_UNSUPPORTED, "a 16-bit dw of more than 2^27 rows needs moe_grouped_linear_dw_long");
   if (R > 1 && (ld_dy < N || ld_x < K)) return fail(MOE_ERR_INVALID_ARG, "row pitches must be >= the rows' length");
   CUtensorMap a, b;
   MOE_TRY(map_rows(&a, x, 2, R, K, ld_x, 64, 64, "x"));
@@ -142,7 +148,7 @@ int grouped_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const
   g.out = dw;
   g.ld_out = K;
   g.sums = static_cast<uint4*>(workspace);
-  if (workspace && dw_workspace(R, dw_dtype) > 0)
+  if (parts)
     return dtype == MOE_F16 ? launch_grouped<kGroupedDw, __half, __half, true>(a, b, b, g, s)
                             : launch_grouped<kGroupedDw, __nv_bfloat16, __nv_bfloat16, true>(a, b, b, g, s);
   if (dtype == MOE_F16)
