@@ -560,10 +560,13 @@ MOE_API int moe_fused_w4(const void* hidden_states, int64_t ld_hidden, const voi
  *   moe_grouped_linear_dw:  dw[e] = sum_r dy[r] x[r]^T over e's rows, 0 without rows; dw [E, N, K] contiguous in
  *                           dtype or MOE_F32
  * Rows of no expert (before offsets[0], from offsets[E] on): 0 where zero_rest != 0, else left as they are; what
- * they hold is never used. Offsets outside [0, R] are clamped. Sums in fp32, one rounding; the same bits on every run,
- * and for a row of y or dx whatever the other rows are and however many.
- * Requirements: dtype MOE_F16 / MOE_BF16; 1 <= E <= 1024; N and K multiples of 8; R, N and K at most 2^31 - 512;
- *   x, dy and w on 16-byte boundaries, row pitches (in elements) of x and dy multiples of 8; outputs share no memory with inputs.
+ * they hold is never used. Offsets outside [0, R] are clamped. Sums in fp32 (the tensor core cuts them towards zero, by
+ * up to 2^-23 for each 16 terms), one rounding; the same bits on every run, and for a row of y or dx whatever the other
+ * rows are and however many.
+ * Requirements: dtype MOE_F16 / MOE_BF16; 1 <= E <= 1024; N and K multiples of 8; R, N and K at most 2^31 - 512, a sum
+ *   that is not cut into parts at most 2^27 terms (K, for dx N, for a 16-bit dw without a workspace R);
+ *   x, dy and w on 16-byte boundaries, row pitches (in elements) of x and dy multiples of 8; outputs share no memory
+ *   with inputs.
  * ---------------------------------------------------------------------------------------- */
 MOE_API int moe_grouped_linear(const void* x, int64_t ld_x, const void* w, const void* offsets, int offsets_dtype, void* out,
                                int64_t ld_out, int64_t num_rows, int64_t num_experts, int64_t out_features,
@@ -630,7 +633,8 @@ MOE_API int moe_combine_rows(const void* y, const int32_t* slot, void* out, int6
 /* ------------------------------------------------------------------------------------------
  * Dense product of int8 rows: out[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] (+ bias[n]).
  * x [M, K] (pitch ld_x) and w [N, K] (contiguous) int8 as moe_quantize_rows_int8 or moe_add_rms_norm write them; out [M, N]
- * (pitch ld_out) MOE_F16, MOE_BF16 or MOE_F32; bias [N] fp32 or NULL. The sum is exact (int32); scales and bias in fp32.
+ * (pitch ld_out) MOE_F16, MOE_BF16 or MOE_F32; bias [N] fp32 or NULL. The sum is exact (int32); its conversion to fp32, the
+ * scales and the bias round in fp32, then once to out_dtype.
  * Requirements: K a multiple of 16 below 131072; M and N at most 2^31 - 512; x and w on 16-byte boundaries, ld_x a
  *   multiple of 16.
  * ---------------------------------------------------------------------------------------- */

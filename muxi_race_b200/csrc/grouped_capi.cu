@@ -59,9 +59,9 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   int64_t pairs = sms / 2;
   auto lane_tiles = [&](int halves) { return (args.lanes + halves * kGgHalf - 1) / (halves * kGgHalf); };
   // Rounds of the SM pairs, the last one cut as GroupedSchedule does, a quarter longer for the small tiles. A tile of 512 lanes takes
-  // 1.8 times as long as one of 256 (8192^3 bf16: 725 us in 7 rounds of those, 760 us in 14 of these; 4096^3: 99 us in 2, 103 us in 3.5),
-  // and more where the reduction has few blocks, as its stores are hidden less (int8, 4095 rows, 7168 x 2048: 56 us, with 256 lanes 49 us);
-  // not for dW, whose stores bound either form (64 experts of 128 rows, 7168 x 2048: 409 us, with 256 lanes 582 us).
+  // 1.8 times as long as one of 256 (8192^3 bf16: 703 us in 7 rounds of those, 738 us in 14 of these; 4096^3: 101 us in 2, 103 us in 3.5),
+  // and more where the reduction has few blocks, as its stores are hidden less (int8, 4095 rows, 7168 x 2048: 65 us, with 256 lanes 56 us);
+  // not for dW, whose stores bound either form (64 experts of 128 rows, 7168 x 2048: 410 us, with 256 lanes 425 us).
   const int64_t blocks = KIND == kDenseInt8 ? args.split_blocks : (args.red + 63) / 64;
   const double unit = KIND == kGroupedDw ? 1.8 : 1.76 + 5.6 / static_cast<double>(blocks);
   auto cost = [&](int halves) {
@@ -77,7 +77,7 @@ int launch_grouped(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap
   if (KIND == kGroupedDw && sizeof(OutT) == 4 && args.rows / args.E > 64 * kGgChunk) args.halves = 1;
   if (lane_tiles(args.halves) * most > kMaxTiles) return fail(MOE_ERR_UNSUPPORTED, "too many output tiles");
   if (lane_tiles(args.halves) * most < pairs) pairs = lane_tiles(args.halves) * most;
-  if (LONG && pairs > kGgSumPairs) pairs = kGgSumPairs;
+  if (LONG && pairs > kGgPairs) pairs = kGgPairs;
   constexpr auto kernel = grouped_gemm_kernel<KIND, T, OutT, LONG>;
   MOE_TRY(allow_smem<kernel>(dev));
   kernel<<<static_cast<unsigned>(2 * pairs), kGgThreads, kGgSmemBytes, s>>>(a, b, b32, args);
@@ -118,7 +118,7 @@ int grouped_rows(const void* in, int64_t ld_in, const void* w, const void* offse
 
 // What a 16-bit dW of R rows needs for the sums of its parts: nothing where no expert can have more rows than a part.
 size_t dw_workspace(int64_t R, int dw_dtype) {
-  return dw_dtype == MOE_F32 || R <= 64 * kGgChunk16 ? 0 : static_cast<size_t>(2 * kGgSumPairs) * kGgSumBytes;
+  return dw_dtype == MOE_F32 || R <= 64 * kGgChunk16 ? 0 : static_cast<size_t>(2 * kGgPairs) * kGgSumBytes;
 }
 
 int grouped_dw(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* offsets, int offsets_dtype, void* dw,
@@ -186,12 +186,13 @@ int int8_stream(const Int8StreamArgs& a, cudaStream_t s) {
 // 9.0 us; N = 7168, K = 2048: 10.5 against 11.5 us, N = 2048, K = 7168: 16 against 12 us).
 bool int8_streams(int64_t M, int64_t N, int64_t K) { return M <= 16 || (M <= 32 && N * K <= (int64_t(1) << 22)); }
 
-// Slices of the reduction: where tiles of 256 x 256 leave half of the 74 CTA pairs or more without work, with at least 4 blocks
+// Slices of the reduction: where tiles of 256 x 256 leave half of a B200's 74 CTA pairs or more without work (a constant, so that
+// the workspace's size depends on the sizes alone), with at least 4 blocks
 // of 128 each (N = 4096, K = 14336, 33 rows: 20 us in 4 slices, 48 us in one; 512 rows: 36 against 51 us).
 int64_t int8_split(int64_t M, int64_t N, int64_t K) {
   if (int8_streams(M, N, K)) return 1;
   const int64_t tiles = (M + kGgTile - 1) / kGgTile * ((N + kGgHalf - 1) / kGgHalf), blocks = (K + 127) / 128;
-  int64_t split = 74 / tiles;
+  int64_t split = kGgPairs / tiles;
   if (split > blocks / 4) split = blocks / 4;
   if (split > 16) split = 16;
   return split < 2 ? 1 : split;
@@ -299,7 +300,7 @@ int moe_int8_linear(const void* x, int64_t ld_x, const float* x_scale, const voi
   const int64_t blocks = (K + 127) / 128, split = int8_split(M, N, K);
   GroupedArgs g{};
   g.split_blocks = static_cast<int>((blocks + split - 1) / split);
-  g.E = g.split = static_cast<int>((blocks + g.split_blocks - 1) / g.split_blocks);  // no empty slices
+  g.E = static_cast<int>((blocks + g.split_blocks - 1) / g.split_blocks);  // no empty slices
   g.rows = M;
   g.lanes = static_cast<int>(N);
   g.red = static_cast<int>(K);

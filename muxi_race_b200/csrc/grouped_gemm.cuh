@@ -16,8 +16,8 @@
 //
 // Bounds: 2 R N K operations at the tensor rate, or the weights' bytes where an expert has fewer than about 250 rows. CTA pairs
 // (cta_group::2) bring each operand into shared memory once for both SMs. A tile is 512 lanes x 256 columns, two MMAs of 256 lanes that
-// share the columns' operand: 48 KiB per SM and 64-element step, where two tiles of 256 lanes take 64 (8192^3 bf16: 725 against 760 us,
-// cuBLAS 690 us in the same run; tensor pipe 95% busy). Its halves fill the 512 TMEM columns and are handed to the epilogue and back
+// share the columns' operand: 48 KiB per SM and 64-element step, where two tiles of 256 lanes take 64 (8192^3 bf16: 703 against 738 us,
+// cuBLAS 676 us in the same run; tensor pipe 95% busy). Its halves fill the 512 TMEM columns and are handed to the epilogue and back
 // one by one: the MMA warp runs the first half of the next tile ahead while the second is still being stored. Where 512 lanes would
 // leave SMs without work, tiles have 256 lanes and take turns with the two accumulators.
 //
@@ -62,7 +62,7 @@ constexpr int kGgColStep = 32;  // columns of cta_group::2 MMAs come in multiple
 constexpr int kGgTableInts = 3 * kGgMaxExperts + 4;
 constexpr int kGgOutBytes = kGgEpiWarps / 2 * 4096;  // the epilogue's staging
 constexpr int kGgSumBytes = 2 * 256 * 128 * 4;  // of a CTA: the sums of a 16-bit dW's parts, 128 lanes x 256 columns of two halves
-constexpr int kGgSumPairs = 74;                 // pairs that there is room for (all of a B200)
+constexpr int kGgPairs = 74;                    // pairs of CTAs of a B200, where a size may not depend on the device
 constexpr int kGgSmemBytes = 1024 + kGgRingBytes + kGgOutBytes + 256 + kGgTableInts * 4;
 static_assert(kGgSmemBytes <= 232448, "exceeds the shared memory of a CTA");
 
@@ -80,7 +80,7 @@ struct GroupedArgs {
   uint4* sums;           // Dw, 16 bits in parts: kGgSumBytes for each CTA
   int zero_rest;         // rows of no group are cleared
   int out16;             // out's rows start on 16 bytes, and lanes come in whole 16 bytes
-  int split, split_blocks;  // int8: slices of the reduction, blocks of each; slice i writes rows [i rows, (i + 1) rows)
+  int split_blocks;      // int8: blocks of each of E slices of the reduction; slice i writes rows [i rows, (i + 1) rows)
   const float* lane_scale;  // int8: ws
   const float* col_scale;   // int8: xs
   const float* bias;        // int8, or null
@@ -127,7 +127,7 @@ __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m
 }
 
 // A whole warp waits: a wait given up by one lane is given up by all. (The hardware suspends a waiting warp for a while; one
-// lane that polls with pauses, while the others stand by, sees the end later: 8192^3 724 us against 704.)
+// lane that polls with pauses, while the others stand by, sees the end later: 8192^3 took 3% longer.)
 __device__ __forceinline__ bool gg_all(bool ok) { return __all_sync(0xffffffffu, ok) != 0; }
 
 // True in one thread of a converged warp.
@@ -196,7 +196,9 @@ struct GroupedSchedule {
   __device__ int tiles() const { return whole + left * lane_parts * col_parts; }
   // The next part of a tile, or the next of this pair's tiles.
   __device__ void next(int& tile, int& row_part, int npairs) const {
-    if (PART > 0 && ++row_part < parts) return;
+    if constexpr (PART > 0) {
+      if (++row_part < parts) return;
+    }
     row_part = 0;
     tile += npairs;
   }
@@ -255,7 +257,7 @@ struct GroupedSchedule {
         t.row0 += c;
     }
     t.part = t.more = 0;
-    if (PART > 0) {
+    if constexpr (PART > 0) {
       parts = 1;
       if (t.kblocks > PART && t.ncols > 0) {
         const int most = (t.kblocks + PART - 1) / PART, per = (t.kblocks + most - 1) / most;

@@ -1,9 +1,9 @@
 // int8_stream.cuh — the dense int8 product for a few rows: the weights go from HBM to registers and nowhere else.
 //
 // out[m, n] = xs[m] ws[n] sum_k x[m, k] w[n, k] (+ bias[n]) is bound by the N K bytes of the weights. A CTA takes 16 of their
-// rows, its 8 warps an eighth of K each. mma.m16n8k32 wants 4-byte pieces of K from its lanes; since a sum may take its terms in
+// rows, its 4, 8 or 16 warps (kI8Warps) equal parts of K. mma.m16n8k32 wants 4-byte pieces of K from its lanes; since a sum may take its terms in
 // any order as long as both operands agree, lane (g, t) loads 16 bytes of K = 64 c + 16 t of rows g and g + 8, and of tokens, and
-// the two halves of those are two MMAs. Eight such loads of the weights are in flight per lane. The warps' whole-number sums
+// the two halves of those are two MMAs. 4 or 8 chunks (kI8Ahead) of two such loads of the weights are in flight per lane. The warps' whole-number sums
 // meet in shared memory: exact in any order. (tcgen05 reads its operands from shared memory, where the weights would have to be
 // written first; for these few columns its rate is not what bounds.)
 #pragma once

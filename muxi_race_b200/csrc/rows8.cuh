@@ -286,7 +286,8 @@ __device__ __forceinline__ int64_t r8_weight_at(const SiluArgs& a, int64_t r) {
   return i >= 0 && i < a.num_weights ? i : -1;
 }
 
-// 64 registers, for four CTAs on an SM (32768 x 2048 bf16 with the int8 copy: 88 us, 95 us with 80).
+// 64 registers, for four CTAs on an SM (32768 x 2048 bf16 with the int8 copy: 89 us, 95 us with 80), although with a copy a few
+// spill (24 to 28 bytes for rows in whole 8s to int8, 44 for single elements in bf16).
 template <typename T, typename Q, int VEC>
 __global__ void __launch_bounds__(kR8Threads, 4) silu_mul_kernel(const SiluArgs a) {
   const int warp = threadIdx.x >> 5, l8 = threadIdx.x & 7, sub = threadIdx.x >> 3 & 3;

@@ -124,9 +124,10 @@ def grouped_linear(
     """``y[r] = w[e] @ x[r]`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of each expert e.
 
     x [R, K] fp16 / bf16 with rows of any pitch that is a multiple of 8, w [E, N, K] (N and K multiples of 8,
-    E <= 1024), offsets [E + 1] int32 / int64, not falling (``moe_align(ids, E, 1).group_offsets``). Rows of no
+    E <= 1024, R, N at most 2^31 - 512, K at most 2^27), offsets [E + 1] int32 / int64, not falling (``moe_align(ids, E, 1).group_offsets``). Rows of no
     expert, before offsets[0] or from offsets[E] on, are 0 in a new result and left as they are in ``out``; what they
-    hold in x is not used. Sums in fp32, rounded once; the same bits on every run, and for a row whatever the others are
+    hold in x is not used. Sums in fp32, which the tensor core cuts towards zero, by up to 2^-23 for each 16 terms (K = 14336: at
+    most 7e-5 of a sum), then rounded once; the same bits on every run, and for a row whatever the others are
     and however many.
 
     Differentiable once in x and w (``out`` is not). ``save=torch.int8`` or ``torch.float8_e4m3fn``: x is kept for the

@@ -26,8 +26,9 @@ def int8_linear(
     """``y = (x @ w.T) * x_scale * w_scale (+ bias)``: x [..., K] int8 with one fp32 scale per row, w [N, K] int8 with one per
     row (output channel), bias [N] fp32; y [..., N] fp16, bf16 or fp32.
 
-    K is a multiple of 16 below 131072; x's rows have any pitch that is a multiple of 16. The sum is exact, scales and
-    bias are applied in fp32, one rounding. ``out`` (rows of any pitch) must not share memory with x. Not differentiable: a
+    K is a multiple of 16 below 131072, M and N at most 2^31 - 512; x's rows have any pitch that is a multiple of 16. The sum is
+    exact in int32; its conversion to fp32 (above 2^24), the two scales and the bias round in fp32, by 4 * 2^-24 in all, and the
+    result is rounded once to its type. ``out`` (rows of any pitch) must not share memory with x. Not differentiable: a
     backward pass that meets the result raises (``out`` carries no graph).
     """
     no_tangents("int8_linear", x_scale, w_scale, bias)
