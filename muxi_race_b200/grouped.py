@@ -245,6 +245,7 @@ class _MoeMlp(torch.autograd.Function):
     def backward(ctx, dout):
         x, x_scale, gate_up, scale, w13, w2, weights, offsets, order, slot, link = ctx.saved_tensors
         need_x, need_w13, need_w2, _, need_weights, *_ = ctx.needs_input_grad
+        no_tangents("moe_mlp's gradient", dout)
         grads = [None] * 7
         with torch.no_grad():
             kept = x

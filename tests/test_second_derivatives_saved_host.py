@@ -136,3 +136,14 @@ def test_moe_mlp_keeps_tokens_for_their_gradient_only(monkeypatch, save, trained
     assert len(tokens) == (1 in trained) and len(copies) == (1 in trained and save is not None)
     out.float().sum().backward()
     assert all(args[i].grad is not None for i in trained)
+
+
+def test_moe_mlp_tangent_of_the_gradient(monkeypatch):
+    """Forward-mode over the backward pass: a tangent of the gradient that reaches the operator would be dropped."""
+    cpu = CpuMlp(monkeypatch)
+    args = [t.clone().requires_grad_() if t.is_floating_point() else t for t in cpu.args]
+    out = grouped._moe_mlp_graph(*args, None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.autograd.grad(out, args[0], dual)
