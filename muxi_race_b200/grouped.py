@@ -219,8 +219,10 @@ def _mlp_forward(x, w13, w2, ids, weights, save):
     valid = offsets.data_ptr() + 4 * E
     xs = _gather(x, order, topk, valid, R)
     gate_up = _rows_product("moe_grouped_linear", xs, "x", w13, offsets, False, None, False)
+    del xs
     h, saved = silu_forward(gate_up, weights, save, order, valid)
     y = _rows_product("moe_grouped_linear", h, "h", w2, offsets, False, None, False)
+    del h
     return _combine(y, slot, T, topk), offsets, order, slot, (gate_up if saved is None else saved)
 
 
